@@ -372,6 +372,68 @@ int lf_pool_dedup_prefix(const lf_pool_meta* m, const lf_prefix_registry* r,
  * queue tail in ascending page-id order. */
 int lf_pool_unregister_all(const lf_pool_meta* m, const lf_prefix_registry* r, void* stream);
 
+/* ---- K/V cache held in 4 bits ------------------------------------------------------------
+ * The reference's cache is 16-bit only (runtime/kv_pool.py:48-101); these are the append, the
+ * decode and the prefill read of the same paged cache at 4.5 bits a value, on the pool's block
+ * tables.  A group is 64 dims of one token of one KV head: with low = min x and
+ * s = bf16((max - low) / 15), a value is held as n = rint((x - low) / s), 0..15 (0 when s is 0),
+ * and stands for n * s + low.  A group that holds a NaN or an infinity, or whose range overflows
+ * fp32, reads back as NaN.  A page of 16 tokens of one KV head is one block of 18 * D bytes
+ * (D = 64 or 128), pages [P][Hkv][18 * D]; byte offsets inside a block, NG = D / 64:
+ *   K code of (token t, dim d)  32-bit word at  t*32*NG + (d%64/16)*8*NG + (d/64)*8 + (d%16/8)*4,
+ *                               bits 4*(e/2) + 16*(e%2), e = d % 8
+ *   V code of (token t, dim d)  16-bit piece at 8*D + (t/8)*256*NG + ((d%64/8)*4 + t%8/2)*8*NG
+ *                               + (d/64)*8 + (d%8/4)*4 + (t%2)*2, bits 4*(d%4)
+ *   params [token][K, V][group][s, low] bf16 at 16*D. */
+
+/* Quantised append (4-bit form of lf_pool_write_kv and lf_pool_write_qkv).  Token t of session i
+ * (cu_tokens[i] <= t < cu_tokens[i+1]) goes to position start_pos[i] + t - cu_tokens[i] of
+ * block-table row seq_ids[i] (seq_ids NULL: row i); block_table is [table_rows][max_pages].
+ * k, v element (layer l, token t, head h, dim d) at l*stride_layer + t*stride_token +
+ * h*stride_head + d.  num_q_heads > 0 (one layer): q rows of num_q_heads * D at t*q_stride_token
+ * are copied to q_out [total_tokens, num_q_heads, D].  rope_cos / rope_sin (nullable): q and k are
+ * rotated as in lf_pool_write_qkv first.  pages is [num_layers][num_pages][Hkv][18 * D].  A row
+ * without a page, or past the rotation table, is not stored: *status (nullable, a pool's sticky
+ * status; nothing is done when it is already set) becomes LF_EINVAL, or, without a status, the
+ * device error word 222.  Strides multiples of 8, buffers 16-byte aligned. */
+int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v, int64_t q_stride_token,
+                 int64_t stride_layer, int64_t stride_token, int64_t stride_head,
+                 const int32_t* block_table, int table_rows, int max_pages, const int32_t* seq_ids,
+                 const int32_t* start_pos, const int32_t* cu_tokens, int n, int total_tokens,
+                 const float* rope_cos, const float* rope_sin, int rope_rows, lf_bf16* q_out,
+                 void* pages, int num_pages, int num_layers, int num_q_heads, int num_kv_heads,
+                 int head_dim, int32_t* status, void* stream);
+
+/* Expands the pages of a batch to bf16 for lf_prefill_paged_fwd (and for reading a session back).
+ * Output pages [out_pages][Hkv][16][D] are compact: the num_prefix_pages shared ones first, then
+ * each session's own pages in session order; out_table [num_seqs][max_pages] holds their ids (-1
+ * past a session's pages).  Rows at or past a session's length are zeros; output pages past the
+ * last session's are not written.  A session whose pages do not fit in out_pages is cut off there,
+ * with -1 in out_table and the device error word 223; a page id outside [0, num_pages) reads page 0
+ * (word 224).  k_out 32-byte aligned. */
+int lf_q4_expand(const void* pages, const int32_t* block_table, const int32_t* seq_lens,
+                 int num_prefix_pages, lf_bf16* k_out, lf_bf16* v_out, int32_t* out_table,
+                 int num_seqs, int num_kv_heads, int head_dim, int num_pages, int max_pages,
+                 int out_pages, void* stream);
+
+/* lf_pool_fork over 4-bit pages [num_layers][num_pages][Hkv][18 * D]. */
+int lf_q4_fork(const lf_pool_meta* m, int src_seq, const int32_t* dst_seqs, int n, int prefix_len,
+               void* pages, int num_layers, int num_kv_heads, int head_dim, void* stream);
+
+/* Paged split-KV decode over 4-bit pages: lf_decode_fwd's arguments and results (a session of
+ * length 0 gives zeros and an lse of -inf), with one array of pages [P][Hkv][18 * D].  Hq / Hkv is 1, 2, 4 or 8.
+ * The workspace comes from lf_q4_decode_workspace_size, the split size from
+ * lf_q4_decode_default_split (sm_count <= 0: the current device's). */
+int lf_q4_decode_default_split(int num_seqs, int num_kv_heads, int max_pages, int num_prefix_pages,
+                               int sm_count, int* pages_per_split);
+int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int head_dim, int max_pages,
+                                int pages_per_split, int num_prefix_pages, size_t* bytes);
+int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32_t* block_table,
+                     const int32_t* seq_lens, int num_prefix_pages, lf_bf16* o, float* lse,
+                     void* workspace, size_t workspace_bytes, int num_seqs, int num_q_heads,
+                     int num_kv_heads, int head_dim, int num_pages, int max_pages,
+                     int pages_per_split, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -86,6 +86,17 @@ _SIGS = {
     "lf_pool_dedup_prefix": [POINTER(PoolMeta), POINTER(PrefixRegistry), _P, _P, _P, c_int, _P, _P],
     "lf_pool_unregister_all": [POINTER(PoolMeta), POINTER(PrefixRegistry), _P],
 }
+_I = c_int
+_SIGS.update({
+    "lf_q4_append": [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _I, _I, _P, _P, _P, _I, _I,
+                     _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P],
+    "lf_q4_expand": [_P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "lf_q4_fork": [POINTER(PoolMeta), _I, _P, _I, _I, _P, _I, _I, _I, _P],
+    "lf_q4_decode_default_split": [_I, _I, _I, _I, _I, POINTER(c_int)],
+    "lf_q4_decode_workspace_size": [_I, _I, _I, _I, _I, _I, POINTER(c_size_t)],
+    "lf_q4_decode_fwd": [_P, _P, _P, _P, _I, _P, _P, _P, c_size_t, _I, _I, _I, _I, _I, _I, _I,
+                         c_float, _P],
+})
 _RESTYPE = {"lf_version": c_char_p, "lf_last_error": c_char_p}
 
 _lib = None

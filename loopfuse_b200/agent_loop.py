@@ -39,8 +39,10 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
+from ._lib import LF_EINVAL, LoopfuseError
 from .llama import GraphedDecode, LlamaShaped
 from .runtime.kv_pool import KVPool, KVState
+from .runtime.kv_pool_q4 import QuantKVPool
 
 PAGE = 16
 
@@ -64,6 +66,7 @@ class AgentLoopConfig:
     # tiny prefill batches (a few returning tools at a time) cost a whole forward each.
     min_prefill_tokens: int = 2048
     max_prefill_wait_ms: float = 25.0
+    kv_bits: int = 16                # 4: sessions' K/V held in 4 bits (QuantKVPool)
     seed: int = 0
 
 
@@ -129,9 +132,12 @@ class AgentLoop:
         pages = self.n_prefix_pages + sum((o + PAGE - 1) // PAGE + 1 for o in own) + 16 + \
             n + min(n, self.PROFILE_SESSIONS) * (self.PROFILE_PREFILL // PAGE + 1)
         mc = model.cfg
-        self.pool = KVPool(num_layers=mc.layers, num_heads=mc.q_heads, num_kv_heads=mc.kv_heads,
-                           head_dim=mc.head_dim, max_seq_len=max_len, max_slots=n + 2,
-                           dtype=torch.bfloat16, device=self.device, num_pages=pages + 1)
+        if cfg.kv_bits not in (4, 16):
+            raise LoopfuseError(LF_EINVAL, f"kv_bits must be 4 or 16, got {cfg.kv_bits}")
+        pool_type = QuantKVPool if cfg.kv_bits == 4 else KVPool
+        self.pool = pool_type(num_layers=mc.layers, num_heads=mc.q_heads, num_kv_heads=mc.kv_heads,
+                              head_dim=mc.head_dim, max_seq_len=max_len, max_slots=n + 2,
+                              dtype=torch.bfloat16, device=self.device, num_pages=pages + 1)
         self.rng = np.random.default_rng(cfg.seed + 17)
         self.root: Optional[KVState] = None
         self.gd: Optional[GraphedDecode] = None
@@ -202,7 +208,8 @@ class AgentLoop:
         from .analysis import kernel_roofline
         from .llama import OpTimer
         c, pool = self.model.cfg, self.pool
-        kv_tok = 2 * c.kv_heads * c.head_dim * 2 * c.layers           # K+V bytes per token
+        # K+V bytes per token of the cache; a 4-bit cache is prefilled from its bf16 expansion
+        kv_tok = c.kv_heads * c.head_dim * c.layers * (4 if self.cfg.kv_bits == 16 else 9 / 8)
         res = {}
         for phase in ("decode", "prefill"):
             chosen = sessions if phase == "decode" else sessions[:self.PROFILE_SESSIONS]

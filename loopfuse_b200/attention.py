@@ -13,6 +13,12 @@ CPU or eager fallback: a missing library, a wrong device or dtype raises.
 * ``decode_attention_fwd(q, k, v)`` -- drop-in for
   ``kernels/triton/decode_attn.py:133-171`` (contiguous ``[B,H,S,D]`` cache):
   the cache is laid out as pages and handed to ``paged_decode``.
+
+K/V may also be held in 4 bits (4.5 with their scales; format in ``include/loopfuse_b200.h``):
+
+* ``append_qkv_q4(...)`` -- split, rotate and quantise a QKV projection's rows into the pages.
+* ``paged_decode_q4(...)`` -- ``paged_decode`` over 4-bit pages.
+* ``expand_pages_q4(...)`` -- a batch's pages as bf16, for ``prefill_paged``.
 """
 from __future__ import annotations
 
@@ -211,3 +217,174 @@ def decode_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     lens = torch.full((B,), S, dtype=torch.int32, device=q.device)
     o = paged_decode(q.reshape(B, H, D).contiguous(), kp, vp, table, lens, scale=scale)
     return o.view(B, H, 1, D)
+
+
+# -- K/V held in 4 bits -------------------------------------------------------------------------------
+def q4_head_dim(pages: torch.Tensor) -> int:
+    """Head dim of 4-bit pages ``[P, Hkv, 18 * D]``: 64 or 128."""
+    _require(pages, "pages", torch.uint8)
+    if pages.dim() != 3 or pages.shape[2] not in (18 * 64, 18 * 128):
+        raise LoopfuseError(_lib.LF_EINVAL, f"4-bit pages must be [P, Hkv, 18 * D] with D 64 or 128, "
+                                            f"got {tuple(pages.shape)}")
+    return pages.shape[2] // 18
+
+
+def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """The device all the given tensors are on."""
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) != 1:
+        raise LoopfuseError(_lib.LF_EINVAL, f"{what}: tensors on different devices: "
+                                            f"{sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def append_qkv_q4(qkv: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
+                  start_pos: torch.Tensor, cu_tokens: torch.Tensor, num_q_heads: int,
+                  rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                  q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Quantised append of one layer: ``qkv [T, (Hq + 2 Hkv) * D]`` (q heads, then k heads, then v
+    heads per row; rows may be strided), the new tokens of N sessions back to back.
+
+    Token ``t`` of session ``i`` (``cu_tokens [N+1]``) goes to position ``start_pos[i] + t -
+    cu_tokens[i]`` of ``block_table [N, max_pages]``, into ``pages [P, Hkv, 18 * D]``; q and k are
+    first rotated with ``rope = (cos, sin)`` (``[rows, D/2]`` fp32, "rotate half").  Returns the
+    rotated q ``[T, Hq, D]`` (``q_out`` when given).  Block-table rows and pages are the caller's to
+    reserve; a token without a page is not stored and is reported by ``lf_device_status``.
+    """
+    D = q4_head_dim(pages)
+    P, Hkv, _ = pages.shape
+    Hq = int(num_q_heads)
+    for t, n in ((block_table, "block_table"), (start_pos, "start_pos"), (cu_tokens, "cu_tokens")):
+        _require(t, n, torch.int32)
+    N = start_pos.shape[0]
+    if block_table.dim() != 2 or block_table.shape[0] != N or start_pos.dim() != 1 or \
+            cu_tokens.shape != (N + 1,):
+        raise LoopfuseError(_lib.LF_EINVAL, "append_qkv_q4: block_table must be [N, max_pages], "
+                                            "start_pos [N], cu_tokens [N + 1]")
+    if not qkv.is_cuda or qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or Hq <= 0 or \
+            qkv.shape[1] != (Hq + 2 * Hkv) * D or qkv.stride(1) != 1 or \
+            (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
+        raise LoopfuseError(_lib.LF_EINVAL, "append_qkv_q4 expects bf16 rows qkv [T, (Hq + 2 Hkv) * D]")
+    T = qkv.shape[0]
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=qkv.dtype, device=qkv.device)
+    _require(q_out, "q_out")
+    if tuple(q_out.shape) != (T, Hq, D):
+        raise LoopfuseError(_lib.LF_EINVAL, f"q_out must be [T, Hq, D] = {(T, Hq, D)}")
+    cos, sin, rows = _rope(rope, D)
+    dev = _one_device("append_qkv_q4", qkv, pages, block_table, start_pos, cu_tokens, q_out, cos, sin)
+    if T == 0 or N == 0:
+        return q_out
+    base, elem, row = qkv.data_ptr(), qkv.element_size(), qkv.stride(0) if T > 1 else qkv.shape[1]
+    with torch.cuda.device(dev):
+        _lib.call("lf_q4_append", base, base + Hq * D * elem, base + (Hq + Hkv) * D * elem, row, 0,
+                  row, D, block_table.data_ptr(), N, block_table.shape[1], None, start_pos.data_ptr(),
+                  cu_tokens.data_ptr(), N, T, cos.data_ptr() if cos is not None else None,
+                  sin.data_ptr() if sin is not None else None, rows, q_out.data_ptr(),
+                  pages.data_ptr(), P, 1, Hq, Hkv, D, None, _stream())
+    return q_out
+
+
+def _rope(rope, D: int):
+    """Checked (cos, sin, rows) of rotation tables; (None, None, 0) without any."""
+    if rope is None:
+        return None, None, 0
+    cos, sin = rope
+    for t in (cos, sin):
+        _require(t, "rope table", torch.float32)
+        if t.dim() != 2 or t.shape[1] != D // 2 or t.shape != cos.shape or t.shape[0] == 0:
+            raise LoopfuseError(_lib.LF_EINVAL, f"rope tables must be [rows, {D // 2}]")
+    return cos, sin, cos.shape[0]
+
+
+def default_pages_per_split_q4(num_seqs: int, num_kv_heads: int, max_pages: int,
+                               num_prefix_pages: int = 0) -> int:
+    """Split size of ``paged_decode_q4`` (``lf_q4_decode_default_split``)."""
+    out = _lib.c_int(0)
+    _lib.call("lf_q4_decode_default_split", int(num_seqs), int(num_kv_heads), int(max_pages),
+              int(num_prefix_pages), _sm_count(), _lib.ctypes.byref(out))
+    return int(out.value)
+
+
+def decode_q4_workspace_bytes(num_seqs: int, num_q_heads: int, head_dim: int, max_pages: int,
+                              pages_per_split: int, num_prefix_pages: int = 0) -> int:
+    n = _lib.c_size_t(0)
+    _lib.call("lf_q4_decode_workspace_size", num_seqs, num_q_heads, head_dim, max_pages,
+              pages_per_split, num_prefix_pages, _lib.ctypes.byref(n))
+    return int(n.value)
+
+
+def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, num_prefix_pages: int = 0,
+                    scale: Optional[float] = None, pages_per_split: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                    return_lse: bool = False):
+    """``paged_decode`` over K/V held in 4 bits: ``q [N, Hq, D]``, ``pages [P, Hkv, 18 * D]`` uint8
+    (one layer), ``block_table [N, max_pages]`` and ``seq_lens [N]`` int32, Hq / Hkv 1, 2, 4 or 8.
+    With ``num_prefix_pages > 0`` the first that many block-table entries must be the same pages
+    for all sessions.  A session of length 0 gives zeros and an LSE of -inf."""
+    _require(q, "q")
+    D = q4_head_dim(pages)
+    _require(block_table, "block_table", torch.int32)
+    _require(seq_lens, "seq_lens", torch.int32)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise LoopfuseError(_lib.LF_EINVAL, f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
+    N, Hq, _ = q.shape
+    P, Hkv, _ = pages.shape
+    if block_table.dim() != 2 or block_table.shape[0] != N or seq_lens.shape != (N,):
+        raise LoopfuseError(_lib.LF_EINVAL, "block_table must be [N,max_pages], seq_lens [N]")
+    dev = _one_device("paged_decode_q4", q, pages, block_table, seq_lens, out, workspace)
+    o = out if out is not None else torch.empty_like(q)
+    _require(o, "out")
+    if o.shape != q.shape:
+        raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: out must have q's shape")
+    lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    if N == 0:
+        return (o, lse) if return_lse else o
+    max_pages = block_table.shape[1]
+    scale = D ** -0.5 if scale is None else float(scale)
+    with torch.cuda.device(dev):
+        pps = pages_per_split or default_pages_per_split_q4(N, Hkv, max_pages, num_prefix_pages)
+        need = decode_q4_workspace_bytes(N, Hq, D, max_pages, pps, num_prefix_pages)
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _lib.call("lf_q4_decode_fwd", q.data_ptr(), pages.data_ptr(), block_table.data_ptr(),
+                  seq_lens.data_ptr(), int(num_prefix_pages), o.data_ptr(),
+                  lse.data_ptr() if lse is not None else None, workspace.data_ptr(),
+                  workspace.numel() * workspace.element_size(), N, Hq, Hkv, D, P, max_pages, pps,
+                  scale, _stream())
+    return (o, lse) if return_lse else o
+
+
+def expand_pages_q4(pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    total_pages: int, num_prefix_pages: int = 0,
+                    out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A batch's 4-bit pages as bf16 pages for ``prefill_paged``: ``(k_pages, v_pages [total_pages,
+    Hkv, 16, D], block_table [N, max_pages])``.
+
+    The shared prefix's pages come first, then each session's own; ``total_pages`` is their number
+    (``num_prefix_pages + sum(max(0, ceil(len / 16) - num_prefix_pages))``; more is allowed, the
+    rest stays unwritten, fewer is an error that ``lf_device_status`` reports).  Rows at or past a
+    session's length are zeros.  ``out`` gives the two page tensors to write."""
+    D = q4_head_dim(pages)
+    _require(block_table, "block_table", torch.int32)
+    _require(seq_lens, "seq_lens", torch.int32)
+    P, Hkv, _ = pages.shape
+    if block_table.dim() != 2 or seq_lens.shape != (block_table.shape[0],):
+        raise LoopfuseError(_lib.LF_EINVAL, "block_table must be [N,max_pages], seq_lens [N]")
+    N, max_pages = block_table.shape
+    shape = (int(total_pages), Hkv, LF_PAGE_SIZE, D)
+    k, v = out if out is not None else (
+        torch.empty(shape, dtype=torch.bfloat16, device=pages.device) for _ in range(2))
+    for t in (k, v):
+        _require(t, "out")
+        if tuple(t.shape) != shape:
+            raise LoopfuseError(_lib.LF_EINVAL, f"expand_pages_q4: out must be two tensors {shape}")
+    dev = _one_device("expand_pages_q4", pages, block_table, seq_lens, k, v)
+    table = torch.empty_like(block_table)
+    with torch.cuda.device(dev):
+        _lib.call("lf_q4_expand", pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                  int(num_prefix_pages), k.data_ptr(), v.data_ptr(), table.data_ptr(), N, Hkv, D, P,
+                  max_pages, shape[0], _stream())
+    return k, v, table

@@ -1,0 +1,391 @@
+// Appending K/V to 4-bit pages, and expanding 4-bit pages to bf16 pages for the prefill kernel.
+//
+// Both are bandwidth-bound passes: the append reads each new K/V value once and writes 4.5 bits of
+// it, the expansion reads 4.5 bits and writes 16.  The format is described in q4_common.cuh.
+#include "pool_common.cuh"
+#include "q4_common.cuh"
+#include "sm100_primitives.cuh"
+
+#include <math.h>
+
+namespace lf {
+namespace q4 {
+
+struct AppendArgs {
+    const uint16_t *q, *k, *v;
+    int64_t q_token, kv_layer, kv_token, kv_head;      // strides in elements
+    const int32_t *table, *seq_ids, *start, *cu;
+    int table_rows, table_stride, n, total;
+    const float *cos, *sin;
+    int rope_rows;
+    uint16_t* q_out;
+    uint8_t* pages;
+    int num_pages, Hq, Hkv;
+    int32_t* status;                                   // a pool's sticky status, or null
+};
+
+__device__ __forceinline__ void report(const AppendArgs& a) {
+    if (a.status != nullptr) atomicCAS(a.status, LF_OK, LF_EINVAL);
+    else atomicCAS(&g_device_error, 0, 222);
+}
+
+// One CTA walks tokens (grid-stride, blockIdx.y the layer); a row of D dims of one head is D / 8
+// lanes of 8 dims, heads ordered q (Hq), k (Hkv), v (Hkv).  Rotation uses the partner lane's 8 dims
+// and rounds every product and sum separately, then to bf16, as an eager fp32 evaluation does; the
+// codes are those of the rounded values.  A row that has no page, or no rotation table row, is not
+// stored and is reported.
+template <int D>
+__global__ void append_kernel(const AppendArgs a) {
+    using F = Fmt<D>;
+    constexpr int LPR = D / 8, RPW = 32 / LPR;          // lanes a row, rows a warp
+    if (a.status != nullptr && *reinterpret_cast<volatile int32_t*>(a.status) != LF_OK) return;
+    const int H = a.Hq + 2 * a.Hkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int l = lane % LPR;
+    const long layer = blockIdx.y;
+    for (int t = blockIdx.x; t < a.total; t += gridDim.x) {
+        int lo = 0, hi = a.n - 1;                      // session i with cu[i] <= t < cu[i+1]
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.cu[mid] <= t) lo = mid; else hi = mid - 1;
+        }
+        const int pos = a.start[lo] + (t - a.cu[lo]);
+        const int row = a.seq_ids != nullptr ? a.seq_ids[lo] : lo;
+        const bool pos_ok = a.cos == nullptr || (pos >= 0 && pos < a.rope_rows);
+        int page = -1;
+        if (row >= 0 && row < a.table_rows && pos >= 0 && pos / kPage < a.table_stride)
+            page = a.table[(long)row * a.table_stride + pos / kPage];
+        const bool page_ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
+        if (!(page_ok && pos_ok) && threadIdx.x == 0) report(a);
+        for (int r0 = warp * RPW; r0 < H; r0 += warps * RPW) {
+            const int h = r0 + lane / LPR;
+            const bool live = h < H;
+            const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
+            const int kh = h - a.Hq - (is_k ? 0 : a.Hkv);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (live) {
+                const uint16_t* src =
+                    is_q ? a.q + t * a.q_token + (long)h * D
+                         : (is_k ? a.k : a.v) + layer * a.kv_layer + t * a.kv_token + kh * a.kv_head;
+                x = *reinterpret_cast<const uint4*>(src + 8 * l);
+            }
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            if (a.cos != nullptr) {                    // every lane of the warp takes the shuffles
+                const float* cp = a.cos + (long)(pos_ok ? pos : 0) * (D / 2) + (8 * l) % (D / 2);
+                const float* sp = a.sin + (long)(pos_ok ? pos : 0) * (D / 2) + (8 * l) % (D / 2);
+                const bool turn = live && (is_q || is_k);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], LPR / 2);
+                    const float2 c = __ldg(reinterpret_cast<const float2*>(cp) + j);
+                    const float2 s = __ldg(reinterpret_cast<const float2*>(sp) + j);
+                    const float al = __fmul_rn(bf16lo_to_f32(w[j]), c.x);
+                    const float ah = __fmul_rn(bf16hi_to_f32(w[j]), c.y);
+                    const float bl = __fmul_rn(bf16lo_to_f32(other), s.x);
+                    const float bh = __fmul_rn(bf16hi_to_f32(other), s.y);
+                    const uint32_t first = pack_bf16x2(__fsub_rn(al, bl), __fsub_rn(ah, bh));
+                    const uint32_t second = pack_bf16x2(__fadd_rn(al, bl), __fadd_rn(ah, bh));
+                    if (turn) w[j] = l < LPR / 2 ? first : second;
+                }
+            }
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[2 * j] = bf16lo_to_f32(w[j]);
+                f[2 * j + 1] = bf16hi_to_f32(w[j]);
+            }
+            float mn = f[0], mx = f[0];
+            bool nan = f[0] != f[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) {
+                mn = fminf(mn, f[j]);
+                mx = fmaxf(mx, f[j]);
+                nan |= f[j] != f[j];
+            }
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) {    // a group is 8 lanes
+                mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            }
+            const unsigned nans = __ballot_sync(0xffffffffu, nan);
+            if (!live) continue;
+            if (is_q) {
+                if (pos_ok)
+                    *reinterpret_cast<uint4*>(a.q_out + ((long)t * a.Hq + h) * D + 8 * l) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                continue;
+            }
+            if (!page_ok || !pos_ok) continue;
+            const float span = __fsub_rn(mx, mn);
+            uint32_t par = 0x7FC07FC0u;                // NaN, NaN
+            uint32_t n[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (((nans >> (lane & 24)) & 0xFFu) == 0 && span < INFINITY) {
+                par = pack_bf16x2(__fdiv_rn(span, 15.f), mn);
+                const float s = bf16lo_to_f32(par);
+                if (s > 0.f) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        n[j] = (uint32_t)fminf(rintf(__fdiv_rn(__fsub_rn(f[j], mn), s)), 15.f);
+                }
+            }
+            const int tok = pos % kPage, grp = l / 8, in = l % 8;   // group, 8-dim piece of it
+            uint8_t* blk = a.pages + ((layer * a.num_pages + page) * a.Hkv + kh) * (long)F::kBlockBytes;
+            if (is_k) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) word |= n[e] << (4 * (e / 2) + 16 * (e % 2));
+                *reinterpret_cast<uint32_t*>(blk + tok * (32 * F::NG) + (in / 2) * (8 * F::NG) +
+                                             grp * 8 + (in % 2) * 4) = word;
+            } else {
+                uint8_t* vp = blk + F::kVOff + (tok / 8) * (256 * F::NG) +
+                              (in * 4 + (tok % 8) / 2) * (8 * F::NG) + grp * 8 + (tok % 2) * 2;
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    *reinterpret_cast<uint16_t*>(vp + 4 * q) = (uint16_t)(
+                        n[4 * q] | (n[4 * q + 1] << 4) | (n[4 * q + 2] << 8) | (n[4 * q + 3] << 12));
+            }
+            if (in == 0)
+                *reinterpret_cast<uint32_t*>(blk + F::kParOff + ((tok * 2 + (is_k ? 0 : 1)) * F::NG + grp) * 4) = par;
+        }
+    }
+}
+
+// -- expansion --------------------------------------------------------------------------------------
+constexpr int kExpWarps = 8;
+constexpr int kExpPages = 8;                           // table columns a CTA expands
+
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, float s0, float b0, float s1, float b1) {
+    // n * s is exact in fp32 (4 by 8 bits), so the value is rounded once here and once to bf16
+    return pack_bf16x2(fmaf((float)(codes & 15u), s0, b0), fmaf((float)((codes >> 16) & 15u), s1, b1));
+}
+
+// CTA (session n, kExpPages columns of its table row): warps take (page, head) pairs.  Output pages
+// are compact: the shared prefix first, then every session's own pages in session order; each CTA
+// finds its session's first one by summing the lengths before it.  Rows at or past the length
+// become zeros, so that the prefill kernel's masked products see no stale bits.
+template <int D>
+__global__ void __launch_bounds__(32 * kExpWarps)
+expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
+              const int32_t* __restrict__ lens, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo,
+              int32_t* __restrict__ out_table, int N, int Hkv, int num_pages, int max_pages,
+              int n_prefix, int out_pages) {
+    using F = Fmt<D>;
+    const int chunks = (max_pages + kExpPages - 1) / kExpPages;
+    const int n = blockIdx.x / chunks, j0 = (blockIdx.x % chunks) * kExpPages;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto held = [&](int i) { return min(max(lens[i], 0), max_pages * kPage); };
+    int own = 0, best = -1, best_n = 0;                // pages before this session's; longest session
+    for (int i = threadIdx.x; i < N; i += 32 * kExpWarps) {
+        const int L = held(i);
+        if (i < n) own += max(0, (L + kPage - 1) / kPage - n_prefix);
+        if (L > best) { best = L; best_n = i; }
+    }
+    __shared__ int s_own[kExpWarps], s_best[kExpWarps], s_arg[kExpWarps];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        own += __shfl_xor_sync(0xffffffffu, own, off);
+        const int ob = __shfl_xor_sync(0xffffffffu, best, off), oa = __shfl_xor_sync(0xffffffffu, best_n, off);
+        if (ob > best || (ob == best && oa < best_n)) { best = ob; best_n = oa; }
+    }
+    if (lane == 0) { s_own[warp] = own; s_best[warp] = best; s_arg[warp] = best_n; }
+    __syncthreads();
+    own = 0;
+    best = -1;
+    best_n = 0;
+#pragma unroll
+    for (int w = 0; w < kExpWarps; ++w) {
+        own += s_own[w];
+        if (s_best[w] > best || (s_best[w] == best && s_arg[w] < best_n)) { best = s_best[w]; best_n = s_arg[w]; }
+    }
+    const int L = held(n), np = (L + kPage - 1) / kPage;
+    const int j_end = min(j0 + kExpPages, max_pages);
+    auto out_page = [&](int j) { return j < n_prefix ? j : n_prefix + own + (j - n_prefix); };
+    if (threadIdx.x < j_end - j0) {
+        const int j = j0 + threadIdx.x;
+        const int o = out_page(j);
+        const bool fits = o < out_pages;
+        out_table[(long)n * max_pages + j] = (j < np || j < n_prefix) && fits ? o : -1;
+        if (j < np && !fits) atomicCAS(&g_device_error, 0, 223);
+    }
+    // shared pages are written once, from the longest session's row
+    const int lead = best_n;
+    for (int u = warp; u < (j_end - j0) * Hkv; u += kExpWarps) {
+        const int j = j0 + u / Hkv, h = u % Hkv;
+        const int o = out_page(j);
+        if (j >= np && !(j < n_prefix)) break;
+        if (o >= out_pages || (j < n_prefix && n != lead)) continue;
+        const int rows = min(kPage, L - j * kPage);     // <= 0: a prefix page past every session
+        int page = rows > 0 ? bt[(long)n * max_pages + j] : 0;
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(num_pages)) {
+            if (lane == 0) atomicCAS(&g_device_error, 0, 224);
+            page = 0;
+        }
+        const uint8_t* blk = pages + ((long)page * Hkv + h) * F::kBlockBytes;
+        const long dst = ((long)o * Hkv + h) * (kPage * D);
+        const int g = lane >> 2, c = lane & 3;
+        constexpr int NW = 2 * F::NG;                  // code words of a lane's vector
+        uint32_t kw[2][NW], vw[2][NW];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint8_t* kp = blk + (half * 8 + g) * (32 * F::NG) + c * (8 * F::NG);
+            const uint8_t* vp = blk + F::kVOff + half * (256 * F::NG) + lane * (8 * F::NG);
+            if constexpr (F::NG == 2) {
+                const uint4 a = ldg_stream(kp), b = ldg_stream(vp);
+                kw[half][0] = a.x; kw[half][1] = a.y; kw[half][2] = a.z; kw[half][3] = a.w;
+                vw[half][0] = b.x; vw[half][1] = b.y; vw[half][2] = b.z; vw[half][3] = b.w;
+            } else {
+                const uint2 a = __ldg(reinterpret_cast<const uint2*>(kp));
+                const uint2 b = __ldg(reinterpret_cast<const uint2*>(vp));
+                kw[half][0] = a.x; kw[half][1] = a.y;
+                vw[half][0] = b.x; vw[half][1] = b.y;
+            }
+        }
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(blk + F::kParOff);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int t = half * 8 + g;                // K: the lane's 16 dims of a group, 32 bytes
+#pragma unroll
+            for (int grp = 0; grp < F::NG; ++grp) {
+                uint32_t out[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (t < rows) {
+                    const uint32_t p = __ldg(par + t * 2 * F::NG + grp);
+                    const float s = bf16lo_to_f32(p), b = bf16hi_to_f32(p);
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            out[4 * w + i] = bf16_pair(kw[half][2 * grp + w] >> (4 * i), s, b, s, b);
+                }
+                sm100::st_global_v8(ko + dst + t * D + grp * kGroup + c * 16, out);
+            }
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {        // V: 8 dims of a group, 16 bytes
+                const int tv = half * 8 + 2 * c + odd;
+#pragma unroll
+                for (int grp = 0; grp < F::NG; ++grp) {
+                    uint32_t out[4] = {0, 0, 0, 0};
+                    if (tv < rows) {
+                        const uint32_t p = __ldg(par + (tv * 2 + 1) * F::NG + grp);
+                        const float s = bf16lo_to_f32(p), b = bf16hi_to_f32(p);
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const uint32_t x = vw[half][2 * grp + w] >> (16 * odd);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                out[2 * w + i] = pack_bf16x2(fmaf((float)((x >> (8 * i)) & 15u), s, b),
+                                                             fmaf((float)((x >> (8 * i + 4)) & 15u), s, b));
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(vo + dst + tv * D + grp * kGroup + g * 8) =
+                        make_uint4(out[0], out[1], out[2], out[3]);
+                }
+            }
+        }
+    }
+}
+
+// The rows a fork needs of a session's partial last page: whole blocks are copied (rows past the
+// prefix are overwritten by the destination's own tokens before anything reads them).
+__global__ void fork_copy_kernel(const int32_t* __restrict__ status, const int32_t* __restrict__ bt,
+                                 int table_stride, int table_rows, int src, const int32_t* __restrict__ dsts,
+                                 int full, uint8_t* __restrict__ pages, int num_pages, long page_bytes) {
+    if (*reinterpret_cast<const volatile int32_t*>(status) != LF_OK) return;
+    const int d = dsts[blockIdx.x];
+    if (d < 0 || d >= table_rows) return;
+    const int sp = bt[(long)src * table_stride + full], dp = bt[(long)d * table_stride + full];
+    if (static_cast<unsigned>(sp) >= static_cast<unsigned>(num_pages) ||
+        static_cast<unsigned>(dp) >= static_cast<unsigned>(num_pages))
+        return;
+    const uint4* from = reinterpret_cast<const uint4*>(pages + ((long)blockIdx.y * num_pages + sp) * page_bytes);
+    uint4* to = reinterpret_cast<uint4*>(pages + ((long)blockIdx.y * num_pages + dp) * page_bytes);
+    for (long i = threadIdx.x; i < page_bytes / 16; i += blockDim.x) to[i] = from[i];
+}
+
+}  // namespace q4
+}  // namespace lf
+
+using namespace lf;
+
+extern "C" int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v,
+                            int64_t q_stride_token, int64_t stride_layer, int64_t stride_token,
+                            int64_t stride_head, const int32_t* block_table, int table_rows,
+                            int max_pages, const int32_t* seq_ids, const int32_t* start_pos,
+                            const int32_t* cu_tokens, int n, int total_tokens, const float* rope_cos,
+                            const float* rope_sin, int rope_rows, lf_bf16* q_out, void* pages,
+                            int num_pages, int num_layers, int num_q_heads, int num_kv_heads,
+                            int head_dim, int32_t* status, void* stream) {
+    LF_CHECK_ARG(n >= 0 && total_tokens >= 0, "q4 append: negative sizes");
+    if (n == 0 || total_tokens == 0) { clear_error(); return LF_OK; }
+    LF_CHECK_ARG(k && v && block_table && start_pos && cu_tokens && pages, "q4 append: null pointer argument");
+    LF_CHECK_ARG(head_dim == 64 || head_dim == 128, "q4 append: head_dim must be 64 or 128 (got %d)", head_dim);
+    LF_CHECK_ARG(num_q_heads >= 0 && num_kv_heads > 0 && num_pages > 0 && max_pages > 0 && table_rows > 0 &&
+                     num_layers > 0 && num_layers <= 65535,
+                 "q4 append: bad shape");
+    LF_CHECK_ARG(num_q_heads == 0 || (q && q_out && num_layers == 1), "q4 append: q needs q_out and one layer");
+    LF_CHECK_ARG(seq_ids != nullptr || n <= table_rows, "q4 append: more sessions than block-table rows");
+    LF_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(pages) &&
+                     q_stride_token % 8 == 0 && stride_layer % 8 == 0 && stride_token % 8 == 0 &&
+                     stride_head % 8 == 0,
+                 "q4 append: rows and pages must be 16-byte aligned");
+    LF_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr), "q4 append: give cos and sin");
+    LF_CHECK_ARG(rope_cos == nullptr || (rope_rows > 0 && aligned16(rope_cos) && aligned16(rope_sin)),
+                 "q4 append: rope tables must be 16-byte aligned with rows > 0");
+    const q4::AppendArgs a{q, k, v, q_stride_token, stride_layer, stride_token, stride_head, block_table,
+                           seq_ids, start_pos, cu_tokens, table_rows, max_pages, n, total_tokens, rope_cos,
+                           rope_sin, rope_rows, q_out, static_cast<uint8_t*>(pages), num_pages, num_q_heads,
+                           num_kv_heads, status};
+    const int rows = num_q_heads + 2 * num_kv_heads, rpw = 256 / head_dim;
+    const int warps = (rows + rpw - 1) / rpw;
+    const int threads = 32 * (warps < 16 ? warps : 16);
+    const int blocks = total_tokens < 148 * 32 ? total_tokens : 148 * 32;
+    const dim3 grid(blocks, num_layers);
+    if (head_dim == 128)
+        q4::append_kernel<128><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+    else
+        q4::append_kernel<64><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+    return launch_status("q4 append");
+}
+
+extern "C" int lf_q4_expand(const void* pages, const int32_t* block_table, const int32_t* seq_lens,
+                            int num_prefix_pages, lf_bf16* k_out, lf_bf16* v_out, int32_t* out_table,
+                            int num_seqs, int num_kv_heads, int head_dim, int num_pages, int max_pages,
+                            int out_pages, void* stream) {
+    LF_CHECK_ARG(num_seqs >= 0, "q4 expand: negative sizes");
+    if (num_seqs == 0) { clear_error(); return LF_OK; }
+    LF_CHECK_ARG(pages && block_table && seq_lens && out_table && out_pages >= 0 &&
+                     (out_pages == 0 || (k_out && v_out)),
+                 "q4 expand: null pointer argument");
+    LF_CHECK_ARG(head_dim == 64 || head_dim == 128, "q4 expand: head_dim must be 64 or 128 (got %d)", head_dim);
+    LF_CHECK_ARG(num_kv_heads > 0 && num_pages > 0 && max_pages > 0 && num_prefix_pages >= 0 &&
+                     num_prefix_pages <= max_pages,
+                 "q4 expand: bad shape");
+    LF_CHECK_ARG(aligned16(pages) && (reinterpret_cast<uintptr_t>(k_out) & 31u) == 0 && aligned16(v_out),
+                 "q4 expand: pages and v_out must be 16-byte aligned, k_out 32-byte aligned");
+    const long blocks = (long)num_seqs * ((max_pages + q4::kExpPages - 1) / q4::kExpPages);
+    LF_CHECK_ARG(blocks <= 2147483647L, "q4 expand: grid limits exceeded");
+    auto launch = [&](auto kernel) {
+        kernel<<<(unsigned)blocks, 32 * q4::kExpWarps, 0, (cudaStream_t)stream>>>(
+            static_cast<const uint8_t*>(pages), block_table, seq_lens, k_out, v_out, out_table, num_seqs,
+            num_kv_heads, num_pages, max_pages, num_prefix_pages, out_pages);
+    };
+    if (head_dim == 128) launch(q4::expand_kernel<128>); else launch(q4::expand_kernel<64>);
+    return launch_status("q4 expand");
+}
+
+extern "C" int lf_q4_fork(const lf_pool_meta* m, int src_seq, const int32_t* dst_seqs, int n,
+                          int prefix_len, void* pages, int num_layers, int num_kv_heads, int head_dim,
+                          void* stream) {
+    LF_CHECK_ARG(pages != nullptr && aligned16(pages) && num_layers > 0 && num_layers <= 65535 &&
+                     num_kv_heads > 0 && (head_dim == 64 || head_dim == 128),
+                 "q4 fork: bad data arguments");
+    const int rc = lf_pool_fork(m, src_seq, dst_seqs, n, prefix_len, nullptr, nullptr, 0, 0, 8, stream);
+    if (rc != LF_OK || n == 0 || prefix_len % LF_PAGE_SIZE == 0) return rc;
+    LF_CHECK_ARG(src_seq >= 0 && src_seq < m->max_seqs && prefix_len > 0 &&
+                     prefix_len <= m->max_pages_per_seq * LF_PAGE_SIZE,
+                 "q4 fork: bad source or prefix");
+    q4::fork_copy_kernel<<<dim3(n, num_layers), 256, 0, (cudaStream_t)stream>>>(
+        m->ctrl + LF_CTRL_STATUS, m->block_table, m->max_pages_per_seq, m->max_seqs, src_seq, dst_seqs,
+        prefix_len / LF_PAGE_SIZE, static_cast<uint8_t*>(pages), m->num_pages,
+        (long)num_kv_heads * 18 * head_dim);
+    return launch_status("q4 fork copy");
+}

@@ -24,9 +24,9 @@ from typing import Dict, List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 
-from . import attention as att
-from ._lib import LF_PAGE_SIZE
+from ._lib import LF_EINVAL, LF_PAGE_SIZE, LoopfuseError
 from .runtime.kv_pool import KVPool, KVState
+from .runtime.kv_pool_q4 import QuantKVPool
 
 
 @dataclass
@@ -73,12 +73,17 @@ class GPT2Model:
                       f"{l}.fc2.w": n(f, d), f"{l}.fc2.b": torch.zeros(d)})
         return w
 
-    def new_pool(self, num_pages: int, max_slots: int, max_seq_len: Optional[int] = None) -> KVPool:
+    def new_pool(self, num_pages: int, max_slots: int, max_seq_len: Optional[int] = None,
+                 kv_bits: int = 16) -> KVPool:
+        """A pool for this model's K/V, in bf16 (``kv_bits`` 16) or in 4 bits (4)."""
         c = self.cfg
-        return KVPool(num_layers=c.layers, num_heads=c.heads, num_kv_heads=c.heads,
-                      head_dim=c.head_dim, max_seq_len=max_seq_len or c.positions,
-                      max_slots=max_slots, dtype=torch.bfloat16, device=self.device,
-                      num_pages=num_pages)
+        if kv_bits not in (4, 16):
+            raise LoopfuseError(LF_EINVAL, f"kv_bits must be 4 or 16, got {kv_bits}")
+        pool_type = QuantKVPool if kv_bits == 4 else KVPool
+        return pool_type(num_layers=c.layers, num_heads=c.heads, num_kv_heads=c.heads,
+                         head_dim=c.head_dim, max_seq_len=max_seq_len or c.positions,
+                         max_slots=max_slots, dtype=torch.bfloat16, device=self.device,
+                         num_pages=num_pages)
 
     def _ln(self, x: torch.Tensor, p: str) -> torch.Tensor:
         return F.layer_norm(x, (self.cfg.d_model,), self.w[p + ".w"], self.w[p + ".b"], self.cfg.eps)
@@ -103,14 +108,13 @@ class GPT2Model:
                          for s0, n in zip(starts_host, counts)])
         decode = all(n == 1 for n in counts)
         if decode:
-            pps = att.default_pages_per_split(len(states), c.heads, table.shape[1], n_prefix_pages)
-            need = att.decode_workspace_bytes(len(states), c.heads, c.head_dim, table.shape[1],
-                                              pps, n_prefix_pages)
+            pps, need = pool.decode_workspace(len(states), c.heads, table.shape[1], n_prefix_pages)
             if self._ws is None or self._ws.numel() < need:
                 self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         else:
             cu = torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32,
                               device=self.device)
+            buffers = pool.prefill_buffers([s.current_len for s in states], n_prefix_pages)
         last = torch.tensor(counts, device=self.device).cumsum(0) - 1
         x = w["wte"][tokens.to(self.device)] + w["wpe"][pos]
         for l in range(c.layers):
@@ -118,12 +122,11 @@ class GPT2Model:
             qkv = (h @ w[f"{l}.attn.w"] + w[f"{l}.attn.b"]).to(torch.bfloat16)
             q = torch.empty((T, c.heads, c.head_dim), dtype=torch.bfloat16, device=self.device)
             pool.write_qkv(states, start, l, qkv, q, counts, index=index)   # no rotary in GPT-2
-            kp, vp = pool.layer_pages(l)
             if decode:
-                a = att.paged_decode(q, kp, vp, table, lens, num_prefix_pages=n_prefix_pages,
-                                     pages_per_split=pps, workspace=self._ws)
+                a = pool.attend_decode(q, l, table, lens, num_prefix_pages=n_prefix_pages,
+                                       pages_per_split=pps, workspace=self._ws)
             else:
-                a = att.prefill_paged(q, kp, vp, table, cu, lens, max(counts))
+                a = pool.attend_prefill(q, l, table, cu, lens, max(counts), buffers)
             a = a.reshape(T, c.d_model).to(self.dtype)
             if attn_last is not None:
                 attn_last.append(a[last])

@@ -24,7 +24,6 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from . import attention as att
 from . import model_ops as mo
 from .runtime.kv_pool import KVPool, KVState
 
@@ -203,10 +202,9 @@ class LlamaShaped:
         if not decode:
             cu = torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32,
                               device=self.device)
+            buffers = pool.prefill_buffers([s.current_len for s in states], n_prefix_pages)
         else:
-            pps = att.default_pages_per_split(len(states), c.kv_heads, table.shape[1], n_prefix_pages)
-            need = att.decode_workspace_bytes(len(states), c.q_heads, c.head_dim, table.shape[1],
-                                              pps, n_prefix_pages)
+            pps, need = pool.decode_workspace(len(states), c.q_heads, table.shape[1], n_prefix_pages)
             if self._ws is None or self._ws.numel() < need:
                 self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         if timer is not None:
@@ -227,13 +225,11 @@ class LlamaShaped:
                 k = self._rope(qkv[:, nq:nq + nk].view(T, c.kv_heads, c.head_dim), cos, sin)
                 v = qkv[:, nq + nk:].reshape(T, c.kv_heads, c.head_dim).contiguous()
                 pool.write_layer(states, start, l, k.contiguous(), v, counts, index=index)
-            kp, vp = pool.layer_pages(l)
             if decode:
-                a = att.paged_decode(q, kp, vp, table, lens,
-                                     num_prefix_pages=n_prefix_pages, pages_per_split=pps,
-                                     workspace=self._ws)
+                a = pool.attend_decode(q, l, table, lens, num_prefix_pages=n_prefix_pages,
+                                       pages_per_split=pps, workspace=self._ws)
             else:
-                a = att.prefill_paged(q, kp, vp, table, cu, lens, max(counts))
+                a = pool.attend_prefill(q, l, table, cu, lens, max(counts), buffers)
             _lap(timer, "attention")
             x, h = self._mlp_block(x, a.view(T, nq), l, timer)
         last = torch.tensor(counts, device=self.device).cumsum(0) - 1
@@ -293,10 +289,8 @@ class GraphedDecode:
              "table": torch.empty((nb, pool.max_pages_per_seq), dtype=torch.int32, device=dev),
              "lens": torch.empty(nb, dtype=torch.int32, device=dev),
              "copied": torch.cuda.Event()}
-        s["pps"] = att.default_pages_per_split(nb, c.kv_heads, pool.max_pages_per_seq, self.npp)
-        s["ws"] = torch.empty(att.decode_workspace_bytes(nb, c.q_heads, c.head_dim,
-                                                         pool.max_pages_per_seq, s["pps"], self.npp),
-                              dtype=torch.uint8, device=dev)
+        s["pps"], need = pool.decode_workspace(nb, c.q_heads, pool.max_pages_per_seq, self.npp)
+        s["ws"] = torch.empty(need, dtype=torch.uint8, device=dev)
         # rows: real sessions take 1 token; a fresh graph's warm-up runs every row as padding
         s["host"][1].fill_(self.pad.slot_id)
         s["dev"].copy_(s["host"])
@@ -329,9 +323,8 @@ class GraphedDecode:
             qkv = h @ m.wqkv[l]
             q = torch.empty((nb, c.q_heads, c.head_dim), dtype=qkv.dtype, device=m.device)
             pool.write_qkv(None, s["start"], l, qkv, q, None, rope=rope, index=index)
-            kp, vp = pool.layer_pages(l)
-            a = att.paged_decode(q, kp, vp, s["table"], s["lens"], num_prefix_pages=self.npp,
-                                 pages_per_split=s["pps"], workspace=s["ws"])
+            a = pool.attend_decode(q, l, s["table"], s["lens"], num_prefix_pages=self.npp,
+                                   pages_per_split=s["pps"], workspace=s["ws"])
             x, h = m._mlp_block(x, a.view(nb, nq), l)
         return torch.argmax(m._norm_in(x, None, m.final_norm) @ m.lm_head, dim=-1)
 

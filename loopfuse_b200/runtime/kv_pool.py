@@ -33,6 +33,7 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _lib
+from .. import attention as att
 from .._lib import LF_PAGE_SIZE, LoopfuseError, PoolMeta
 
 _DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
@@ -96,9 +97,7 @@ class KVPool:
         self.max_pages_per_seq = math.ceil(max_seq_len / LF_PAGE_SIZE)
         self.num_pages = num_pages or max_slots * self.max_pages_per_seq
 
-        shape = (num_layers, self.num_pages, self.num_kv_heads, LF_PAGE_SIZE, head_dim)
-        self.keys = torch.zeros(shape, dtype=dtype, device=dev)
-        self.values = torch.zeros(shape, dtype=dtype, device=dev)
+        self._alloc_storage()
 
         i32 = dict(dtype=torch.int32, device=dev)
         self._free_queue = torch.empty(self.num_pages, **i32)
@@ -134,6 +133,72 @@ class KVPool:
                    dtype=_DTYPES.get(kv_config.get("dtype", "fp16"), torch.float16),
                    device=device, max_slots=max_slots,
                    num_kv_heads=kv_config.get("num_kv_heads"), num_pages=num_pages)
+
+    # -- storage: what a pool with another page format replaces ------------------------------
+    def _alloc_storage(self) -> None:
+        shape = (self.num_layers, self.num_pages, self.num_kv_heads, LF_PAGE_SIZE, self.head_dim)
+        self.keys = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        self.values = torch.zeros(shape, dtype=self.dtype, device=self.device)
+
+    def _storage_bytes(self) -> int:
+        return (self.keys.numel() + self.values.numel()) * self.keys.element_size()
+
+    def _write_kv(self, ids, start, cu, n, total, keys, values, s_layer, s_token, s_head, layer,
+                  layers, stream) -> None:
+        """Store ``total`` tokens' K/V of ``layers`` layers from ``layer`` on (strides in elements)."""
+        off = layer * self.keys.stride(0) * self.keys.element_size()
+        self._call("lf_pool_write_kv", self._meta_ref(), ids.data_ptr(), start.data_ptr(),
+                   cu.data_ptr(), n, total, keys.data_ptr(), values.data_ptr(), s_layer, s_token,
+                   s_head, self.keys.data_ptr() + off, self.values.data_ptr() + off, layers,
+                   self.num_kv_heads, self.head_dim, self._stream(stream))
+        self._bytes_written += 2 * layers * total * self.num_kv_heads * self.head_dim * \
+            self.keys.element_size()
+
+    def _write_qkv(self, ids, start, cu, total, layer, qkv, q_out, rope, stream) -> None:
+        cos, sin = rope if rope is not None else (None, None)
+        Hq, Hkv, D, elem = q_out.shape[1], self.num_kv_heads, self.head_dim, self.keys.element_size()
+        off = layer * self.keys.stride(0) * elem
+        self._call("lf_pool_write_qkv", self._meta_ref(), ids.data_ptr(), start.data_ptr(),
+                   cu.data_ptr(), ids.numel(), total, qkv.data_ptr(), qkv.stride(0),
+                   cos.data_ptr() if cos is not None else None,
+                   sin.data_ptr() if sin is not None else None,
+                   cos.shape[0] if cos is not None else 0, q_out.data_ptr(),
+                   self.keys.data_ptr() + off, self.values.data_ptr() + off, Hq, Hkv, D,
+                   self._stream(stream))
+        self._bytes_written += 2 * total * Hkv * D * elem
+
+    def _fork_data(self, src: int, ids: torch.Tensor, n: int, prefix_len: int) -> None:
+        self._call("lf_pool_fork", self._meta_ref(), src, ids.data_ptr(), n, prefix_len,
+                   self.keys.data_ptr(), self.values.data_ptr(), self.num_layers,
+                   self.num_kv_heads, self.head_dim, self._stream())
+
+    # -- attention over the pool's pages, whatever their format --------------------------------
+    def decode_workspace(self, n: int, num_q_heads: int, width: int,
+                         num_prefix_pages: int = 0) -> Tuple[int, int]:
+        """(pages per split, workspace bytes) of ``attend_decode`` for ``n`` sessions."""
+        pps = att.default_pages_per_split(n, self.num_kv_heads, width, num_prefix_pages)
+        return pps, att.decode_workspace_bytes(n, num_q_heads, self.head_dim, width, pps,
+                                               num_prefix_pages)
+
+    def attend_decode(self, q: torch.Tensor, layer: int, table: torch.Tensor, lens: torch.Tensor,
+                      num_prefix_pages: int = 0, pages_per_split: Optional[int] = None,
+                      workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One-token attention ``[N, Hq, D]`` of a batch over one layer's pages."""
+        kp, vp = self.layer_pages(layer)
+        return att.paged_decode(q, kp, vp, table, lens, num_prefix_pages=num_prefix_pages,
+                                pages_per_split=pages_per_split, workspace=workspace)
+
+    def prefill_buffers(self, lengths: Sequence[int], num_prefix_pages: int = 0):
+        """What ``attend_prefill`` needs besides the pages, made once per forward: ``lengths`` are
+        the sessions' lengths with their new tokens, the first ``num_prefix_pages`` pages the same
+        for all of them.  Nothing for bf16 pages."""
+        return None
+
+    def attend_prefill(self, q: torch.Tensor, layer: int, table: torch.Tensor, cu: torch.Tensor,
+                       lens: torch.Tensor, max_new: int, buffers=None) -> torch.Tensor:
+        """Causal attention ``[T, Hq, D]`` of a batch's new tokens over one layer's pages."""
+        kp, vp = self.layer_pages(layer)
+        return att.prefill_paged(q, kp, vp, table, cu, lens, max_new)
 
     # -- plumbing -------------------------------------------------------------
     def _meta_ref(self):
@@ -220,7 +285,7 @@ class KVPool:
     def hbm_usage_bytes(self) -> int:
         meta = sum(t.numel() * 4 for t in (self._free_queue, self._refcount, self._table,
                                             self._seq_len, self._ctrl, self._scratch))
-        return (self.keys.numel() + self.values.numel()) * self.keys.element_size() + meta
+        return self._storage_bytes() + meta
 
     def stats(self) -> dict:
         ctrl = self._ctrl.tolist()
@@ -299,14 +364,8 @@ class KVPool:
                     tuple(t.shape) != (total, self.num_kv_heads, self.head_dim):
                 raise LoopfuseError(_lib.LF_EINVAL, "write_layer expects contiguous "
                                                     "[T_total, Hkv, D] tensors of the pool dtype")
-        elem = self.keys.element_size()
-        layer_off = layer * self.keys.stride(0) * elem
-        self._call("lf_pool_write_kv", self._meta_ref(), ids.data_ptr(), start.data_ptr(),
-                   cu_t.data_ptr(), len(states), total, keys.data_ptr(), values.data_ptr(), 0,
-                   keys.stride(0), keys.stride(1), self.keys.data_ptr() + layer_off,
-                   self.values.data_ptr() + layer_off, 1, self.num_kv_heads, self.head_dim,
-                   self._stream(stream))
-        self._bytes_written += 2 * keys.numel() * elem
+        self._write_kv(ids, start, cu_t, len(states), total, keys, values, 0, keys.stride(0),
+                       keys.stride(1), layer, 1, stream)
 
     def append(self, states: Sequence[KVState], keys: Sequence[torch.Tensor],
                values: Sequence[torch.Tensor], layout: str = "lthd",
@@ -344,12 +403,9 @@ class KVPool:
             cu.append(cu[-1] + c)
         ids = self._ids([s.slot_id for s in states])
         cu_t = self._ids(cu)
-        self._call("lf_pool_write_kv", self._meta_ref(), ids.data_ptr(), start.data_ptr(),
-                   cu_t.data_ptr(), len(states), total, k_all.data_ptr(), v_all.data_ptr(), sl,
-                   st_tok, st_head, self.keys.data_ptr(), self.values.data_ptr(), self.num_layers,
-                   self.num_kv_heads, self.head_dim, self._stream(stream))
+        self._write_kv(ids, start, cu_t, len(states), total, k_all, v_all, sl, st_tok, st_head, 0,
+                       self.num_layers, stream)
         self._write_count += 1
-        self._bytes_written += 2 * k_all.numel() * k_all.element_size()
 
     def fork(self, state: KVState, prefix_len: Optional[int] = None, n: int = 1) -> List[KVState]:
         """``n`` new sessions sharing ``state``'s first ``prefix_len`` tokens (KV fusion)."""
@@ -362,9 +418,7 @@ class KVPool:
                                f"Increase max_slots or wait for a trajectory to complete.")
         dsts = [self.allocate_slot() for _ in range(n)]
         ids = self._ids([d.slot_id for d in dsts])
-        self._call("lf_pool_fork", self._meta_ref(), state.slot_id, ids.data_ptr(), n, prefix_len,
-                   self.keys.data_ptr(), self.values.data_ptr(), self.num_layers,
-                   self.num_kv_heads, self.head_dim, self._stream())
+        self._fork_data(state.slot_id, ids, n, prefix_len)
         if self._oversubscribed and prefix_len % LF_PAGE_SIZE:
             try:
                 self._raise_if_failed("fork")
@@ -455,25 +509,13 @@ class KVPool:
         if q_out.dtype != self.dtype or not q_out.is_contiguous() or \
                 tuple(q_out.shape) != (total, Hq, D):
             raise LoopfuseError(_lib.LF_EINVAL, "write_qkv: q_out must be contiguous [T, Hq, D]")
-        cos = sin = None
-        rows = 0
         if rope is not None:
-            cos, sin = rope
-            for t in (cos, sin):
+            for t in rope:
                 if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
                         t.shape[1] != D // 2 or t.device != self.device:
                     raise LoopfuseError(_lib.LF_EINVAL, "write_qkv: rope tables must be "
                                                         "contiguous fp32 [rows, D/2] on the pool device")
-            rows = cos.shape[0]
-        elem = self.keys.element_size()
-        layer_off = layer * self.keys.stride(0) * elem
-        self._call("lf_pool_write_qkv", self._meta_ref(), ids.data_ptr(), start.data_ptr(),
-                   cu_t.data_ptr(), ids.numel(), total, qkv.data_ptr(), qkv.stride(0),
-                   cos.data_ptr() if cos is not None else None,
-                   sin.data_ptr() if sin is not None else None, rows, q_out.data_ptr(),
-                   self.keys.data_ptr() + layer_off, self.values.data_ptr() + layer_off, Hq, Hkv, D,
-                   self._stream(stream))
-        self._bytes_written += 2 * total * Hkv * D * elem
+        self._write_qkv(ids, start, cu_t, total, layer, qkv, q_out, rope, stream)
 
     # -- prefix-hash dedup (content-addressed KV fusion) ----------------------------------
     def _registry(self) -> "_lib.PrefixRegistry":
