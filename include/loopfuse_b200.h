@@ -434,6 +434,52 @@ int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32_t* block_t
                      int num_kv_heads, int head_dim, int num_pages, int max_pages,
                      int pages_per_split, float scale, void* stream);
 
+/* ---- log probabilities of given tokens -------------------------------------------------------
+ * For each of `rows` rows of `vocab` logits (dtype LF_BF16, LF_FP16 or LF_FP32; row_stride
+ * elements apart, any alignment of the element type), p = softmax(row) in fp32:
+ *   logprob[r] = ln p[tokens[r]]  (0 for a negative token: none given; NaN, and the device error
+ *                word 231, for one >= vocab),
+ *   entropy[r] = -sum p ln p,
+ *   top_ids[r][0..top_k), top_logprobs[r][..]: the top_k (0..32, at most vocab) largest logits in
+ *                falling order, ties to the lowest index, and their ln p.
+ * Logits of -inf have no probability.  A row of nothing else has logprob -inf and entropy 0; a row
+ * with a NaN or +inf has NaN in every probability and the entropy (NaN sorts above all).  tokens are
+ * int64 (tokens_64bit != 0) or int32.  No workspace.  The reference returns logits only
+ * (runtime/executor.py:220-231). */
+#define LF_BF16 0
+#define LF_FP16 1
+#define LF_FP32 2
+int lf_token_logprobs(const void* logits, int dtype, int64_t row_stride, const void* tokens,
+                      int tokens_64bit, int rows, int vocab, int top_k, float* logprob,
+                      float* entropy, int64_t* top_ids, float* top_logprobs, void* stream);
+
+/* ---- low-rank adapters beside a shared projection ----------------------------------------------
+ * out[t] = y[t] + scale[a] * (x[t] . A[a]) . B[a] for the tokens of n sessions back to back
+ * (session i owns rows cu_tokens[i] .. cu_tokens[i+1]-1 and uses adapter a = adapter_ids[i], -1:
+ * none, its rows are y's).  No reference counterpart (one set of weights per program).
+ *
+ * lf_lora_plan sorts a batch's rows by adapter on the device, once for every projection of the
+ * batch: a stable order, so results do not depend on anything but the inputs.  An adapter id
+ * outside [-1, num_adapters) counts as none (device error word 241); offsets that are not 0 ..
+ * total_tokens in rising order give an empty plan (word 242) that writes nothing.
+ *
+ * lf_lora_add: x [total_tokens][inputs], y and out [total_tokens][outputs] (strides in elements,
+ * multiples of 8; out may be y), a [num_adapters][inputs][rank], b [num_adapters][rank][outputs],
+ * scale [num_adapters] (nullable: 1), all bf16 but the fp32 scale; inputs and outputs multiples of
+ * 8; rank 16, 32, 64 or 128 (zero columns of A and rows of B pad a smaller one).  x . A is summed
+ * in fp32 and scale * (x . A) is rounded once to bf16; y is added in fp32 and the sum rounded once.
+ * n, total_tokens and num_adapters are the plan's.  num_adapters <= 4096. */
+int lf_lora_plan_size(int n, int total_tokens, int num_adapters, size_t* bytes);
+int lf_lora_plan(const int32_t* adapter_ids, const int32_t* cu_tokens, int n, int total_tokens,
+                 int num_adapters, void* plan, size_t plan_bytes, void* stream);
+int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int rank,
+                           int sm_count, size_t* bytes);
+int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x, int64_t x_stride,
+                const lf_bf16* a, const lf_bf16* b, const float* scale, const void* plan, int n,
+                int total_tokens, int num_adapters, int inputs, int outputs, int rank, lf_bf16* out,
+                int64_t out_stride, void* workspace, size_t workspace_bytes, int sm_count,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

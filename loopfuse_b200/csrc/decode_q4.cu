@@ -99,7 +99,9 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 
 // Codes 4 i .. 4 i + 3 of both halves of a word as the bf16 pair 128 + n.
 __device__ __forceinline__ uint32_t codes(uint32_t w, int i) {
-    return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+    uint32_t r;                                // (w & mask) | bits: one instruction
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> (4 * i)), "n"(0x000F000F), "r"(0x43004300u));
+    return r;
 }
 
 // A warp's attention state: 8 columns (query rows), of which this lane holds 2c and 2c + 1.

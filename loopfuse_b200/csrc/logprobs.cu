@@ -1,0 +1,416 @@
+// Log probabilities of given tokens, the entropy of each distribution and its top alternatives, from
+// a batch of logits rows, in one pass over them.
+//
+// Per row, with m = max x:  s = sum e^(x - m),  w = sum e^(x - m) (x - m),
+//   log p(token) = (x_token - m) - ln s,   entropy = ln s - w / s,
+// and the k largest logits, ties to the lowest index.  w is taken around the running maximum, so that
+// a peaked distribution's small entropy is not a difference of large numbers; -inf logits (banned
+// tokens) enter both sums as zeros.
+//
+// Work is bound by reading the logits (at 2 bytes a value an SM receives about 12 values a clock, and
+// one value costs about 8 lane-instructions, one of them an exponential, of the 128 it can issue).
+// A row is taken by a cluster of 1 to 8 CTAs, so that small batches fill the chip; a warp streams
+// slices of 8 vectors of 16 bytes per lane with the next slice already in flight.  Every lane keeps
+// its own (m, s, w) and rescales once a slice.  The top list is a warp's: lane i holds the i-th
+// largest so far as a 64-bit key (value, then lowest index), and a slice is searched only when some
+// lane's maximum reaches the list's k-th value.  The first threshold is the k-th largest of the 32
+// lane maxima of the first slice, which about 32 elements of it pass.  Lists are merged by bitonic
+// exchanges, in the CTA through shared memory and in the cluster through distributed shared memory:
+// one launch, no workspace, no atomics, the same result in every run.
+#include "lf_common.cuh"
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+namespace lf {
+namespace logprobs {
+
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kVecs = 8;                               // 16-byte vectors of a lane's slice
+constexpr int kMaxParts = 8;                           // CTAs of a row (portable cluster size)
+constexpr unsigned kAll = 0xffffffffu;
+
+typedef unsigned long long u64;
+
+template <int DT> struct Elem;                         // 0 bf16, 1 fp16, 2 fp32
+template <> struct Elem<0> {
+    typedef uint16_t T;
+    static constexpr int N = 8;
+    static constexpr uint32_t kNegInf = 0xFF80FF80u;
+    static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = bf16lo_to_f32(w); f[1] = bf16hi_to_f32(w); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+};
+template <> struct Elem<1> {
+    typedef uint16_t T;
+    static constexpr int N = 8;
+    static constexpr uint32_t kNegInf = 0xFC00FC00u;
+    static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        f[0] = v.x;
+        f[1] = v.y;
+    }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+};
+template <> struct Elem<2> {
+    typedef uint32_t T;
+    static constexpr int N = 4;
+    static constexpr uint32_t kNegInf = 0xFF800000u;
+    static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Largest of a vector's values (NaN if one is).
+template <int DT>
+__device__ __forceinline__ float vec_max(const uint4& v) {
+    if constexpr (DT == 2) {
+        return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
+                       max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else {
+        float f[2];
+        Elem<DT>::unpack(Elem<DT>::max2(Elem<DT>::max2(v.x, v.y), Elem<DT>::max2(v.z, v.w)), f);
+        return max_nan(f[0], f[1]);
+    }
+}
+
+// The values of a vector, in order.
+template <int DT>
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[Elem<DT>::N]) {
+    constexpr int P = Elem<DT>::N / 4;
+    Elem<DT>::unpack(v.x, f);
+    Elem<DT>::unpack(v.y, f + P);
+    Elem<DT>::unpack(v.z, f + 2 * P);
+    Elem<DT>::unpack(v.w, f + 3 * P);
+}
+
+// Keys order by value (NaN above all, both zeros alike), then by lowest index; 0 is below every key.
+__device__ __forceinline__ u64 make_key(float x, uint32_t index) {
+    uint32_t b = __float_as_uint(x + 0.f);             // -0 + 0 = +0
+    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    if (x != x) b = 0xFFFFFFFFu;
+    return ((u64)b << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ float key_value(u64 k) {
+    const uint32_t b = (uint32_t)(k >> 32);
+    return __uint_as_float((b & 0x80000000u) ? (b & 0x7FFFFFFFu) : ~b);
+}
+__device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
+
+// Sorts a bitonic sequence over the lanes, largest first.
+__device__ __forceinline__ u64 bitonic_merge(u64 k, int lane) {
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) {
+        const u64 o = __shfl_xor_sync(kAll, k, j);
+        const bool upper = (lane & j) == 0;            // keeps the larger
+        k = ((o > k) == upper) ? o : k;
+    }
+    return k;
+}
+__device__ __forceinline__ u64 sort_desc(u64 k, int lane) {
+#pragma unroll
+    for (int size = 2; size < 32; size <<= 1)
+#pragma unroll
+        for (int j = size >> 1; j > 0; j >>= 1) {
+            const u64 o = __shfl_xor_sync(kAll, k, j);
+            const bool upper = ((lane & j) == 0) == ((lane & size) == 0);
+            k = ((o > k) == upper) ? o : k;
+        }
+    return bitonic_merge(k, lane);
+}
+// The 32 largest of two sorted lists, sorted.
+__device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
+    const u64 r = __shfl_sync(kAll, b, 31 - lane);
+    return bitonic_merge(a > r ? a : r, lane);
+}
+
+struct Stat {                                          // of a set of values
+    float m, s, w;
+};
+__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
+    const float m = max_nan(a.m, b.m);
+    if (!(m > -INFINITY)) return Stat{m, 0.f, 0.f};    // nothing yet, or NaN
+    // an empty side has s = w = 0: its difference is clamped like an element's
+    const float da = fmaxf(a.m - m, -1e30f), db = fmaxf(b.m - m, -1e30f);
+    const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
+    return Stat{m, fa * a.s + fb * b.s, fa * (a.w + da * a.s) + fb * (b.w + db * b.s)};
+}
+
+struct Args {
+    const void* x;
+    int64_t stride;                                    // elements
+    const void* tokens;
+    int tokens64, vocab, k, parts;
+    float *logprob, *entropy;
+    int64_t* ids;
+    float* top;
+};
+
+template <int DT, bool kTop>
+__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
+    using E = Elem<DT>;
+    typedef typename E::T T;
+    constexpr int N = E::N;
+    constexpr uint32_t kSlice = 32u * N * kVecs;       // values of a warp's slice
+    __shared__ u64 s_list[kWarps][32];
+    __shared__ Stat s_stat[kWarps];
+    __shared__ u64 c_list[kMaxParts][32];              // the cluster's, in its first CTA
+    __shared__ Stat c_stat[kMaxParts];
+    const int part = blockIdx.x % a.parts;
+    const long row = blockIdx.x / a.parts;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const T* x = static_cast<const T*>(a.x) + row * a.stride;
+    // Positions u = v + lead count from the 16-byte boundary at or before the row, so that vectors
+    // are aligned; the row is [lead, end).
+    const uint32_t lead = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    const uint32_t end = lead + (uint32_t)a.vocab;
+    const T* base = x - lead;
+    const uint32_t slices = (end + kSlice - 1) / kSlice;
+    const uint32_t per = (slices + a.parts - 1) / a.parts;
+    const uint32_t s_end = min(slices, (part + 1) * per);
+
+    auto load = [&](uint32_t slice, uint4 (&v)[kVecs]) {
+        const uint32_t u0 = slice * kSlice + lane * N;
+        if (slice * kSlice >= lead && (slice + 1) * kSlice <= end) {   // warp-uniform: whole slice
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) v[i] = ldg_stream(base + u0 + i * 32 * N);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const uint32_t u = u0 + i * 32 * N;
+            uint32_t w[4] = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+            if (u >= lead && u + N <= end) {
+                v[i] = ldg_stream(base + u);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (u + e >= lead && u + e < end) {
+                    if constexpr (DT == 2) w[e] = base[u + e];
+                    else w[e / 2] = (w[e / 2] & (e % 2 ? 0x0000FFFFu : 0xFFFF0000u)) | ((uint32_t)base[u + e] << (16 * (e % 2)));
+                }
+            v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    };
+
+    Stat st{-INFINITY, 0.f, 0.f};
+    u64 list = 0, kth = 0;                             // this lane's entry; the k-th entry
+    float thr = -INFINITY;                             // no value below it enters the list
+    bool first = true;
+    uint4 cur[kVecs], nxt[kVecs];
+    uint32_t sl = part * per + warp;
+    if (sl < s_end) load(sl, cur);
+    for (; sl < s_end; sl += kWarps) {
+        if (sl + kWarps < s_end) load(sl + kWarps, nxt);
+        float vm[kVecs];
+        float lm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            vm[i] = vec_max<DT>(cur[i]);
+            lm = max_nan(lm, vm[i]);
+        }
+        const float m = max_nan(st.m, lm);
+        const float ref = m == -INFINITY ? 0.f : m;    // every value so far is -inf: all terms are 0
+        if (m != st.m) {
+            const float d = fmaxf(st.m - ref, -1e30f), f = fast_exp2(d * kLog2e);
+            st.w = f * (st.w + d * st.s);
+            st.s *= f;
+            st.m = m;
+        }
+        float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};    // short chains of additions
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            float f[N];
+            unpack<DT>(cur[i], f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float d = fmaxf(f[e] - ref, -1e30f);
+                const float p = fast_exp2(d * kLog2e);
+                s[e & 1] += p;
+                w[e & 1] = fmaf(p, d, w[e & 1]);
+            }
+        }
+        st.s += s[0] + s[1];
+        st.w += w[0] + w[1];
+        if constexpr (kTop) {
+            if (first) {
+                // k lanes have a value >= the k-th largest lane maximum, so it bounds the k-th value
+                int rank = 0;
+                for (int j = 0; j < 32; ++j) {
+                    const float o = __shfl_sync(kAll, lm, j);
+                    rank += (o > lm || o != o || (o == lm && j < lane)) ? 1 : 0;
+                }
+                const unsigned at = __ballot_sync(kAll, rank == a.k - 1);
+                thr = at != 0 ? __shfl_sync(kAll, lm, __ffs(at) - 1) : -INFINITY;
+                if (thr != thr) thr = -INFINITY;
+                first = false;
+            }
+            if (__any_sync(kAll, !(lm < thr))) {
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    if (!__any_sync(kAll, !(vm[i] < thr))) continue;
+                    float f[N];
+                    unpack<DT>(cur[i], f);
+                    const uint32_t u = sl * kSlice + (i * 32 + lane) * N;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const bool valid = u + e >= lead && u + e < end;
+                        const u64 key = valid && !(f[e] < thr) ? make_key(f[e], u + e - lead) : 0;
+                        unsigned in = __ballot_sync(kAll, key > kth);
+                        if (in == 0) continue;
+                        if (__popc(in) > 6) {          // many at once: sort them and merge
+                            list = merge_lists(list, sort_desc(key > kth ? key : 0, lane), lane);
+                            kth = __shfl_sync(kAll, list, a.k - 1);
+                        } else {
+                            while (in != 0) {
+                                const u64 c = __shfl_sync(kAll, key, __ffs(in) - 1);
+                                in &= in - 1;
+                                const int pos = __popc(__ballot_sync(kAll, list > c));
+                                const u64 up = __shfl_up_sync(kAll, list, 1);
+                                list = lane < pos ? list : (lane == pos ? c : up);
+                            }
+                            kth = __shfl_sync(kAll, list, a.k - 1);
+                        }
+                        if (kth != 0) {                // a NaN there lets everything be looked at
+                            const float v = key_value(kth);
+                            thr = v != v ? -INFINITY : v;
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) cur[i] = nxt[i];
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        const Stat o{__shfl_xor_sync(kAll, st.m, off), __shfl_xor_sync(kAll, st.s, off),
+                     __shfl_xor_sync(kAll, st.w, off)};
+        st = merge(st, o);
+    }
+    // A tree over lists in shared memory, halving the number of lists: warp i takes i and i + half.
+    auto tree = [&](u64 (*lists)[32], Stat* stats, int count) {
+        for (int n = count; n > 1; n = (n + 1) / 2) {
+            const int half = (n + 1) / 2;
+            __syncthreads();
+            if (warp < n - half) {
+                if (kTop) lists[warp][lane] = merge_lists(lists[warp][lane], lists[warp + half][lane], lane);
+                const Stat r = merge(stats[warp], stats[warp + half]);
+                __syncwarp();
+                if (lane == 0) stats[warp] = r;
+            }
+        }
+        __syncthreads();
+    };
+    if (kTop) s_list[warp][lane] = list;
+    if (lane == 0) s_stat[warp] = st;
+    tree(s_list, s_stat, kWarps);
+    u64(*lists)[32] = s_list;
+    Stat* stats = s_stat;
+    if (a.parts > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if (warp == 0) {
+            if (kTop) *cluster.map_shared_rank(&c_list[part][lane], 0) = s_list[0][lane];
+            if (lane == 0) *cluster.map_shared_rank(&c_stat[part], 0) = s_stat[0];
+        }
+        cluster.sync();
+        if (part != 0) return;
+        lists = c_list;
+        stats = c_stat;
+        tree(lists, stats, a.parts);
+    }
+    if (warp != 0) return;
+    st = stats[0];
+    const bool none = st.m == -INFINITY, bad = !(st.m < INFINITY);
+    const float ln_s = none || bad ? 0.f : logf(st.s);
+    auto logp = [&](float v) { return bad ? NAN : (none ? -INFINITY : (v - st.m) - ln_s); };
+    if (kTop && lane < a.k) {
+        const u64 k = lists[0][lane];
+        a.ids[row * a.k + lane] = (int64_t)key_index(k);
+        a.top[row * a.k + lane] = logp(key_value(k));
+    }
+    if (lane == 0) {
+        const int64_t tok = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row]
+                                       : (int64_t)static_cast<const int32_t*>(a.tokens)[row];
+        float lp = 0.f;                                // a negative token: none was given
+        if (tok >= a.vocab) {
+            atomicCAS(&g_device_error, 0, 231);
+            lp = NAN;
+        } else if (tok >= 0) {
+            float f[2];
+            E::unpack((uint32_t)x[tok], f);
+            lp = logp(f[0]);
+        }
+        a.logprob[row] = lp;
+        a.entropy[row] = bad ? NAN : (none ? 0.f : ln_s - st.w / st.s);
+    }
+}
+
+template <int DT>
+static int launch(const Args& a, int rows, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long)rows * a.parts));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)a.parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (a.k > 0) LF_CHECK_CUDA((cudaLaunchKernelEx(&cfg, logprobs_kernel<DT, true>, a)));
+    else LF_CHECK_CUDA((cudaLaunchKernelEx(&cfg, logprobs_kernel<DT, false>, a)));
+    return launch_status("token logprobs");
+}
+
+}  // namespace logprobs
+}  // namespace lf
+
+using namespace lf;
+
+extern "C" int lf_token_logprobs(const void* logits, int dtype, int64_t row_stride, const void* tokens,
+                                 int tokens_64bit, int rows, int vocab, int top_k, float* logprob,
+                                 float* entropy, int64_t* top_ids, float* top_logprobs, void* stream) {
+    LF_CHECK_ARG(rows >= 0 && vocab > 0, "token logprobs: rows >= 0 and vocab > 0 are needed");
+    LF_CHECK_ARG(dtype >= 0 && dtype <= 2, "token logprobs: dtype must be LF_BF16, LF_FP16 or LF_FP32");
+    LF_CHECK_ARG(top_k >= 0 && top_k <= 32 && top_k <= vocab, "token logprobs: top_k must be 0..32 and at most vocab");
+    LF_CHECK_ARG(vocab <= (1 << 30), "token logprobs: vocab too large");
+    LF_CHECK_ARG(rows <= 1 || row_stride >= vocab, "token logprobs: rows overlap");
+    if (rows == 0) { clear_error(); return LF_OK; }
+    LF_CHECK_ARG(logits && tokens && logprob && entropy && (top_k == 0 || (top_ids && top_logprobs)),
+                 "token logprobs: null pointer argument");
+    LF_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % (dtype == 2 ? 4 : 2) == 0, "token logprobs: unaligned logits");
+    int dev = 0, sms = 0;
+    LF_CHECK_CUDA(cudaGetDevice(&dev));
+    LF_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    // CTAs of a row: doubled while the grid leaves SMs with less than two and a warp keeps a slice
+    const int slice = dtype == 2 ? 1024 : 2048;
+    int parts = 1;
+    while (parts < logprobs::kMaxParts && (long)rows * parts < 2L * sms &&
+           (long)vocab > (long)parts * logprobs::kWarps * slice)
+        parts *= 2;
+    LF_CHECK_ARG((long)rows * parts <= 2147483647L, "token logprobs: grid limits exceeded");
+    const logprobs::Args a{logits, row_stride, tokens, tokens_64bit != 0, vocab, top_k, parts,
+                           logprob, entropy, top_ids, top_logprobs};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == 0) return logprobs::launch<0>(a, rows, st);
+    if (dtype == 1) return logprobs::launch<1>(a, rows, st);
+    return logprobs::launch<2>(a, rows, st);
+}

@@ -1,0 +1,538 @@
+// Low-rank adapters of many requests beside a shared projection:
+//   out[t] = y[t] + scale[a] (x[t] A[a]) B[a],   a = the adapter of token t's session (or none).
+//
+// Three kernels.  `plan` sorts the tokens by adapter on the device, once per batch: a stable order
+// (adapter, then token) and a list of tiles of up to 64 rows of one adapter, so that the products
+// share an adapter's weights between its sessions.  `shrink` computes h = x A per (tile, slice of the
+// inputs) into fp32 partials; `expand` sums a tile's partials in slice order, rounds scale * h once to
+// bf16 (the operand type; an error of at most 2^-8 of the adapter's own contribution) and adds h B
+// to y in fp32, rounded once.  No atomics: the same bits in every run.
+//
+// Both products have a rank of 16 to 128 on one side, so the work is bound by moving x, y, A and B:
+// tiles come in by cp.async several stages ahead (rows of x and y are gathered, 16 bytes a copy),
+// the products are warp-level m16n8k16.
+#include "lf_common.cuh"
+#include "pool_common.cuh"
+#include "sm100_primitives.cuh"
+
+namespace lf {
+namespace lora {
+
+constexpr int kTile = 64;                              // rows of a tile
+constexpr int kMaxAdapters = 4096;
+constexpr int kHeader = 4;                             // ints before the tiles: [0] = number of tiles
+
+// Layout of a plan (int32): header, tiles [max_tiles][4] = {adapter (-1: none), first row, rows, 0},
+// order [total] = token of every sorted row, starts [n] = first sorted row of every session.
+struct Plan {
+    int32_t *head, *tiles, *order, *starts;
+};
+inline long max_tiles(int total, int n, int adapters) {
+    const long parts = n < adapters + 1 ? n : adapters + 1;
+    return (total + kTile - 1) / kTile + parts;
+}
+inline Plan views(int32_t* p, int total, int n, int adapters) {
+    Plan v;
+    v.head = p;
+    v.tiles = p + kHeader;
+    v.order = v.tiles + 4 * max_tiles(total, n, adapters);
+    v.starts = v.order + total;
+    return v;
+}
+
+// One CTA.  Bucket b < adapters holds adapter b's sessions, bucket `adapters` those without one.
+__global__ void __launch_bounds__(pool::kMetaThreads)
+plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int n, int total, int adapters,
+            Plan p) {
+    extern __shared__ int sm[];
+    __shared__ int buf[32];
+    int* tot = sm;                                     // [adapters + 1] tokens
+    int* off = sm + adapters + 1;                      // first sorted row
+    int* til = off + adapters + 1;                     // first tile
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto bucket = [&](int i) {
+        const int a = ids[i];
+        return a >= 0 && a < adapters ? a : adapters;
+    };
+    // tokens outside [0, total) are cut off: a plan never names a row that does not exist
+    auto lo = [&](int i) { return min(max(cu[i], 0), total); };
+    auto count = [&](int i) { return max(0, min(max(cu[i + 1], 0), total) - lo(i)); };
+    for (int b = threadIdx.x; b <= adapters; b += pool::kMetaThreads) tot[b] = 0;
+    __syncthreads();
+    int sum = 0;
+    for (int i0 = 0; i0 < n; i0 += pool::kMetaThreads) {
+        const int i = i0 + threadIdx.x;
+        const int c = i < n ? count(i) : 0;
+        if (i < n) {
+            if (c > 0) atomicAdd(&tot[bucket(i)], c);
+            if (ids[i] < -1 || ids[i] >= adapters) atomicCAS(&g_device_error, 0, 241);
+        }
+        int t = 0;
+        pool::block_excl_scan(c, &t, buf);
+        sum += t;
+    }
+    // offsets that overlap or leave tokens out give no plan: rows would be written twice or not at all
+    const bool bad = sum != total || (n > 0 && (cu[0] != 0 || cu[n] != total));
+    if (bad) {
+        if (threadIdx.x == 0) {
+            atomicCAS(&g_device_error, 0, 242);
+            p.head[0] = 0;
+        }
+        return;
+    }
+    __syncthreads();
+    int rows = 0, tiles = 0;
+    for (int b0 = 0; b0 <= adapters; b0 += pool::kMetaThreads) {
+        const int b = b0 + threadIdx.x;
+        const int c = b <= adapters ? tot[b] : 0;
+        int t = 0;
+        const int r = rows + pool::block_excl_scan(c, &t, buf);
+        rows += t;
+        const int k = tiles + pool::block_excl_scan((c + kTile - 1) / kTile, &t, buf);
+        tiles += t;
+        if (b <= adapters) {
+            off[b] = r;
+            til[b] = k;
+        }
+    }
+    if (threadIdx.x == 0) p.head[0] = tiles;
+    __syncthreads();
+    for (int b = warp; b <= adapters; b += pool::kMetaThreads / 32) {
+        if (tot[b] == 0) continue;
+        int run = off[b];
+        for (int i0 = 0; i0 < n; i0 += 32) {           // the bucket's sessions, in order
+            const int i = i0 + lane;
+            const int c = i < n && bucket(i) == b ? count(i) : 0;
+            int incl = c;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += o;
+            }
+            if (i < n && bucket(i) == b) p.starts[i] = run + incl - c;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        for (int k = lane; k < (tot[b] + kTile - 1) / kTile; k += 32)
+            reinterpret_cast<int4*>(p.tiles)[til[b] + k] =
+                make_int4(b == adapters ? -1 : b, off[b] + kTile * k, min(kTile, tot[b] - kTile * k), 0);
+    }
+    __syncthreads();
+    constexpr int kBig = 1024;                         // sessions that the whole CTA copies
+    for (int i = warp; i < n; i += pool::kMetaThreads / 32) {
+        const int c = count(i);
+        if (c < kBig)
+            for (int j = lane; j < c; j += 32) p.order[p.starts[i] + j] = lo(i) + j;
+    }
+    if (total >= kBig)
+        for (int i = 0; i < n; ++i) {
+            const int c = count(i);
+            if (c >= kBig)
+                for (int j = threadIdx.x; j < c; j += pool::kMetaThreads) p.order[p.starts[i] + j] = lo(i) + j;
+        }
+}
+
+// -- products ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+    const int n = on ? 16 : 0;                         // 0: fill with zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct Args {
+    const uint16_t *x, *y, *a, *b;
+    uint16_t* out;
+    const float* scale;
+    float* part;                                       // [slices][total][R]
+    const int32_t *head, *tiles, *order;
+    int64_t x_stride, y_stride, out_stride;            // elements between rows
+    int total, K, N, slices, k_per;                    // k_per: inputs of a slice, a multiple of kStep
+    int cols;                                          // expand: column blocks of a CTA
+};
+
+constexpr int kStep = 64;                              // inputs of a stage
+constexpr int kStages = 4;
+constexpr int kShrinkWarps = 8;
+
+// Row of `r` 16-byte chunks in shared memory, chunk index xor-ed with the row: ldmatrix without
+// bank conflicts for rows of 128 bytes and more; for shorter rows several rows share 128 bytes.
+template <int CH>
+__device__ __forceinline__ uint32_t at(int row, int chunk) {
+    if constexpr (CH >= 8) return (uint32_t)((row * CH + (chunk & ~7) + ((chunk ^ row) & 7)) * 16);
+    else return (uint32_t)((row * CH + (chunk ^ ((row / (8 / CH)) & (CH - 1)))) * 16);
+}
+
+template <int R>
+struct ShrinkSmem {
+    static constexpr int kX = kTile * kStep * 2, kA = kStep * R * 2;
+    static constexpr int kRing = kStages * (kX + kA);
+    static constexpr int kRed = kShrinkWarps * 16 * R * 4;   // partial accumulators of the warps
+    static constexpr int kBytes = kRing > kRed ? kRing : kRed;
+};
+
+// CTA (slice of the inputs, tile).  Warps split the tile's 16-row blocks, and, where the tile has
+// fewer than eight, the 16-input steps of a stage; those partial sums are added in warp order.
+template <int R>
+__global__ void __launch_bounds__(32 * kShrinkWarps)
+shrink_kernel(const Args g) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tile = blockIdx.y, slice = blockIdx.x;
+    if (tile >= g.head[0]) return;
+    const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
+    if (t.x < 0) return;
+    const int rows = t.z, first = t.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int k0 = slice * g.k_per, k1 = min(g.K, k0 + g.k_per);
+    const int steps = (k1 - k0 + kStep - 1) / kStep;
+    const uint32_t base = sm100::smem_addr(smem);
+    constexpr int XC = kStep / 8, AC = R / 8;          // chunks of a row
+    constexpr int SZ = ShrinkSmem<R>::kX + ShrinkSmem<R>::kA;
+    const uint16_t* A = g.a + (long)t.x * g.K * R;
+    const int blocks = (rows + 15) / 16;
+    const int mb = blocks <= 1 ? 1 : (blocks <= 2 ? 2 : 4);   // row blocks, rounded up; kw warps each
+    const int kw = kShrinkWarps / mb;
+    // this thread's x rows: chunk c of rows r0, r0 + 32
+    const int xc = threadIdx.x % XC, xr = threadIdx.x / XC;
+    const uint16_t* xrow[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = xr + 32 * i;
+        xrow[i] = g.x + (r < rows ? (long)g.order[first + r] : 0) * g.x_stride + 8 * xc;
+    }
+    auto load = [&](int s) {
+        if (s < steps) {
+            const uint32_t st = base + (uint32_t)((s % kStages) * SZ);
+            const int k = k0 + s * kStep;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = xr + 32 * i;
+                if (r < 16 * mb) {
+                    const bool on = r < rows && k + 8 * xc < k1;
+                    cp16(st + at<XC>(r, xc), on ? xrow[i] + k : g.x, on);
+                }
+            }
+            for (int c = threadIdx.x; c < kStep * AC; c += 32 * kShrinkWarps) {
+                const int kr = c / AC, cc = c % AC;
+                const bool on = k + kr < k1;
+                cp16(st + ShrinkSmem<R>::kX + at<AC>(kr, cc), on ? A + (long)(k + kr) * R + 8 * cc : g.a, on);
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) load(s);
+    float acc[R / 8][4];
+#pragma unroll
+    for (int j = 0; j < R / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    const int m = warp % mb, kk0 = warp / mb;
+    for (int s = 0; s < steps; ++s) {
+        cp_wait<kStages - 2>();
+        __syncthreads();
+        load(s + kStages - 1);
+        const uint32_t st = base + (uint32_t)((s % kStages) * SZ);
+        for (int kk = kk0; kk < kStep / 16; kk += kw) {
+            uint32_t a[4];
+            ldsm4(st + at<XC>(16 * m + (lane & 15), 2 * kk + (lane >> 4)), a);
+#pragma unroll
+            for (int j = 0; j < R / 16; ++j) {
+                uint32_t b[4];
+                ldsm4_t(st + ShrinkSmem<R>::kX + at<AC>(16 * kk + (lane & 15), 2 * j + (lane >> 4)), b);
+                mma(acc[2 * j], a, b[0], b[1]);
+                mma(acc[2 * j + 1], a, b[2], b[3]);
+            }
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();
+    const int gq = lane >> 2, c = lane & 3;
+    float* red = reinterpret_cast<float*>(smem);       // [kw][16 mb][R]
+#pragma unroll
+    for (int j = 0; j < R / 8; ++j) {
+        float* p = red + (long)(kk0 * 16 * mb + 16 * m + gq) * R + 8 * j + 2 * c;
+        *reinterpret_cast<float2*>(p) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(p + 8 * R) = make_float2(acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    const int used = kw < kStep / 16 ? kw : kStep / 16;  // warps past a stage's steps hold zeros
+    float* dst = g.part + ((long)slice * g.total + first) * R;
+    for (int i = threadIdx.x * 4; i < rows * R; i += 32 * kShrinkWarps * 4) {
+        float4 v = *reinterpret_cast<const float4*>(red + i);
+        for (int w = 1; w < used; ++w) {
+            const float4 o = *reinterpret_cast<const float4*>(red + (long)w * 16 * mb * R + i);
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        *reinterpret_cast<float4*>(dst + i) = v;
+    }
+}
+
+constexpr int kCols = 128;                             // columns of an expand block
+constexpr int kExpandWarps = 4;                        // 32 columns each
+
+template <int R>
+struct ExpandSmem {
+    static constexpr int kH = kTile * R * 2, kB = R * kCols * 2, kY = kTile * kCols * 2;
+    static constexpr int kBytes = kH + kB + kY;
+};
+
+// CTA (group of column blocks, tile): h of the tile once, then per block of 128 columns
+// y + h B, staged in shared memory.
+template <int R>
+__global__ void __launch_bounds__(32 * kExpandWarps)
+expand_kernel(const Args g) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tile = blockIdx.y;
+    if (tile >= g.head[0]) return;
+    const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
+    const int rows = t.z, first = t.y;
+    const bool copy_only = t.x < 0;
+    if (copy_only && g.y == g.out) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int YC = kCols / 8, HC = R / 8;
+    constexpr int T = 32 * kExpandWarps;
+    const uint32_t sh = sm100::smem_addr(smem), sb = sh + ExpandSmem<R>::kH, sy = sb + ExpandSmem<R>::kB;
+    uint8_t* yb = smem + ExpandSmem<R>::kH + ExpandSmem<R>::kB;
+    const uint16_t* B = g.b + (long)(copy_only ? 0 : t.x) * R * g.N;
+    const int c = threadIdx.x % YC, r0 = threadIdx.x / YC;      // this thread's chunk column, row
+    const int blocks = (rows + 15) / 16;
+    auto load = [&](int n0) {
+        const bool on = n0 + 8 * c < g.N;
+        for (int r = r0; r < rows; r += T / YC) {
+            const long tok = g.order[first + r];
+            cp16(sy + at<YC>(r, c), on ? g.y + tok * g.y_stride + n0 + 8 * c : g.y, on);
+        }
+        if (!copy_only)
+            for (int k = r0; k < R; k += T / YC)
+                cp16(sb + at<YC>(k, c), on ? B + (long)k * g.N + n0 + 8 * c : g.b, on);
+        cp_commit();
+    };
+    const int n_first = blockIdx.x * g.cols * kCols;
+    load(n_first);
+    if (!copy_only) {                                  // h: partials summed in slice order, scaled, rounded
+        const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+        for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
+            const int r = i / HC, ch = i % HC;
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (r < rows)
+                for (int s = 0; s < g.slices; ++s) {
+                    const float4* p = reinterpret_cast<const float4*>(g.part + ((long)s * g.total + first + r) * R + 8 * ch);
+                    const float4 a = p[0], b = p[1];
+                    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+                }
+            *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
+                make_uint4(pack_bf16x2(v[0] * sc, v[1] * sc), pack_bf16x2(v[2] * sc, v[3] * sc),
+                           pack_bf16x2(v[4] * sc, v[5] * sc), pack_bf16x2(v[6] * sc, v[7] * sc));
+        }
+    }
+    for (int blk = 0; blk < g.cols; ++blk) {
+        const int n0 = n_first + blk * kCols;
+        if (n0 >= g.N) break;
+        if (blk > 0) load(n0);
+        cp_wait<0>();
+        __syncthreads();
+        if (!copy_only) {
+            const int gq = lane >> 2, cq = lane & 3;
+            for (int m = 0; m < blocks; ++m) {
+                float acc[4][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < R / 16; ++kk) {
+                    uint32_t a[4];
+                    ldsm4(sh + at<HC>(16 * m + (lane & 15), 2 * kk + (lane >> 4)), a);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t b[4];
+                        ldsm4_t(sb + at<YC>(16 * kk + (lane & 15), 4 * warp + 2 * j + (lane >> 4)), b);
+                        mma(acc[2 * j], a, b[0], b[1]);
+                        mma(acc[2 * j + 1], a, b[2], b[3]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int r = 16 * m + gq + 8 * half;
+                        if (r < rows) {
+                            uint32_t* p = reinterpret_cast<uint32_t*>(yb + at<YC>(r, 4 * warp + j)) + cq;
+                            const uint32_t w = *p;
+                            *p = pack_bf16x2(bf16lo_to_f32(w) + acc[j][2 * half], bf16hi_to_f32(w) + acc[j][2 * half + 1]);
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        if (n0 + 8 * c < g.N)
+            for (int r = r0; r < rows; r += T / YC)
+                *reinterpret_cast<uint4*>(g.out + (long)g.order[first + r] * g.out_stride + n0 + 8 * c) =
+                    *reinterpret_cast<const uint4*>(yb + at<YC>(r, c));
+        __syncthreads();                               // the block's buffers are free
+    }
+}
+
+inline int slices_for(int total, int n, int adapters, int K, int sms) {
+    // Slices of the inputs so that a small batch still fills the SMs, 256 inputs at least.
+    const long tiles = max_tiles(total, n, adapters);
+    int s = 1;
+    while (s < 32 && tiles * s < sms && K >= 2 * s * 256) s *= 2;
+    return s;
+}
+
+template <int R>
+static int launch(const Args& g, int tiles, cudaStream_t st) {
+    static PerContextOnce once;
+    const int rc = once.run([] {
+        LF_CHECK_CUDA(cudaFuncSetAttribute(shrink_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           ShrinkSmem<R>::kBytes));
+        LF_CHECK_CUDA(cudaFuncSetAttribute(expand_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           ExpandSmem<R>::kBytes));
+        return LF_OK;
+    });
+    if (rc != LF_OK) return rc;
+    shrink_kernel<R><<<dim3(g.slices, tiles), 32 * kShrinkWarps, ShrinkSmem<R>::kBytes, st>>>(g);
+    const int e = launch_status("lora shrink");
+    if (e != LF_OK) return e;
+    const int groups = ((g.N + kCols - 1) / kCols + g.cols - 1) / g.cols;
+    expand_kernel<R><<<dim3(groups, tiles), 32 * kExpandWarps, ExpandSmem<R>::kBytes, st>>>(g);
+    return launch_status("lora expand");
+}
+
+static int sm_count(int* out) {
+    int dev = 0;
+    LF_CHECK_CUDA(cudaGetDevice(&dev));
+    LF_CHECK_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+    return LF_OK;
+}
+
+static int check_sizes(int n, int total, int adapters) {
+    LF_CHECK_ARG(n >= 0 && total >= 0, "lora: negative sizes");
+    LF_CHECK_ARG(adapters > 0 && adapters <= kMaxAdapters, "lora: 1..%d adapters", kMaxAdapters);
+    LF_CHECK_ARG(n > 0 || total == 0, "lora: tokens without sessions");
+    LF_CHECK_ARG(total <= 64 * 60000, "lora: too many tokens");
+    return LF_OK;
+}
+
+}  // namespace lora
+}  // namespace lf
+
+using namespace lf;
+
+extern "C" int lf_lora_plan_size(int n, int total_tokens, int num_adapters, size_t* bytes) {
+    LF_CHECK_ARG(bytes != nullptr, "lora plan: bytes is null");
+    const int rc = lora::check_sizes(n, total_tokens, num_adapters);
+    if (rc != LF_OK) return rc;
+    *bytes = 4 * (size_t)(lora::kHeader + 4 * lora::max_tiles(total_tokens, n, num_adapters) + total_tokens + n);
+    clear_error();
+    return LF_OK;
+}
+
+extern "C" int lf_lora_plan(const int32_t* adapter_ids, const int32_t* cu_tokens, int n, int total_tokens,
+                            int num_adapters, void* plan, size_t plan_bytes, void* stream) {
+    size_t need = 0;
+    int rc = lf_lora_plan_size(n, total_tokens, num_adapters, &need);
+    if (rc != LF_OK) return rc;
+    LF_CHECK_ARG(plan != nullptr && aligned16(plan) && plan_bytes >= need, "lora plan: needs %zu bytes, 16-byte aligned", need);
+    LF_CHECK_ARG(n == 0 || (adapter_ids && cu_tokens), "lora plan: null pointer argument");
+    static PerContextOnce once;
+    rc = once.run([] {
+        LF_CHECK_CUDA(cudaFuncSetAttribute(lora::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           3 * (lora::kMaxAdapters + 1) * 4));
+        return LF_OK;
+    });
+    if (rc != LF_OK) return rc;
+    const lora::Plan p = lora::views(static_cast<int32_t*>(plan), total_tokens, n, num_adapters);
+    lora::plan_kernel<<<1, pool::kMetaThreads, 3 * (num_adapters + 1) * 4, (cudaStream_t)stream>>>(
+        adapter_ids, cu_tokens, n, total_tokens, num_adapters, p);
+    return launch_status("lora plan");
+}
+
+extern "C" int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int rank,
+                                      int sm_count, size_t* bytes) {
+    LF_CHECK_ARG(bytes != nullptr, "lora: bytes is null");
+    int rc = lora::check_sizes(n, total_tokens, num_adapters);
+    if (rc != LF_OK) return rc;
+    LF_CHECK_ARG(inputs > 0 && rank > 0, "lora: bad workspace arguments");
+    if (sm_count <= 0) {
+        rc = lora::sm_count(&sm_count);
+        if (rc != LF_OK) return rc;
+    }
+    *bytes = (size_t)lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count) * total_tokens * rank * 4;
+    clear_error();
+    return LF_OK;
+}
+
+extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x, int64_t x_stride,
+                           const lf_bf16* a, const lf_bf16* b, const float* scale, const void* plan, int n,
+                           int total_tokens, int num_adapters, int inputs, int outputs, int rank,
+                           lf_bf16* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                           int sm_count, void* stream) {
+    int rc = lora::check_sizes(n, total_tokens, num_adapters);
+    if (rc != LF_OK) return rc;
+    LF_CHECK_ARG(rank == 16 || rank == 32 || rank == 64 || rank == 128,
+                 "lora: rank must be 16, 32, 64 or 128 (got %d; pad A and B with zeros)", rank);
+    LF_CHECK_ARG(inputs > 0 && inputs % 8 == 0 && outputs > 0 && outputs % 8 == 0,
+                 "lora: inputs and outputs must be positive multiples of 8");
+    if (total_tokens == 0) { clear_error(); return LF_OK; }
+    LF_CHECK_ARG(y && x && a && b && plan && out && workspace, "lora: null pointer argument");
+    LF_CHECK_ARG(aligned16(y) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(out) &&
+                     aligned16(plan) && aligned16(workspace) && y_stride % 8 == 0 && x_stride % 8 == 0 &&
+                     out_stride % 8 == 0,
+                 "lora: rows must be 16-byte aligned");
+    LF_CHECK_ARG(total_tokens == 1 || (y_stride >= outputs && out_stride >= outputs && x_stride >= 0),
+                 "lora: rows of y or out overlap");
+    LF_CHECK_ARG(y != out || y_stride == out_stride, "lora: in place, y and out need the same rows");
+    if (sm_count <= 0) {
+        rc = lora::sm_count(&sm_count);
+        if (rc != LF_OK) return rc;
+    }
+    lora::Args g{};
+    g.slices = lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count);
+    const size_t need = (size_t)g.slices * total_tokens * rank * 4;
+    LF_CHECK_ARG(workspace_bytes >= need, "lora: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
+    const lora::Plan p = lora::views(const_cast<int32_t*>(static_cast<const int32_t*>(plan)), total_tokens, n, num_adapters);
+    g.x = x;
+    g.y = y;
+    g.a = a;
+    g.b = b;
+    g.out = out;
+    g.scale = scale;
+    g.part = static_cast<float*>(workspace);
+    g.head = p.head;
+    g.tiles = p.tiles;
+    g.order = p.order;
+    g.x_stride = x_stride;
+    g.y_stride = y_stride;
+    g.out_stride = out_stride;
+    g.total = total_tokens;
+    g.K = inputs;
+    g.N = outputs;
+    const int steps = (inputs + lora::kStep - 1) / lora::kStep;
+    g.k_per = (steps + g.slices - 1) / g.slices * lora::kStep;
+    const int tiles = (int)lora::max_tiles(total_tokens, n, num_adapters);
+    // Column blocks of a CTA: 4 once that still leaves about eight CTAs an SM, so that h is formed
+    // once for them.
+    const long blocks = (outputs + lora::kCols - 1) / lora::kCols;
+    g.cols = blocks * tiles >= 32L * sm_count ? 4 : 1;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (rank) {
+        case 16: return lora::launch<16>(g, tiles, st);
+        case 32: return lora::launch<32>(g, tiles, st);
+        case 64: return lora::launch<64>(g, tiles, st);
+        default: return lora::launch<128>(g, tiles, st);
+    }
+}

@@ -13,7 +13,11 @@ appended to the pool layer by layer (``KVPool.reserve`` once per forward, ``writ
 layer).
 
 ``forward(tokens, pool, states, counts)`` advances every listed session by ``counts[i]`` tokens
-(``tokens`` holds them back to back) and returns the greedy next token of each session.
+(``tokens`` holds them back to back) and returns the greedy next token of each session, with their
+log probabilities and top alternatives when asked (``top_logprobs``); ``score`` returns the log
+probability of every given token.  ``pool`` is a ``KVPool`` or, with K/V held in 4 bits, a
+``QuantKVPool``.  ``adapters`` (``LoraAdapters``) with ``adapter_ids`` adds each session's own
+low-rank adapter to the four projections of every layer (``model_ops.lora_add``).
 """
 from __future__ import annotations
 
@@ -79,6 +83,62 @@ class OpTimer:
 def _lap(timer: Optional[OpTimer], name: str) -> None:
     if timer is not None:
         timer.lap(name)
+
+
+class LoraAdapters:
+    """Low-rank adapters of the four projections of every layer, ``num_adapters`` of rank ``rank``:
+    per layer and projection ``a [num_adapters, inputs, rank]``, ``b [num_adapters, rank, outputs]``
+    (bf16, in ``weights``), and one ``scale [num_adapters]`` (fp32).  Ranks are 16, 32, 64 or 128;
+    a smaller adapter is padded with zeros (``set``).  ``seed`` None leaves all of them zero."""
+
+    def __init__(self, cfg: LlamaConfig, num_adapters: int, rank: int, device="cuda",
+                 seed: Optional[int] = None, std: float = 0.02):
+        if rank not in mo.LORA_RANKS:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"rank {rank} is not one of {mo.LORA_RANKS}")
+        c = cfg
+        self.num_adapters, self.rank, self.device = num_adapters, rank, torch.device(device)
+        nq = c.q_heads * c.head_dim
+        self.shapes = {"qkv": (c.d_model, nq + 2 * c.kv_heads * c.head_dim), "o": (nq, c.d_model),
+                       "gate_up": (c.d_model, 2 * c.ffn), "down": (c.ffn, c.d_model)}
+        g = None
+        if seed is not None:
+            g = torch.Generator(device=self.device).manual_seed(seed)
+
+        def w(*shape):
+            if g is None:
+                return torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+            return (torch.randn(shape, generator=g, device=self.device) * std).bfloat16()
+        self.weights = [{k: (w(num_adapters, i, rank), w(num_adapters, rank, o))
+                         for k, (i, o) in self.shapes.items()} for _ in range(c.layers)]
+        self.scale = torch.ones(num_adapters, dtype=torch.float32, device=self.device)
+
+    def set(self, index: int, layer: int, name: str, a: torch.Tensor, b: torch.Tensor,
+            scale: float = 1.0) -> None:
+        """Adapter ``index`` of one projection: ``a [inputs, r]``, ``b [r, outputs]``, r <= rank."""
+        i, o = self.shapes[name]
+        r = a.shape[1]
+        if tuple(a.shape) != (i, r) or tuple(b.shape) != (r, o) or r > self.rank or \
+                not 0 <= index < self.num_adapters:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"adapter of {name} must be [{i}, r], [r, {o}] with "
+                                                     f"r <= {self.rank}")
+        wa, wb = self.weights[layer][name]
+        wa[index].zero_()
+        wb[index].zero_()
+        wa[index, :, :r] = a
+        wb[index, :r] = b
+        self.scale[index] = scale
+
+
+class _Adapted:
+    """The adapters of one batch: its rows sorted once, then one call per projection."""
+
+    def __init__(self, adapters: LoraAdapters, ids: torch.Tensor, cu: torch.Tensor, total: int):
+        self.adapters = adapters
+        self.plan = mo.lora_plan(ids, cu, total, adapters.num_adapters)
+
+    def add(self, y: torch.Tensor, x: torch.Tensor, layer: int, name: str) -> torch.Tensor:
+        a, b = self.adapters.weights[layer][name]
+        return mo.lora_add(y, x, a, b, self.plan, self.adapters.scale)
 
 
 class LlamaShaped:
@@ -160,21 +220,28 @@ class LlamaShaped:
         return self._rmsnorm(x, w) if w is not None else None
 
     def _mlp_block(self, x: torch.Tensor, attn: torch.Tensor, l: int,
-                   timer: Optional[OpTimer] = None):
+                   timer: Optional[OpTimer] = None, adapted: Optional[_Adapted] = None):
         """Rest of layer ``l`` after attention: output projection, residual, FFN norm, SwiGLU
         FFN, residual, and the next layer's input norm.  Returns (x, normed input of l + 1)."""
         c = self.cfg
+        def add(y, inp, name):
+            if adapted is not None:
+                adapted.add(y, inp, l, name)
+                _lap(timer, "adapters")
         o = attn @ self.wo[l]
         _lap(timer, "o_gemm")
+        add(o, attn, "o")
         h = self._norm_in(x, o, self.ffn_norm[l])
         _lap(timer, "add_rmsnorm")
         gu = h @ self.w13[l]
         _lap(timer, "gate_up_gemm")
+        add(gu, h, "gate_up")
         act = mo.swiglu(gu) if self.fused_ops else F.silu(gu[:, :c.ffn]) * gu[:, c.ffn:]
         _lap(timer, "swiglu")
         nxt = self.attn_norm[l + 1] if l + 1 < c.layers else None
         d = act @ self.w2[l]
         _lap(timer, "down_gemm")
+        add(d, act, "down")
         out = self._norm_in(x, d, nxt)
         _lap(timer, "add_rmsnorm")
         return x, out
@@ -183,7 +250,49 @@ class LlamaShaped:
     @torch.no_grad()
     def forward(self, tokens: torch.Tensor, pool: KVPool, states: Sequence[KVState],
                 counts: Sequence[int], n_prefix_pages: int = 0,
-                return_logits: bool = False, timer: Optional[OpTimer] = None) -> torch.Tensor:
+                return_logits: bool = False, timer: Optional[OpTimer] = None,
+                adapters: Optional[LoraAdapters] = None,
+                adapter_ids: Optional[Sequence[int]] = None, top_logprobs: Optional[int] = None):
+        """Advance each session by ``counts[i]`` tokens; the greedy next token of each (their fp32
+        logits with ``return_logits``).  With ``top_logprobs`` (0 to 32 alternatives): ``(tokens,
+        TokenLogprobs)`` of the tokens chosen.  ``adapter_ids`` names each session's adapter (-1:
+        none).  ``n_prefix_pages``: leading pages that are the same for every session listed."""
+        x = self._trunk(tokens, pool, states, counts, n_prefix_pages, timer, adapters, adapter_ids)
+        last = torch.tensor([int(n) for n in counts], device=self.device).cumsum(0) - 1
+        h = self._norm_in(x[last].contiguous(), None, self.final_norm)
+        logits = h @ self.lm_head
+        _lap(timer, "lm_head")
+        if return_logits:
+            out = logits.float()
+        else:
+            out = torch.argmax(logits, dim=-1)
+            if top_logprobs is not None:
+                out = out, mo.token_logprobs(logits, out, top_k=top_logprobs)
+        _lap(timer, "argmax")
+        return out
+
+    @torch.no_grad()
+    def score(self, tokens: torch.Tensor, pool: KVPool, states: Sequence[KVState],
+              counts: Sequence[int], n_prefix_pages: int = 0,
+              adapters: Optional[LoraAdapters] = None, adapter_ids: Optional[Sequence[int]] = None,
+              top_k: int = 0, rows: int = 2048) -> mo.TokenLogprobs:
+        """Advance each session by its tokens and score them: entry ``t`` holds the log probability
+        of the session's token ``t + 1`` given those up to ``t`` (0 at a session's last token, whose
+        successor is not given), the entropy and the ``top_k`` alternatives there.  The LM head runs
+        ``rows`` positions at a time, so no logits of the whole batch are held."""
+        counts = [int(n) for n in counts]
+        tokens = tokens.to(self.device).long()
+        x = self._trunk(tokens, pool, states, counts, n_prefix_pages, None, adapters, adapter_ids)
+        nxt = torch.full_like(tokens, -1)
+        nxt[:-1] = tokens[1:]
+        nxt[torch.tensor([n for n in counts if n], device=self.device).cumsum(0) - 1] = -1
+        h = self._norm_in(x, None, self.final_norm)
+        parts = [mo.token_logprobs(h[i:i + rows] @ self.lm_head, nxt[i:i + rows], top_k)
+                 for i in range(0, h.shape[0], rows)]
+        return mo.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
+
+    def _trunk(self, tokens, pool, states, counts, n_prefix_pages, timer, adapters, adapter_ids):
+        """Every layer for the batch's new tokens; returns the residual stream ``[T, d_model]``."""
         c = self.cfg
         counts = [int(x) for x in counts]
         T = sum(counts)
@@ -207,6 +316,11 @@ class LlamaShaped:
             pps, need = pool.decode_workspace(len(states), c.q_heads, table.shape[1], n_prefix_pages)
             if self._ws is None or self._ws.numel() < need:
                 self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        adapted = None
+        if adapters is not None:
+            if adapter_ids is None or len(adapter_ids) != len(states):
+                raise _lib.LoopfuseError(_lib.LF_EINVAL, "adapters need one adapter id per session")
+            adapted = _Adapted(adapters, pool._ids(adapter_ids), index[1], T)
         if timer is not None:
             timer.lap("setup")
         x = self.embed[tokens]
@@ -216,6 +330,9 @@ class LlamaShaped:
         for l in range(c.layers):
             qkv = h @ self.wqkv[l]
             _lap(timer, "qkv_gemm")
+            if adapted is not None:
+                adapted.add(qkv, h, l, "qkv")
+                _lap(timer, "adapters")
             if self.fused_qkv:
                 q = torch.empty((T, c.q_heads, c.head_dim), dtype=qkv.dtype, device=self.device)
                 pool.write_qkv(states, start, l, qkv, q, counts, rope=rope, index=index)
@@ -231,14 +348,8 @@ class LlamaShaped:
             else:
                 a = pool.attend_prefill(q, l, table, cu, lens, max(counts), buffers)
             _lap(timer, "attention")
-            x, h = self._mlp_block(x, a.view(T, nq), l, timer)
-        last = torch.tensor(counts, device=self.device).cumsum(0) - 1
-        h = self._norm_in(x[last].contiguous(), None, self.final_norm)
-        logits = h @ self.lm_head
-        _lap(timer, "lm_head")
-        out = logits.float() if return_logits else torch.argmax(logits, dim=-1)
-        _lap(timer, "argmax")
-        return out
+            x, h = self._mlp_block(x, a.view(T, nq), l, timer, adapted)
+        return x
 
     # -- AgentExecutor model contract ------------------------------------------------------------
     def prefill(self, tokens: torch.Tensor, kv_state: KVState, attention=None) -> torch.Tensor:
@@ -265,7 +376,7 @@ class GraphedDecode:
 
     A decode step of the model is ~700 kernel launches, so at small batches the host's launch
     rate, not the GPU, sets the step time.  Here a step is: one pinned host -> device copy of
-    (tokens, slot ids, counts), one graph replay (pool reserve and block-table gather, every
+    (tokens, slot ids, counts, adapter ids), one graph replay (pool reserve and block-table gather, every
     layer, final norm, LM head, argmax), and the caller's read of the result.  A batch of n
     sessions runs in the graph of the smallest bucket >= n; rows past n take 0 new tokens in
     ``pad`` (a ``KVPool.pad_session``): their pages never grow and their outputs are ignored.
@@ -273,8 +384,10 @@ class GraphedDecode:
     output (``raise_if_failed`` after the caller's sync).
     """
 
-    def __init__(self, model: "LlamaShaped", pool: KVPool, pad: KVState, n_prefix_pages: int = 0):
+    def __init__(self, model: "LlamaShaped", pool: KVPool, pad: KVState, n_prefix_pages: int = 0,
+                 adapters: Optional[LoraAdapters] = None):
         self.model, self.pool, self.pad, self.npp = model, pool, pad, n_prefix_pages
+        self.adapters = adapters
         self.graphs = {}
         self.status_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
 
@@ -282,8 +395,8 @@ class GraphedDecode:
         m, pool, dev = self.model, self.pool, self.model.device
         c = m.cfg
         s = {"nb": nb,
-             "host": torch.zeros((3, nb), dtype=torch.int32, pin_memory=True),
-             "dev": torch.zeros((3, nb), dtype=torch.int32, device=dev),
+             "host": torch.zeros((4, nb), dtype=torch.int32, pin_memory=True),
+             "dev": torch.zeros((4, nb), dtype=torch.int32, device=dev),
              "cu": torch.arange(nb + 1, dtype=torch.int32, device=dev),
              "start": torch.zeros(nb, dtype=torch.int32, device=dev),
              "table": torch.empty((nb, pool.max_pages_per_seq), dtype=torch.int32, device=dev),
@@ -293,6 +406,7 @@ class GraphedDecode:
         s["ws"] = torch.empty(need, dtype=torch.uint8, device=dev)
         # rows: real sessions take 1 token; a fresh graph's warm-up runs every row as padding
         s["host"][1].fill_(self.pad.slot_id)
+        s["host"][3].fill_(-1)
         s["dev"].copy_(s["host"])
         m.rope_tables(pool.max_seq_len + 1)
         side = torch.cuda.Stream(device=dev)
@@ -316,16 +430,21 @@ class GraphedDecode:
         pool.gather_device(ids, nb, s["table"], s["lens"])
         rope = (m._cos, m._sin)
         index = (ids, s["cu"], nb)
+        adapted = None
+        if self.adapters is not None:
+            adapted = _Adapted(self.adapters, s["dev"][3], s["cu"], nb)
         x = m.embed[toks.long()]
         nq = c.q_heads * c.head_dim
         h = m._norm_in(x, None, m.attn_norm[0])
         for l in range(c.layers):
             qkv = h @ m.wqkv[l]
+            if adapted is not None:
+                adapted.add(qkv, h, l, "qkv")
             q = torch.empty((nb, c.q_heads, c.head_dim), dtype=qkv.dtype, device=m.device)
             pool.write_qkv(None, s["start"], l, qkv, q, None, rope=rope, index=index)
             a = pool.attend_decode(q, l, s["table"], s["lens"], num_prefix_pages=self.npp,
                                    pages_per_split=s["pps"], workspace=s["ws"])
-            x, h = m._mlp_block(x, a.view(nb, nq), l)
+            x, h = m._mlp_block(x, a.view(nb, nq), l, adapted=adapted)
         return torch.argmax(m._norm_in(x, None, m.final_norm) @ m.lm_head, dim=-1)
 
     def prepare(self, max_batch: int) -> None:
@@ -336,10 +455,14 @@ class GraphedDecode:
             if b >= max_batch:
                 break
 
-    def step(self, states: Sequence[KVState], tokens: Sequence[int]) -> torch.Tensor:
+    def step(self, states: Sequence[KVState], tokens: Sequence[int],
+             adapter_ids: Optional[Sequence[int]] = None) -> torch.Tensor:
         """Advance each session by its token; returns the device tensor of greedy next tokens
-        (the first ``len(states)`` rows are valid)."""
+        (the first ``len(states)`` rows are valid).  ``adapter_ids``: each session's adapter (-1 or
+        not given: none), when the graphs were built with ``adapters``."""
         n = len(states)
+        if adapter_ids is not None and (self.adapters is None or len(adapter_ids) != n):
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, "adapter_ids need adapters and one id per session")
         nb = _bucket(n)
         s = self.graphs.get(nb)
         if s is None:
@@ -356,6 +479,9 @@ class GraphedDecode:
         host[0, n:] = 0
         host[1, n:] = self.pad.slot_id
         host[2, n:] = 0
+        host[3] = -1
+        if adapter_ids is not None:
+            host[3, :n] = torch.as_tensor(list(adapter_ids), dtype=torch.int32)
         s["dev"].copy_(host, non_blocking=True)
         s["copied"].record()
         s["graph"].replay()

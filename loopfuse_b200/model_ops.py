@@ -1,5 +1,7 @@
-"""Decoder ops on the sm_100a library: residual add + RMSNorm, the SwiGLU gate, and a
-weight-streaming tcgen05 GEMM for decode batches (``gemm_skinny``).
+"""Decoder ops on the sm_100a library: residual add + RMSNorm, the SwiGLU gate, a
+weight-streaming tcgen05 GEMM for decode batches (``gemm_skinny``), low-rank adapters of many
+sessions beside a shared projection (``lora_plan`` / ``lora_add``), and the log probabilities of
+given tokens with entropy and top alternatives (``token_logprobs``).
 
 Each is one bandwidth-bound kernel in place of the chain of torch elementwise passes a model
 would otherwise run around its GEMMs (``lf_add_rmsnorm`` / ``lf_swiglu`` in
@@ -9,7 +11,8 @@ output is rounded to bf16 before the gate multiply.
 """
 from __future__ import annotations
 
-from typing import Optional
+from dataclasses import dataclass
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -102,3 +105,132 @@ def gemm_skinny(x: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] = 
     _lib.call("lf_gemm_skinny", x.data_ptr(), w.data_ptr(), out.data_ptr(), m, n, k,
               workspace.data_ptr(), workspace.numel(), sms, _stream())
     return out
+
+
+# -- log probabilities --------------------------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor          # [T] fp32: ln p of the given token
+    entropy: torch.Tensor          # [T] fp32: -sum p ln p
+    top_ids: torch.Tensor          # [T, k] int64: the k most likely tokens, ties to the lowest id
+    top_logprobs: torch.Tensor     # [T, k] fp32
+
+
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TOP_LOGPROBS = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """Log probability of ``tokens [T]`` (int64 or int32) under ``softmax(logits [T, V])``, each
+    row's entropy and its ``top_k`` (at most 32) most likely tokens, in one pass over the logits.
+
+    ``logits`` is bf16, fp16 or fp32, rows contiguous (their stride is free).  A negative token
+    means none was given: its logprob is 0.  A token >= V gives NaN and is reported by
+    ``lf_device_status``.  -inf logits have no probability; a row of nothing else has logprob -inf and
+    entropy 0; a row with a NaN or +inf has NaN probabilities and entropy."""
+    if logits.device.type != "cuda" or tokens.device != logits.device:
+        raise LoopfuseError(_lib.LF_EINVAL, "token_logprobs: logits and tokens must be on one CUDA device")
+    if logits.dtype not in _LOGIT_TYPES or logits.dim() != 2 or \
+            (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise LoopfuseError(_lib.LF_EINVAL, "token_logprobs: logits must be bf16, fp16 or fp32 [T, V] "
+                                            "with contiguous rows")
+    T, V = logits.shape
+    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != (T,) or not tokens.is_contiguous():
+        raise LoopfuseError(_lib.LF_EINVAL, f"token_logprobs: tokens must be contiguous int64 or int32 [{T}]")
+    k = int(top_k)
+    if not 0 <= k <= min(MAX_TOP_LOGPROBS, V):
+        raise LoopfuseError(_lib.LF_EINVAL, f"token_logprobs: top_k = {k} outside 0..{min(MAX_TOP_LOGPROBS, V)}")
+    dev = logits.device
+    out = TokenLogprobs(torch.empty(T, dtype=torch.float32, device=dev),
+                        torch.empty(T, dtype=torch.float32, device=dev),
+                        torch.empty((T, k), dtype=torch.int64, device=dev),
+                        torch.empty((T, k), dtype=torch.float32, device=dev))
+    if T == 0:
+        return out
+    with torch.cuda.device(dev):
+        _lib.call("lf_token_logprobs", logits.data_ptr(), _LOGIT_TYPES[logits.dtype], logits.stride(0),
+                  tokens.data_ptr(), int(tokens.dtype == torch.int64), T, V, k, out.logprob.data_ptr(),
+                  out.entropy.data_ptr(), out.top_ids.data_ptr() if k else None,
+                  out.top_logprobs.data_ptr() if k else None, _stream())
+    return out
+
+
+# -- low-rank adapters ----------------------------------------------------------------------------
+LORA_RANKS = (16, 32, 64, 128)
+
+
+@dataclass
+class LoraPlan:
+    """A batch's rows sorted by adapter (``lora_plan``); used by every ``lora_add`` of the batch."""
+    buffer: torch.Tensor
+    sessions: int
+    total_tokens: int
+    num_adapters: int
+
+
+def lora_plan(adapter_ids: torch.Tensor, cu_tokens: torch.Tensor, total_tokens: int,
+              num_adapters: int) -> LoraPlan:
+    """Sort a batch's rows by adapter on the device, once for all its projections.
+
+    ``adapter_ids [N]`` int32 on the GPU: the adapter of each session (-1: none); ``cu_tokens
+    [N + 1]``: session ``i`` owns rows ``cu_tokens[i] .. cu_tokens[i + 1]``, ``total_tokens`` in
+    all.  Ids outside ``[-1, num_adapters)`` count as none; they, and offsets that are not rising
+    from 0 to ``total_tokens`` (nothing is written then), are reported by ``lf_device_status``."""
+    for t, n in ((adapter_ids, "adapter_ids"), (cu_tokens, "cu_tokens")):
+        if t.device.type != "cuda" or t.dtype != torch.int32 or not t.is_contiguous():
+            raise LoopfuseError(_lib.LF_EINVAL, f"lora_plan: {n} must be a contiguous CUDA int32 tensor")
+    n = adapter_ids.shape[0] if adapter_ids.dim() == 1 else -1
+    if cu_tokens.shape != (n + 1,) or cu_tokens.device != adapter_ids.device:
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_plan: adapter_ids [N] and cu_tokens [N + 1] on one device")
+    size = _lib.c_size_t(0)
+    _lib.call("lf_lora_plan_size", n, int(total_tokens), int(num_adapters), _lib.ctypes.byref(size))
+    buf = torch.empty(size.value, dtype=torch.uint8, device=adapter_ids.device)
+    with torch.cuda.device(adapter_ids.device):
+        _lib.call("lf_lora_plan", adapter_ids.data_ptr(), cu_tokens.data_ptr(), n, int(total_tokens),
+                  int(num_adapters), buf.data_ptr(), buf.numel(), _stream())
+    return LoraPlan(buf, n, int(total_tokens), int(num_adapters))
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan,
+             scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[t] + scale[i] * (x[t] @ a[i]) @ b[i]``, ``i`` the adapter of token ``t``'s session.
+
+    ``y [T, N]`` and ``x [T, K]`` bf16 rows (contiguous, row stride a multiple of 8), ``a
+    [adapters, K, R]``, ``b [adapters, R, N]`` bf16, ``scale [adapters]`` fp32 (None: 1); R is 16,
+    32, 64 or 128 (pad with zeros), K and N multiples of 8.  In place on ``y`` unless ``out`` is
+    given; rows without an adapter keep (or, with ``out``, are) ``y``'s."""
+    res = y if out is None else out
+    for t, n, dim in ((y, "y", 2), (x, "x", 2), (res, "out", 2), (a, "a", 3), (b, "b", 3)):
+        if t.device.type != "cuda" or t.dtype != torch.bfloat16 or t.dim() != dim or \
+                t.device != plan.buffer.device:
+            raise LoopfuseError(_lib.LF_EINVAL, f"lora_add: {n} must be a {dim}-d bf16 tensor on the plan's device")
+    T, K = x.shape
+    N, R = y.shape[1], a.shape[2]
+    if T != plan.total_tokens or y.shape[0] != T or res.shape != y.shape or \
+            tuple(a.shape) != (plan.num_adapters, K, R) or tuple(b.shape) != (plan.num_adapters, R, N):
+        raise LoopfuseError(_lib.LF_EINVAL, f"lora_add: y {tuple(y.shape)}, x {tuple(x.shape)}, "
+                                            f"a {tuple(a.shape)}, b {tuple(b.shape)} and a plan of "
+                                            f"{plan.total_tokens} tokens, {plan.num_adapters} adapters do not match")
+    if not (a.is_contiguous() and b.is_contiguous()):
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_add: a and b must be contiguous")
+    for t in (y, x, res):
+        if t.stride(1) != 1 or (T > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
+            raise LoopfuseError(_lib.LF_EINVAL, "lora_add: rows must be contiguous, their stride a multiple of 8")
+    if R not in LORA_RANKS:
+        raise LoopfuseError(_lib.LF_EINVAL, f"lora_add: rank {R} is not one of {LORA_RANKS} (pad with zeros)")
+    if scale is not None and (scale.device != y.device or scale.dtype != torch.float32 or
+                              tuple(scale.shape) != (plan.num_adapters,) or not scale.is_contiguous()):
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_add: scale must be fp32 [adapters] on y's device")
+    if T == 0:
+        return res
+    with torch.cuda.device(y.device):
+        sms = _sm_count(y.device)
+        need = _lib.c_size_t(0)
+        _lib.call("lf_lora_workspace_size", plan.sessions, T, plan.num_adapters, K, R, sms,
+                  _lib.ctypes.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=y.device)
+        rows = [t.stride(0) if T > 1 else t.shape[1] for t in (y, x, res)]
+        _lib.call("lf_lora_add", y.data_ptr(), rows[0], x.data_ptr(), rows[1], a.data_ptr(), b.data_ptr(),
+                  scale.data_ptr() if scale is not None else None, plan.buffer.data_ptr(), plan.sessions,
+                  T, plan.num_adapters, K, N, R, res.data_ptr(), rows[2], ws.data_ptr(), ws.numel(), sms,
+                  _stream())
+    return res
