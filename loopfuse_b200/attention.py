@@ -23,11 +23,13 @@ K/V may also be held in 4 bits (4.5 with their scales; format in ``include/loopf
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+from ._launch import launch, sm_count
 from ._lib import LF_PAGE_SIZE, LoopfuseError
 
 SM_COUNT = 148          # B200; the split heuristic uses the current device's count when it can
@@ -231,11 +233,11 @@ def q4_head_dim(pages: torch.Tensor) -> int:
 
 def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
     """The device all the given tensors are on."""
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) != 1:
-        raise LoopfuseError(_lib.LF_EINVAL, f"{what}: tensors on different devices: "
-                                            f"{sorted(map(str, devs))}")
-    return devs.pop()
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise LoopfuseError(_lib.LF_EINVAL, f"{what}: tensors on {dev} and {t.device}")
+    return dev
 
 
 def append_qkv_q4(qkv: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
@@ -276,12 +278,11 @@ def append_qkv_q4(qkv: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
     if T == 0 or N == 0:
         return q_out
     base, elem, row = qkv.data_ptr(), qkv.element_size(), qkv.stride(0) if T > 1 else qkv.shape[1]
-    with torch.cuda.device(dev):
-        _lib.call("lf_q4_append", base, base + Hq * D * elem, base + (Hq + Hkv) * D * elem, row, 0,
-                  row, D, block_table.data_ptr(), N, block_table.shape[1], None, start_pos.data_ptr(),
-                  cu_tokens.data_ptr(), N, T, cos.data_ptr() if cos is not None else None,
-                  sin.data_ptr() if sin is not None else None, rows, q_out.data_ptr(),
-                  pages.data_ptr(), P, 1, Hq, Hkv, D, None, _stream())
+    launch("lf_q4_append", dev, base, base + Hq * D * elem, base + (Hq + Hkv) * D * elem, row, 0,
+           row, D, block_table.data_ptr(), N, block_table.shape[1], None, start_pos.data_ptr(),
+           cu_tokens.data_ptr(), N, T, cos.data_ptr() if cos is not None else None,
+           sin.data_ptr() if sin is not None else None, rows, q_out.data_ptr(), pages.data_ptr(), P,
+           1, Hq, Hkv, D, None)
     return q_out
 
 
@@ -300,12 +301,18 @@ def _rope(rope, D: int):
 def default_pages_per_split_q4(num_seqs: int, num_kv_heads: int, max_pages: int,
                                num_prefix_pages: int = 0) -> int:
     """Split size of ``paged_decode_q4`` (``lf_q4_decode_default_split``)."""
+    return _split_q4(int(num_seqs), int(num_kv_heads), int(max_pages), int(num_prefix_pages), _sm_count())
+
+
+@lru_cache(maxsize=4096)
+def _split_q4(num_seqs: int, num_kv_heads: int, max_pages: int, num_prefix_pages: int, sms: int) -> int:
     out = _lib.c_int(0)
-    _lib.call("lf_q4_decode_default_split", int(num_seqs), int(num_kv_heads), int(max_pages),
-              int(num_prefix_pages), _sm_count(), _lib.ctypes.byref(out))
+    _lib.call("lf_q4_decode_default_split", num_seqs, num_kv_heads, max_pages, num_prefix_pages, sms,
+              _lib.ctypes.byref(out))
     return int(out.value)
 
 
+@lru_cache(maxsize=4096)
 def decode_q4_workspace_bytes(num_seqs: int, num_q_heads: int, head_dim: int, max_pages: int,
                               pages_per_split: int, num_prefix_pages: int = 0) -> int:
     n = _lib.c_size_t(0)
@@ -341,18 +348,16 @@ def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
     lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if N == 0:
         return (o, lse) if return_lse else o
-    max_pages = block_table.shape[1]
+    max_pages, npre = block_table.shape[1], int(num_prefix_pages)
     scale = D ** -0.5 if scale is None else float(scale)
-    with torch.cuda.device(dev):
-        pps = pages_per_split or default_pages_per_split_q4(N, Hkv, max_pages, num_prefix_pages)
-        need = decode_q4_workspace_bytes(N, Hq, D, max_pages, pps, num_prefix_pages)
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _lib.call("lf_q4_decode_fwd", q.data_ptr(), pages.data_ptr(), block_table.data_ptr(),
-                  seq_lens.data_ptr(), int(num_prefix_pages), o.data_ptr(),
-                  lse.data_ptr() if lse is not None else None, workspace.data_ptr(),
-                  workspace.numel() * workspace.element_size(), N, Hq, Hkv, D, P, max_pages, pps,
-                  scale, _stream())
+    pps = pages_per_split or _split_q4(N, Hkv, max_pages, npre, sm_count(dev.index))
+    need = decode_q4_workspace_bytes(N, Hq, D, max_pages, pps, npre)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    launch("lf_q4_decode_fwd", dev, q.data_ptr(), pages.data_ptr(), block_table.data_ptr(),
+           seq_lens.data_ptr(), npre, o.data_ptr(), lse.data_ptr() if lse is not None else None,
+           workspace.data_ptr(), workspace.numel() * workspace.element_size(), N, Hq, Hkv, D, P,
+           max_pages, pps, scale)
     return (o, lse) if return_lse else o
 
 
@@ -383,8 +388,7 @@ def expand_pages_q4(pages: torch.Tensor, block_table: torch.Tensor, seq_lens: to
             raise LoopfuseError(_lib.LF_EINVAL, f"expand_pages_q4: out must be two tensors {shape}")
     dev = _one_device("expand_pages_q4", pages, block_table, seq_lens, k, v)
     table = torch.empty_like(block_table)
-    with torch.cuda.device(dev):
-        _lib.call("lf_q4_expand", pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-                  int(num_prefix_pages), k.data_ptr(), v.data_ptr(), table.data_ptr(), N, Hkv, D, P,
-                  max_pages, shape[0], _stream())
+    launch("lf_q4_expand", dev, pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+           int(num_prefix_pages), k.data_ptr(), v.data_ptr(), table.data_ptr(), N, Hkv, D, P, max_pages,
+           shape[0])
     return k, v, table

@@ -11,12 +11,16 @@
 // one value costs about 8 lane-instructions, one of them an exponential, of the 128 it can issue).
 // A row is taken by a cluster of 1 to 8 CTAs, so that small batches fill the chip; a warp streams
 // slices of 8 vectors of 16 bytes per lane with the next slice already in flight.  Every lane keeps
-// its own (m, s, w) and rescales once a slice.  The top list is a warp's: lane i holds the i-th
-// largest so far as a 64-bit key (value, then lowest index), and a slice is searched only when some
-// lane's maximum reaches the list's k-th value.  The first threshold is the k-th largest of the 32
-// lane maxima of the first slice, which about 32 elements of it pass.  Lists are merged by bitonic
-// exchanges, in the CTA through shared memory and in the cluster through distributed shared memory:
-// one launch, no workspace, no atomics, the same result in every run.
+// its own (m, s, w) and rescales once a slice.
+//
+// The alternatives are found among whole vectors: the k vectors with the largest maxima (ties to the
+// lowest index) hold the k largest values, since a value of any other vector is beaten by each of
+// their k maxima.  A warp keeps its best vectors as a sorted list, lane i the i-th as a 64-bit key
+// (maximum, then lowest index); it starts from the lanes' best vectors of the first slice, and a
+// later slice is searched only when some lane's maximum reaches the list's k-th.  Lists are merged by
+// bitonic exchanges, in the CTA through shared memory and in the cluster through distributed shared
+// memory, and the values of the last k vectors are read again and sorted: one launch, no workspace,
+// no atomics, the same result in every run.
 #include "lf_common.cuh"
 
 #include <cooperative_groups.h>
@@ -211,8 +215,8 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
     };
 
     Stat st{-INFINITY, 0.f, 0.f};
-    u64 list = 0, kth = 0;                             // this lane's entry; the k-th entry
-    float thr = -INFINITY;                             // no value below it enters the list
+    u64 list = 0, kth = 0, own = 0;                    // this lane's entry; the k-th entry
+    float thr = -INFINITY;                             // no vector below it enters the list
     bool first = true;
     uint4 cur[kVecs], nxt[kVecs];
     uint32_t sl = part * per + warp;
@@ -250,49 +254,47 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
         st.s += s[0] + s[1];
         st.w += w[0] + w[1];
         if constexpr (kTop) {
-            if (first) {
-                // k lanes have a value >= the k-th largest lane maximum, so it bounds the k-th value
-                int rank = 0;
-                for (int j = 0; j < 32; ++j) {
-                    const float o = __shfl_sync(kAll, lm, j);
-                    rank += (o > lm || o != o || (o == lm && j < lane)) ? 1 : 0;
-                }
-                const unsigned at = __ballot_sync(kAll, rank == a.k - 1);
-                thr = at != 0 ? __shfl_sync(kAll, lm, __ffs(at) - 1) : -INFINITY;
-                if (thr != thr) thr = -INFINITY;
+            const uint32_t v0 = sl * (kSlice / N) + lane;     // this lane's vectors: v0 + 32 i
+            auto key_of = [&](int i) {                 // a vector without a value of the row has none
+                const uint32_t v = v0 + 32 * i;
+                return v * N + N > lead && v * N < end ? make_key(vm[i], v) : 0;
+            };
+            if (first) {                               // the list starts from the lanes' best vectors
                 first = false;
+                u64 best = 0;
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    const u64 k = key_of(i);
+                    best = k > best ? k : best;
+                }
+                list = sort_desc(best, lane);
+                kth = __shfl_sync(kAll, list, a.k - 1);
+                own = best;
             }
             if (__any_sync(kAll, !(lm < thr))) {
 #pragma unroll
                 for (int i = 0; i < kVecs; ++i) {
-                    if (!__any_sync(kAll, !(vm[i] < thr))) continue;
-                    float f[N];
-                    unpack<DT>(cur[i], f);
-                    const uint32_t u = sl * kSlice + (i * 32 + lane) * N;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const bool valid = u + e >= lead && u + e < end;
-                        const u64 key = valid && !(f[e] < thr) ? make_key(f[e], u + e - lead) : 0;
-                        unsigned in = __ballot_sync(kAll, key > kth);
-                        if (in == 0) continue;
-                        if (__popc(in) > 6) {          // many at once: sort them and merge
-                            list = merge_lists(list, sort_desc(key > kth ? key : 0, lane), lane);
-                            kth = __shfl_sync(kAll, list, a.k - 1);
-                        } else {
-                            while (in != 0) {
-                                const u64 c = __shfl_sync(kAll, key, __ffs(in) - 1);
-                                in &= in - 1;
-                                const int pos = __popc(__ballot_sync(kAll, list > c));
-                                const u64 up = __shfl_up_sync(kAll, list, 1);
-                                list = lane < pos ? list : (lane == pos ? c : up);
-                            }
-                            kth = __shfl_sync(kAll, list, a.k - 1);
-                        }
-                        if (kth != 0) {                // a NaN there lets everything be looked at
-                            const float v = key_value(kth);
-                            thr = v != v ? -INFINITY : v;
+                    u64 key = !(vm[i] < thr) ? key_of(i) : 0;
+                    if (key == own) key = 0;           // in the list already
+                    unsigned in = __ballot_sync(kAll, key > kth);
+                    if (in == 0) continue;
+                    if (__popc(in) > 6) {              // many at once: sort them and merge
+                        list = merge_lists(list, sort_desc(key > kth ? key : 0, lane), lane);
+                    } else {
+                        while (in != 0) {
+                            const u64 c = __shfl_sync(kAll, key, __ffs(in) - 1);
+                            in &= in - 1;
+                            const int pos = __popc(__ballot_sync(kAll, list > c));
+                            const u64 up = __shfl_up_sync(kAll, list, 1);
+                            list = lane < pos ? list : (lane == pos ? c : up);
                         }
                     }
+                    kth = __shfl_sync(kAll, list, a.k - 1);
+                }
+                own = 0;
+                if (kth != 0) {                        // a NaN there lets everything be looked at
+                    const float v = key_value(kth);
+                    thr = v != v ? -INFINITY : v;
                 }
             }
         }
@@ -341,10 +343,43 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
     const bool none = st.m == -INFINITY, bad = !(st.m < INFINITY);
     const float ln_s = none || bad ? 0.f : logf(st.s);
     auto logp = [&](float v) { return bad ? NAN : (none ? -INFINITY : (v - st.m) - ln_s); };
-    if (kTop && lane < a.k) {
-        const u64 k = lists[0][lane];
-        a.ids[row * a.k + lane] = (int64_t)key_index(k);
-        a.top[row * a.k + lane] = logp(key_value(k));
+    if (kTop) {
+        // The values of the k best vectors that reach the k-th vector's maximum hold the k best values
+        // (at least k do); they are gathered, sorted 32 at a time and merged.
+        const u64 mine = lists[0][lane];
+        const bool have = mine != 0 && lane < a.k;
+        const uint32_t u = key_index(mine) * N;
+        const u64 last = __shfl_sync(kAll, mine, a.k - 1);   // 0: fewer than k vectors
+        const float bar = last == 0 ? -INFINITY : key_value(last);
+        u64 best = 0, key = 0;
+        int count = 0;                                 // candidates waiting in `key`, one a lane
+        for (int e = 0; e < N; ++e) {
+            const uint32_t p = u + e;
+            float f[2] = {-INFINITY, 0.f};
+            const bool valid = have && p >= lead && p < end;
+            if (valid) E::unpack((uint32_t)base[p], f);
+            const bool in = valid && !(f[0] < bar);
+            const unsigned mask = __ballot_sync(kAll, in);
+            if (mask == 0) continue;
+            const u64 cand = in ? make_key(f[0], p - lead) : 0;
+            const int n = __popc(mask);
+            if (count + n > 32) {
+                best = merge_lists(best, sort_desc(key, lane), lane);
+                key = 0;
+                count = 0;
+            }
+            // the j-th candidate goes to lane count + j
+            const int j = lane - count;
+            const int src = j >= 0 && j < n ? (int)__fns(mask, 0, j + 1) : 0;
+            const u64 got = __shfl_sync(kAll, cand, src);
+            if (j >= 0 && j < n) key = got;
+            count += n;
+        }
+        best = merge_lists(best, sort_desc(key, lane), lane);
+        if (lane < a.k) {
+            a.ids[row * a.k + lane] = (int64_t)key_index(best);
+            a.top[row * a.k + lane] = logp(key_value(best));
+        }
     }
     if (lane == 0) {
         const int64_t tok = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row]

@@ -12,11 +12,13 @@ output is rounded to bf16 before the gate multiply.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
+from ._launch import launch, sm_count
 from ._lib import LoopfuseError
 
 
@@ -146,11 +148,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
                         torch.empty((T, k), dtype=torch.float32, device=dev))
     if T == 0:
         return out
-    with torch.cuda.device(dev):
-        _lib.call("lf_token_logprobs", logits.data_ptr(), _LOGIT_TYPES[logits.dtype], logits.stride(0),
-                  tokens.data_ptr(), int(tokens.dtype == torch.int64), T, V, k, out.logprob.data_ptr(),
-                  out.entropy.data_ptr(), out.top_ids.data_ptr() if k else None,
-                  out.top_logprobs.data_ptr() if k else None, _stream())
+    launch("lf_token_logprobs", dev, logits.data_ptr(), _LOGIT_TYPES[logits.dtype], logits.stride(0),
+           tokens.data_ptr(), int(tokens.dtype == torch.int64), T, V, k, out.logprob.data_ptr(),
+           out.entropy.data_ptr(), out.top_ids.data_ptr() if k else None,
+           out.top_logprobs.data_ptr() if k else None)
     return out
 
 
@@ -181,13 +182,26 @@ def lora_plan(adapter_ids: torch.Tensor, cu_tokens: torch.Tensor, total_tokens: 
     n = adapter_ids.shape[0] if adapter_ids.dim() == 1 else -1
     if cu_tokens.shape != (n + 1,) or cu_tokens.device != adapter_ids.device:
         raise LoopfuseError(_lib.LF_EINVAL, "lora_plan: adapter_ids [N] and cu_tokens [N + 1] on one device")
+    total, adapters, dev = int(total_tokens), int(num_adapters), adapter_ids.device
+    size = _plan_bytes(n, total, adapters)
+    buf = torch.empty(size, dtype=torch.uint8, device=dev)
+    launch("lf_lora_plan", dev, adapter_ids.data_ptr(), cu_tokens.data_ptr(), n, total, adapters,
+           buf.data_ptr(), size)
+    return LoraPlan(buf, n, total, adapters)
+
+
+@lru_cache(maxsize=4096)
+def _plan_bytes(n: int, total: int, adapters: int) -> int:
     size = _lib.c_size_t(0)
-    _lib.call("lf_lora_plan_size", n, int(total_tokens), int(num_adapters), _lib.ctypes.byref(size))
-    buf = torch.empty(size.value, dtype=torch.uint8, device=adapter_ids.device)
-    with torch.cuda.device(adapter_ids.device):
-        _lib.call("lf_lora_plan", adapter_ids.data_ptr(), cu_tokens.data_ptr(), n, int(total_tokens),
-                  int(num_adapters), buf.data_ptr(), buf.numel(), _stream())
-    return LoraPlan(buf, n, int(total_tokens), int(num_adapters))
+    _lib.call("lf_lora_plan_size", n, total, adapters, _lib.ctypes.byref(size))
+    return int(size.value)
+
+
+@lru_cache(maxsize=4096)
+def _lora_workspace_bytes(n: int, total: int, adapters: int, inputs: int, rank: int, sms: int) -> int:
+    need = _lib.c_size_t(0)
+    _lib.call("lf_lora_workspace_size", n, total, adapters, inputs, rank, sms, _lib.ctypes.byref(need))
+    return int(need.value)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan,
@@ -222,15 +236,13 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         raise LoopfuseError(_lib.LF_EINVAL, "lora_add: scale must be fp32 [adapters] on y's device")
     if T == 0:
         return res
-    with torch.cuda.device(y.device):
-        sms = _sm_count(y.device)
-        need = _lib.c_size_t(0)
-        _lib.call("lf_lora_workspace_size", plan.sessions, T, plan.num_adapters, K, R, sms,
-                  _lib.ctypes.byref(need))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=y.device)
-        rows = [t.stride(0) if T > 1 else t.shape[1] for t in (y, x, res)]
-        _lib.call("lf_lora_add", y.data_ptr(), rows[0], x.data_ptr(), rows[1], a.data_ptr(), b.data_ptr(),
-                  scale.data_ptr() if scale is not None else None, plan.buffer.data_ptr(), plan.sessions,
-                  T, plan.num_adapters, K, N, R, res.data_ptr(), rows[2], ws.data_ptr(), ws.numel(), sms,
-                  _stream())
+    dev = y.device
+    sms = sm_count(dev.index)
+    need = _lora_workspace_bytes(plan.sessions, T, plan.num_adapters, K, R, sms)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    launch("lf_lora_add", dev, y.data_ptr(), y.stride(0) if T > 1 else N, x.data_ptr(),
+           x.stride(0) if T > 1 else K, a.data_ptr(), b.data_ptr(),
+           scale.data_ptr() if scale is not None else None, plan.buffer.data_ptr(), plan.sessions, T,
+           plan.num_adapters, K, N, R, res.data_ptr(), res.stride(0) if T > 1 else N, ws.data_ptr(), need,
+           sms)
     return res
