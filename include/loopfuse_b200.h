@@ -422,17 +422,16 @@ int lf_q4_fork(const lf_pool_meta* m, int src_seq, const int32_t* dst_seqs, int 
 
 /* Paged split-KV decode over 4-bit pages: lf_decode_fwd's arguments and results (a session of
  * length 0 gives zeros and an lse of -inf), with one array of pages [P][Hkv][18 * D].  Hq / Hkv is 1, 2, 4 or 8.
- * The workspace comes from lf_q4_decode_workspace_size, the split size from
- * lf_q4_decode_default_split (sm_count <= 0: the current device's). */
-int lf_q4_decode_default_split(int num_seqs, int num_kv_heads, int max_pages, int num_prefix_pages,
-                               int sm_count, int* pages_per_split);
-int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int head_dim, int max_pages,
-                                int pages_per_split, int num_prefix_pages, size_t* bytes);
+ * The workspace comes from lf_q4_decode_workspace_size (sm_count <= 0, in both: the current
+ * device's).  The sessions' own pages are cut into equal ranges, a few per SM; there is no split
+ * size to choose. */
+int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                                int max_pages, int num_prefix_pages, int sm_count, size_t* bytes);
 int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32_t* block_table,
                      const int32_t* seq_lens, int num_prefix_pages, lf_bf16* o, float* lse,
                      void* workspace, size_t workspace_bytes, int num_seqs, int num_q_heads,
-                     int num_kv_heads, int head_dim, int num_pages, int max_pages,
-                     int pages_per_split, float scale, void* stream);
+                     int num_kv_heads, int head_dim, int num_pages, int max_pages, float scale,
+                     int sm_count, void* stream);
 
 /* ---- log probabilities of given tokens -------------------------------------------------------
  * For each of `rows` rows of `vocab` logits (dtype LF_BF16, LF_FP16 or LF_FP32; row_stride

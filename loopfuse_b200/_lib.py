@@ -92,10 +92,9 @@ _SIGS.update({
                      _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P],
     "lf_q4_expand": [_P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "lf_q4_fork": [POINTER(PoolMeta), _I, _P, _I, _I, _P, _I, _I, _I, _P],
-    "lf_q4_decode_default_split": [_I, _I, _I, _I, _I, POINTER(c_int)],
-    "lf_q4_decode_workspace_size": [_I, _I, _I, _I, _I, _I, POINTER(c_size_t)],
-    "lf_q4_decode_fwd": [_P, _P, _P, _P, _I, _P, _P, _P, c_size_t, _I, _I, _I, _I, _I, _I, _I,
-                         c_float, _P],
+    "lf_q4_decode_workspace_size": [_I, _I, _I, _I, _I, _I, _I, POINTER(c_size_t)],
+    "lf_q4_decode_fwd": [_P, _P, _P, _P, _I, _P, _P, _P, c_size_t, _I, _I, _I, _I, _I, _I, c_float,
+                         _I, _P],
     "lf_token_logprobs": [_P, _I, c_int64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "lf_lora_plan_size": [_I, _I, _I, POINTER(c_size_t)],
     "lf_lora_plan": [_P, _P, _I, _I, _I, _P, c_size_t, _P],

@@ -298,34 +298,20 @@ def _rope(rope, D: int):
     return cos, sin, cos.shape[0]
 
 
-def default_pages_per_split_q4(num_seqs: int, num_kv_heads: int, max_pages: int,
-                               num_prefix_pages: int = 0) -> int:
-    """Split size of ``paged_decode_q4`` (``lf_q4_decode_default_split``)."""
-    return _split_q4(int(num_seqs), int(num_kv_heads), int(max_pages), int(num_prefix_pages), _sm_count())
-
-
 @lru_cache(maxsize=4096)
-def _split_q4(num_seqs: int, num_kv_heads: int, max_pages: int, num_prefix_pages: int, sms: int) -> int:
-    out = _lib.c_int(0)
-    _lib.call("lf_q4_decode_default_split", num_seqs, num_kv_heads, max_pages, num_prefix_pages, sms,
-              _lib.ctypes.byref(out))
-    return int(out.value)
-
-
-@lru_cache(maxsize=4096)
-def decode_q4_workspace_bytes(num_seqs: int, num_q_heads: int, head_dim: int, max_pages: int,
-                              pages_per_split: int, num_prefix_pages: int = 0) -> int:
+def decode_q4_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                              max_pages: int, num_prefix_pages: int = 0, sms: int = 0) -> int:
+    """Workspace of ``paged_decode_q4`` on a device of ``sms`` SMs (0: the current one)."""
     n = _lib.c_size_t(0)
-    _lib.call("lf_q4_decode_workspace_size", num_seqs, num_q_heads, head_dim, max_pages,
-              pages_per_split, num_prefix_pages, _lib.ctypes.byref(n))
+    _lib.call("lf_q4_decode_workspace_size", num_seqs, num_q_heads, num_kv_heads, head_dim, max_pages,
+              num_prefix_pages, sms or _sm_count(), _lib.ctypes.byref(n))
     return int(n.value)
 
 
 def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
                     seq_lens: torch.Tensor, num_prefix_pages: int = 0,
-                    scale: Optional[float] = None, pages_per_split: Optional[int] = None,
-                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
-                    return_lse: bool = False):
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None, return_lse: bool = False):
     """``paged_decode`` over K/V held in 4 bits: ``q [N, Hq, D]``, ``pages [P, Hkv, 18 * D]`` uint8
     (one layer), ``block_table [N, max_pages]`` and ``seq_lens [N]`` int32, Hq / Hkv 1, 2, 4 or 8.
     With ``num_prefix_pages > 0`` the first that many block-table entries must be the same pages
@@ -350,14 +336,14 @@ def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
         return (o, lse) if return_lse else o
     max_pages, npre = block_table.shape[1], int(num_prefix_pages)
     scale = D ** -0.5 if scale is None else float(scale)
-    pps = pages_per_split or _split_q4(N, Hkv, max_pages, npre, sm_count(dev.index))
-    need = decode_q4_workspace_bytes(N, Hq, D, max_pages, pps, npre)
+    sms = sm_count(dev.index)
+    need = decode_q4_workspace_bytes(N, Hq, Hkv, D, max_pages, npre, sms)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     launch("lf_q4_decode_fwd", dev, q.data_ptr(), pages.data_ptr(), block_table.data_ptr(),
            seq_lens.data_ptr(), npre, o.data_ptr(), lse.data_ptr() if lse is not None else None,
            workspace.data_ptr(), workspace.numel() * workspace.element_size(), N, Hq, Hkv, D, P,
-           max_pages, pps, scale)
+           max_pages, scale, sms)
     return (o, lse) if return_lse else o
 
 

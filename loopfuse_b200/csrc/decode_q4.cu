@@ -16,14 +16,18 @@
 // A warp's lane holds 16-byte vectors of codes that are its operand registers (no ldmatrix, no
 // bank conflicts); a page of one KV head is one block of 18 D bytes, brought in by one bulk copy.
 //
-// Work items (CTAs of four warps):
-//   own     (split, KV head, session): the columns are the GQA group's heads; the warps take the
-//           split's pages round-robin, each with its own ring of kOwnStages pages.
+// Work of CTAs of four warps, one launch:
+//   own     the sessions' own pages, two at a time (a unit), in the order (session, KV head, unit),
+//           are cut into equal ranges, one per resident CTA, so that long and short sessions fill
+//           the chip alike and a CTA starts up once: its warps take a range's units in turn, each
+//           with a ring of kStages units whose copies run on across sessions and heads.  The
+//           columns are the GQA group's heads.
 //   prefix  (chunk, KV head, group of 4 * 8/G sessions): the pages of a shared prefix; the 8
 //           columns of a warp are G heads of 8/G sessions, and the four warps use the same staged
 //           pages for different sessions, so that a prefix page is read once per 32 columns.
-// Every item writes unnormalised fp32 partials (o, max, sum) to its slots; combine merges a row's
-// slots in slot order.
+// Every piece writes unnormalised fp32 partials (o, max, sum); a range's piece of item (session, KV
+// head) is partial number CTA + item, which no two pieces share as both grow along the ranges.
+// combine merges a row's partials, in order.
 //
 // Every barrier wait is bounded (site 221 in the device error word); a warp that gives up stops
 // computing and lets the copies in flight land, bounded again, before it leaves.
@@ -40,21 +44,35 @@ using decode::checked_page;
 using decode::kThreads;
 using decode::kWarps;
 
-constexpr int kStages = 4;                     // pages in flight per warp
-constexpr int kSlots = kWarps * kStages;       // page buffers of a CTA
+constexpr int kUnit = 2;                       // pages of a barrier, a softmax step, a buffer
+constexpr int kStages = 3;                     // units in flight per warp
+constexpr int kSlots = kWarps * kStages;       // buffers of a CTA
+constexpr int kPerSm = 3;                      // resident CTAs of an SM
+constexpr int kMinUnits = kWarps;              // units of a range
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct DecodeArgs {
     const uint16_t* q;
     const uint8_t* pages;
     const int32_t *bt, *lens;
-    float* part_o;
-    float2* part_ml;
+    float *own_o, *pre_o;                      // [ctas + N * Hkv][G][D]; [N][Hq][n_chunks][D]
+    float2 *own_ml, *pre_ml;                   // (max, sum) of each
+    int2* span;                                // [N * Hkv] first and last CTA of an item
     int N, Hq, Hkv, G, num_pages, max_pages;
     int n_prefix, chunk, n_chunks, groups;     // shared prefix: pages, pages a chunk, chunks, session groups
-    int pps, max_split, n_slots;
-    float qscale;                              // scale * log2(e)
+    int ctas;                                  // ranges of the own pages
+    float qscale;                              // |scale| * log2(e)
+    uint32_t flip;                             // sign bits of a negative scale
 };
+
+__device__ __forceinline__ int held(const DecodeArgs& a, int n) {
+    return n < a.N ? min(max(a.lens[n], 0), a.max_pages * kPage) : 0;
+}
+// Units of a session's own pages.
+__device__ __forceinline__ int own_units(const DecodeArgs& a, int n) {
+    const int own = (held(a, n) + kPage - 1) / kPage - a.n_prefix;
+    return own > 0 ? (own + kUnit - 1) / kUnit : 0;
+}
 
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
     if (sm100::mbar_try_wait(bar, parity)) return true;
@@ -87,14 +105,14 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
     return r;
 }
 
-// D += A . B, m16n8k16, bf16 operands, fp32 accumulators.
+// D = A . B + C, m16n8k16, bf16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                    uint32_t b0, uint32_t b1) {
+                                    uint32_t b0, uint32_t b1, const float (&c)[4]) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 // Codes 4 i .. 4 i + 3 of both halves of a word as the bf16 pair 128 + n.
@@ -104,175 +122,240 @@ __device__ __forceinline__ uint32_t codes(uint32_t w, int i) {
     return r;
 }
 
-// A warp's attention state: 8 columns (query rows), of which this lane holds 2c and 2c + 1.
-template <int D>
+// A warp's attention state: B blocks of 8 columns (query rows), of which this lane holds 2c and
+// 2c + 1.  Scores are kept unscaled (q's sign carries the scale's), maxima too.
+template <int D, int B>
 struct State {
     static constexpr int NG = Fmt<D>::NG;
-    uint32_t qb[NG][4][2];                     // Q^T operand, column g
-    float qsum[NG][2];                         // sums of columns 2c, 2c + 1 over each group
-    float o[NG][4][4];                         // O^T: m-tile (16 dims) x 4
-    float corr[NG][4];                         // -136 sum(bf16(p s)): rows are equal
-    float bias[NG][2];                         // this lane's share of sum p (b + 8 s)
-    float m0, m1, l0, l1;
+    uint32_t qb[B][NG][4][2];                  // Q^T operand, column g
+    float qsum[B][NG][2];                      // sums of columns 2c, 2c + 1 over each group
+    float o[B][NG][4][4];                      // O^T: m-tile (16 dims) x 4
+    float corr[B][NG][4];                      // -136 sum(bf16(p s)): rows are equal
+    float bias[B][NG][2];                      // this lane's share of sum p (b + 8 s)
+    float m[B][2], l[B][2];
 
-    // `row` is column g's query row (null: the column is unused).
-    __device__ __forceinline__ void init(const uint16_t* row, int c) {
-        float part[NG];
+    // `row` is column g's query row (null: the column is unused); `flip` is 0x80008000 for a
+    // negative scale.
+    __device__ __forceinline__ void init(int b, const uint16_t* row, uint32_t flip, int c) {
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
-            uint4 a = make_uint4(0, 0, 0, 0), b = a;
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
             if (row != nullptr) {
-                a = *reinterpret_cast<const uint4*>(row + gr * kGroup + c * 16);
-                b = *reinterpret_cast<const uint4*>(row + gr * kGroup + c * 16 + 8);
+                x = *reinterpret_cast<const uint4*>(row + gr * kGroup + c * 16);
+                y = *reinterpret_cast<const uint4*>(row + gr * kGroup + c * 16 + 8);
             }
-            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            part[gr] = 0.f;
+            const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            float part = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                qb[b][gr][k / 2][k % 2] = w[k] ^ flip;
+                part += bf16lo_to_f32(w[k] ^ flip) + bf16hi_to_f32(w[k] ^ flip);
+            }
+            part += __shfl_xor_sync(0xffffffffu, part, 1);
+            part += __shfl_xor_sync(0xffffffffu, part, 2);
+            qsum[b][gr][0] = __shfl_sync(0xffffffffu, part, 8 * c);
+            qsum[b][gr][1] = __shfl_sync(0xffffffffu, part, 8 * c + 4);
+            bias[b][gr][0] = bias[b][gr][1] = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                qb[gr][k][0] = w[2 * k];
-                qb[gr][k][1] = w[2 * k + 1];
-            }
+                corr[b][gr][k] = 0.f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) part[gr] += bf16lo_to_f32(w[k]) + bf16hi_to_f32(w[k]);
-            part[gr] += __shfl_xor_sync(0xffffffffu, part[gr], 1);
-            part[gr] += __shfl_xor_sync(0xffffffffu, part[gr], 2);
-            qsum[gr][0] = __shfl_sync(0xffffffffu, part[gr], 8 * c);
-            qsum[gr][1] = __shfl_sync(0xffffffffu, part[gr], 8 * c + 4);
-            bias[gr][0] = bias[gr][1] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                corr[gr][k] = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[gr][k][j] = 0.f;
+                for (int j = 0; j < 4; ++j) o[b][gr][k][j] = 0.f;
             }
         }
-        m0 = m1 = -INFINITY;
-        l0 = l1 = 0.f;
+        m[b][0] = m[b][1] = -INFINITY;
+        l[b][0] = l[b][1] = 0.f;
     }
 
-    // Applies one staged page whose first token is `tok0`; L0, L1 are the lengths of columns 2c and
-    // 2c + 1.  kMasked: some token of the page may be at or past a column's length.  Such tokens
-    // take no part, whatever their codes and scales hold.
+    // Applies kUnit staged pages, tokens tok0 .. tok0 + 16 kUnit - 1; len[b] are the lengths of the
+    // lane's columns.  kMasked: some token may be at or past a column's length.  Such tokens take no
+    // part, whatever their codes and scales hold.
     template <bool kMasked>
-    __device__ __forceinline__ void page(uint32_t blk, int tok0, int L0, int L1, float qscale, int lane) {
+    __device__ __forceinline__ void unit(uint32_t base, int tok0, const int (&len)[B][2], float qscale, int lane) {
         const int g = lane >> 2, c = lane & 3;
-        uint32_t pa[2 * NG], pb[2 * NG];       // params of tokens g, g + 8: K groups, V groups
-        lds<2 * NG>(blk + Fmt<D>::kParOff + g * (8 * NG), pa);
-        lds<2 * NG>(blk + Fmt<D>::kParOff + (g + 8) * (8 * NG), pb);
-        float s[4] = {0.f, 0.f, 0.f, 0.f};     // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
-        {
-            uint32_t ka[2 * NG], kb[2 * NG];
+        float s[B][kUnit][4];                  // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
+        uint32_t vp[kUnit][2][NG];             // V params of tokens g, g + 8
+#pragma unroll
+        for (int pg = 0; pg < kUnit; ++pg) {
+            const uint32_t blk = base + (uint32_t)(pg * Fmt<D>::kBlockBytes);
+            uint32_t pa[2 * NG], pb[2 * NG], ka[2 * NG], kb[2 * NG];
+            lds<2 * NG>(blk + Fmt<D>::kParOff + g * (8 * NG), pa);
+            lds<2 * NG>(blk + Fmt<D>::kParOff + (g + 8) * (8 * NG), pb);
             lds<2 * NG>(blk + g * (32 * NG) + c * (8 * NG), ka);
             lds<2 * NG>(blk + (g + 8) * (32 * NG) + c * (8 * NG), kb);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                vp[pg][0][gr] = pa[NG + gr];
+                vp[pg][1][gr] = pb[NG + gr];
+                float acc[B][4];
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        mma(acc, codes(ka[2 * gr + w], 2 * k), codes(kb[2 * gr + w], 2 * k),
-                            codes(ka[2 * gr + w], 2 * k + 1), codes(kb[2 * gr + w], 2 * k + 1),
-                            qb[gr][2 * w + k][0], qb[gr][2 * w + k][1]);
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t a0 = codes(ka[2 * gr + w], 2 * k), a1 = codes(kb[2 * gr + w], 2 * k);
+                        const uint32_t a2 = codes(ka[2 * gr + w], 2 * k + 1), a3 = codes(kb[2 * gr + w], 2 * k + 1);
+#pragma unroll
+                        for (int b = 0; b < B; ++b) {
+                            if (w == 0 && k == 0) {    // the accumulators start from -128 sum(q)
+                                const float q0 = -128.f * qsum[b][gr][0], q1 = -128.f * qsum[b][gr][1];
+                                const float start[4] = {q0, q1, q0, q1};
+                                mma(acc[b], a0, a1, a2, a3, qb[b][gr][0][0], qb[b][gr][0][1], start);
+                            } else {
+                                mma(acc[b], a0, a1, a2, a3, qb[b][gr][2 * w + k][0], qb[b][gr][2 * w + k][1], acc[b]);
+                            }
+                        }
+                    }
                 const float sa = bf16lo_to_f32(pa[gr]), sb = bf16lo_to_f32(pb[gr]);
-                const float ba = fmaf(-128.f, sa, bf16hi_to_f32(pa[gr]));
-                const float bb = fmaf(-128.f, sb, bf16hi_to_f32(pb[gr]));
-                s[0] = fmaf(sa, acc[0], fmaf(ba, qsum[gr][0], s[0]));
-                s[1] = fmaf(sa, acc[1], fmaf(ba, qsum[gr][1], s[1]));
-                s[2] = fmaf(sb, acc[2], fmaf(bb, qsum[gr][0], s[2]));
-                s[3] = fmaf(sb, acc[3], fmaf(bb, qsum[gr][1], s[3]));
+                const float ba = bf16hi_to_f32(pa[gr]), bb = bf16hi_to_f32(pb[gr]);
+#pragma unroll
+                for (int b = 0; b < B; ++b) {
+                    float(&t)[4] = s[b][pg];
+                    if (gr == 0) {
+                        t[0] = ba * qsum[b][gr][0];
+                        t[1] = ba * qsum[b][gr][1];
+                        t[2] = bb * qsum[b][gr][0];
+                        t[3] = bb * qsum[b][gr][1];
+                    } else {
+                        t[0] = fmaf(ba, qsum[b][gr][0], t[0]);
+                        t[1] = fmaf(ba, qsum[b][gr][1], t[1]);
+                        t[2] = fmaf(bb, qsum[b][gr][0], t[2]);
+                        t[3] = fmaf(bb, qsum[b][gr][1], t[3]);
+                    }
+                    t[0] = fmaf(sa, acc[b][0], t[0]);
+                    t[1] = fmaf(sa, acc[b][1], t[1]);
+                    t[2] = fmaf(sb, acc[b][2], t[2]);
+                    t[3] = fmaf(sb, acc[b][3], t[3]);
+                }
+            }
+        }
+        bool keep[B][kUnit][4];
+        if (kMasked) {
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int pg = 0; pg < kUnit; ++pg)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        keep[b][pg][j] = tok0 + kPage * pg + g + 8 * (j / 2) < len[b][j % 2];
+                        s[b][pg][j] = keep[b][pg][j] ? s[b][pg][j] : -INFINITY;
+                    }
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            float x0 = fmaxf(s[b][0][0], s[b][0][2]), x1 = fmaxf(s[b][0][1], s[b][0][3]);
+#pragma unroll
+            for (int pg = 1; pg < kUnit; ++pg) {
+                x0 = fmaxf(x0, fmaxf(s[b][pg][0], s[b][pg][2]));
+                x1 = fmaxf(x1, fmaxf(s[b][pg][1], s[b][pg][3]));
+            }
+            // Only lanes of the column need agree, and only when the maximum grows.
+            if (__any_sync(0xffffffffu, x0 > m[b][0] || x1 > m[b][1])) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+                }
+                const float n0 = fmaxf(m[b][0], x0), n1 = fmaxf(m[b][1], x1);
+                const float a0 = m[b][0] == n0 ? 1.f : fast_exp2((m[b][0] - n0) * qscale);
+                const float a1 = m[b][1] == n1 ? 1.f : fast_exp2((m[b][1] - n1) * qscale);
+                // (a column that had met no token has sums of zero: any finite factor will do)
+                const float f0 = m[b][0] == -INFINITY ? 0.f : a0, f1 = m[b][1] == -INFINITY ? 0.f : a1;
+                m[b][0] = n0;
+                m[b][1] = n1;
+                l[b][0] *= f0;
+                l[b][1] *= f1;
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                    bias[b][gr][0] *= f0;
+                    bias[b][gr][1] *= f1;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) corr[b][gr][j] *= (j & 1) ? f1 : f0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[b][gr][k][j] *= (j & 1) ? f1 : f0;
+                }
+            }
+            // a column that has met no token yet keeps a maximum of -inf; its scores are all -inf
+            const float r0 = (kMasked && m[b][0] == -INFINITY) ? 0.f : m[b][0] * -qscale;
+            const float r1 = (kMasked && m[b][1] == -INFINITY) ? 0.f : m[b][1] * -qscale;
+#pragma unroll
+            for (int pg = 0; pg < kUnit; ++pg)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float e = fast_exp2(fmaf(s[b][pg][j], qscale, (j & 1) ? r1 : r0));
+                    s[b][pg][j] = !kMasked || keep[b][pg][j] ? e : 0.f;
+                }
+#pragma unroll
+            for (int pg = 0; pg < kUnit; ++pg) {
+                l[b][0] += s[b][pg][0] + s[b][pg][2];
+                l[b][1] += s[b][pg][1] + s[b][pg][3];
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] *= qscale;
-        bool keep[4] = {true, true, true, true};
-        if (kMasked) {
-            keep[0] = tok0 + g < L0;
-            keep[1] = tok0 + g < L1;
-            keep[2] = tok0 + g + 8 < L0;
-            keep[3] = tok0 + g + 8 < L1;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] = keep[j] ? s[j] : -INFINITY;
-        }
-        float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
-        }
-        if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-            const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-            const float a0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), a1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= a0;
-            l1 *= a1;
+        for (int pg = 0; pg < kUnit; ++pg) {
+            const uint32_t blk = base + (uint32_t)(pg * Fmt<D>::kBlockBytes) + Fmt<D>::kVOff;
+            uint32_t va[2 * NG], vb[2 * NG];   // tokens 2c, 2c + 1 and 2c + 8, 2c + 9
+            lds<2 * NG>(blk + lane * (8 * NG), va);
+            lds<2 * NG>(blk + 256 * NG + lane * (8 * NG), vb);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                bias[gr][0] *= a0;
-                bias[gr][1] *= a1;
+                const float sa = bf16lo_to_f32(vp[pg][0][gr]), sb = bf16lo_to_f32(vp[pg][1][gr]);
+                const float ba = fmaf(8.f, sa, bf16hi_to_f32(vp[pg][0][gr]));
+                const float bb = fmaf(8.f, sb, bf16hi_to_f32(vp[pg][1][gr]));
+                uint32_t b0[B], b1[B];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) corr[gr][j] *= (j & 1) ? a1 : a0;
+                for (int b = 0; b < B; ++b) {
+                    const float(&e)[4] = s[b][pg];
+                    float p[4] = {e[0] * sa, e[1] * sa, e[2] * sb, e[3] * sb};
+                    if (kMasked) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                        for (int j = 0; j < 4; ++j) p[j] = keep[b][pg][j] ? p[j] : 0.f;
+                        bias[b][gr][0] += (keep[b][pg][0] ? e[0] * ba : 0.f) + (keep[b][pg][2] ? e[2] * bb : 0.f);
+                        bias[b][gr][1] += (keep[b][pg][1] ? e[1] * ba : 0.f) + (keep[b][pg][3] ? e[3] * bb : 0.f);
+                    } else {
+                        bias[b][gr][0] = fmaf(e[0], ba, fmaf(e[2], bb, bias[b][gr][0]));
+                        bias[b][gr][1] = fmaf(e[1], ba, fmaf(e[3], bb, bias[b][gr][1]));
+                    }
+                    b0[b] = movm_t(pack_bf16x2(p[0], p[1]));
+                    b1[b] = movm_t(pack_bf16x2(p[2], p[3]));
+                    mma(corr[b][gr], 0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u, b0[b], b1[b], corr[b][gr]);   // bf16 -136
+                }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[gr][k][j] *= (j & 1) ? a1 : a0;
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t a0 = codes(va[2 * gr + w], 2 * k), a1 = codes(va[2 * gr + w], 2 * k + 1);
+                        const uint32_t a2 = codes(vb[2 * gr + w], 2 * k), a3 = codes(vb[2 * gr + w], 2 * k + 1);
+#pragma unroll
+                        for (int b = 0; b < B; ++b)
+                            mma(o[b][gr][2 * w + k], a0, a1, a2, a3, b0[b], b1[b], o[b][gr][2 * w + k]);
+                    }
             }
-        }
-        // a column that has met no token yet keeps a maximum of -inf; its scores are all -inf
-        const float r0 = (kMasked && m0 == -INFINITY) ? 0.f : m0, r1 = (kMasked && m1 == -INFINITY) ? 0.f : m1;
-        float e[4] = {fast_exp2(s[0] - r0), fast_exp2(s[1] - r1), fast_exp2(s[2] - r0), fast_exp2(s[3] - r1)};
-        l0 += e[0] + e[2];
-        l1 += e[1] + e[3];
-        uint32_t va[2 * NG], vb[2 * NG];       // tokens 2c, 2c + 1 and 2c + 8, 2c + 9
-        lds<2 * NG>(blk + Fmt<D>::kVOff + lane * (8 * NG), va);
-        lds<2 * NG>(blk + Fmt<D>::kVOff + 256 * NG + lane * (8 * NG), vb);
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-            const float sa = bf16lo_to_f32(pa[NG + gr]), sb = bf16lo_to_f32(pb[NG + gr]);
-            const float ba = fmaf(8.f, sa, bf16hi_to_f32(pa[NG + gr]));
-            const float bb = fmaf(8.f, sb, bf16hi_to_f32(pb[NG + gr]));
-            float p[4] = {e[0] * sa, e[1] * sa, e[2] * sb, e[3] * sb};
-            float t0 = e[0] * ba, t1 = e[1] * ba, t2 = e[2] * bb, t3 = e[3] * bb;
-            if (kMasked) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = keep[j] ? p[j] : 0.f;
-                t0 = keep[0] ? t0 : 0.f;
-                t1 = keep[1] ? t1 : 0.f;
-                t2 = keep[2] ? t2 : 0.f;
-                t3 = keep[3] ? t3 : 0.f;
-            }
-            bias[gr][0] += t0 + t2;
-            bias[gr][1] += t1 + t3;
-            const uint32_t b0 = movm_t(pack_bf16x2(p[0], p[1])), b1 = movm_t(pack_bf16x2(p[2], p[3]));
-            mma(corr[gr], 0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u, b0, b1);   // bf16 -136
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    mma(o[gr][2 * w + k], codes(va[2 * gr + w], 2 * k), codes(va[2 * gr + w], 2 * k + 1),
-                        codes(vb[2 * gr + w], 2 * k), codes(vb[2 * gr + w], 2 * k + 1), b0, b1);
         }
     }
 
     // Sums over the lanes that share a column; o then holds the whole unnormalised rows.
     __device__ __forceinline__ void finish() {
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, off);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+        for (int b = 0; b < B; ++b) {
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-                bias[gr][0] += __shfl_xor_sync(0xffffffffu, bias[gr][0], off);
-                bias[gr][1] += __shfl_xor_sync(0xffffffffu, bias[gr][1], off);
+            for (int off = 4; off < 32; off <<= 1) {
+                l[b][0] += __shfl_xor_sync(0xffffffffu, l[b][0], off);
+                l[b][1] += __shfl_xor_sync(0xffffffffu, l[b][1], off);
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                    bias[b][gr][0] += __shfl_xor_sync(0xffffffffu, bias[b][gr][0], off);
+                    bias[b][gr][1] += __shfl_xor_sync(0xffffffffu, bias[b][gr][1], off);
+                }
             }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[b][gr][k][j] += corr[b][gr][j & 1] + bias[b][gr][j & 1];
         }
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[gr][k][j] += corr[gr][j & 1] + bias[gr][j & 1];
     }
 };
 
@@ -281,134 +364,245 @@ __device__ __forceinline__ int out_dim(int gr, int k, int g) { return gr * kGrou
 
 template <int D>
 struct Smem {
-    static constexpr int kRing = kSlots * Fmt<D>::kBlockBytes;
+    static constexpr int kUnitBytes = kUnit * Fmt<D>::kBlockBytes;
+    static constexpr int kRing = kSlots * kUnitBytes;
     static constexpr int kMerge = kWarps * 8 * (D + 2) * 4;
-    static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + 128;
+    static constexpr int kBytes = kRing + kMerge + 128;
 };
 
-// Own pages of one session: one split of one KV head.
+// Sum over the CTA's threads (every thread gets it).
+__device__ __forceinline__ long cta_sum(long v, long* buf) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+    __syncthreads();
+    long r = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) r += buf[w];
+    __syncthreads();
+    return r;
+}
+
+// Where a range starts: session n, the first of its units u_n in the flat order before the heads.
+struct Place {
+    long before;                               // units (of one head) of the sessions before n
+    int n;
+};
+
+// A run of units [j, j1) of (session n, KV head h), and how many units follow it in the range.
+struct Segment {
+    int n, h, j, j1, u;
+    long left;
+    // Moves on to the next segment; false at the range's end.
+    __device__ __forceinline__ bool next(const DecodeArgs& a) {
+        if (left <= 0) return false;
+        if (++h == a.Hkv) {
+            h = 0;
+            do { u = own_units(a, ++n); } while (u == 0 && n < a.N);
+            if (u == 0) return false;                            // (not met: units are left)
+        }
+        j = 0;
+        j1 = (int)min((long)u, left);
+        left -= j1;
+        return true;
+    }
+};
+
+// The sessions' own pages: range `cta` of them.
 template <int D>
-__device__ __forceinline__ void own_item(const DecodeArgs& a, uint8_t* smem, uint64_t* bars, int split,
-                                         int h, int n) {
+__device__ __forceinline__ void own_range(const DecodeArgs& a, uint8_t* smem, uint64_t* bars, int cta) {
     using F = Fmt<D>;
+    constexpr int UB = Smem<D>::kUnitBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int L = min(max(a.lens[n], 0), a.max_pages * kPage);
-    const int npages = (L + kPage - 1) / kPage;
-    const int p_begin = a.n_prefix + split * a.pps;
-    if (p_begin >= npages) return;
-    const int n_local = min(a.pps, npages - p_begin);
-    const int mine = n_local > warp ? (n_local - warp + kWarps - 1) / kWarps : 0;
-    const int32_t* row = a.bt + (size_t)n * a.max_pages;
-    const uint32_t ring = sm100::smem_addr(smem) + (uint32_t)(warp * kStages * F::kBlockBytes);
+    __shared__ long buf[kWarps];
+    __shared__ Place s_place;
+    const uint32_t ring = sm100::smem_addr(smem) + (uint32_t)(warp * kStages * UB);
     const uint32_t bar = sm100::smem_addr(bars + warp * kStages);
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) sm100::mbar_init(bar + 8 * i, 1);
         sm100::fence_barrier_init();
     }
-    __syncwarp();
-    const uint64_t policy = sm100::l2_evict_first_policy();      // read once
-    int ids = 0, batch = -1;
-    auto issue = [&](int k) {                                    // warp-uniform
-        if (k >= mine) return;
-        if ((k >> 5) != batch) {                                 // ids of 32 pages, one per lane
-            batch = k >> 5;
-            const int j = warp + kWarps * ((batch << 5) + lane);
-            ids = j < n_local ? checked_page(row[p_begin + j], a.num_pages) : 0;
+    long mine = 0;
+    for (int n = threadIdx.x; n < a.N; n += kThreads) mine += own_units(a, n);
+    const long total = cta_sum(mine, buf) * a.Hkv;
+    const long share = max((total + a.ctas - 1) / a.ctas, (long)kMinUnits);
+    const long begin = cta * share;
+    if (begin >= total) return;
+    long before = 0;                                             // sessions, a CTA's width at a time
+    for (int n0 = 0;; n0 += kThreads) {                          // ends: begin < total
+        const int n = n0 + threadIdx.x;
+        const int u = n < a.N ? own_units(a, n) : 0;
+        const long sum = cta_sum(u, buf);
+        if (begin >= (before + sum) * a.Hkv) {
+            before += sum;
+            continue;
         }
-        const int page = __shfl_sync(0xffffffffu, ids, k & 31);
-        if (lane == 0) {
-            const int st = k % kStages;
-            sm100::mbar_arrive_expect_tx(bar + 8 * st, F::kBlockBytes);
-            bulk_load(ring + (uint32_t)(st * F::kBlockBytes),
-                      a.pages + ((size_t)page * a.Hkv + h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
-        }
-    };
+        long excl = u;                                           // exclusive prefix within the CTA
 #pragma unroll
-    for (int k = 0; k < kStages; ++k) issue(k);
-    State<D> st;
-    st.init(g < a.G ? a.q + ((size_t)n * a.Hq + h * a.G + g) * D : nullptr, c);
-    bool failed = false;
-    int done = 0;
-    for (int k = 0; k < mine; ++k) {
-        const int sl = k % kStages;
-        if (!__all_sync(0xffffffffu, wait_full(bar + 8 * sl, (uint32_t)((k / kStages) & 1)))) {
-            if (lane == 0) atomicCAS(&g_device_error, 0, 221);
-            failed = true;
-            break;
+        for (int off = 1; off < 32; off <<= 1) {
+            const long o = __shfl_up_sync(0xffffffffu, excl, off);
+            if (lane >= off) excl += o;
         }
-        done = k + 1;
-        const uint32_t blk = ring + (uint32_t)(sl * F::kBlockBytes);
-        const int tok0 = (p_begin + warp + kWarps * k) * kPage;
-        if (tok0 + kPage <= L) st.template page<false>(blk, tok0, L, L, a.qscale, lane);
-        else st.template page<true>(blk, tok0, L, L, a.qscale, lane);
-        __syncwarp();                                            // every lane has read the buffer
-        issue(k + kStages);
+        if (lane == 31) buf[warp] = excl;
+        __syncthreads();
+        excl -= u;
+        for (int w = 0; w < warp; ++w) excl += buf[w];
+        if (u > 0 && begin >= (before + excl) * a.Hkv && begin < (before + excl + u) * a.Hkv)
+            s_place = Place{before + excl, n};
+        __syncthreads();
+        break;
     }
-    if (failed && lane == 0)                                     // let the copies in flight land
-        for (int k = done + 1; k < min(mine, done + kStages); ++k)
-            wait_full(bar + 8 * (k % kStages), (uint32_t)((k / kStages) & 1));
-    st.finish();
-
-    __syncthreads();                                             // the rings are idle: merge in them
-    float* sm_m = reinterpret_cast<float*>(smem);                // [kWarps][8]
+    Segment seg;                                                 // what the warps compute on
+    seg.n = s_place.n;
+    seg.u = own_units(a, seg.n);
+    {
+        const long in = begin - s_place.before * a.Hkv, len = min(share, total - begin);
+        seg.h = (int)(in / seg.u);
+        seg.j = (int)(in % seg.u);
+        seg.j1 = (int)min((long)seg.u, seg.j + len);
+        seg.left = len - (seg.j1 - seg.j);
+    }
+    // What this warp copies: a segment of its own that runs ahead.  Page ids of 16 of its units at a
+    // time, one page per lane (lane 2 i + p: page p of the i-th).
+    Segment pre = seg;
+    pre.j += warp;
+    bool more = true;
+    int ids = 0, ids_from = -1, ids_at = 0;                      // units ids_from + 4 i; next i
+    uint32_t issued = 0;
+    const uint64_t policy = sm100::l2_evict_first_policy();      // read once
+    auto issue = [&]() {                                         // warp-uniform: one unit, if any is left
+        while (more && pre.j >= pre.j1) {
+            more = pre.next(a);
+            pre.j = warp;
+            ids_from = -1;
+        }
+        if (!more) return;
+        if (ids_from < 0 || ids_at == 16) {
+            ids_from = pre.j;
+            ids_at = 0;
+            const int p = a.n_prefix + (pre.j + kWarps * (lane / kUnit)) * kUnit + lane % kUnit;
+            const int np = (held(a, pre.n) + kPage - 1) / kPage;
+            ids = p < np ? checked_page(a.bt[(size_t)pre.n * a.max_pages + p], a.num_pages) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, ids_at * kUnit + lane % kUnit);
+        const int last = __shfl_sync(0xffffffffu, page, kUnit - 1);
+        const int st = issued % kStages;
+        if (lane == 0) sm100::mbar_arrive_expect_tx(bar + 8 * st, last >= 0 ? UB : F::kBlockBytes);
+        __syncwarp();
+        if (lane < kUnit && page >= 0)
+            bulk_load(ring + (uint32_t)(st * UB + lane * F::kBlockBytes),
+                      a.pages + ((size_t)page * a.Hkv + pre.h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
+        ++issued;
+        ++ids_at;
+        pre.j += kWarps;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kStages; ++k) issue();
+    float* sm_m = reinterpret_cast<float*>(smem + Smem<D>::kRing);   // [kWarps][8]
     float* sm_l = sm_m + kWarps * 8;
     float* sm_o = sm_l + kWarps * 8;                             // [kWarps][8][D]
-    if (g == 0) {
-        sm_m[warp * 8 + 2 * c] = st.m0;
-        sm_m[warp * 8 + 2 * c + 1] = st.m1;
-        sm_l[warp * 8 + 2 * c] = st.l0;
-        sm_l[warp * 8 + 2 * c + 1] = st.l1;
-    }
-#pragma unroll
-    for (int gr = 0; gr < F::NG; ++gr)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float* r0 = sm_o + (size_t)(warp * 8 + 2 * c) * D + out_dim(gr, k, g);
-            *reinterpret_cast<float2*>(r0) = make_float2(st.o[gr][k][0], st.o[gr][k][2]);
-            *reinterpret_cast<float2*>(r0 + D) = make_float2(st.o[gr][k][1], st.o[gr][k][3]);
+    uint32_t used = 0;
+    bool failed = false;
+    do {
+        const int L = held(a, seg.n), item = seg.n * a.Hkv + seg.h;
+        const int len[1][2] = {{L, L}};
+        State<D, 1> st;
+        st.init(0, g < a.G ? a.q + ((size_t)seg.n * a.Hq + seg.h * a.G + g) * D : nullptr, a.flip, c);
+        for (int j = seg.j + warp; j < seg.j1 && !failed; j += kWarps) {
+            const int sl = used % kStages;
+            if (!__all_sync(0xffffffffu, wait_full(bar + 8 * sl, (used / kStages) & 1))) {
+                if (lane == 0) {
+                    atomicCAS(&g_device_error, 0, 221);          // let the copies in flight land
+                    for (uint32_t k = used; k < issued; ++k) wait_full(bar + 8 * (k % kStages), (k / kStages) & 1);
+                }
+                failed = true;
+                break;
+            }
+            const uint32_t blk = ring + (uint32_t)(sl * UB);
+            const int tok0 = (a.n_prefix + j * kUnit) * kPage;
+            if (tok0 + kUnit * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
+            else st.template unit<true>(blk, tok0, len, a.qscale, lane);
+            __syncwarp();                                        // every lane has read the buffer
+            ++used;
+            issue();
         }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < a.G * D; idx += kThreads) {
-        const int hd = idx / D, d = idx % D;
-        float M = -INFINITY;
+        st.finish();
+        __syncthreads();                                         // the last merge's readers are done
+        if (g == 0) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * 8 + hd]);
-        float acc = 0.f, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float mw = sm_m[w * 8 + hd];
-            if (mw == -INFINITY && sm_l[w * 8 + hd] == 0.f) continue;   // a warp without pages
-            const float sc = fast_exp2(mw - M);
-            acc = fmaf(sc, sm_o[(size_t)(w * 8 + hd) * D + d], acc);
-            l = fmaf(sc, sm_l[w * 8 + hd], l);
+            for (int j = 0; j < 2; ++j) {
+                sm_m[warp * 8 + 2 * c + j] = st.m[0][j];
+                sm_l[warp * 8 + 2 * c + j] = st.l[0][j];
+            }
         }
-        const size_t slot = ((size_t)n * a.Hq + h * a.G + hd) * a.n_slots + a.n_chunks + split;
-        a.part_o[slot * D + d] = acc;
-        if (d == 0) a.part_ml[slot] = make_float2(M, l);
-    }
+        if (2 * c < a.G) {
+#pragma unroll
+            for (int gr = 0; gr < F::NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float* r0 = sm_o + (size_t)(warp * 8 + 2 * c) * D + out_dim(gr, k, g);
+                    *reinterpret_cast<float2*>(r0) = make_float2(st.o[0][gr][k][0], st.o[0][gr][k][2]);
+                    *reinterpret_cast<float2*>(r0 + D) = make_float2(st.o[0][gr][k][1], st.o[0][gr][k][3]);
+                }
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < a.G * D / 4; idx += kThreads) {
+            const int hd = idx / (D / 4), d = 4 * (idx % (D / 4));
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * 8 + hd]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float mw = sm_m[w * 8 + hd], lw = sm_l[w * 8 + hd];
+                if (mw == -INFINITY && lw == 0.f) continue;      // a warp without units
+                const float sc = mw == M ? 1.f : fast_exp2((mw - M) * a.qscale);
+                const float4 x = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * 8 + hd) * D + d);
+                acc.x = fmaf(sc, x.x, acc.x);
+                acc.y = fmaf(sc, x.y, acc.y);
+                acc.z = fmaf(sc, x.z, acc.z);
+                acc.w = fmaf(sc, x.w, acc.w);
+                l = fmaf(sc, lw, l);
+            }
+            const size_t slot = (size_t)(cta + item) * a.G + hd;
+            *reinterpret_cast<float4*>(a.own_o + slot * D + d) = acc;
+            if (d == 0) a.own_ml[slot] = make_float2(M, l);
+        }
+        if (threadIdx.x == 0) {
+            if (seg.j == 0) a.span[item].x = cta;
+            if (seg.j1 == seg.u) a.span[item].y = cta;
+        }
+    } while (seg.next(a));
 }
 
-// One chunk of the shared prefix for 4 * 8/G sessions of one KV head.  The page buffers are one ring
-// of two halves of kSlots / 2 pages, refilled half by half after a CTA barrier.
+// One chunk of the shared prefix for the sessions of four warps (8 columns each) of one KV head.  The
+// buffers are one ring of two halves, refilled half by half after a CTA barrier.
 template <int D>
 __device__ __forceinline__ void prefix_item(const DecodeArgs& a, uint8_t* smem, uint64_t* bars, int chunk,
                                             int h, int group) {
     using F = Fmt<D>;
-    constexpr int kHalf = kSlots / 2;
+    constexpr int UB = Smem<D>::kUnitBytes, kHalf = kSlots / 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int spw = 8 / a.G;                                     // sessions of a warp
     const int first = group * kWarps * spw;
     const int p_begin = chunk * a.chunk, p_end = min(p_begin + a.chunk, a.n_prefix);
-    auto held = [&](int n) { return n < a.N ? min(max(a.lens[n], 0), a.max_pages * kPage) : 0; };
     // The page ids come from the group's longest session, whose row holds every page that any
     // session here needs; pages past its length are not read.
     int best = -1, lead = first;
-    for (int i = 0; i < kWarps * spw; ++i) {
-        const int L = held(first + i);
-        if (L > best) { best = L; lead = first + i; }
+    if (lane < kWarps * spw) {
+        best = held(a, first + lane);
+        lead = first + lane;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        const int ob = __shfl_xor_sync(0xffffffffu, best, off), ol = __shfl_xor_sync(0xffffffffu, lead, off);
+        if (ob > best || (ob == best && ol < lead)) { best = ob; lead = ol; }
     }
     const int pages = min(p_end, (best + kPage - 1) / kPage) - p_begin;
     if (pages <= 0) return;                                      // combine reads no slot of this chunk
+    const int units = (pages + kUnit - 1) / kUnit;
     const int32_t* row = a.bt + (size_t)lead * a.max_pages + p_begin;
     const uint32_t ring = sm100::smem_addr(smem), bar = sm100::smem_addr(bars);
     if (threadIdx.x == 0) {
@@ -418,42 +612,45 @@ __device__ __forceinline__ void prefix_item(const DecodeArgs& a, uint8_t* smem, 
     __syncthreads();
     uint64_t policy;
     asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
-    auto issue_half = [&](int k0) {                              // pages k0 .. k0 + kHalf - 1, warp 0
+    const uint8_t* head = a.pages + (size_t)h * F::kBlockBytes;
+    auto issue_half = [&](int k0) {                              // units k0 .. k0 + kHalf - 1, one a lane of warp 0
         const int k = k0 + lane;
-        if (warp == 0 && lane < kHalf && k < pages) {
-            const int page = checked_page(row[k], a.num_pages);
-            const int sl = k % kSlots;
-            sm100::mbar_arrive_expect_tx(bar + 8 * sl, F::kBlockBytes);
-            bulk_load(ring + (uint32_t)(sl * F::kBlockBytes),
-                      a.pages + ((size_t)page * a.Hkv + h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * sl, policy);
+        if (warp == 0 && lane < kHalf && k < units) {
+            const int sl = k % kSlots, have = min(kUnit, pages - k * kUnit);
+            sm100::mbar_arrive_expect_tx(bar + 8 * sl, have * F::kBlockBytes);
+            for (int i = 0; i < have; ++i)
+                bulk_load(ring + (uint32_t)(sl * UB + i * F::kBlockBytes),
+                          head + (size_t)checked_page(row[k * kUnit + i], a.num_pages) * a.Hkv * F::kBlockBytes,
+                          F::kBlockBytes, bar + 8 * sl, policy);
         }
     };
     issue_half(0);
     issue_half(kHalf);
-    const int base = first + warp * spw;                         // this warp's sessions
-    const int n_g = base + g / a.G, L0 = held(base + (2 * c) / a.G), L1 = held(base + (2 * c + 1) / a.G);
-    State<D> st;
-    st.init(n_g < a.N ? a.q + ((size_t)n_g * a.Hq + h * a.G + g % a.G) * D : nullptr, c);
-    int lmin = min(L0, L1);
+    const int end = (p_begin + pages) * kPage;                   // a unit's missing page is past it
+    const int base = first + warp * spw, n_g = base + g / a.G;
+    const int len[1][2] = {{min(end, held(a, base + (2 * c) / a.G)), min(end, held(a, base + (2 * c + 1) / a.G))}};
+    int lmin = min(len[0][0], len[0][1]);
+    State<D, 1> st;
+    st.init(0, n_g < a.N ? a.q + ((size_t)n_g * a.Hq + h * a.G + g % a.G) * D : nullptr, a.flip, c);
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) lmin = min(lmin, __shfl_xor_sync(0xffffffffu, lmin, off));
     bool failed = false;
-    for (int k0 = 0; k0 < pages; k0 += kHalf) {
-        for (int k = k0; k < min(k0 + kHalf, pages); ++k) {
+    for (int k0 = 0; k0 < units; k0 += kHalf) {
+        for (int k = k0; k < min(k0 + kHalf, units); ++k) {
             const int sl = k % kSlots;
             if (!failed && !__all_sync(0xffffffffu, wait_full(bar + 8 * sl, (uint32_t)((k / kSlots) & 1)))) {
                 if (lane == 0) atomicCAS(&g_device_error, 0, 221);
                 failed = true;
             }
             if (failed) continue;
-            const uint32_t blk = ring + (uint32_t)(sl * F::kBlockBytes);
-            const int tok0 = (p_begin + k) * kPage;
-            if (tok0 + kPage <= lmin) st.template page<false>(blk, tok0, L0, L1, a.qscale, lane);
-            else st.template page<true>(blk, tok0, L0, L1, a.qscale, lane);
+            const uint32_t blk = ring + (uint32_t)(sl * UB);
+            const int tok0 = (p_begin + k * kUnit) * kPage;
+            if (tok0 + kUnit * kPage <= lmin) st.template unit<false>(blk, tok0, len, a.qscale, lane);
+            else st.template unit<true>(blk, tok0, len, a.qscale, lane);
         }
         if (__syncthreads_or(failed)) {                          // every warp is done with this half
             const int k = k0 + lane;                             // copies may still be landing
-            if (warp == 0 && lane < kSlots && k < pages) wait_full(bar + 8 * (k % kSlots), (uint32_t)((k / kSlots) & 1));
+            if (warp == 0 && lane < kSlots && k < units) wait_full(bar + 8 * (k % kSlots), (uint32_t)((k / kSlots) & 1));
             break;
         }
         issue_half(k0 + kSlots);
@@ -464,34 +661,29 @@ __device__ __forceinline__ void prefix_item(const DecodeArgs& a, uint8_t* smem, 
     for (int col = 0; col < 2; ++col) {
         const int j = 2 * c + col, n = base + j / a.G;
         if (n >= a.N) continue;
-        const size_t slot = ((size_t)n * a.Hq + h * a.G + j % a.G) * a.n_slots + chunk;
+        const size_t slot = ((size_t)n * a.Hq + h * a.G + j % a.G) * a.n_chunks + chunk;
 #pragma unroll
         for (int gr = 0; gr < F::NG; ++gr)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<float2*>(a.part_o + slot * D + out_dim(gr, k, g)) =
-                    make_float2(st.o[gr][k][col], st.o[gr][k][2 + col]);
-        if (g == 0) a.part_ml[slot] = col ? make_float2(st.m1, st.l1) : make_float2(st.m0, st.l0);
+                *reinterpret_cast<float2*>(a.pre_o + slot * D + out_dim(gr, k, g)) =
+                    make_float2(st.o[0][gr][k][col], st.o[0][gr][k][2 + col]);
+        if (g == 0) a.pre_ml[slot] = make_float2(st.m[0][col], st.l[0][col]);
     }
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const DecodeArgs a) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
     __shared__ __align__(8) uint64_t bars[kSlots];
-    long item = blockIdx.x;
-    const long n_pre = (long)a.n_chunks * a.Hkv * a.groups;
-    if (item < n_pre) {
-        const int chunk = (int)(item % a.n_chunks);
-        item /= a.n_chunks;
-        prefix_item<D>(a, smem, bars, chunk, (int)(item % a.Hkv), (int)(item / a.Hkv));
-        return;
-    }
-    item -= n_pre;
-    const int split = (int)(item % a.max_split);
-    item /= a.max_split;
-    own_item<D>(a, smem, bars, split, (int)(item % a.Hkv), (int)(item / a.Hkv));
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // combine may be brought in
+    const int n_pre = a.n_chunks * a.Hkv * a.groups;
+    const int item = blockIdx.x;
+    if (item < n_pre)
+        prefix_item<D>(a, smem, bars, item % a.n_chunks, item / a.n_chunks % a.Hkv, item / a.n_chunks / a.Hkv);
+    else
+        own_range<D>(a, smem, bars, item - n_pre);
 }
 
 // One warp per (session, query head): merges the row's partials, the prefix chunks first, by their
@@ -502,20 +694,22 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     const int lane = threadIdx.x & 31;
     const long row = (long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (row >= (long)a.N * a.Hq) return;
-    const int n = (int)(row / a.Hq);
-    const int L = min(max(a.lens[n], 0), a.max_pages * kPage);
-    const int npages = (L + kPage - 1) / kPage;
+    const int n = (int)(row / a.Hq), hq = (int)(row % a.Hq), item = n * a.Hkv + hq / a.G;
+    const int npages = (held(a, n) + kPage - 1) / kPage;
     const int chunks = a.n_prefix > 0 ? (min(npages, a.n_prefix) + a.chunk - 1) / a.chunk : 0;
-    const int splits = npages > a.n_prefix ? (npages - a.n_prefix + a.pps - 1) / a.pps : 0;
-    const int total = chunks + splits;
-    const float2* ml = a.part_ml + row * a.n_slots;
-    const float* po = a.part_o + row * (long)a.n_slots * D;
-    auto slot = [&](int j) { return j < chunks ? j : a.n_chunks + (j - chunks); };
+    asm volatile("griddepcontrol.wait;" ::: "memory");        // the partials are written
+    const int2 span = npages > a.n_prefix ? a.span[item] : make_int2(0, -1);
+    const int total = chunks + span.y - span.x + 1;
+    const long own0 = (long)(span.x + item) * a.G + hq % a.G, pre0 = row * a.n_chunks;
+    auto ml = [&](int j) { return j < chunks ? a.pre_ml[pre0 + j] : a.own_ml[own0 + (long)(j - chunks) * a.G]; };
+    constexpr int V = D / 32;                              // dims of a lane
+    auto vec = [&](int j) {
+        return (j < chunks ? a.pre_o + (pre0 + j) * D : a.own_o + (own0 + (long)(j - chunks) * a.G) * D) + V * lane;
+    };
     float M = -INFINITY;
-    for (int j = lane; j < total; j += 32) M = fmaxf(M, ml[slot(j)].x);
+    for (int j = lane; j < total; j += 32) M = fmaxf(M, ml(j).x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    constexpr int V = D / 32;                              // dims of a lane
     float acc[V], l = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
@@ -523,15 +717,15 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     for (int j0 = 0; j0 < total; j0 += 32) {
         float w = 0.f;
         if (j0 + lane < total) {
-            const float2 e = ml[slot(j0 + lane)];
-            w = fast_exp2(e.x - ref);
+            const float2 e = ml(j0 + lane);
+            w = e.x == -INFINITY ? 0.f : fast_exp2((e.x - ref) * a.qscale);
             l = fmaf(w, e.y, l);
         }
         const int end = min(32, total - j0);
 #pragma unroll 4
         for (int t = 0; t < end; ++t) {
             const float wt = __shfl_sync(0xffffffffu, w, t);
-            const float* src = po + (long)slot(j0 + t) * D + V * lane;
+            const float* src = vec(j0 + t);
             if constexpr (V == 4) {
                 const float4 x = *reinterpret_cast<const float4*>(src);
                 acc[0] = fmaf(wt, x.x, acc[0]);
@@ -551,26 +745,36 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     uint32_t* dst = reinterpret_cast<uint32_t*>(o + row * D) + (V / 2) * lane;
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) dst[i] = pack_bf16x2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    if (lse != nullptr && lane == 0) lse[row] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+    if (lse != nullptr && lane == 0) lse[row] = l != 0.f ? (ref * a.qscale + log2f(l)) * kLn2 : -INFINITY;
 }
 
 // -- sizes ------------------------------------------------------------------------------------------
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-// Pages of a prefix chunk: halved from the whole prefix down to 16 while the items stay under about
-// four per SM.
+// Pages of a prefix chunk: halved from the whole prefix, down to 16, while the items are fewer than
+// two per SM.
 inline int prefix_chunk(int N, int G, int Hkv, int n_prefix, int sms) {
     const long groups = ceil_div((long)N * G, 8 * kWarps);
     int c = n_prefix;
-    while (c > 16 && groups * Hkv * ceil_div(n_prefix, c) < 4L * sms) c = (c + 1) / 2;
+    while (c > 16 && groups * Hkv * ceil_div(n_prefix, c) < 2L * sms) c = (c + 1) / 2;
     return c > 0 ? c : 1;
 }
 
-inline int own_splits(int max_pages, int n_prefix, int pps) { return ceil_div(max_pages - n_prefix, pps); }
-
-constexpr int kMinChunk = 16;
-inline size_t slots_bound(int max_pages, int n_prefix, int pps) {
-    return (size_t)own_splits(max_pages, n_prefix, pps) + (size_t)ceil_div(n_prefix, kMinChunk / 2);
+// Sizes of the workspace's parts, in their order.
+struct Sizes {
+    size_t own, pre, items;                    // partials of the ranges, of the prefix; spans
+    int chunk, n_chunks, ctas;
+    size_t bytes(int D) const { return (own + pre) * (D * sizeof(float) + sizeof(float2)) + items * sizeof(int2); }
+};
+inline Sizes sizes(int N, int Hq, int Hkv, int n_prefix, int max_pages, int sms) {
+    Sizes s;
+    s.ctas = n_prefix < max_pages ? kPerSm * sms : 0;
+    s.items = (size_t)N * Hkv;
+    s.own = s.ctas > 0 ? (s.ctas + s.items) * (Hq / Hkv) : 0;
+    s.chunk = prefix_chunk(N, Hq / Hkv, Hkv, n_prefix, sms);
+    s.n_chunks = ceil_div(n_prefix, s.chunk);
+    s.pre = (size_t)N * Hq * s.n_chunks;
+    return s;
 }
 
 static int sm_count(int* out) {
@@ -589,15 +793,21 @@ static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st)
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
-    const long items = (long)a.n_chunks * a.Hkv * a.groups + (long)a.max_split * a.Hkv * a.N;
+    const long items = (long)a.n_chunks * a.Hkv * a.groups + a.ctas;
     LF_CHECK_ARG(items <= 2147483647L, "q4 decode: grid limits exceeded");
-    if (items > 0) {
-        decode_kernel<D><<<(unsigned)items, kThreads, Smem<D>::kBytes, st>>>(a);
-        const int e = launch_status("q4 decode");
-        if (e != LF_OK) return e;
-    }
-    const long rows = (long)a.N * a.Hq;
-    combine_kernel<D><<<(unsigned)ceil_div(rows, kWarps), kThreads, 0, st>>>(a, o, lse);
+    decode_kernel<D><<<(unsigned)items, kThreads, Smem<D>::kBytes, st>>>(a);
+    const int e = launch_status("q4 decode");
+    if (e != LF_OK) return e;
+    cudaLaunchConfig_t cfg = {};               // launched while the first kernel still runs; it waits itself
+    cfg.gridDim = dim3((unsigned)ceil_div((long)a.N * a.Hq, kWarps));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<D>, a, o, lse));
     return launch_status("q4 decode combine");
 }
 
@@ -606,33 +816,17 @@ static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st)
 
 using namespace lf;
 
-extern "C" int lf_q4_decode_default_split(int num_seqs, int num_kv_heads, int max_pages,
-                                          int num_prefix_pages, int sm_count, int* pages_per_split) {
-    LF_CHECK_ARG(pages_per_split != nullptr, "q4 decode split: out pointer is null");
-    LF_CHECK_ARG(num_seqs >= 0 && num_kv_heads > 0 && max_pages > 0 && num_prefix_pages >= 0 &&
-                     num_prefix_pages <= max_pages,
-                 "q4 decode split: bad arguments");
+extern "C" int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                                           int max_pages, int num_prefix_pages, int sm_count, size_t* bytes) {
+    LF_CHECK_ARG(bytes != nullptr, "q4 decode: bytes is null");
+    LF_CHECK_ARG(num_seqs >= 0 && num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0 &&
+                     head_dim > 0 && max_pages > 0 && num_prefix_pages >= 0 && num_prefix_pages <= max_pages,
+                 "q4 decode: bad workspace arguments");
     if (sm_count <= 0) {
         const int rc = q4::sm_count(&sm_count);
         if (rc != LF_OK) return rc;
     }
-    // Pages are split until there are about eight items an SM, down to one page for each warp.
-    const long own = max_pages - num_prefix_pages;
-    int pps = 128;
-    while (pps > 4 && (long)num_seqs * num_kv_heads * ((own + pps - 1) / pps) < 8L * sm_count) pps /= 2;
-    *pages_per_split = pps;
-    clear_error();
-    return LF_OK;
-}
-
-extern "C" int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int head_dim, int max_pages,
-                                           int pages_per_split, int num_prefix_pages, size_t* bytes) {
-    LF_CHECK_ARG(bytes != nullptr, "q4 decode: bytes is null");
-    LF_CHECK_ARG(num_seqs >= 0 && num_q_heads > 0 && head_dim > 0 && max_pages > 0 && pages_per_split > 0 &&
-                     num_prefix_pages >= 0 && num_prefix_pages <= max_pages,
-                 "q4 decode: bad workspace arguments");
-    *bytes = (size_t)num_seqs * num_q_heads * q4::slots_bound(max_pages, num_prefix_pages, pages_per_split) *
-             ((size_t)head_dim * sizeof(float) + sizeof(float2));
+    *bytes = q4::sizes(num_seqs, num_q_heads, num_kv_heads, num_prefix_pages, max_pages, sm_count).bytes(head_dim);
     clear_error();
     return LF_OK;
 }
@@ -640,8 +834,8 @@ extern "C" int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int he
 extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32_t* block_table,
                                 const int32_t* seq_lens, int num_prefix_pages, lf_bf16* o, float* lse,
                                 void* workspace, size_t workspace_bytes, int num_seqs, int num_q_heads,
-                                int num_kv_heads, int head_dim, int num_pages, int max_pages,
-                                int pages_per_split, float scale, void* stream) {
+                                int num_kv_heads, int head_dim, int num_pages, int max_pages, float scale,
+                                int sm_count, void* stream) {
     LF_CHECK_ARG(num_seqs >= 0, "q4 decode: negative sizes");
     if (num_seqs == 0) { clear_error(); return LF_OK; }
     LF_CHECK_ARG(q && pages && block_table && seq_lens && o && workspace, "q4 decode: null pointer argument");
@@ -652,22 +846,28 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
                  "q4 decode: need Hq a multiple of Hkv");
     const int G = num_q_heads / num_kv_heads;
     LF_CHECK_ARG(G == 1 || G == 2 || G == 4 || G == 8, "q4 decode: Hq/Hkv must be 1, 2, 4 or 8 (got %d)", G);
-    LF_CHECK_ARG(num_pages > 0 && max_pages > 0 && max_pages <= (1 << 26) && pages_per_split > 0,
-                 "q4 decode: num_pages, max_pages and pages_per_split must be > 0");
+    LF_CHECK_ARG(num_pages > 0 && max_pages > 0 && max_pages <= (1 << 26),
+                 "q4 decode: num_pages and max_pages must be > 0 (at most 2^26 pages a session)");
+    LF_CHECK_ARG((long)num_seqs * num_q_heads <= (1L << 30), "q4 decode: too many sessions");
     LF_CHECK_ARG(num_prefix_pages >= 0 && num_prefix_pages <= max_pages,
                  "q4 decode: num_prefix_pages out of range");
-    size_t need = 0;
-    lf_q4_decode_workspace_size(num_seqs, num_q_heads, head_dim, max_pages, pages_per_split,
-                                num_prefix_pages, &need);
-    LF_CHECK_ARG(workspace_bytes >= need, "q4 decode: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
-    int sms = 0;
-    const int rc = q4::sm_count(&sms);
-    if (rc != LF_OK) return rc;
+    if (sm_count <= 0) {
+        const int rc = q4::sm_count(&sm_count);
+        if (rc != LF_OK) return rc;
+    }
+    const q4::Sizes z = q4::sizes(num_seqs, num_q_heads, num_kv_heads, num_prefix_pages, max_pages, sm_count);
+    LF_CHECK_ARG(workspace_bytes >= z.bytes(head_dim), "q4 decode: workspace too small (%zu < %zu bytes)",
+                 workspace_bytes, z.bytes(head_dim));
     q4::DecodeArgs a{};
     a.q = q;
     a.pages = static_cast<const uint8_t*>(pages);
     a.bt = block_table;
     a.lens = seq_lens;
+    a.own_o = static_cast<float*>(workspace);
+    a.pre_o = a.own_o + z.own * head_dim;
+    a.own_ml = reinterpret_cast<float2*>(a.pre_o + z.pre * head_dim);
+    a.pre_ml = a.own_ml + z.own;
+    a.span = reinterpret_cast<int2*>(a.pre_ml + z.pre);
     a.N = num_seqs;
     a.Hq = num_q_heads;
     a.Hkv = num_kv_heads;
@@ -675,15 +875,12 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
     a.num_pages = num_pages;
     a.max_pages = max_pages;
     a.n_prefix = num_prefix_pages;
-    a.chunk = q4::prefix_chunk(num_seqs, G, num_kv_heads, num_prefix_pages, sms);
-    a.n_chunks = q4::ceil_div(num_prefix_pages, a.chunk);
+    a.chunk = z.chunk;
+    a.n_chunks = z.n_chunks;
     a.groups = q4::ceil_div(num_seqs, q4::kWarps * (8 / G));
-    a.pps = pages_per_split;
-    a.max_split = q4::own_splits(max_pages, num_prefix_pages, pages_per_split);
-    a.n_slots = a.max_split + a.n_chunks;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)num_seqs * num_q_heads * a.n_slots * head_dim);
-    a.qscale = scale * kLog2e;
+    a.ctas = z.ctas;
+    a.qscale = fabsf(scale) * kLog2e;
+    a.flip = scale < 0.f ? 0x80008000u : 0u;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return head_dim == 128 ? q4::launch<128>(a, o, lse, st) : q4::launch<64>(a, o, lse, st);
 }

@@ -119,16 +119,15 @@ class QuantKVPool(KVPool):
     # -- attention --------------------------------------------------------------------------------
     def decode_workspace(self, n: int, num_q_heads: int, width: int,
                          num_prefix_pages: int = 0) -> Tuple[int, int]:
-        pps = att.default_pages_per_split_q4(n, self.num_kv_heads, width, num_prefix_pages)
-        return pps, att.decode_q4_workspace_bytes(n, num_q_heads, self.head_dim, width, pps,
-                                                  num_prefix_pages)
+        return 0, att.decode_q4_workspace_bytes(n, num_q_heads, self.num_kv_heads, self.head_dim, width,
+                                                num_prefix_pages)
 
     def attend_decode(self, q: torch.Tensor, layer: int, table: torch.Tensor, lens: torch.Tensor,
                       num_prefix_pages: int = 0, pages_per_split: Optional[int] = None,
                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        # the decode cuts the pages itself: no split size
         return att.paged_decode_q4(q, self.pages[layer], table, lens,
-                                   num_prefix_pages=num_prefix_pages,
-                                   pages_per_split=pages_per_split, workspace=workspace)
+                                   num_prefix_pages=num_prefix_pages, workspace=workspace)
 
     def prefill_buffers(self, lengths: Sequence[int], num_prefix_pages: int = 0):
         total = num_prefix_pages + sum(max(0, -(-int(n) // LF_PAGE_SIZE) - num_prefix_pages)

@@ -54,7 +54,7 @@ def table_for(lens, npre=0, gen=None, width=None):
     return table, max(1, n_ids)
 
 
-def check_decode(lens, Hq, Hkv, D, npre=0, pps=None, scale=None, width=None, seed=0, spoil=False):
+def check_decode(lens, Hq, Hkv, D, npre=0, scale=None, width=None, seed=0, spoil=False):
     gen = torch.Generator().manual_seed(seed + sum(lens) + Hq)
     table, P = table_for(lens, npre, gen, width)
     pages = random_pages(gen, P, Hkv, D)
@@ -67,7 +67,7 @@ def check_decode(lens, Hq, Hkv, D, npre=0, pps=None, scale=None, width=None, see
     q = torch.randn(len(lens), Hq, D, generator=gen).bfloat16()
     o, lse = att.paged_decode_q4(q.cuda(), pages.cuda(), table.cuda(),
                                  torch.tensor(lens, dtype=torch.int32).cuda(), num_prefix_pages=npre,
-                                 scale=scale, pages_per_split=pps, return_lse=True)
+                                 scale=scale, return_lse=True)
     ro, rl, to, tl = q4.decode(q, pages, table, lens, scale if scale is not None else D ** -0.5)
     err = (o.double().cpu() - ro).abs()
     assert bool((err <= to).all()), (err / to.clamp_min(1e-30)).max()
@@ -83,9 +83,11 @@ def test_decode_matches_the_oracle(Hq, Hkv, D):
     check_decode([0, 1, 15, 16, 17, 333, 64], Hq, Hkv, D, spoil=True)
 
 
-@pytest.mark.parametrize("pps", [1, 3, 4, 7, 64])
-def test_decode_split_sizes(pps):
-    check_decode([513, 1, 0, 1000], 8, 2, 128, pps=pps)
+@pytest.mark.parametrize("lens", [[513, 1, 0, 1000], [0, 0, 0], [0, 0, 40, 0, 0, 3000, 0, 2, 0], [16] * 300,
+                                  [1 + (i * 37) % 700 for i in range(150)], [33] * 129 + [0] * 140 + [5000]])
+def test_decode_ranges_over_sessions_of_all_lengths(lens):
+    check_decode(lens, 4, 2, 64, spoil=True)
+    check_decode(lens[:40], 8, 1, 128)
 
 
 def test_decode_one_long_session_and_a_wide_table():
@@ -310,13 +312,13 @@ def test_decode_repeats_bit_for_bit_and_takes_a_given_workspace():
     table, P = table_for(lens, 1, gen)
     pages, q = random_pages(gen, P, 2, 128).cuda(), torch.randn(4, 8, 128, generator=gen).bfloat16().cuda()
     lens_d = torch.tensor(lens, dtype=torch.int32).cuda()
-    need = att.decode_q4_workspace_bytes(4, 8, 128, table.shape[1], 4, 1)
+    need = att.decode_q4_workspace_bytes(4, 8, 2, 128, table.shape[1], 1)
     ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")       # NaN bits
     out = torch.full_like(q, math.nan)
-    a = att.paged_decode_q4(q, pages, table.cuda(), lens_d, 1, pages_per_split=4, workspace=ws, out=out)
+    a = att.paged_decode_q4(q, pages, table.cuda(), lens_d, 1, workspace=ws, out=out)
     assert a.data_ptr() == out.data_ptr()
     for _ in range(3):
-        assert torch.equal(a, att.paged_decode_q4(q, pages, table.cuda(), lens_d, 1, pages_per_split=4))
+        assert torch.equal(a, att.paged_decode_q4(q, pages, table.cuda(), lens_d, 1))
 
 
 # -- the pool ---------------------------------------------------------------------------------------

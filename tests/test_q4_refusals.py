@@ -48,13 +48,14 @@ def test_tensors_off_the_gpu_and_of_other_types_are_refused():
     (dict(head_dim=96), b"head_dim"), (dict(num_q_heads=6), b"1, 2, 4 or 8"), (dict(num_q_heads=5), b"multiple"),
     (dict(q=P + 2), b"aligned"), (dict(pages=P + 8), b"aligned"), (dict(q=None), b"null"),
     (dict(num_prefix_pages=5), b"num_prefix_pages"), (dict(num_prefix_pages=-1), b"num_prefix_pages"),
-    (dict(workspace_bytes=16), b"workspace"), (dict(pages_per_split=0), b"pages_per_split"),
+    (dict(workspace_bytes=16), b"workspace"), (dict(max_pages=1 << 27), b"max_pages"),
+    (dict(num_seqs=1 << 29), b"too many"),
     (dict(num_seqs=-1), b"negative"), (dict(max_pages=0), b"max_pages"),
 ])
 def test_decode_arguments(change, words):
     a = dict(q=P, pages=P, block_table=P, seq_lens=P, num_prefix_pages=0, o=P, lse=None, workspace=P,
              workspace_bytes=1 << 30, num_seqs=2, num_q_heads=4, num_kv_heads=2, head_dim=128, num_pages=8,
-             max_pages=4, pages_per_split=4, scale=1.0, stream=None)
+             max_pages=4, scale=1.0, sm_count=148, stream=None)
     a.update(change)
     lib = _lib.lib()
     assert lib.lf_q4_decode_fwd(*a.values()) == _lib.LF_EINVAL
@@ -94,7 +95,7 @@ def test_expand_arguments(change, words):
 def test_empty_calls_do_nothing():
     lib = _lib.lib()
     assert lib.lf_q4_expand(None, None, None, 0, None, None, None, 0, 1, 64, 1, 1, 0, None) == _lib.LF_OK
-    assert lib.lf_q4_decode_fwd(None, None, None, None, 0, None, None, None, 0, 0, 4, 2, 128, 1, 1, 1, 1.0,
+    assert lib.lf_q4_decode_fwd(None, None, None, None, 0, None, None, None, 0, 0, 4, 2, 128, 1, 1, 1.0, 148,
                                 None) == _lib.LF_OK
 
 
@@ -111,9 +112,8 @@ def test_fork_and_pool_arguments():
         QuantKVPool(1, 1, 64, 64, device="cpu")
 
 
-def test_split_sizes_and_workspace():
-    n = ctypes.c_int(0)
-    for seqs, hkv, pages, npre in [(1, 8, 49, 0), (64, 8, 1024, 0), (256, 8, 119, 0), (1, 1, 1, 0), (4, 2, 50, 50)]:
-        _lib.call("lf_q4_decode_default_split", seqs, hkv, pages, npre, 148, ctypes.byref(n))
-        assert 4 <= n.value <= 128 and n.value & (n.value - 1) == 0
-    assert att.decode_q4_workspace_bytes(3, 4, 128, 10, 4) == 3 * 4 * 3 * (128 * 4 + 8)
+def test_workspace():
+    """(444 ranges + N Hkv items) x G partials, prefix chunks x N Hq partials, one span per item."""
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 0, 148) == (444 + 6) * 2 * (512 + 8) + 6 * 8
+    # a prefix of 16 pages or less is one chunk; no own pages, no ranges
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 10, 148) == 3 * 4 * (512 + 8) + 6 * 8
