@@ -377,8 +377,8 @@ int lf_pool_unregister_all(const lf_pool_meta* m, const lf_prefix_registry* r, v
  * decode and the prefill read of the same paged cache at 4.5 bits a value, on the pool's block
  * tables.  A group is 64 dims of one token of one KV head: with low = min x and
  * s = bf16((max - low) / 15), a value is held as n = rint((x - low) / s), 0..15 (0 when s is 0),
- * and stands for n * s + low.  A group that holds a NaN or an infinity, or whose range overflows
- * fp32, reads back as NaN.  A page of 16 tokens of one KV head is one block of 18 * D bytes
+ * and stands for n * s + low.  A group that holds a NaN or an infinity, or whose values span 2^60
+ * or more, reads back as NaN.  A page of 16 tokens of one KV head is one block of 18 * D bytes
  * (D = 64 or 128), pages [P][Hkv][18 * D]; byte offsets inside a block, NG = D / 64:
  *   K code of (token t, dim d)  32-bit word at  t*32*NG + (d%64/16)*8*NG + (d/64)*8 + (d%16/8)*4,
  *                               bits 4*(e/2) + 16*(e%2), e = d % 8

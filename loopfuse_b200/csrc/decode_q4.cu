@@ -4,11 +4,16 @@
 // The codes are never expanded to values.  With the scales taken out of the products,
 //   q . k_t = sum over groups of  s_t (q . n_t) + b_t sum(q)
 //   o       = sum over tokens of  (p_t s_t) n_t + p_t b_t,
-// the matrix products run on the codes themselves: (word >> 4 i) & 0x000F000F, or-ed with 0x4300
-// twice, is a pair of bf16 operands 128 + n, exact, one shift and one logic instruction a pair.  The
-// 128 goes into the bias of the scores (b - 128 s), and is removed from the output with a product
-// by the constant -136 on the same bf16 probabilities: what the rounding of p s to bf16 multiplies
-// is then n - 8, centred in the range, and b + 8 s is applied with unrounded fp32 probabilities.
+// the matrix products run on the codes themselves.  A bf16 bit pattern below 256 stands for
+// 2^-133 times the pattern: the subnormals and the first normals share their step.  So a code of bits
+// 0..3 is n 2^-133 as it stands, one of bits 4..7 is 16 n 2^-133, and the two pairs of a word's low
+// bytes cost one mask each, those of its high bytes one shift more; the products are exact.  The
+// powers of two are balanced by 2^64 in the other operand (q, or p s, which therefore has to stay
+// below 2^63: the append stores no larger scale) and removed where sums are used; the factor 16 goes
+// into q, or out of every second output dim at the end.  Probabilities times scales are
+// rounded to bf16; a product of the same rounded values with the constant -8 is added to o and
+// b + 8 s applied with unrounded probabilities, so that the rounding (2^-9 on average) multiplies
+// n - 8, centred in the range, not n.
 //
 // As in the bf16 decode a page's 16 tokens are the M rows of m16n8k16:
 //   S^T [16 tokens x 8 columns]  = codes_k [16 x D] . q^T [D x 8]       per group, D/16 MMAs
@@ -45,7 +50,7 @@ using decode::kThreads;
 using decode::kWarps;
 
 constexpr int kUnit = 2;                       // pages of a barrier, a softmax step, a buffer
-constexpr int kStages = 3;                     // units in flight per warp
+constexpr int kStages = 2;                     // units in flight per warp
 constexpr int kSlots = kWarps * kStages;       // buffers of a CTA
 constexpr int kPerSm = 3;                      // resident CTAs of an SM
 constexpr int kMinUnits = kWarps;              // units of a range
@@ -61,7 +66,7 @@ struct DecodeArgs {
     int N, Hq, Hkv, G, num_pages, max_pages;
     int n_prefix, chunk, n_chunks, groups;     // shared prefix: pages, pages a chunk, chunks, session groups
     int ctas;                                  // ranges of the own pages
-    float qscale;                              // |scale| * log2(e)
+    float qscale;                              // |scale| * log2(e) * 2^69
     uint32_t flip;                             // sign bits of a negative scale
 };
 
@@ -115,22 +120,28 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Codes 4 i .. 4 i + 3 of both halves of a word as the bf16 pair 128 + n.
+// Codes i of both halves of a word, as the bf16 pair n 2^-133 (i even) or 16 n 2^-133 (i odd).
 __device__ __forceinline__ uint32_t codes(uint32_t w, int i) {
-    uint32_t r;                                // (w & mask) | bits: one instruction
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> (4 * i)), "n"(0x000F000F), "r"(0x43004300u));
+    return (i < 2 ? w : w >> 8) & (i % 2 == 0 ? 0x000F000Fu : 0x00F000F0u);
+}
+constexpr float kUp = 18446744073709551616.f;            // 2^64, in q and in p s
+constexpr float kDown = 590295810358705651712.f;         // 2^69 = 2^133 / 2^64
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
 // A warp's attention state: B blocks of 8 columns (query rows), of which this lane holds 2c and
-// 2c + 1.  Scores are kept unscaled (q's sign carries the scale's), maxima too.
+// 2c + 1.  Scores and maxima are kept as q . k 2^-69 (q's sign carries the scale's).
 template <int D, int B>
 struct State {
     static constexpr int NG = Fmt<D>::NG;
-    uint32_t qb[B][NG][4][2];                  // Q^T operand, column g
-    float qsum[B][NG][2];                      // sums of columns 2c, 2c + 1 over each group
-    float o[B][NG][4][4];                      // O^T: m-tile (16 dims) x 4
-    float corr[B][NG][4];                      // -136 sum(bf16(p s)): rows are equal
+    uint32_t qb[B][NG][4][2];                  // Q^T operand, column g: q 2^64, q 2^60
+    float qsum[B][NG][2];                      // sums of columns 2c, 2c + 1 over each group, 2^-69
+    float o[B][NG][4][4];                      // O^T: m-tile (16 dims) x 4; 2^-69, 2^-65 in rows g + 8
+    float corr[B][NG][4];                      // -8 sum(bf16(p s)): the same in every m-tile
     float bias[B][NG][2];                      // this lane's share of sum p (b + 8 s)
     float m[B][2], l[B][2];
 
@@ -148,11 +159,12 @@ struct State {
             float part = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                qb[b][gr][k / 2][k % 2] = w[k] ^ flip;
+                qb[b][gr][k / 2][k % 2] = mul_bf16x2(w[k] ^ flip, k % 2 == 0 ? 0x5F805F80u : 0x5D805D80u);
                 part += bf16lo_to_f32(w[k] ^ flip) + bf16hi_to_f32(w[k] ^ flip);
             }
             part += __shfl_xor_sync(0xffffffffu, part, 1);
             part += __shfl_xor_sync(0xffffffffu, part, 2);
+            part *= 1.f / kDown;
             qsum[b][gr][0] = __shfl_sync(0xffffffffu, part, 8 * c);
             qsum[b][gr][1] = __shfl_sync(0xffffffffu, part, 8 * c + 4);
             bias[b][gr][0] = bias[b][gr][1] = 0.f;
@@ -196,10 +208,9 @@ struct State {
                         const uint32_t a2 = codes(ka[2 * gr + w], 2 * k + 1), a3 = codes(kb[2 * gr + w], 2 * k + 1);
 #pragma unroll
                         for (int b = 0; b < B; ++b) {
-                            if (w == 0 && k == 0) {    // the accumulators start from -128 sum(q)
-                                const float q0 = -128.f * qsum[b][gr][0], q1 = -128.f * qsum[b][gr][1];
-                                const float start[4] = {q0, q1, q0, q1};
-                                mma(acc[b], a0, a1, a2, a3, qb[b][gr][0][0], qb[b][gr][0][1], start);
+                            if (w == 0 && k == 0) {
+                                const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma(acc[b], a0, a1, a2, a3, qb[b][gr][0][0], qb[b][gr][0][1], zero);
                             } else {
                                 mma(acc[b], a0, a1, a2, a3, qb[b][gr][2 * w + k][0], qb[b][gr][2 * w + k][1], acc[b]);
                             }
@@ -303,11 +314,12 @@ struct State {
                 const float sa = bf16lo_to_f32(vp[pg][0][gr]), sb = bf16lo_to_f32(vp[pg][1][gr]);
                 const float ba = fmaf(8.f, sa, bf16hi_to_f32(vp[pg][0][gr]));
                 const float bb = fmaf(8.f, sb, bf16hi_to_f32(vp[pg][1][gr]));
+                const float ua = sa * kUp, ub = sb * kUp;
                 uint32_t b0[B], b1[B];
 #pragma unroll
                 for (int b = 0; b < B; ++b) {
                     const float(&e)[4] = s[b][pg];
-                    float p[4] = {e[0] * sa, e[1] * sa, e[2] * sb, e[3] * sb};
+                    float p[4] = {e[0] * ua, e[1] * ua, e[2] * ub, e[3] * ub};
                     if (kMasked) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) p[j] = keep[b][pg][j] ? p[j] : 0.f;
@@ -319,7 +331,8 @@ struct State {
                     }
                     b0[b] = movm_t(pack_bf16x2(p[0], p[1]));
                     b1[b] = movm_t(pack_bf16x2(p[2], p[3]));
-                    mma(corr[b][gr], 0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u, b0[b], b1[b], corr[b][gr]);   // bf16 -136
+                    // -8 2^-133 in rows g, -128 2^-133 in rows g + 8
+                    mma(corr[b][gr], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0[b], b1[b], corr[b][gr]);
                 }
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
@@ -354,7 +367,8 @@ struct State {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[b][gr][k][j] += corr[b][gr][j & 1] + bias[b][gr][j & 1];
+                    for (int j = 0; j < 4; ++j)
+                        o[b][gr][k][j] = fmaf(o[b][gr][k][j] + corr[b][gr][j], j < 2 ? kDown : kDown / 16.f, bias[b][gr][j & 1]);
         }
     }
 };
@@ -879,7 +893,7 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
     a.n_chunks = z.n_chunks;
     a.groups = q4::ceil_div(num_seqs, q4::kWarps * (8 / G));
     a.ctas = z.ctas;
-    a.qscale = fabsf(scale) * kLog2e;
+    a.qscale = fabsf(scale) * kLog2e * q4::kDown;
     a.flip = scale < 0.f ? 0x80008000u : 0u;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return head_dim == 128 ? q4::launch<128>(a, o, lse, st) : q4::launch<64>(a, o, lse, st);

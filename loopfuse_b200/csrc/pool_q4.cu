@@ -119,7 +119,7 @@ __global__ void append_kernel(const AppendArgs a) {
             const float span = __fsub_rn(mx, mn);
             uint32_t par = 0x7FC07FC0u;                // NaN, NaN
             uint32_t n[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (((nans >> (lane & 24)) & 0xFFu) == 0 && span < INFINITY) {
+            if (((nans >> (lane & 24)) & 0xFFu) == 0 && span < kMaxSpan) {
                 par = pack_bf16x2(__fdiv_rn(span, 15.f), mn);
                 const float s = bf16lo_to_f32(par);
                 if (s > 0.f) {

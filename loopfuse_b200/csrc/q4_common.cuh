@@ -4,7 +4,8 @@
 // A group is 64 dims of one token of one KV head.  With low = min x and s = bf16((max - low) / 15),
 // a value is held as n = rint((x - low) / s) in 0..15 (0 when s is 0) and stands for n * s + low;
 // low is a bf16 input value, so it is held exactly.  4.5 bits a value.  A group with a NaN or an
-// infinity, or whose range overflows fp32, is stored with s = low = NaN and reads back as NaN.
+// infinity, or whose values span 2^60 or more (the decode multiplies scales by 2^64), is stored with
+// s = low = NaN and reads back as NaN.
 //
 // A page of one KV head is one block of 18 * D bytes (1152 or 2304: a multiple of 128):
 //   K codes  [token 16][c 4][group D/64][word 2]           32-bit words: 8 dims of a token each;
@@ -24,6 +25,7 @@ namespace q4 {
 
 constexpr int kPage = LF_PAGE_SIZE;
 constexpr int kGroup = 64;
+constexpr float kMaxSpan = 1152921504606846976.f;      // 2^60
 
 template <int D>
 struct Fmt {

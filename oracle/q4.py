@@ -20,8 +20,8 @@ def quantise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]
     """``(codes int64 [..., D], s [..., D/64], low [..., D/64])`` (float64) of ``x [..., D]``."""
     g = x.double().unflatten(-1, (-1, GROUP))
     low, high = g.amin(-1), g.amax(-1)
-    span = (high - low).float()                       # overflows to inf where fp32 does
-    bad = ~torch.isfinite(span) | torch.isnan(g).any(-1)
+    span = (high - low).float()
+    bad = ~(span < 2.0 ** 60) | torch.isnan(g).any(-1)
     s = (span.double() / 15).to(torch.bfloat16).double()
     n = ((g - low[..., None]) / torch.where(s > 0, s, torch.ones_like(s))[..., None]).round()
     n = torch.where((s > 0)[..., None] & ~bad[..., None], n.clamp(0, 15), torch.zeros_like(n))
@@ -80,8 +80,8 @@ def decode(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: List
 
     The bound counts: o's rounding to bf16 (half a step, 2^-8); the rounding of ``p s`` to bf16,
     which multiplies ``n - 8`` (2^-8 of ``sum p s |n - 8|``); the scores' fp32 sums of products
-    ``q (128 + n) s``, five additions of magnitude at most ``143 s sum |q|`` with 2^-22 each (truncating
-    accumulators); fp32 exponentials and sums (2^-20 of ``sum p |v|``)."""
+    ``q n s`` and of ``b sum(q)``, seven additions of magnitude at most ``(15 s + |b|) sum |q|`` with
+    2^-22 each (truncating accumulators); fp32 exponentials and sums (2^-20 of ``sum p |v|``)."""
     N, Hq, D = q.shape
     Hkv = pages.shape[1]
     G, ng = Hq // Hkv, D // GROUP
@@ -93,13 +93,14 @@ def decode(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: List
             continue
         blk = pages[table[i, :-(-L // PAGE)].long()]
         k, v, spread = (x.transpose(1, 2).reshape(-1, Hkv, D)[:L] for x in unpack(blk))
-        s_k = blk[..., 16 * D:].contiguous().view(torch.bfloat16).double().unflatten(-1, (PAGE, 2, ng, 2))[..., 0, :, 0]
-        s_k = s_k.transpose(1, 2).reshape(-1, Hkv, ng)[:L]
+        par = blk[..., 16 * D:].contiguous().view(torch.bfloat16).double().unflatten(-1, (PAGE, 2, ng, 2))[..., 0, :, :]
+        par = par.transpose(1, 2).reshape(-1, Hkv, ng, 2)[:L]
+        most = 15 * par[..., 0] + par[..., 1].abs()
         for h in range(Hq):
             x = q[i, h].double()
             sc = scale * (k[:, h // G] @ x)
-            size = (s_k[:, h // G] * x.abs().unflatten(0, (ng, GROUP)).sum(-1)).sum(-1).max()
-            delta = float(abs(scale) * 5 * 143 * 2 ** -22 * size) + 2 ** -21
+            size = (most[:, h // G] * x.abs().unflatten(0, (ng, GROUP)).sum(-1)).sum(-1).max()
+            delta = float(abs(scale) * 7 * 2 ** -22 * size) + 2 ** -21
             lse[i, h] = torch.logsumexp(sc, 0)
             p = torch.softmax(sc, 0)
             o[i, h] = p @ v[:, h // G]
