@@ -21,17 +21,19 @@
 // A warp's lane holds 16-byte vectors of codes that are its operand registers (no ldmatrix, no
 // bank conflicts); a page of one KV head is one block of 18 D bytes, brought in by one bulk copy.
 //
-// Work of CTAs of four warps, one launch:
+// Work:
 //   own     the sessions' own pages, two at a time (a unit), in the order (session, KV head, unit),
-//           are cut into equal ranges, one per resident CTA, so that long and short sessions fill
-//           the chip alike and a CTA starts up once: its warps take a range's units in turn, each
-//           with a ring of kStages units whose copies run on across sessions and heads.  The
-//           columns are the GQA group's heads.
-//   prefix  (chunk, KV head, group of 4 * 8/G sessions): the pages of a shared prefix; the 8
-//           columns of a warp are G heads of 8/G sessions, and the four warps use the same staged
-//           pages for different sessions, so that a prefix page is read once per 32 columns.
+//           are cut into equal ranges, one per resident warp, so that long and short sessions fill
+//           the chip alike and a warp starts up once.  A warp works alone, with a ring of kStages
+//           units whose copies run on across heads and sessions (the queries of a head come with
+//           its first unit).  The columns are the GQA group's heads.
+//   prefix  (chunk, KV head, group of 4 * 8/G sessions): the pages of a shared prefix; the 8 columns of
+//           a warp are G heads of 8/G sessions, and the four warps use the same staged pages, so
+//           that a prefix page is read once per 32 columns.  A kernel of its own, next to which the
+//           own one starts.  (Two blocks of 8 columns a warp, unpacking a page once for both: 227
+//           registers and half the warps, 65.6 against 57.6 us with 64 sessions on 4096 tokens.)
 // Every piece writes unnormalised fp32 partials (o, max, sum); a range's piece of item (session, KV
-// head) is partial number CTA + item, which no two pieces share as both grow along the ranges.
+// head) is partial number range + item, which no two pieces share as both grow along the ranges.
 // combine merges a row's partials, in order.
 //
 // Every barrier wait is bounded (site 221 in the device error word); a warp that gives up stops
@@ -49,23 +51,24 @@ using decode::checked_page;
 using decode::kThreads;
 using decode::kWarps;
 
-constexpr int kUnit = 2;                       // pages of a barrier, a softmax step, a buffer
-constexpr int kStages = 2;                     // units in flight per warp
-constexpr int kSlots = kWarps * kStages;       // buffers of a CTA
-constexpr int kPerSm = 3;                      // resident CTAs of an SM
-constexpr int kMinUnits = kWarps;              // units of a range
+constexpr int kUnit = 2;                       // own: pages of a barrier, a softmax step, a buffer
+constexpr int kStages = 2;                     // own: units in flight per warp
+constexpr int kPerSm = 3;                      // own: resident CTAs of an SM
+constexpr int kMinUnits = 2;                   // own: units of a range
+constexpr int kBlocks = 1;                     // prefix: blocks of 8 columns of a warp
+constexpr int kRing = 16;                      // prefix: pages staged in a CTA, in two halves
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct DecodeArgs {
     const uint16_t* q;
     const uint8_t* pages;
     const int32_t *bt, *lens;
-    float *own_o, *pre_o;                      // [ctas + N * Hkv][G][D]; [N][Hq][n_chunks][D]
+    float *own_o, *pre_o;                      // [ranges + N * Hkv][G][D]; [N][Hq][n_chunks][D]
     float2 *own_ml, *pre_ml;                   // (max, sum) of each
-    int2* span;                                // [N * Hkv] first and last CTA of an item
+    int2* span;                                // [N * Hkv] first and last range of an item
     int N, Hq, Hkv, G, num_pages, max_pages;
     int n_prefix, chunk, n_chunks, groups;     // shared prefix: pages, pages a chunk, chunks, session groups
-    int ctas;                                  // ranges of the own pages
+    int ranges;                                // of the own pages: one per warp
     float qscale;                              // |scale| * log2(e) * 2^69
     uint32_t flip;                             // sign bits of a negative scale
 };
@@ -79,12 +82,18 @@ __device__ __forceinline__ int own_units(const DecodeArgs& a, int n) {
     return own > 0 ? (own + kUnit - 1) / kUnit : 0;
 }
 
+// Waits for a phase; false after kWaitNs.
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
     if (sm100::mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = sm100::global_timer_ns();
     while (!sm100::mbar_try_wait(bar, parity))
         if (sm100::global_timer_ns() - t0 > kWaitNs) return false;
     return true;
+}
+// The same for a whole warp, the answer uniform; a phase that is there costs a poll and a vote.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, sm100::mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, wait_full(bar, parity));
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar,
@@ -135,7 +144,7 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 
 // A warp's attention state: B blocks of 8 columns (query rows), of which this lane holds 2c and
 // 2c + 1.  Scores and maxima are kept as q . k 2^-69 (q's sign carries the scale's).
-template <int D, int B>
+template <int D, int B, int U>
 struct State {
     static constexpr int NG = Fmt<D>::NG;
     uint32_t qb[B][NG][4][2];                  // Q^T operand, column g: q 2^64, q 2^60
@@ -179,16 +188,16 @@ struct State {
         l[b][0] = l[b][1] = 0.f;
     }
 
-    // Applies kUnit staged pages, tokens tok0 .. tok0 + 16 kUnit - 1; len[b] are the lengths of the
+    // Applies U staged pages, tokens tok0 .. tok0 + 16 U - 1; len[b] are the lengths of the
     // lane's columns.  kMasked: some token may be at or past a column's length.  Such tokens take no
     // part, whatever their codes and scales hold.
     template <bool kMasked>
     __device__ __forceinline__ void unit(uint32_t base, int tok0, const int (&len)[B][2], float qscale, int lane) {
         const int g = lane >> 2, c = lane & 3;
-        float s[B][kUnit][4];                  // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
-        uint32_t vp[kUnit][2][NG];             // V params of tokens g, g + 8
+        float s[B][U][4];                  // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
+        uint32_t vp[U][2][NG];             // V params of tokens g, g + 8
 #pragma unroll
-        for (int pg = 0; pg < kUnit; ++pg) {
+        for (int pg = 0; pg < U; ++pg) {
             const uint32_t blk = base + (uint32_t)(pg * Fmt<D>::kBlockBytes);
             uint32_t pa[2 * NG], pb[2 * NG], ka[2 * NG], kb[2 * NG];
             lds<2 * NG>(blk + Fmt<D>::kParOff + g * (8 * NG), pa);
@@ -239,12 +248,12 @@ struct State {
                 }
             }
         }
-        bool keep[B][kUnit][4];
+        bool keep[B][U][4];
         if (kMasked) {
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int pg = 0; pg < kUnit; ++pg)
+                for (int pg = 0; pg < U; ++pg)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         keep[b][pg][j] = tok0 + kPage * pg + g + 8 * (j / 2) < len[b][j % 2];
@@ -255,7 +264,7 @@ struct State {
         for (int b = 0; b < B; ++b) {
             float x0 = fmaxf(s[b][0][0], s[b][0][2]), x1 = fmaxf(s[b][0][1], s[b][0][3]);
 #pragma unroll
-            for (int pg = 1; pg < kUnit; ++pg) {
+            for (int pg = 1; pg < U; ++pg) {
                 x0 = fmaxf(x0, fmaxf(s[b][pg][0], s[b][pg][2]));
                 x1 = fmaxf(x1, fmaxf(s[b][pg][1], s[b][pg][3]));
             }
@@ -291,20 +300,20 @@ struct State {
             const float r0 = (kMasked && m[b][0] == -INFINITY) ? 0.f : m[b][0] * -qscale;
             const float r1 = (kMasked && m[b][1] == -INFINITY) ? 0.f : m[b][1] * -qscale;
 #pragma unroll
-            for (int pg = 0; pg < kUnit; ++pg)
+            for (int pg = 0; pg < U; ++pg)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float e = fast_exp2(fmaf(s[b][pg][j], qscale, (j & 1) ? r1 : r0));
                     s[b][pg][j] = !kMasked || keep[b][pg][j] ? e : 0.f;
                 }
 #pragma unroll
-            for (int pg = 0; pg < kUnit; ++pg) {
+            for (int pg = 0; pg < U; ++pg) {
                 l[b][0] += s[b][pg][0] + s[b][pg][2];
                 l[b][1] += s[b][pg][1] + s[b][pg][3];
             }
         }
 #pragma unroll
-        for (int pg = 0; pg < kUnit; ++pg) {
+        for (int pg = 0; pg < U; ++pg) {
             const uint32_t blk = base + (uint32_t)(pg * Fmt<D>::kBlockBytes) + Fmt<D>::kVOff;
             uint32_t va[2 * NG], vb[2 * NG];   // tokens 2c, 2c + 1 and 2c + 8, 2c + 9
             lds<2 * NG>(blk + lane * (8 * NG), va);
@@ -376,12 +385,13 @@ struct State {
 // Dim of accumulator row g of m-tile k of group gr (row g + 8 is the next dim).
 __device__ __forceinline__ int out_dim(int gr, int k, int g) { return gr * kGroup + 8 * g + 2 * k; }
 
+// -- own pages ----------------------------------------------------------------------------------------
 template <int D>
-struct Smem {
+struct OwnSmem {
     static constexpr int kUnitBytes = kUnit * Fmt<D>::kBlockBytes;
-    static constexpr int kRing = kSlots * kUnitBytes;
-    static constexpr int kMerge = kWarps * 8 * (D + 2) * 4;
-    static constexpr int kBytes = kRing + kMerge + 128;
+    static constexpr int kQ = 8 * D * 2;                   // queries of a KV head, at most 8 rows
+    static constexpr int kWarp = kStages * kUnitBytes + 2 * kQ;
+    static constexpr int kBytes = kWarps * kWarp + 128;
 };
 
 // Sum over the CTA's threads (every thread gets it).
@@ -397,15 +407,9 @@ __device__ __forceinline__ long cta_sum(long v, long* buf) {
     return r;
 }
 
-// Where a range starts: session n, the first of its units u_n in the flat order before the heads.
-struct Place {
-    long before;                               // units (of one head) of the sessions before n
-    int n;
-};
-
 // A run of units [j, j1) of (session n, KV head h), and how many units follow it in the range.
 struct Segment {
-    int n, h, j, j1, u;
+    int n, h, j, j1, u, L;
     long left;
     // Moves on to the next segment; false at the range's end.
     __device__ __forceinline__ bool next(const DecodeArgs& a) {
@@ -414,6 +418,7 @@ struct Segment {
             h = 0;
             do { u = own_units(a, ++n); } while (u == 0 && n < a.N);
             if (u == 0) return false;                            // (not met: units are left)
+            L = held(a, n);
         }
         j = 0;
         j1 = (int)min((long)u, left);
@@ -422,15 +427,21 @@ struct Segment {
     }
 };
 
-// The sessions' own pages: range `cta` of them.
 template <int D>
-__device__ __forceinline__ void own_range(const DecodeArgs& a, uint8_t* smem, uint64_t* bars, int cta) {
+__global__ void __launch_bounds__(kThreads, kPerSm) own_kernel(const DecodeArgs a) {
     using F = Fmt<D>;
-    constexpr int UB = Smem<D>::kUnitBytes;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    constexpr int UB = OwnSmem<D>::kUnitBytes;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    __shared__ __align__(8) uint64_t bars[kWarps * kStages];
     __shared__ long buf[kWarps];
-    __shared__ Place s_place;
-    const uint32_t ring = sm100::smem_addr(smem) + (uint32_t)(warp * kStages * UB);
+    __shared__ long s_before[kWarps];          // units of one head before session s_n[w]
+    __shared__ int s_n[kWarps];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // combine may be brought in
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    uint8_t* mem = smem + warp * OwnSmem<D>::kWarp;
+    const uint8_t* qbuf = mem + kStages * UB;
+    const uint32_t ring = sm100::smem_addr(mem), qring = ring + kStages * UB;
     const uint32_t bar = sm100::smem_addr(bars + warp * kStages);
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) sm100::mbar_init(bar + 8 * i, 1);
@@ -439,175 +450,171 @@ __device__ __forceinline__ void own_range(const DecodeArgs& a, uint8_t* smem, ui
     long mine = 0;
     for (int n = threadIdx.x; n < a.N; n += kThreads) mine += own_units(a, n);
     const long total = cta_sum(mine, buf) * a.Hkv;
-    const long share = max((total + a.ctas - 1) / a.ctas, (long)kMinUnits);
-    const long begin = cta * share;
-    if (begin >= total) return;
-    long before = 0;                                             // sessions, a CTA's width at a time
-    for (int n0 = 0;; n0 += kThreads) {                          // ends: begin < total
+    const long share = max((total + a.ranges - 1) / a.ranges, (long)kMinUnits);
+    const int range = blockIdx.x * kWarps + warp;
+    const long begin = range * share, cta_begin = (long)blockIdx.x * kWarps * share;
+    // Sessions where the CTA's ranges start, a CTA's width of sessions at a time.
+    const long cta_last = min(cta_begin + (kWarps - 1) * share, total - 1);
+    long before = 0;
+    for (int n0 = 0; n0 < a.N && cta_begin < total && before * a.Hkv <= cta_last; n0 += kThreads) {
         const int n = n0 + threadIdx.x;
         const int u = n < a.N ? own_units(a, n) : 0;
-        const long sum = cta_sum(u, buf);
-        if (begin >= (before + sum) * a.Hkv) {
-            before += sum;
-            continue;
-        }
-        long excl = u;                                           // exclusive prefix within the CTA
+        long incl = u;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const long o = __shfl_up_sync(0xffffffffu, excl, off);
-            if (lane >= off) excl += o;
+            const long o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
         }
-        if (lane == 31) buf[warp] = excl;
+        if (lane == 31) buf[warp] = incl;
         __syncthreads();
-        excl -= u;
+        long excl = before + incl - u;
         for (int w = 0; w < warp; ++w) excl += buf[w];
-        if (u > 0 && begin >= (before + excl) * a.Hkv && begin < (before + excl + u) * a.Hkv)
-            s_place = Place{before + excl, n};
+        for (int w = 0; w < kWarps; ++w) before += buf[w];
+        for (int w = 0; w < kWarps; ++w) {
+            const long at = cta_begin + w * share;
+            if (at >= excl * a.Hkv && at < (excl + u) * a.Hkv) {
+                s_before[w] = excl;
+                s_n[w] = n;
+            }
+        }
         __syncthreads();
-        break;
     }
-    Segment seg;                                                 // what the warps compute on
-    seg.n = s_place.n;
-    seg.u = own_units(a, seg.n);
-    {
-        const long in = begin - s_place.before * a.Hkv, len = min(share, total - begin);
-        seg.h = (int)(in / seg.u);
-        seg.j = (int)(in % seg.u);
-        seg.j1 = (int)min((long)seg.u, seg.j + len);
-        seg.left = len - (seg.j1 - seg.j);
-    }
-    // What this warp copies: a segment of its own that runs ahead.  Page ids of 16 of its units at a
-    // time, one page per lane (lane 2 i + p: page p of the i-th).
-    Segment pre = seg;
-    pre.j += warp;
-    bool more = true;
-    int ids = 0, ids_from = -1, ids_at = 0;                      // units ids_from + 4 i; next i
-    uint32_t issued = 0;
-    const uint64_t policy = sm100::l2_evict_first_policy();      // read once
-    auto issue = [&]() {                                         // warp-uniform: one unit, if any is left
-        while (more && pre.j >= pre.j1) {
-            more = pre.next(a);
-            pre.j = warp;
-            ids_from = -1;
+    if (begin < total) {
+        Segment seg;                                             // what the warp computes on
+        seg.n = s_n[warp];
+        seg.u = own_units(a, seg.n);
+        seg.L = held(a, seg.n);
+        {
+            const long in = begin - s_before[warp] * a.Hkv, len = min(share, total - begin);
+            seg.h = (int)(in / seg.u);
+            seg.j = (int)(in % seg.u);
+            seg.j1 = (int)min((long)seg.u, seg.j + len);
+            seg.left = len - (seg.j1 - seg.j);
         }
-        if (!more) return;
-        if (ids_from < 0 || ids_at == 16) {
-            ids_from = pre.j;
-            ids_at = 0;
-            const int p = a.n_prefix + (pre.j + kWarps * (lane / kUnit)) * kUnit + lane % kUnit;
-            const int np = (held(a, pre.n) + kPage - 1) / kPage;
-            ids = p < np ? checked_page(a.bt[(size_t)pre.n * a.max_pages + p], a.num_pages) : -1;
-        }
-        const int page = __shfl_sync(0xffffffffu, ids, ids_at * kUnit + lane % kUnit);
-        const int last = __shfl_sync(0xffffffffu, page, kUnit - 1);
-        const int st = issued % kStages;
-        if (lane == 0) sm100::mbar_arrive_expect_tx(bar + 8 * st, last >= 0 ? UB : F::kBlockBytes);
+        // What it copies: a segment that runs ahead.  Page ids of 16 units at a time, one page per
+        // lane (lane 2 i + p: page p of the i-th).
+        Segment pre = seg;
+        bool more = true, fresh = true;                          // fresh: the segment's first unit
+        int ids = 0, ids_at = 16;
+        uint32_t issued = 0, used = 0, q_in = 0;
+        const uint64_t policy = sm100::l2_evict_first_policy();  // read once
+        auto issue = [&]() {                                     // warp-uniform: one unit, if any is left
+            if (more && pre.j >= pre.j1) {
+                more = pre.next(a);
+                fresh = true;
+                ids_at = 16;
+            }
+            if (!more) return;
+            if (ids_at == 16) {
+                ids_at = 0;
+                const int p = a.n_prefix + (pre.j + lane / kUnit) * kUnit + lane % kUnit;
+                ids = p < (pre.L + kPage - 1) / kPage ? checked_page(a.bt[(size_t)pre.n * a.max_pages + p], a.num_pages) : -1;
+            }
+            const int page = __shfl_sync(0xffffffffu, ids, ids_at * kUnit + lane % kUnit);
+            const int last = __shfl_sync(0xffffffffu, page, kUnit - 1);
+            const int st = issued % kStages;
+            const uint32_t q_bytes = a.G * D * 2;
+            if (lane == 0)
+                sm100::mbar_arrive_expect_tx(bar + 8 * st, (last >= 0 ? UB : F::kBlockBytes) + (fresh ? q_bytes : 0));
+            __syncwarp();
+            if (lane < kUnit && page >= 0)
+                bulk_load(ring + (uint32_t)(st * UB + lane * F::kBlockBytes),
+                          a.pages + ((size_t)page * a.Hkv + pre.h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
+            if (fresh && lane == kUnit)
+                bulk_load(qring + (q_in & 1) * OwnSmem<D>::kQ, a.q + ((size_t)pre.n * a.Hq + pre.h * a.G) * D, q_bytes,
+                          bar + 8 * st, policy);
+            q_in += fresh;
+            fresh = false;
+            ++issued;
+            ++ids_at;
+            ++pre.j;
+        };
         __syncwarp();
-        if (lane < kUnit && page >= 0)
-            bulk_load(ring + (uint32_t)(st * UB + lane * F::kBlockBytes),
-                      a.pages + ((size_t)page * a.Hkv + pre.h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
-        ++issued;
-        ++ids_at;
-        pre.j += kWarps;
-    };
-    __syncwarp();
 #pragma unroll
-    for (int k = 0; k < kStages; ++k) issue();
-    float* sm_m = reinterpret_cast<float*>(smem + Smem<D>::kRing);   // [kWarps][8]
-    float* sm_l = sm_m + kWarps * 8;
-    float* sm_o = sm_l + kWarps * 8;                             // [kWarps][8][D]
-    uint32_t used = 0;
-    bool failed = false;
-    do {
-        const int L = held(a, seg.n), item = seg.n * a.Hkv + seg.h;
-        const int len[1][2] = {{L, L}};
-        State<D, 1> st;
-        st.init(0, g < a.G ? a.q + ((size_t)seg.n * a.Hq + seg.h * a.G + g) * D : nullptr, a.flip, c);
-        for (int j = seg.j + warp; j < seg.j1 && !failed; j += kWarps) {
-            const int sl = used % kStages;
-            if (!__all_sync(0xffffffffu, wait_full(bar + 8 * sl, (used / kStages) & 1))) {
-                if (lane == 0) {
-                    atomicCAS(&g_device_error, 0, 221);          // let the copies in flight land
-                    for (uint32_t k = used; k < issued; ++k) wait_full(bar + 8 * (k % kStages), (k / kStages) & 1);
+        for (int k = 0; k < kStages; ++k) issue();
+        uint32_t q_out = 0;
+        bool failed = false;
+        do {
+            const int item = seg.n * a.Hkv + seg.h, L = seg.L;
+            const int len[1][2] = {{L, L}};
+            State<D, 1, kUnit> st;
+            for (int j = seg.j; j < seg.j1; ++j) {
+                const int sl = used % kStages;
+                if (!warp_wait(bar + 8 * sl, (used / kStages) & 1)) {
+                    if (lane == 0) {
+                        atomicCAS(&g_device_error, 0, 221);      // let the copies in flight land
+                        for (uint32_t k = used; k < issued; ++k) wait_full(bar + 8 * (k % kStages), (k / kStages) & 1);
+                    }
+                    failed = true;
+                    break;
                 }
-                failed = true;
-                break;
-            }
-            const uint32_t blk = ring + (uint32_t)(sl * UB);
-            const int tok0 = (a.n_prefix + j * kUnit) * kPage;
-            if (tok0 + kUnit * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
-            else st.template unit<true>(blk, tok0, len, a.qscale, lane);
-            __syncwarp();                                        // every lane has read the buffer
-            ++used;
-            issue();
-        }
-        st.finish();
-        __syncthreads();                                         // the last merge's readers are done
-        if (g == 0) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                sm_m[warp * 8 + 2 * c + j] = st.m[0][j];
-                sm_l[warp * 8 + 2 * c + j] = st.l[0][j];
-            }
-        }
-        if (2 * c < a.G) {
-#pragma unroll
-            for (int gr = 0; gr < F::NG; ++gr)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float* r0 = sm_o + (size_t)(warp * 8 + 2 * c) * D + out_dim(gr, k, g);
-                    *reinterpret_cast<float2*>(r0) = make_float2(st.o[0][gr][k][0], st.o[0][gr][k][2]);
-                    *reinterpret_cast<float2*>(r0 + D) = make_float2(st.o[0][gr][k][1], st.o[0][gr][k][3]);
+                if (j == seg.j) {
+                    const uint16_t* rows = reinterpret_cast<const uint16_t*>(qbuf + (q_out & 1) * OwnSmem<D>::kQ);
+                    st.init(0, g < a.G ? rows + g * D : nullptr, a.flip, c);
+                    ++q_out;
                 }
-        }
-        __syncthreads();
-        for (int idx = threadIdx.x; idx < a.G * D / 4; idx += kThreads) {
-            const int hd = idx / (D / 4), d = 4 * (idx % (D / 4));
-            float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * 8 + hd]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float mw = sm_m[w * 8 + hd], lw = sm_l[w * 8 + hd];
-                if (mw == -INFINITY && lw == 0.f) continue;      // a warp without units
-                const float sc = mw == M ? 1.f : fast_exp2((mw - M) * a.qscale);
-                const float4 x = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * 8 + hd) * D + d);
-                acc.x = fmaf(sc, x.x, acc.x);
-                acc.y = fmaf(sc, x.y, acc.y);
-                acc.z = fmaf(sc, x.z, acc.z);
-                acc.w = fmaf(sc, x.w, acc.w);
-                l = fmaf(sc, lw, l);
+                const uint32_t blk = ring + (uint32_t)(sl * UB);
+                const int tok0 = (a.n_prefix + j * kUnit) * kPage;
+                if (tok0 + kUnit * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
+                else st.template unit<true>(blk, tok0, len, a.qscale, lane);
+                __syncwarp();                                    // every lane has read the buffer
+                ++used;
+                issue();
             }
-            const size_t slot = (size_t)(cta + item) * a.G + hd;
-            *reinterpret_cast<float4*>(a.own_o + slot * D + d) = acc;
-            if (d == 0) a.own_ml[slot] = make_float2(M, l);
-        }
-        if (threadIdx.x == 0) {
-            if (seg.j == 0) a.span[item].x = cta;
-            if (seg.j1 == seg.u) a.span[item].y = cta;
-        }
-    } while (seg.next(a));
+            if (failed) break;
+            st.finish();
+            // Columns 2c and 2c + 1 are heads of the group; lane g holds 2 dims of each m-tile.
+            const size_t slot = (size_t)(range + item) * a.G;
+#pragma unroll
+            for (int col = 0; col < 2; ++col) {
+                if (2 * c + col >= a.G) continue;
+                float* dst = a.own_o + (slot + 2 * c + col) * D;
+#pragma unroll
+                for (int gr = 0; gr < F::NG; ++gr)
+#pragma unroll
+                    for (int k = 0; k < 4; k += 2)
+                        *reinterpret_cast<float4*>(dst + out_dim(gr, k, g)) =
+                            make_float4(st.o[0][gr][k][col], st.o[0][gr][k][2 + col],
+                                        st.o[0][gr][k + 1][col], st.o[0][gr][k + 1][2 + col]);
+                if (g == 0) a.own_ml[slot + 2 * c + col] = make_float2(st.m[0][col], st.l[0][col]);
+            }
+            if (lane == 0) {
+                if (seg.j == 0) a.span[item].x = range;
+                if (seg.j1 == seg.u) a.span[item].y = range;
+            }
+        } while (seg.next(a));
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");           // the prefix kernel's partials are there too
 }
 
-// One chunk of the shared prefix for the sessions of four warps (8 columns each) of one KV head.  The
-// buffers are one ring of two halves, refilled half by half after a CTA barrier.
+// -- shared prefix --------------------------------------------------------------------------------------
 template <int D>
-__device__ __forceinline__ void prefix_item(const DecodeArgs& a, uint8_t* smem, uint64_t* bars, int chunk,
-                                            int h, int group) {
+struct PrefixSmem {
+    static constexpr int kBytes = kRing * Fmt<D>::kBlockBytes + 128;
+};
+
+// One chunk of the prefix for the sessions of four warps (kBlocks blocks of 8 columns each) of one KV
+// head.  The staged pages are a ring of two halves, refilled half by half after a CTA barrier.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a) {
     using F = Fmt<D>;
-    constexpr int UB = Smem<D>::kUnitBytes, kHalf = kSlots / 2;
+    constexpr int kHalf = kRing / 2;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    __shared__ __align__(8) uint64_t bars[kRing];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the own pages need nothing from here
+    const int chunk = blockIdx.x % a.n_chunks, h = blockIdx.x / a.n_chunks % a.Hkv;
+    const int group = blockIdx.x / a.n_chunks / a.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int spw = 8 / a.G;                                     // sessions of a warp
-    const int first = group * kWarps * spw;
+    const int spb = 8 / a.G;                                     // sessions of a block
+    const int first = group * kWarps * kBlocks * spb;
     const int p_begin = chunk * a.chunk, p_end = min(p_begin + a.chunk, a.n_prefix);
     // The page ids come from the group's longest session, whose row holds every page that any
     // session here needs; pages past its length are not read.
     int best = -1, lead = first;
-    if (lane < kWarps * spw) {
-        best = held(a, first + lane);
-        lead = first + lane;
+    for (int i = lane; i < kWarps * kBlocks * spb; i += 32) {
+        const int L = held(a, first + i);
+        if (L > best) { best = L; lead = first + i; }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -616,89 +623,82 @@ __device__ __forceinline__ void prefix_item(const DecodeArgs& a, uint8_t* smem, 
     }
     const int pages = min(p_end, (best + kPage - 1) / kPage) - p_begin;
     if (pages <= 0) return;                                      // combine reads no slot of this chunk
-    const int units = (pages + kUnit - 1) / kUnit;
     const int32_t* row = a.bt + (size_t)lead * a.max_pages + p_begin;
     const uint32_t ring = sm100::smem_addr(smem), bar = sm100::smem_addr(bars);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kSlots; ++i) sm100::mbar_init(bar + 8 * i, 1);
+        for (int i = 0; i < kRing; ++i) sm100::mbar_init(bar + 8 * i, 1);
         sm100::fence_barrier_init();
     }
     __syncthreads();
     uint64_t policy;
     asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
-    const uint8_t* head = a.pages + (size_t)h * F::kBlockBytes;
-    auto issue_half = [&](int k0) {                              // units k0 .. k0 + kHalf - 1, one a lane of warp 0
+    auto issue_half = [&](int k0) {                              // pages k0 .. k0 + kHalf - 1, one a lane of warp 0
         const int k = k0 + lane;
-        if (warp == 0 && lane < kHalf && k < units) {
-            const int sl = k % kSlots, have = min(kUnit, pages - k * kUnit);
-            sm100::mbar_arrive_expect_tx(bar + 8 * sl, have * F::kBlockBytes);
-            for (int i = 0; i < have; ++i)
-                bulk_load(ring + (uint32_t)(sl * UB + i * F::kBlockBytes),
-                          head + (size_t)checked_page(row[k * kUnit + i], a.num_pages) * a.Hkv * F::kBlockBytes,
-                          F::kBlockBytes, bar + 8 * sl, policy);
+        if (warp == 0 && lane < kHalf && k < pages) {
+            const int sl = k % kRing, page = checked_page(row[k], a.num_pages);
+            sm100::mbar_arrive_expect_tx(bar + 8 * sl, F::kBlockBytes);
+            bulk_load(ring + (uint32_t)(sl * F::kBlockBytes),
+                      a.pages + ((size_t)page * a.Hkv + h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * sl, policy);
         }
     };
     issue_half(0);
     issue_half(kHalf);
-    const int end = (p_begin + pages) * kPage;                   // a unit's missing page is past it
-    const int base = first + warp * spw, n_g = base + g / a.G;
-    const int len[1][2] = {{min(end, held(a, base + (2 * c) / a.G)), min(end, held(a, base + (2 * c + 1) / a.G))}};
-    int lmin = min(len[0][0], len[0][1]);
-    State<D, 1> st;
-    st.init(0, n_g < a.N ? a.q + ((size_t)n_g * a.Hq + h * a.G + g % a.G) * D : nullptr, a.flip, c);
+    State<D, kBlocks, 1> st;
+    int len[kBlocks][2], lmin = 0x7FFFFFFF;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const int base = first + (warp * kBlocks + b) * spb, n_g = base + g / a.G;
+        len[b][0] = held(a, base + (2 * c) / a.G);
+        len[b][1] = held(a, base + (2 * c + 1) / a.G);
+        lmin = min(lmin, min(len[b][0], len[b][1]));
+        st.init(b, n_g < a.N ? a.q + ((size_t)n_g * a.Hq + h * a.G + g % a.G) * D : nullptr, a.flip, c);
+    }
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) lmin = min(lmin, __shfl_xor_sync(0xffffffffu, lmin, off));
     bool failed = false;
-    for (int k0 = 0; k0 < units; k0 += kHalf) {
-        for (int k = k0; k < min(k0 + kHalf, units); ++k) {
-            const int sl = k % kSlots;
-            if (!failed && !__all_sync(0xffffffffu, wait_full(bar + 8 * sl, (uint32_t)((k / kSlots) & 1)))) {
+    for (int k0 = 0; k0 < pages; k0 += kHalf) {
+        for (int k = k0; k < min(k0 + kHalf, pages); ++k) {
+            const int sl = k % kRing;
+            if (!failed && !warp_wait(bar + 8 * sl, (uint32_t)((k / kRing) & 1))) {
                 if (lane == 0) atomicCAS(&g_device_error, 0, 221);
                 failed = true;
             }
             if (failed) continue;
-            const uint32_t blk = ring + (uint32_t)(sl * UB);
-            const int tok0 = (p_begin + k * kUnit) * kPage;
-            if (tok0 + kUnit * kPage <= lmin) st.template unit<false>(blk, tok0, len, a.qscale, lane);
+            const uint32_t blk = ring + (uint32_t)(sl * F::kBlockBytes);
+            const int tok0 = (p_begin + k) * kPage;
+            if (tok0 + kPage <= lmin) st.template unit<false>(blk, tok0, len, a.qscale, lane);
             else st.template unit<true>(blk, tok0, len, a.qscale, lane);
         }
         if (__syncthreads_or(failed)) {                          // every warp is done with this half
             const int k = k0 + lane;                             // copies may still be landing
-            if (warp == 0 && lane < kSlots && k < units) wait_full(bar + 8 * (k % kSlots), (uint32_t)((k / kSlots) & 1));
+            if (warp == 0 && lane < kRing && k < pages) wait_full(bar + 8 * (k % kRing), (uint32_t)((k / kRing) & 1));
             break;
         }
-        issue_half(k0 + kSlots);
+        issue_half(k0 + kRing);
     }
     st.finish();
     // rows of columns 2c and 2c + 1 go straight to their slots
 #pragma unroll
-    for (int col = 0; col < 2; ++col) {
-        const int j = 2 * c + col, n = base + j / a.G;
-        if (n >= a.N) continue;
-        const size_t slot = ((size_t)n * a.Hq + h * a.G + j % a.G) * a.n_chunks + chunk;
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-        for (int gr = 0; gr < F::NG; ++gr)
+        for (int col = 0; col < 2; ++col) {
+            const int j = 2 * c + col, n = first + (warp * kBlocks + b) * spb + j / a.G;
+            if (n >= a.N) continue;
+            const size_t slot = ((size_t)n * a.Hq + h * a.G + j % a.G) * a.n_chunks + chunk;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<float2*>(a.pre_o + slot * D + out_dim(gr, k, g)) =
-                    make_float2(st.o[0][gr][k][col], st.o[0][gr][k][2 + col]);
-        if (g == 0) a.pre_ml[slot] = make_float2(st.m[0][col], st.l[0][col]);
-    }
+            for (int gr = 0; gr < F::NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 4; k += 2)
+                    *reinterpret_cast<float4*>(a.pre_o + slot * D + out_dim(gr, k, g)) =
+                        make_float4(st.o[b][gr][k][col], st.o[b][gr][k][2 + col],
+                                    st.o[b][gr][k + 1][col], st.o[b][gr][k + 1][2 + col]);
+            if (g == 0) a.pre_ml[slot] = make_float2(st.m[b][col], st.l[b][col]);
+        }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const DecodeArgs a) {
-    extern __shared__ __align__(128) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-    __shared__ __align__(8) uint64_t bars[kSlots];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // combine may be brought in
-    const int n_pre = a.n_chunks * a.Hkv * a.groups;
-    const int item = blockIdx.x;
-    if (item < n_pre)
-        prefix_item<D>(a, smem, bars, item % a.n_chunks, item / a.n_chunks % a.Hkv, item / a.n_chunks / a.Hkv);
-    else
-        own_range<D>(a, smem, bars, item - n_pre);
-}
+template <int V> struct Vec;
+template <> struct Vec<2> { typedef float2 T; };
+template <> struct Vec<4> { typedef float4 T; };
 
 // One warp per (session, query head): merges the row's partials, the prefix chunks first, by their
 // maxima.  A row without tokens gives zeros and an lse of -inf.
@@ -712,7 +712,9 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     const int npages = (held(a, n) + kPage - 1) / kPage;
     const int chunks = a.n_prefix > 0 ? (min(npages, a.n_prefix) + a.chunk - 1) / a.chunk : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");        // the partials are written
-    const int2 span = npages > a.n_prefix ? a.span[item] : make_int2(0, -1);
+    int2 span = npages > a.n_prefix ? a.span[item] : make_int2(0, -1);
+    span.x = max(0, min(span.x, a.ranges - 1));               // (a range that gave up leaves any bits there)
+    span.y = max(span.x - 1, min(span.y, a.ranges - 1));
     const int total = chunks + span.y - span.x + 1;
     const long own0 = (long)(span.x + item) * a.G + hq % a.G, pre0 = row * a.n_chunks;
     auto ml = [&](int j) { return j < chunks ? a.pre_ml[pre0 + j] : a.own_ml[own0 + (long)(j - chunks) * a.G]; };
@@ -720,38 +722,43 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     auto vec = [&](int j) {
         return (j < chunks ? a.pre_o + (pre0 + j) * D : a.own_o + (own0 + (long)(j - chunks) * a.G) * D) + V * lane;
     };
-    float M = -INFINITY;
-    for (int j = lane; j < total; j += 32) M = fmaxf(M, ml(j).x);
+    typedef typename Vec<V>::T VT;
+    // the first slots' vectors are on their way while the weights are formed
+    constexpr int kEarly = 4;
+    VT early[kEarly];
+#pragma unroll
+    for (int t = 0; t < kEarly; ++t)
+        if (t < total) early[t] = *reinterpret_cast<const VT*>(vec(t));
+    float2 e = make_float2(-INFINITY, 0.f);
+    if (lane < total) e = ml(lane);
+    float M = e.x;
+    for (int j = lane + 32; j < total; j += 32) M = fmaxf(M, ml(j).x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
     float acc[V], l = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     const float ref = M == -INFINITY ? 0.f : M;
+    auto add = [&](float wt, const VT& x) {
+        const float* f = reinterpret_cast<const float*>(&x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(wt, f[i], acc[i]);
+    };
     for (int j0 = 0; j0 < total; j0 += 32) {
-        float w = 0.f;
-        if (j0 + lane < total) {
-            const float2 e = ml(j0 + lane);
-            w = e.x == -INFINITY ? 0.f : fast_exp2((e.x - ref) * a.qscale);
-            l = fmaf(w, e.y, l);
-        }
+        if (j0 > 0) e = j0 + lane < total ? ml(j0 + lane) : make_float2(-INFINITY, 0.f);
+        const float w = e.x == -INFINITY ? 0.f : fast_exp2((e.x - ref) * a.qscale);
+        l = fmaf(w, e.y, l);
         const int end = min(32, total - j0);
-#pragma unroll 4
-        for (int t = 0; t < end; ++t) {
-            const float wt = __shfl_sync(0xffffffffu, w, t);
-            const float* src = vec(j0 + t);
-            if constexpr (V == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(src);
-                acc[0] = fmaf(wt, x.x, acc[0]);
-                acc[1] = fmaf(wt, x.y, acc[1]);
-                acc[2] = fmaf(wt, x.z, acc[2]);
-                acc[3] = fmaf(wt, x.w, acc[3]);
-            } else {
-                const float2 x = *reinterpret_cast<const float2*>(src);
-                acc[0] = fmaf(wt, x.x, acc[0]);
-                acc[1] = fmaf(wt, x.y, acc[1]);
+        if (j0 == 0) {
+#pragma unroll
+            for (int t = 0; t < kEarly; ++t) {
+                const float wt = __shfl_sync(0xffffffffu, w, t);
+                if (t < total) add(wt, early[t]);
             }
         }
+#pragma unroll 4
+        for (int t = j0 == 0 ? kEarly : 0; t < end; ++t)
+            add(__shfl_sync(0xffffffffu, w, t), *reinterpret_cast<const VT*>(vec(j0 + t)));
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
@@ -768,7 +775,7 @@ inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 // Pages of a prefix chunk: halved from the whole prefix, down to 16, while the items are fewer than
 // two per SM.
 inline int prefix_chunk(int N, int G, int Hkv, int n_prefix, int sms) {
-    const long groups = ceil_div((long)N * G, 8 * kWarps);
+    const long groups = ceil_div((long)N * G, 8 * kWarps * kBlocks);
     int c = n_prefix;
     while (c > 16 && groups * Hkv * ceil_div(n_prefix, c) < 2L * sms) c = (c + 1) / 2;
     return c > 0 ? c : 1;
@@ -777,14 +784,14 @@ inline int prefix_chunk(int N, int G, int Hkv, int n_prefix, int sms) {
 // Sizes of the workspace's parts, in their order.
 struct Sizes {
     size_t own, pre, items;                    // partials of the ranges, of the prefix; spans
-    int chunk, n_chunks, ctas;
+    int chunk, n_chunks, ranges;
     size_t bytes(int D) const { return (own + pre) * (D * sizeof(float) + sizeof(float2)) + items * sizeof(int2); }
 };
 inline Sizes sizes(int N, int Hq, int Hkv, int n_prefix, int max_pages, int sms) {
     Sizes s;
-    s.ctas = n_prefix < max_pages ? kPerSm * sms : 0;
+    s.ranges = n_prefix < max_pages ? kPerSm * sms * kWarps : 0;
     s.items = (size_t)N * Hkv;
-    s.own = s.ctas > 0 ? (s.ctas + s.items) * (Hq / Hkv) : 0;
+    s.own = s.ranges > 0 ? (s.ranges + s.items) * (Hq / Hkv) : 0;
     s.chunk = prefix_chunk(N, Hq / Hkv, Hkv, n_prefix, sms);
     s.n_chunks = ceil_div(n_prefix, s.chunk);
     s.pre = (size_t)N * Hq * s.n_chunks;
@@ -798,31 +805,45 @@ static int sm_count(int* out) {
     return LF_OK;
 }
 
-template <int D>
-static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st) {
-    static PerContextOnce once;
-    const int rc = once.run([] {
-        LF_CHECK_CUDA(cudaFuncSetAttribute(decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           Smem<D>::kBytes));
-        return LF_OK;
-    });
-    if (rc != LF_OK) return rc;
-    const long items = (long)a.n_chunks * a.Hkv * a.groups + a.ctas;
-    LF_CHECK_ARG(items <= 2147483647L, "q4 decode: grid limits exceeded");
-    decode_kernel<D><<<(unsigned)items, kThreads, Smem<D>::kBytes, st>>>(a);
-    const int e = launch_status("q4 decode");
-    if (e != LF_OK) return e;
-    cudaLaunchConfig_t cfg = {};               // launched while the first kernel still runs; it waits itself
-    cfg.gridDim = dim3((unsigned)ceil_div((long)a.N * a.Hq, kWarps));
+// `after`: may start while the stream's last kernel still runs (and waits for it itself).
+template <class... P, class... A>
+static int start(const char* what, bool after, void (*kernel)(P...), long blocks, size_t smem, cudaStream_t st, A... args) {
+    LF_CHECK_ARG(blocks <= 2147483647L, "%s: grid limits exceeded", what);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
-    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<D>, a, o, lse));
-    return launch_status("q4 decode combine");
+    cfg.numAttrs = after ? 1 : 0;
+    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return launch_status(what);
+}
+
+template <int D>
+static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st) {
+    static PerContextOnce once;
+    int rc = once.run([] {
+        LF_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           OwnSmem<D>::kBytes));
+        LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           PrefixSmem<D>::kBytes));
+        return LF_OK;
+    });
+    if (rc != LF_OK) return rc;
+    const long shared = (long)a.n_chunks * a.Hkv * a.groups;
+    if (shared > 0) {
+        rc = start("q4 decode prefix", false, prefix_kernel<D>, shared, PrefixSmem<D>::kBytes, st, a);
+        if (rc != LF_OK) return rc;
+    }
+    if (a.ranges > 0) {
+        rc = start("q4 decode", shared > 0, own_kernel<D>, a.ranges / kWarps, OwnSmem<D>::kBytes, st, a);
+        if (rc != LF_OK) return rc;
+    }
+    return start("q4 decode combine", true, combine_kernel<D>, ceil_div((long)a.N * a.Hq, kWarps), 0, st, a, o, lse);
 }
 
 }  // namespace q4
@@ -891,8 +912,8 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
     a.n_prefix = num_prefix_pages;
     a.chunk = z.chunk;
     a.n_chunks = z.n_chunks;
-    a.groups = q4::ceil_div(num_seqs, q4::kWarps * (8 / G));
-    a.ctas = z.ctas;
+    a.groups = q4::ceil_div(num_seqs, q4::kWarps * q4::kBlocks * (8 / G));
+    a.ranges = z.ranges;
     a.qscale = fabsf(scale) * kLog2e * q4::kDown;
     a.flip = scale < 0.f ? 0x80008000u : 0u;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

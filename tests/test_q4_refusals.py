@@ -113,7 +113,7 @@ def test_fork_and_pool_arguments():
 
 
 def test_workspace():
-    """(444 ranges + N Hkv items) x G partials, prefix chunks x N Hq partials, one span per item."""
-    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 0, 148) == (444 + 6) * 2 * (512 + 8) + 6 * 8
+    """(148 x 12 ranges + N Hkv items) x G partials, prefix chunks x N Hq partials, a span per item."""
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 0, 148) == (1776 + 6) * 2 * (512 + 8) + 6 * 8
     # a prefix of 16 pages or less is one chunk; no own pages, no ranges
     assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 10, 148) == 3 * 4 * (512 + 8) + 6 * 8
