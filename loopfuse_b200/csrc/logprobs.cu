@@ -7,10 +7,14 @@
 // a peaked distribution's small entropy is not a difference of large numbers; -inf logits (banned
 // tokens) enter both sums as zeros.
 //
-// Work is bound by reading the logits (at 2 bytes a value an SM receives about 12 values a clock, and
-// one value costs about 8 lane-instructions, one of them an exponential, of the 128 it can issue).
+// Work is bound by reading the logits: at 2 bytes a value an SM receives about 12 values a clock, and
+// can issue 128 lane-instructions.  So the sums are kept in the log2 domain,
+//   t = (x - m) log2 e,  s = sum 2^t,  w = sum 2^t t,
+// on packed pairs of fp32 (two values an instruction), -inf being raised to a finite value first:
+// about 5 instructions a value, one of them the exponential.  Maxima are taken on packed 16-bit pairs.
+// x - m, not a multiply-add with a rounded m log2 e: a certain token's t is exactly 0.
 // A row is taken by a cluster of 1 to 8 CTAs, so that small batches fill the chip; a warp streams
-// slices of 8 vectors of 16 bytes per lane with the next slice already in flight.  Every lane keeps
+// slices of 4 vectors of 16 bytes per lane with the next slice already in flight.  Every lane keeps
 // its own (m, s, w) and rescales once a slice.
 //
 // The alternatives are found among whole vectors: the k vectors with the largest maxima (ties to the
@@ -35,17 +39,21 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kVecs = 8;                               // 16-byte vectors of a lane's slice
+constexpr int kVecs = 4;                               // 16-byte vectors of a lane's slice
+constexpr int kPerSm = 3;                              // resident CTAs of an SM
 constexpr int kMaxParts = 8;                           // CTAs of a row (portable cluster size)
 constexpr unsigned kAll = 0xffffffffu;
 
 typedef unsigned long long u64;
+constexpr float kHuge = 1.3e36f;                       // 2^120: maxima past it are far from the type's end
 
 template <int DT> struct Elem;                         // 0 bf16, 1 fp16, 2 fp32
 template <> struct Elem<0> {
     typedef uint16_t T;
     static constexpr int N = 8;
     static constexpr uint32_t kNegInf = 0xFF80FF80u;
+    static constexpr uint32_t kFloor = 0xFE80FE80u;    // -2^126
+    static constexpr float kLowest = -1.3e36f;         // maxima from here on are far above the floor
     static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = bf16lo_to_f32(w); f[1] = bf16hi_to_f32(w); }
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
         uint32_t r;
@@ -57,6 +65,8 @@ template <> struct Elem<1> {
     typedef uint16_t T;
     static constexpr int N = 8;
     static constexpr uint32_t kNegInf = 0xFC00FC00u;
+    static constexpr uint32_t kFloor = 0xFBFFFBFFu;    // -65504
+    static constexpr float kLowest = -60000.f;
     static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
         const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
         f[0] = v.x;
@@ -72,12 +82,40 @@ template <> struct Elem<2> {
     typedef uint32_t T;
     static constexpr int N = 4;
     static constexpr uint32_t kNegInf = 0xFF800000u;
+    static constexpr uint32_t kFloor = 0xFE800000u;    // -2^126
+    static constexpr float kLowest = -1.3e36f;
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
     static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Packed pairs of fp32.
+__device__ __forceinline__ u64 pair(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(u64 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 
@@ -144,16 +182,22 @@ __device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
     return bitonic_merge(a > r ? a : r, lane);
 }
 
-struct Stat {                                          // of a set of values
+struct Stat {                                          // of a set of values: maximum, sums around it
     float m, s, w;
+    // The sums around a larger maximum.
+    __device__ __forceinline__ void raise(float m2) {
+        const float d = fmaxf((m - m2) * kLog2e, -1e30f);   // finite: from -inf, s and w are 0
+        const float f = fast_exp2(d);
+        w = f * (w + d * s);
+        s *= f;
+        m = m2;
+    }
 };
-__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
+__device__ __forceinline__ Stat merge(Stat a, Stat b) {
     const float m = max_nan(a.m, b.m);
-    if (!(m > -INFINITY)) return Stat{m, 0.f, 0.f};    // nothing yet, or NaN
-    // an empty side has s = w = 0: its difference is clamped like an element's
-    const float da = fmaxf(a.m - m, -1e30f), db = fmaxf(b.m - m, -1e30f);
-    const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
-    return Stat{m, fa * a.s + fb * b.s, fa * (a.w + da * a.s) + fb * (b.w + db * b.s)};
+    if (m != a.m) a.raise(m);
+    if (m != b.m) b.raise(m);
+    return Stat{m, a.s + b.s, a.w + b.w};
 }
 
 struct Args {
@@ -166,8 +210,12 @@ struct Args {
     float* top;
 };
 
+__device__ __forceinline__ int64_t token(const Args& a, long row) {
+    return a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : (int64_t)static_cast<const int32_t*>(a.tokens)[row];
+}
+
 template <int DT, bool kTop>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a) {
     using E = Elem<DT>;
     typedef typename E::T T;
     constexpr int N = E::N;
@@ -214,15 +262,18 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
         }
     };
 
+    __shared__ float s_tok;
+    if (part == 0 && threadIdx.x == kThreads - 1) {    // the token's own logit, on its way meanwhile
+        const int64_t tok = token(a, row);
+        float f[2] = {0.f, 0.f};
+        if (tok >= 0 && tok < a.vocab) E::unpack((uint32_t)x[tok], f);
+        s_tok = f[0];
+    }
     Stat st{-INFINITY, 0.f, 0.f};
     u64 list = 0, kth = 0, own = 0;                    // this lane's entry; the k-th entry
     float thr = -INFINITY;                             // no vector below it enters the list
     bool first = true;
-    uint4 cur[kVecs], nxt[kVecs];
-    uint32_t sl = part * per + warp;
-    if (sl < s_end) load(sl, cur);
-    for (; sl < s_end; sl += kWarps) {
-        if (sl + kWarps < s_end) load(sl + kWarps, nxt);
+    auto slice = [&](uint32_t sl, const uint4 (&cur)[kVecs]) {
         float vm[kVecs];
         float lm = -INFINITY;
 #pragma unroll
@@ -230,29 +281,49 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
             vm[i] = vec_max<DT>(cur[i]);
             lm = max_nan(lm, vm[i]);
         }
-        const float m = max_nan(st.m, lm);
-        const float ref = m == -INFINITY ? 0.f : m;    // every value so far is -inf: all terms are 0
-        if (m != st.m) {
-            const float d = fmaxf(st.m - ref, -1e30f), f = fast_exp2(d * kLog2e);
-            st.w = f * (st.w + d * st.s);
-            st.s *= f;
-            st.m = m;
-        }
-        float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};    // short chains of additions
+        if (!(lm <= st.m)) st.raise(max_nan(st.m, lm));
+        const bool none = st.m == -INFINITY;           // every value so far is -inf: all terms are 0
+        if (__all_sync(kAll, none || (st.m >= E::kLowest && st.m < kHuge))) {
+            const float M = none ? 0.f : -st.m;
+            const u64 M2 = pair(M, M), L2 = pair(kLog2e, kLog2e);
+            u64 s2 = 0, w2 = 0;
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            float f[N];
-            unpack<DT>(cur[i], f);
+            for (int i = 0; i < kVecs; ++i) {
+                const uint32_t v[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+                float f[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float d = fmaxf(f[e] - ref, -1e30f);
-                const float p = fast_exp2(d * kLog2e);
-                s[e & 1] += p;
-                w[e & 1] = fmaf(p, d, w[e & 1]);
+                for (int e = 0; e < 4; ++e) E::unpack(E::max2(v[e], E::kFloor), f + e * (N / 4));
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const u64 t2 = mul2(add2(pair(f[e], f[e + 1]), M2), L2);
+                    float t0, t1;
+                    split(t2, t0, t1);
+                    const u64 p2 = pair(fast_exp2(t0), fast_exp2(t1));
+                    s2 = add2(s2, p2);
+                    w2 = fma2(p2, t2, w2);
+                }
+            }
+            float s0, s1, w0, w1;
+            split(s2, s0, s1);
+            split(w2, w0, w1);
+            if (!none) {
+                st.s += s0 + s1;
+                st.w += w0 + w1;
+            }
+        } else if (!none) {                            // maxima out of range: differences, one by one
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                float f[N];
+                unpack<DT>(cur[i], f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float t = fmaxf((f[e] - st.m) * kLog2e, -1e30f);
+                    const float p = fast_exp2(t);
+                    st.s += p;
+                    st.w = fmaf(p, t, st.w);
+                }
             }
         }
-        st.s += s[0] + s[1];
-        st.w += w[0] + w[1];
         if constexpr (kTop) {
             const uint32_t v0 = sl * (kSlice / N) + lane;     // this lane's vectors: v0 + 32 i
             auto key_of = [&](int i) {                 // a vector without a value of the row has none
@@ -298,8 +369,20 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) cur[i] = nxt[i];
+    };
+    {
+        uint4 va[kVecs], vb[kVecs];                    // two slices in turn: one is used, one on its way
+        uint32_t sl = part * per + warp;
+        if (sl < s_end) load(sl, va);
+        while (sl < s_end) {
+            if (sl + kWarps < s_end) load(sl + kWarps, vb);
+            slice(sl, va);
+            sl += kWarps;
+            if (sl >= s_end) break;
+            if (sl + kWarps < s_end) load(sl + kWarps, va);
+            slice(sl, vb);
+            sl += kWarps;
+        }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -353,15 +436,21 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
         const float bar = last == 0 ? -INFINITY : key_value(last);
         u64 best = 0, key = 0;
         int count = 0;                                 // candidates waiting in `key`, one a lane
+        float val[N];
+#pragma unroll
         for (int e = 0; e < N; ++e) {
             const uint32_t p = u + e;
             float f[2] = {-INFINITY, 0.f};
-            const bool valid = have && p >= lead && p < end;
-            if (valid) E::unpack((uint32_t)base[p], f);
-            const bool in = valid && !(f[0] < bar);
+            if (have && p >= lead && p < end) E::unpack((uint32_t)base[p], f);
+            val[e] = f[0];
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t p = u + e;
+            const bool in = have && p >= lead && p < end && !(val[e] < bar);
             const unsigned mask = __ballot_sync(kAll, in);
             if (mask == 0) continue;
-            const u64 cand = in ? make_key(f[0], p - lead) : 0;
+            const u64 cand = in ? make_key(val[e], p - lead) : 0;
             const int n = __popc(mask);
             if (count + n > 32) {
                 best = merge_lists(best, sort_desc(key, lane), lane);
@@ -382,19 +471,11 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a) {
         }
     }
     if (lane == 0) {
-        const int64_t tok = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row]
-                                       : (int64_t)static_cast<const int32_t*>(a.tokens)[row];
-        float lp = 0.f;                                // a negative token: none was given
-        if (tok >= a.vocab) {
-            atomicCAS(&g_device_error, 0, 231);
-            lp = NAN;
-        } else if (tok >= 0) {
-            float f[2];
-            E::unpack((uint32_t)x[tok], f);
-            lp = logp(f[0]);
-        }
-        a.logprob[row] = lp;
-        a.entropy[row] = bad ? NAN : (none ? 0.f : ln_s - st.w / st.s);
+        const int64_t tok = token(a, row);
+        if (tok >= a.vocab) atomicCAS(&g_device_error, 0, 231);
+        // a negative token: none was given
+        a.logprob[row] = tok < 0 ? 0.f : (tok >= a.vocab ? NAN : logp(s_tok));
+        a.entropy[row] = bad ? NAN : (none ? 0.f : ln_s - st.w / st.s * kLn2);
     }
 }
 
@@ -435,10 +516,10 @@ extern "C" int lf_token_logprobs(const void* logits, int dtype, int64_t row_stri
     int dev = 0, sms = 0;
     LF_CHECK_CUDA(cudaGetDevice(&dev));
     LF_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    // CTAs of a row: doubled while the grid leaves SMs with less than two and a warp keeps a slice
-    const int slice = dtype == 2 ? 1024 : 2048;
+    // CTAs of a row: doubled while all of them stay resident at once and a warp keeps a slice
+    const int slice = 32 * logprobs::kVecs * (dtype == 2 ? 4 : 8);
     int parts = 1;
-    while (parts < logprobs::kMaxParts && (long)rows * parts < 2L * sms &&
+    while (parts < logprobs::kMaxParts && 2L * rows * parts <= (long)logprobs::kPerSm * sms &&
            (long)vocab > (long)parts * logprobs::kWarps * slice)
         parts *= 2;
     LF_CHECK_ARG((long)rows * parts <= 2147483647L, "token logprobs: grid limits exceeded");

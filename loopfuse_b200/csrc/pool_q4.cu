@@ -57,6 +57,19 @@ __global__ void append_kernel(const AppendArgs a) {
             page = a.table[(long)row * a.table_stride + pos / kPage];
         const bool page_ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
         if (!(page_ok && pos_ok) && threadIdx.x == 0) report(a);
+        float cs[8], sn[8];                            // this lane's dims, the same in every row
+        if (a.cos != nullptr) {
+            const long off = (long)(pos_ok ? pos : 0) * (D / 2) + (8 * l) % (D / 2);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos + off) + j);
+                const float4 n = __ldg(reinterpret_cast<const float4*>(a.sin + off) + j);
+                const float sign = l < LPR / 2 ? -1.f : 1.f;
+                cs[4 * j] = c.x; cs[4 * j + 1] = c.y; cs[4 * j + 2] = c.z; cs[4 * j + 3] = c.w;
+                sn[4 * j] = sign * n.x; sn[4 * j + 1] = sign * n.y;
+                sn[4 * j + 2] = sign * n.z; sn[4 * j + 3] = sign * n.w;
+            }
+        }
         for (int r0 = warp * RPW; r0 < H; r0 += warps * RPW) {
             const int h = r0 + lane / LPR;
             const bool live = h < H;
@@ -70,23 +83,24 @@ __global__ void append_kernel(const AppendArgs a) {
                 x = *reinterpret_cast<const uint4*>(src + 8 * l);
             }
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            if (a.cos != nullptr) {                    // every lane of the warp takes the shuffles
-                const float* cp = a.cos + (long)(pos_ok ? pos : 0) * (D / 2) + (8 * l) % (D / 2);
-                const float* sp = a.sin + (long)(pos_ok ? pos : 0) * (D / 2) + (8 * l) % (D / 2);
-                const bool turn = live && (is_q || is_k);
+            const bool turn = live && (is_q || is_k);
+            if (a.cos != nullptr && __any_sync(0xffffffffu, turn)) {   // every lane takes the shuffles
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], LPR / 2);
-                    const float2 c = __ldg(reinterpret_cast<const float2*>(cp) + j);
-                    const float2 s = __ldg(reinterpret_cast<const float2*>(sp) + j);
-                    const float al = __fmul_rn(bf16lo_to_f32(w[j]), c.x);
-                    const float ah = __fmul_rn(bf16hi_to_f32(w[j]), c.y);
-                    const float bl = __fmul_rn(bf16lo_to_f32(other), s.x);
-                    const float bh = __fmul_rn(bf16hi_to_f32(other), s.y);
-                    const uint32_t first = pack_bf16x2(__fsub_rn(al, bl), __fsub_rn(ah, bh));
-                    const uint32_t second = pack_bf16x2(__fadd_rn(al, bl), __fadd_rn(ah, bh));
-                    if (turn) w[j] = l < LPR / 2 ? first : second;
+                    // x1 c - x2 s in the first half of a row, x2 c + x1 s in the second (sn is -s, s)
+                    const float lo = __fadd_rn(__fmul_rn(bf16lo_to_f32(w[j]), cs[2 * j]),
+                                               __fmul_rn(bf16lo_to_f32(other), sn[2 * j]));
+                    const float hi = __fadd_rn(__fmul_rn(bf16hi_to_f32(w[j]), cs[2 * j + 1]),
+                                               __fmul_rn(bf16hi_to_f32(other), sn[2 * j + 1]));
+                    if (turn) w[j] = pack_bf16x2(lo, hi);
                 }
+            }
+            if (__all_sync(0xffffffffu, is_q || !live)) {   // query rows: no groups to form
+                if (live && pos_ok)
+                    *reinterpret_cast<uint4*>(a.q_out + ((long)t * a.Hq + h) * D + 8 * l) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                continue;
             }
             float f[8];
 #pragma unroll
@@ -335,8 +349,10 @@ extern "C" int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v
                            rope_sin, rope_rows, q_out, static_cast<uint8_t*>(pages), num_pages, num_q_heads,
                            num_kv_heads, status};
     const int rows = num_q_heads + 2 * num_kv_heads, rpw = 256 / head_dim;
-    const int warps = (rows + rpw - 1) / rpw;
-    const int threads = 32 * (warps < 16 ? warps : 16);
+    // A token's rows are spread over 16 warps while there are few tokens, over 4 once the tokens fill
+    // the chip by themselves (what a warp looks up once per token then serves more rows).
+    const int warps = (rows + rpw - 1) / rpw, most = total_tokens >= 148 * 4 ? 4 : 16;
+    const int threads = 32 * (warps < most ? warps : most);
     const int blocks = total_tokens < 148 * 32 ? total_tokens : 148 * 32;
     const dim3 grid(blocks, num_layers);
     if (head_dim == 128)
