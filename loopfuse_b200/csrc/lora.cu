@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(pool::kMetaThreads)
 plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int n, int total, int adapters,
             Plan p) {
     extern __shared__ int sm[];
-    __shared__ int buf[32];
+    __shared__ int2 buf[32];
     int* tot = sm;                                     // [adapters + 1] tokens
     int* off = sm + adapters + 1;                      // first sorted row
     int* til = off + adapters + 1;                     // first tile
@@ -59,41 +59,47 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int
     auto count = [&](int i) { return max(0, min(max(cu[i + 1], 0), total) - lo(i)); };
     for (int b = threadIdx.x; b <= adapters; b += pool::kMetaThreads) tot[b] = 0;
     __syncthreads();
-    int sum = 0;
-    for (int i0 = 0; i0 < n; i0 += pool::kMetaThreads) {
-        const int i = i0 + threadIdx.x;
-        const int c = i < n ? count(i) : 0;
-        if (i < n) {
-            if (c > 0) atomicAdd(&tot[bucket(i)], c);
-            if (ids[i] < -1 || ids[i] >= adapters) atomicCAS(&g_device_error, 0, 241);
+    for (int i = threadIdx.x; i < n; i += pool::kMetaThreads) {
+        const int c = count(i);
+        if (c > 0) atomicAdd(&tot[bucket(i)], c);
+        if (ids[i] < -1 || ids[i] >= adapters) atomicCAS(&g_device_error, 0, 241);
+    }
+    __syncthreads();
+    int rows = 0, tiles = 0;                           // exclusive sums over the buckets
+    for (int b0 = 0; b0 <= adapters; b0 += pool::kMetaThreads) {
+        const int b = b0 + threadIdx.x;
+        const int c = b <= adapters ? tot[b] : 0, k = (c + kTile - 1) / kTile;
+        int xc = c, xk = k;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int oc = __shfl_up_sync(0xffffffffu, xc, d), ok = __shfl_up_sync(0xffffffffu, xk, d);
+            if (lane >= d) { xc += oc; xk += ok; }
         }
-        int t = 0;
-        pool::block_excl_scan(c, &t, buf);
-        sum += t;
+        if (lane == 31) buf[warp] = make_int2(xc, xk);
+        __syncthreads();
+        int2 w = buf[lane];                            // every warp scans the warps' sums
+        const int2 mine = w;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int oc = __shfl_up_sync(0xffffffffu, w.x, d), ok = __shfl_up_sync(0xffffffffu, w.y, d);
+            if (lane >= d) { w.x += oc; w.y += ok; }
+        }
+        const int bc = __shfl_sync(0xffffffffu, w.x - mine.x, warp), bk = __shfl_sync(0xffffffffu, w.y - mine.y, warp);
+        if (b <= adapters) {
+            off[b] = rows + bc + xc - c;
+            til[b] = tiles + bk + xk - k;
+        }
+        rows += __shfl_sync(0xffffffffu, w.x, 31);
+        tiles += __shfl_sync(0xffffffffu, w.y, 31);
+        __syncthreads();
     }
     // offsets that overlap or leave tokens out give no plan: rows would be written twice or not at all
-    const bool bad = sum != total || (n > 0 && (cu[0] != 0 || cu[n] != total));
-    if (bad) {
+    if (rows != total || (n > 0 && (cu[0] != 0 || cu[n] != total))) {
         if (threadIdx.x == 0) {
             atomicCAS(&g_device_error, 0, 242);
             p.head[0] = 0;
         }
         return;
-    }
-    __syncthreads();
-    int rows = 0, tiles = 0;
-    for (int b0 = 0; b0 <= adapters; b0 += pool::kMetaThreads) {
-        const int b = b0 + threadIdx.x;
-        const int c = b <= adapters ? tot[b] : 0;
-        int t = 0;
-        const int r = rows + pool::block_excl_scan(c, &t, buf);
-        rows += t;
-        const int k = tiles + pool::block_excl_scan((c + kTile - 1) / kTile, &t, buf);
-        tiles += t;
-        if (b <= adapters) {
-            off[b] = r;
-            til[b] = k;
-        }
     }
     if (threadIdx.x == 0) p.head[0] = tiles;
     __syncthreads();
@@ -160,7 +166,7 @@ struct Args {
     const uint16_t *x, *y, *a, *b;
     uint16_t* out;
     const float* scale;
-    float* part;                                       // [slices][total][R]
+    float* part;                                       // [slices][total][R]; with one slice, h [total][R] bf16
     const int32_t *head, *tiles, *order;
     int64_t x_stride, y_stride, out_stride;            // elements between rows
     int total, K, N, slices, k_per;                    // k_per: inputs of a slice, a multiple of kStep
@@ -168,7 +174,7 @@ struct Args {
 };
 
 constexpr int kStep = 64;                              // inputs of a stage
-constexpr int kStages = 4;
+constexpr int kStages = 8;
 constexpr int kShrinkWarps = 8;
 
 // Row of `r` 16-byte chunks in shared memory, chunk index xor-ed with the row: ldmatrix without
@@ -193,6 +199,10 @@ template <int R>
 __global__ void __launch_bounds__(32 * kShrinkWarps)
 shrink_kernel(const Args g) {
     extern __shared__ __align__(128) uint8_t smem[];
+    // x, y and the plan are there, and this memory's last readers are done; from here on the expansion
+    // may be brought in and fetch y and B
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tile = blockIdx.y, slice = blockIdx.x;
     if (tile >= g.head[0]) return;
     const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
@@ -278,118 +288,156 @@ shrink_kernel(const Args g) {
             const float4 o = *reinterpret_cast<const float4*>(red + (long)w * 16 * mb * R + i);
             v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
         }
-        *reinterpret_cast<float4*>(dst + i) = v;
+        if (g.slices > 1) {
+            *reinterpret_cast<float4*>(dst + i) = v;
+        } else {
+            const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.part) + (long)first * R + i) =
+                make_uint2(pack_bf16x2(v.x * sc, v.y * sc), pack_bf16x2(v.z * sc, v.w * sc));
+        }
     }
 }
 
 constexpr int kCols = 128;                             // columns of an expand block
-constexpr int kExpandWarps = 4;                        // 32 columns each
+constexpr int kExpandWarps = 8;                        // 16 columns each
 
 template <int R>
 struct ExpandSmem {
     static constexpr int kH = kTile * R * 2, kB = R * kCols * 2, kY = kTile * kCols * 2;
-    static constexpr int kBytes = kH + kB + kY;
+    static constexpr int kBuf = kB + kY;
+    static constexpr int kBytes = kH + 2 * kBuf;
 };
 
-// CTA (group of column blocks, tile): h of the tile once, then per block of 128 columns
-// y + h B, staged in shared memory.
+// CTA (group of column blocks, tile): h of the tile once, then per block of 128 columns y + h B,
+// staged in shared memory, the next block's y and B on their way meanwhile.
 template <int R>
 __global__ void __launch_bounds__(32 * kExpandWarps)
 expand_kernel(const Args g) {
+    using S = ExpandSmem<R>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tile = blockIdx.y;
-    if (tile >= g.head[0]) return;
-    const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
+    const bool none = tile >= g.head[0];
+    const int4 t = none ? make_int4(-1, 0, 0, 0) : reinterpret_cast<const int4*>(g.tiles)[tile];
     const int rows = t.z, first = t.y;
     const bool copy_only = t.x < 0;
-    if (copy_only && g.y == g.out) return;
+    if (none || (copy_only && g.y == g.out)) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // no CTA ends before the kernel it follows
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int YC = kCols / 8, HC = R / 8;
-    constexpr int T = 32 * kExpandWarps;
-    const uint32_t sh = sm100::smem_addr(smem), sb = sh + ExpandSmem<R>::kH, sy = sb + ExpandSmem<R>::kB;
-    uint8_t* yb = smem + ExpandSmem<R>::kH + ExpandSmem<R>::kB;
+    constexpr int T = 32 * kExpandWarps, RS = T / YC, NR = kTile / RS;   // rows of a pass, passes
+    const uint32_t sh = sm100::smem_addr(smem);
     const uint16_t* B = g.b + (long)(copy_only ? 0 : t.x) * R * g.N;
-    const int c = threadIdx.x % YC, r0 = threadIdx.x / YC;      // this thread's chunk column, row
+    const int c = threadIdx.x % YC, r0 = threadIdx.x / YC;      // this thread's chunk column, first row
     const int blocks = (rows + 15) / 16;
-    auto load = [&](int n0) {
-        const bool on = n0 + 8 * c < g.N;
-        for (int r = r0; r < rows; r += T / YC) {
-            const long tok = g.order[first + r];
-            cp16(sy + at<YC>(r, c), on ? g.y + tok * g.y_stride + n0 + 8 * c : g.y, on);
+    int tok[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) tok[i] = r0 + i * RS < rows ? g.order[first + r0 + i * RS] : -1;
+    const int n_first = blockIdx.x * g.cols * kCols;
+    const int n_blocks = min(g.cols, (g.N - n_first + kCols - 1) / kCols);
+    // A thread copies in and writes out the same pieces of y, so a buffer's y needs no barrier between.
+    auto load = [&](int blk) {
+        if (blk < n_blocks) {
+            const int col = n_first + blk * kCols + 8 * c;
+            const uint32_t sb = sh + S::kH + (blk & 1) * S::kBuf, sy = sb + S::kB;
+            const bool on = col < g.N;
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (tok[i] >= 0) cp16(sy + at<YC>(r0 + i * RS, c), on ? g.y + tok[i] * g.y_stride + col : g.y, on);
+            if (!copy_only)
+#pragma unroll
+                for (int k = 0; k < R / RS; ++k)
+                    cp16(sb + at<YC>(r0 + k * RS, c), on ? B + (long)(r0 + k * RS) * g.N + col : g.b, on);
         }
-        if (!copy_only)
-            for (int k = r0; k < R; k += T / YC)
-                cp16(sb + at<YC>(k, c), on ? B + (long)k * g.N + n0 + 8 * c : g.b, on);
         cp_commit();
     };
-    const int n_first = blockIdx.x * g.cols * kCols;
-    load(n_first);
-    if (!copy_only) {                                  // h: partials summed in slice order, scaled, rounded
-        const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
-        for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
-            const int r = i / HC, ch = i % HC;
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (r < rows)
-                for (int s = 0; s < g.slices; ++s) {
-                    const float4* p = reinterpret_cast<const float4*>(g.part + ((long)s * g.total + first + r) * R + 8 * ch);
-                    const float4 a = p[0], b = p[1];
-                    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-                    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    load(0);
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // h is there
+    if (!copy_only) {
+        if (g.slices == 1) {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(g.part) + (long)first * R;
+            for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
+                const int r = i / HC, ch = i % HC;
+                *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
+                    r < rows ? *reinterpret_cast<const uint4*>(h + (long)r * R + 8 * ch) : make_uint4(0, 0, 0, 0);
+            }
+        } else {                                       // partials summed in slice order, scaled, rounded
+            const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+            for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
+                const int r = i / HC, ch = i % HC;
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (r < rows) {
+#pragma unroll 4
+                    for (int s = 0; s < g.slices; ++s) {
+                        const float4* p = reinterpret_cast<const float4*>(g.part + ((long)s * g.total + first + r) * R + 8 * ch);
+                        const float4 a = p[0], b = p[1];
+                        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+                    }
                 }
-            *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
-                make_uint4(pack_bf16x2(v[0] * sc, v[1] * sc), pack_bf16x2(v[2] * sc, v[3] * sc),
-                           pack_bf16x2(v[4] * sc, v[5] * sc), pack_bf16x2(v[6] * sc, v[7] * sc));
+                *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
+                    make_uint4(pack_bf16x2(v[0] * sc, v[1] * sc), pack_bf16x2(v[2] * sc, v[3] * sc),
+                               pack_bf16x2(v[4] * sc, v[5] * sc), pack_bf16x2(v[6] * sc, v[7] * sc));
+            }
         }
     }
-    for (int blk = 0; blk < g.cols; ++blk) {
-        const int n0 = n_first + blk * kCols;
-        if (n0 >= g.N) break;
-        if (blk > 0) load(n0);
-        cp_wait<0>();
+    for (int blk = 0; blk < n_blocks; ++blk) {
+        load(blk + 1);
+        cp_wait<1>();
         __syncthreads();
+        const uint32_t sb = sh + S::kH + (blk & 1) * S::kBuf;
+        uint8_t* yb = smem + S::kH + (blk & 1) * S::kBuf + S::kB;
         if (!copy_only) {
             const int gq = lane >> 2, cq = lane & 3;
+            constexpr int CJ = kCols / kExpandWarps / 16;   // 16-column pieces of a warp
+            uint32_t b[R / 16][CJ][4];                 // B of this warp's columns, for every row block
+#pragma unroll
+            for (int kk = 0; kk < R / 16; ++kk)
+#pragma unroll
+                for (int j = 0; j < CJ; ++j)
+                    ldsm4_t(sb + at<YC>(16 * kk + (lane & 15), 2 * (CJ * warp + j) + (lane >> 4)), b[kk][j]);
             for (int m = 0; m < blocks; ++m) {
-                float acc[4][4] = {};
+                float acc[2 * CJ][4] = {};
 #pragma unroll
                 for (int kk = 0; kk < R / 16; ++kk) {
                     uint32_t a[4];
                     ldsm4(sh + at<HC>(16 * m + (lane & 15), 2 * kk + (lane >> 4)), a);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t b[4];
-                        ldsm4_t(sb + at<YC>(16 * kk + (lane & 15), 4 * warp + 2 * j + (lane >> 4)), b);
-                        mma(acc[2 * j], a, b[0], b[1]);
-                        mma(acc[2 * j + 1], a, b[2], b[3]);
+                    for (int j = 0; j < CJ; ++j) {
+                        mma(acc[2 * j], a, b[kk][j][0], b[kk][j][1]);
+                        mma(acc[2 * j + 1], a, b[kk][j][2], b[kk][j][3]);
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 2 * CJ; ++j)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
+                    for (int half = 0; half < 2; ++half) {   // rows past the tile's are scratch
                         const int r = 16 * m + gq + 8 * half;
-                        if (r < rows) {
-                            uint32_t* p = reinterpret_cast<uint32_t*>(yb + at<YC>(r, 4 * warp + j)) + cq;
-                            const uint32_t w = *p;
-                            *p = pack_bf16x2(bf16lo_to_f32(w) + acc[j][2 * half], bf16hi_to_f32(w) + acc[j][2 * half + 1]);
-                        }
+                        uint32_t* p = reinterpret_cast<uint32_t*>(yb + at<YC>(r, 2 * CJ * warp + j)) + cq;
+                        const uint32_t w = *p;
+                        *p = pack_bf16x2(bf16lo_to_f32(w) + acc[j][2 * half], bf16hi_to_f32(w) + acc[j][2 * half + 1]);
                     }
             }
             __syncthreads();
         }
-        if (n0 + 8 * c < g.N)
-            for (int r = r0; r < rows; r += T / YC)
-                *reinterpret_cast<uint4*>(g.out + (long)g.order[first + r] * g.out_stride + n0 + 8 * c) =
-                    *reinterpret_cast<const uint4*>(yb + at<YC>(r, c));
-        __syncthreads();                               // the block's buffers are free
+        const int col = n_first + blk * kCols + 8 * c;
+        if (col < g.N) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (tok[i] >= 0)
+                    *reinterpret_cast<uint4*>(g.out + tok[i] * g.out_stride + col) =
+                        *reinterpret_cast<const uint4*>(yb + at<YC>(r0 + i * RS, c));
+        }
     }
 }
 
 inline int slices_for(int total, int n, int adapters, int K, int sms) {
-    // Slices of the inputs so that a small batch still fills the SMs, 256 inputs at least.
+    // Slices of the inputs, 256 at least, so that a small batch still gives three quarters of the SMs
+    // work; one slice where the tiles do by themselves, and h is then final.
     const long tiles = max_tiles(total, n, adapters);
     int s = 1;
-    while (s < 32 && tiles * s < sms && K >= 2 * s * 256) s *= 2;
+    while (s < 32 && 4 * tiles * s < 3L * sms && K >= 2 * s * 256) s *= 2;
     return s;
 }
 
@@ -404,11 +452,22 @@ static int launch(const Args& g, int tiles, cudaStream_t st) {
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
-    shrink_kernel<R><<<dim3(g.slices, tiles), 32 * kShrinkWarps, ShrinkSmem<R>::kBytes, st>>>(g);
-    const int e = launch_status("lora shrink");
-    if (e != LF_OK) return e;
-    const int groups = ((g.N + kCols - 1) / kCols + g.cols - 1) / g.cols;
-    expand_kernel<R><<<dim3(groups, tiles), 32 * kExpandWarps, ExpandSmem<R>::kBytes, st>>>(g);
+    // Both may start while the kernel before them still runs; they wait for it themselves.
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    cfg.stream = st;
+    cfg.gridDim = dim3(g.slices, tiles);
+    cfg.blockDim = dim3(32 * kShrinkWarps);
+    cfg.dynamicSmemBytes = ShrinkSmem<R>::kBytes;
+    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, shrink_kernel<R>, g));
+    cfg.gridDim = dim3(((g.N + kCols - 1) / kCols + g.cols - 1) / g.cols, tiles);
+    cfg.blockDim = dim3(32 * kExpandWarps);
+    cfg.dynamicSmemBytes = ExpandSmem<R>::kBytes;
+    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, expand_kernel<R>, g));
     return launch_status("lora expand");
 }
 

@@ -11,6 +11,17 @@
 namespace lf {
 namespace q4 {
 
+constexpr uint32_t kSigns = 0x80008000u;
+constexpr float kMagic = 12582912.f;                   // 1.5 * 2^23
+constexpr uint32_t kMagicBits = 0x4B400000u;
+constexpr float kSmallest = 1e-27f;                    // about 2^-90: smaller scales divide plainly
+
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 struct AppendArgs {
     const uint16_t *q, *k, *v;
     int64_t q_token, kv_layer, kv_token, kv_head;      // strides in elements
@@ -102,26 +113,15 @@ __global__ void append_kernel(const AppendArgs a) {
                         make_uint4(w[0], w[1], w[2], w[3]);
                 continue;
             }
-            float f[8];
+            // {-min, max} of the group (8 lanes) as a bf16 pair, NaN if it holds one
+            uint32_t ext;
+            {
+                const uint32_t hi = max2(max2(w[0], w[1]), max2(w[2], w[3]));
+                const uint32_t lo = max2(max2(w[0] ^ kSigns, w[1] ^ kSigns), max2(w[2] ^ kSigns, w[3] ^ kSigns));
+                ext = max2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[2 * j] = bf16lo_to_f32(w[j]);
-                f[2 * j + 1] = bf16hi_to_f32(w[j]);
+                for (int off = 1; off < 8; off <<= 1) ext = max2(ext, __shfl_xor_sync(0xffffffffu, ext, off));
             }
-            float mn = f[0], mx = f[0];
-            bool nan = f[0] != f[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) {
-                mn = fminf(mn, f[j]);
-                mx = fmaxf(mx, f[j]);
-                nan |= f[j] != f[j];
-            }
-#pragma unroll
-            for (int off = 1; off < 8; off <<= 1) {    // a group is 8 lanes
-                mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            }
-            const unsigned nans = __ballot_sync(0xffffffffu, nan);
             if (!live) continue;
             if (is_q) {
                 if (pos_ok)
@@ -130,33 +130,57 @@ __global__ void append_kernel(const AppendArgs a) {
                 continue;
             }
             if (!page_ok || !pos_ok) continue;
-            const float span = __fsub_rn(mx, mn);
+            const float mn = -bf16lo_to_f32(ext), span = __fsub_rn(bf16hi_to_f32(ext), mn);
             uint32_t par = 0x7FC07FC0u;                // NaN, NaN
-            uint32_t n[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (((nans >> (lane & 24)) & 0xFFu) == 0 && span < kMaxSpan) {
+            uint32_t n[8];                             // the codes plus kMagicBits
+#pragma unroll
+            for (int j = 0; j < 8; ++j) n[j] = kMagicBits;
+            if (span < kMaxSpan) {                     // (not NaN)
                 par = pack_bf16x2(__fdiv_rn(span, 15.f), mn);
                 const float s = bf16lo_to_f32(par);
-                if (s > 0.f) {
+                float d[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    d[2 * j] = __fsub_rn(bf16lo_to_f32(w[j]), mn);
+                    d[2 * j + 1] = __fsub_rn(bf16hi_to_f32(w[j]), mn);
+                }
+                if (s >= kSmallest) {
+                    // d / s rounded to nearest from the rounded reciprocal and the exact remainder of the
+                    // first quotient (Markstein's theorem); at most 15.03, so that adding 1.5 * 2^23
+                    // leaves rint(d / s), ties to even, in the low bits.
+                    const float r = __frcp_rn(s);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float q0 = __fmul_rn(d[j], r);
+                        const float q1 = fmaf(fmaf(-q0, s, d[j]), r, q0);
+                        n[j] = __float_as_uint(__fadd_rn(q1, kMagic));
+                    }
+                } else if (s > 0.f) {                  // remainders would underflow
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        n[j] = (uint32_t)fminf(rintf(__fdiv_rn(__fsub_rn(f[j], mn), s)), 15.f);
+                        n[j] = __float_as_uint(__fadd_rn(fminf(rintf(__fdiv_rn(d[j], s)), 15.f), kMagic));
                 }
             }
             const int tok = pos % kPage, grp = l / 8, in = l % 8;   // group, 8-dim piece of it
             uint8_t* blk = a.pages + ((layer * a.num_pages + page) * a.Hkv + kh) * (long)F::kBlockBytes;
-            if (is_k) {
-                uint32_t word = 0;
+            if (is_k) {                                // sums modulo 2^32; the magic bits' sum goes off
+                uint32_t word = 0, magic = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) word |= n[e] << (4 * (e / 2) + 16 * (e % 2));
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t at = 1u << (4 * (e / 2) + 16 * (e % 2));
+                    word += n[e] * at;
+                    magic += kMagicBits * at;
+                }
                 *reinterpret_cast<uint32_t*>(blk + tok * (32 * F::NG) + (in / 2) * (8 * F::NG) +
-                                             grp * 8 + (in % 2) * 4) = word;
+                                             grp * 8 + (in % 2) * 4) = word - magic;
             } else {
                 uint8_t* vp = blk + F::kVOff + (tok / 8) * (256 * F::NG) +
                               (in * 4 + (tok % 8) / 2) * (8 * F::NG) + grp * 8 + (tok % 2) * 2;
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
                     *reinterpret_cast<uint16_t*>(vp + 4 * q) = (uint16_t)(
-                        n[4 * q] | (n[4 * q + 1] << 4) | (n[4 * q + 2] << 8) | (n[4 * q + 3] << 12));
+                        n[4 * q] + n[4 * q + 1] * 16u + n[4 * q + 2] * 256u + n[4 * q + 3] * 4096u -
+                        kMagicBits * 0x1111u);
             }
             if (in == 0)
                 *reinterpret_cast<uint32_t*>(blk + F::kParOff + ((tok * 2 + (is_k ? 0 : 1)) * F::NG + grp) * 4) = par;
@@ -168,9 +192,14 @@ __global__ void append_kernel(const AppendArgs a) {
 constexpr int kExpWarps = 8;
 constexpr int kExpPages = 8;                           // table columns a CTA expands
 
-__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, float s0, float b0, float s1, float b1) {
-    // n * s is exact in fp32 (4 by 8 bits), so the value is rounded once here and once to bf16
-    return pack_bf16x2(fmaf((float)(codes & 15u), s0, b0), fmaf((float)((codes >> 16) & 15u), s1, b1));
+// The pair of codes at bits 0..3 of both halves, as values: n s + b rounded once to bf16.  128 + n is put
+// together from bits and 128 taken off again, both exact.
+__device__ __forceinline__ uint32_t values(uint32_t w, uint32_t s2, uint32_t b2) {
+    uint32_t n, r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(n) : "r"(w), "n"(0x000F000F), "r"(0x43004300u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(n) : "r"(n), "r"(0x43004300u));
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(n), "r"(s2), "r"(b2));
+    return r;
 }
 
 // CTA (session n, kExpPages columns of its table row): warps take (page, head) pairs.  Output pages
@@ -223,11 +252,16 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
     }
     // shared pages are written once, from the longest session's row
     const int lead = best_n;
-    for (int u = warp; u < (j_end - j0) * Hkv; u += kExpWarps) {
-        const int j = j0 + u / Hkv, h = u % Hkv;
+    const int g = lane >> 2, c = lane & 3;
+    constexpr int NW = 2 * F::NG;                      // code words of a lane's vector
+    // Pages this CTA writes: its own ones, and, in the lead session, the shared ones.
+    const int j_last = min(j_end, max(np, n == lead ? n_prefix : 0));
+    const int j_first = n == lead ? j0 : max(j0, n_prefix);
+    const int units = max(0, j_last - j_first) * Hkv;
+    for (int u = warp; u < units; u += kExpWarps) {
+        const int j = j_first + u / Hkv, h = u % Hkv;
         const int o = out_page(j);
-        if (j >= np && !(j < n_prefix)) break;
-        if (o >= out_pages || (j < n_prefix && n != lead)) continue;
+        if (o >= out_pages) break;
         const int rows = min(kPage, L - j * kPage);     // <= 0: a prefix page past every session
         int page = rows > 0 ? bt[(long)n * max_pages + j] : 0;
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(num_pages)) {
@@ -236,11 +270,10 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
         }
         const uint8_t* blk = pages + ((long)page * Hkv + h) * F::kBlockBytes;
         const long dst = ((long)o * Hkv + h) * (kPage * D);
-        const int g = lane >> 2, c = lane & 3;
-        constexpr int NW = 2 * F::NG;                  // code words of a lane's vector
-        uint32_t kw[2][NW], vw[2][NW];
+        uint32_t kw[2][NW], vw[2][NW], pk[2][F::NG], pv[2][2][F::NG];
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(blk + F::kParOff);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < 2; ++half) {         // all loads before the first use
             const uint8_t* kp = blk + (half * 8 + g) * (32 * F::NG) + c * (8 * F::NG);
             const uint8_t* vp = blk + F::kVOff + half * (256 * F::NG) + lane * (8 * F::NG);
             if constexpr (F::NG == 2) {
@@ -253,8 +286,13 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
                 kw[half][0] = a.x; kw[half][1] = a.y;
                 vw[half][0] = b.x; vw[half][1] = b.y;
             }
+#pragma unroll
+            for (int grp = 0; grp < F::NG; ++grp) {
+                pk[half][grp] = __ldg(par + (half * 8 + g) * 2 * F::NG + grp);
+                pv[half][0][grp] = __ldg(par + ((half * 8 + 2 * c) * 2 + 1) * F::NG + grp);
+                pv[half][1][grp] = __ldg(par + ((half * 8 + 2 * c) * 2 + 3) * F::NG + grp);
+            }
         }
-        const uint32_t* par = reinterpret_cast<const uint32_t*>(blk + F::kParOff);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int t = half * 8 + g;                // K: the lane's 16 dims of a group, 32 bytes
@@ -262,37 +300,32 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
             for (int grp = 0; grp < F::NG; ++grp) {
                 uint32_t out[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                 if (t < rows) {
-                    const uint32_t p = __ldg(par + t * 2 * F::NG + grp);
-                    const float s = bf16lo_to_f32(p), b = bf16hi_to_f32(p);
+                    const uint32_t p = pk[half][grp];
+                    const uint32_t s2 = __byte_perm(p, p, 0x1010), b2 = __byte_perm(p, p, 0x3232);
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            out[4 * w + i] = bf16_pair(kw[half][2 * grp + w] >> (4 * i), s, b, s, b);
+                        for (int i = 0; i < 4; ++i) out[4 * w + i] = values(kw[half][2 * grp + w] >> (4 * i), s2, b2);
                 }
                 sm100::st_global_v8(ko + dst + t * D + grp * kGroup + c * 16, out);
             }
+            // V: tokens t0, t0 + 1 (a word's halves), 8 dims of a group, 16 bytes each
+            const int t0 = half * 8 + 2 * c;
 #pragma unroll
-            for (int odd = 0; odd < 2; ++odd) {        // V: 8 dims of a group, 16 bytes
-                const int tv = half * 8 + 2 * c + odd;
+            for (int grp = 0; grp < F::NG; ++grp) {
+                const uint32_t p0 = pv[half][0][grp], p1 = pv[half][1][grp];
+                const uint32_t s2 = __byte_perm(p0, p1, 0x5410), b2 = __byte_perm(p0, p1, 0x7632);
+                uint32_t even[4], odd[4];
 #pragma unroll
-                for (int grp = 0; grp < F::NG; ++grp) {
-                    uint32_t out[4] = {0, 0, 0, 0};
-                    if (tv < rows) {
-                        const uint32_t p = __ldg(par + (tv * 2 + 1) * F::NG + grp);
-                        const float s = bf16lo_to_f32(p), b = bf16hi_to_f32(p);
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const uint32_t x = vw[half][2 * grp + w] >> (16 * odd);
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                out[2 * w + i] = pack_bf16x2(fmaf((float)((x >> (8 * i)) & 15u), s, b),
-                                                             fmaf((float)((x >> (8 * i + 4)) & 15u), s, b));
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(vo + dst + tv * D + grp * kGroup + g * 8) =
-                        make_uint4(out[0], out[1], out[2], out[3]);
+                for (int i = 0; i < 4; ++i) {          // dims 2 i, 2 i + 1 of both tokens
+                    const uint32_t w = vw[half][2 * grp + i / 2] >> (8 * (i % 2));
+                    const uint32_t x = values(w, s2, b2), y = values(w >> 4, s2, b2);
+                    even[i] = t0 < rows ? __byte_perm(x, y, 0x5410) : 0u;
+                    odd[i] = t0 + 1 < rows ? __byte_perm(x, y, 0x7632) : 0u;
                 }
+                uint16_t* to = vo + dst + t0 * D + grp * kGroup + g * 8;
+                *reinterpret_cast<uint4*>(to) = make_uint4(even[0], even[1], even[2], even[3]);
+                *reinterpret_cast<uint4*>(to + D) = make_uint4(odd[0], odd[1], odd[2], odd[3]);
             }
         }
     }
