@@ -15,6 +15,8 @@
 #include "pool_common.cuh"
 #include "sm100_primitives.cuh"
 
+#include <algorithm>
+
 namespace lf {
 namespace lora {
 
@@ -46,6 +48,7 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int
             Plan p) {
     extern __shared__ int sm[];
     __shared__ int2 buf[32];
+    __shared__ int s_big;
     int* tot = sm;                                     // [adapters + 1] tokens
     int* off = sm + adapters + 1;                      // first sorted row
     int* til = off + adapters + 1;                     // first tile
@@ -57,10 +60,13 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int
     // tokens outside [0, total) are cut off: a plan never names a row that does not exist
     auto lo = [&](int i) { return min(max(cu[i], 0), total); };
     auto count = [&](int i) { return max(0, min(max(cu[i + 1], 0), total) - lo(i)); };
+    constexpr int kBig = 1024;                         // tokens of a session that the whole CTA copies
     for (int b = threadIdx.x; b <= adapters; b += pool::kMetaThreads) tot[b] = 0;
+    if (threadIdx.x == 0) s_big = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += pool::kMetaThreads) {
         const int c = count(i);
+        if (c >= kBig) s_big = 1;
         if (c > 0) atomicAdd(&tot[bucket(i)], c);
         if (ids[i] < -1 || ids[i] >= adapters) atomicCAS(&g_device_error, 0, 241);
     }
@@ -123,13 +129,12 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int
                 make_int4(b == adapters ? -1 : b, off[b] + kTile * k, min(kTile, tot[b] - kTile * k), 0);
     }
     __syncthreads();
-    constexpr int kBig = 1024;                         // sessions that the whole CTA copies
     for (int i = warp; i < n; i += pool::kMetaThreads / 32) {
         const int c = count(i);
         if (c < kBig)
             for (int j = lane; j < c; j += 32) p.order[p.starts[i] + j] = lo(i) + j;
     }
-    if (total >= kBig)
+    if (s_big)
         for (int i = 0; i < n; ++i) {
             const int c = count(i);
             if (c >= kBig)
@@ -173,8 +178,8 @@ struct Args {
     int cols;                                          // expand: column blocks of a CTA
 };
 
-constexpr int kStep = 64;                              // inputs of a stage
-constexpr int kStages = 8;
+constexpr int kStep = 128;                             // inputs of a stage
+constexpr int kStages = 3;
 constexpr int kShrinkWarps = 8;
 
 // Row of `r` 16-byte chunks in shared memory, chunk index xor-ed with the row: ldmatrix without
@@ -218,12 +223,13 @@ shrink_kernel(const Args g) {
     const int blocks = (rows + 15) / 16;
     const int mb = blocks <= 1 ? 1 : (blocks <= 2 ? 2 : 4);   // row blocks, rounded up; kw warps each
     const int kw = kShrinkWarps / mb;
-    // this thread's x rows: chunk c of rows r0, r0 + 32
+    // this thread's x rows: chunk xc of rows xr, xr + XR, ...
+    constexpr int XR = 32 * kShrinkWarps / XC, XN = kTile / XR;   // rows of a pass, passes
     const int xc = threadIdx.x % XC, xr = threadIdx.x / XC;
-    const uint16_t* xrow[2];
+    const uint16_t* xrow[XN];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = xr + 32 * i;
+    for (int i = 0; i < XN; ++i) {
+        const int r = xr + XR * i;
         xrow[i] = g.x + (r < rows ? (long)g.order[first + r] : 0) * g.x_stride + 8 * xc;
     }
     auto load = [&](int s) {
@@ -231,8 +237,8 @@ shrink_kernel(const Args g) {
             const uint32_t st = base + (uint32_t)((s % kStages) * SZ);
             const int k = k0 + s * kStep;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = xr + 32 * i;
+            for (int i = 0; i < XN; ++i) {
+                const int r = xr + XR * i;
                 if (r < 16 * mb) {
                     const bool on = r < rows && k + 8 * xc < k1;
                     cp16(st + at<XC>(r, xc), on ? xrow[i] + k : g.x, on);
@@ -299,7 +305,7 @@ shrink_kernel(const Args g) {
 }
 
 constexpr int kCols = 128;                             // columns of an expand block
-constexpr int kExpandWarps = 8;                        // 16 columns each
+constexpr int kExpandWarps = 4;                        // 32 columns each
 
 template <int R>
 struct ExpandSmem {
@@ -433,12 +439,19 @@ expand_kernel(const Args g) {
 }
 
 inline int slices_for(int total, int n, int adapters, int K, int sms) {
-    // Slices of the inputs, 256 at least, so that a small batch still gives three quarters of the SMs
-    // work; one slice where the tiles do by themselves, and h is then final.
+    // Slices of the inputs, 256 at least, until the CTAs are one and a half per SM (two fit on an SM).
     const long tiles = max_tiles(total, n, adapters);
     int s = 1;
-    while (s < 32 && 4 * tiles * s < 3L * sms && K >= 2 * s * 256) s *= 2;
+    while (s < 32 && 2 * tiles * s < 3L * sms && K >= 2 * s * 256) s *= 2;
     return s;
+}
+
+// Column blocks of a CTA: as many as leave about four waves of resident CTAs (h is formed once for
+// them; fewer, longer CTAs end less evenly).
+inline int column_blocks(int blocks, int tiles, int rank, int sms) {
+    const long bytes = 128L * rank + 2L * (256L * rank + 16384) + 1024;   // shared memory of a CTA
+    const long slots = sms * std::max(1L, std::min(8L, 233472L / bytes));
+    return (int)std::max(1L, std::min(32L, (long)blocks * tiles / (4 * slots)));
 }
 
 template <int R>
@@ -583,10 +596,7 @@ extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x,
     const int steps = (inputs + lora::kStep - 1) / lora::kStep;
     g.k_per = (steps + g.slices - 1) / g.slices * lora::kStep;
     const int tiles = (int)lora::max_tiles(total_tokens, n, num_adapters);
-    // Column blocks of a CTA: 4 once that still leaves about eight CTAs an SM, so that h is formed
-    // once for them.
-    const long blocks = (outputs + lora::kCols - 1) / lora::kCols;
-    g.cols = blocks * tiles >= 32L * sm_count ? 4 : 1;
+    g.cols = lora::column_blocks((outputs + lora::kCols - 1) / lora::kCols, tiles, rank, sm_count);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (rank) {
         case 16: return lora::launch<16>(g, tiles, st);

@@ -46,7 +46,7 @@ __device__ __forceinline__ void report(const AppendArgs& a) {
 // codes are those of the rounded values.  A row that has no page, or no rotation table row, is not
 // stored and is reported.
 template <int D>
-__global__ void append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
     using F = Fmt<D>;
     constexpr int LPR = D / 8, RPW = 32 / LPR;          // lanes a row, rows a warp
     if (a.status != nullptr && *reinterpret_cast<volatile int32_t*>(a.status) != LF_OK) return;
@@ -55,10 +55,21 @@ __global__ void append_kernel(const AppendArgs a) {
     const int l = lane % LPR;
     const long layer = blockIdx.y;
     for (int t = blockIdx.x; t < a.total; t += gridDim.x) {
-        int lo = 0, hi = a.n - 1;                      // session i with cu[i] <= t < cu[i+1]
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.cu[mid] <= t) lo = mid; else hi = mid - 1;
+        // This warp's first row is on its way while the token is looked up.
+        auto source = [&](int h) -> const uint16_t* {
+            if (h < a.Hq) return a.q + t * a.q_token + (long)h * D + 8 * l;
+            const bool k = h < a.Hq + a.Hkv;
+            return (k ? a.k : a.v) + layer * a.kv_layer + t * a.kv_token + (h - a.Hq - (k ? 0 : a.Hkv)) * a.kv_head + 8 * l;
+        };
+        uint4 ahead = make_uint4(0, 0, 0, 0);
+        if (warp * RPW + lane / LPR < H) ahead = *reinterpret_cast<const uint4*>(source(warp * RPW + lane / LPR));
+        int lo = 0;                                    // the last session i with cu[i] <= t, 32 probes at a time
+        for (int len = a.n; len > 1;) {
+            const int step = (len + 31) / 32, i = lo + lane * step;
+            const bool below = lane * step < len && a.cu[i] <= t;
+            const int k = max(0, 31 - __clz(__ballot_sync(0xffffffffu, below)));
+            lo += k * step;
+            len = min(step, len - k * step);
         }
         const int pos = a.start[lo] + (t - a.cu[lo]);
         const int row = a.seq_ids != nullptr ? a.seq_ids[lo] : lo;
@@ -86,13 +97,9 @@ __global__ void append_kernel(const AppendArgs a) {
             const bool live = h < H;
             const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
             const int kh = h - a.Hq - (is_k ? 0 : a.Hkv);
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (live) {
-                const uint16_t* src =
-                    is_q ? a.q + t * a.q_token + (long)h * D
-                         : (is_k ? a.k : a.v) + layer * a.kv_layer + t * a.kv_token + kh * a.kv_head;
-                x = *reinterpret_cast<const uint4*>(src + 8 * l);
-            }
+            const uint4 x = ahead;
+            ahead = make_uint4(0, 0, 0, 0);
+            if (h + warps * RPW < H) ahead = *reinterpret_cast<const uint4*>(source(h + warps * RPW));
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
             const bool turn = live && (is_q || is_k);
             if (a.cos != nullptr && __any_sync(0xffffffffu, turn)) {   // every lane takes the shuffles
@@ -190,7 +197,7 @@ __global__ void append_kernel(const AppendArgs a) {
 
 // -- expansion --------------------------------------------------------------------------------------
 constexpr int kExpWarps = 8;
-constexpr int kExpPages = 8;                           // table columns a CTA expands
+constexpr int kExpPages = 2;                           // table columns a CTA expands (8: 101 against 93 us)
 
 // The pair of codes at bits 0..3 of both halves, as values: n s + b rounded once to bf16.  128 + n is put
 // together from bits and 128 taken off again, both exact.
@@ -382,9 +389,9 @@ extern "C" int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v
                            rope_sin, rope_rows, q_out, static_cast<uint8_t*>(pages), num_pages, num_q_heads,
                            num_kv_heads, status};
     const int rows = num_q_heads + 2 * num_kv_heads, rpw = 256 / head_dim;
-    // A token's rows are spread over 16 warps while there are few tokens, over 4 once the tokens fill
+    // A token's rows are spread over 16 warps while there are few tokens, over 2 once the tokens fill
     // the chip by themselves (what a warp looks up once per token then serves more rows).
-    const int warps = (rows + rpw - 1) / rpw, most = total_tokens >= 148 * 4 ? 4 : 16;
+    const int warps = (rows + rpw - 1) / rpw, most = total_tokens >= 148 * 4 ? 2 : 16;
     const int threads = 32 * (warps < most ? warps : most);
     const int blocks = total_tokens < 148 * 32 ? total_tokens : 148 * 32;
     const dim3 grid(blocks, num_layers);
