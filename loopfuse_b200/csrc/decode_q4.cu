@@ -53,7 +53,7 @@ using decode::kWarps;
 
 constexpr int kUnit = 2;                       // own: pages of a barrier, a softmax step, a buffer
 constexpr int kStages = 2;                     // own: units in flight per warp
-constexpr int kPerSm = 3;                      // own: resident CTAs of an SM
+constexpr int per_sm(int D) { return D == 64 ? 4 : 3; }   // own: resident CTAs of an SM (registers)
 constexpr int kMinUnits = 2;                   // own: units of a range
 constexpr int kBlocks = 1;                     // prefix: blocks of 8 columns of a warp
 constexpr int kRing = 16;                      // prefix: pages staged in a CTA, in two halves
@@ -428,7 +428,7 @@ struct Segment {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, kPerSm) own_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeArgs a) {
     using F = Fmt<D>;
     constexpr int UB = OwnSmem<D>::kUnitBytes;
     extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -787,9 +787,9 @@ struct Sizes {
     int chunk, n_chunks, ranges;
     size_t bytes(int D) const { return (own + pre) * (D * sizeof(float) + sizeof(float2)) + items * sizeof(int2); }
 };
-inline Sizes sizes(int N, int Hq, int Hkv, int n_prefix, int max_pages, int sms) {
+inline Sizes sizes(int N, int Hq, int Hkv, int D, int n_prefix, int max_pages, int sms) {
     Sizes s;
-    s.ranges = n_prefix < max_pages ? kPerSm * sms * kWarps : 0;
+    s.ranges = n_prefix < max_pages ? per_sm(D) * sms * kWarps : 0;
     s.items = (size_t)N * Hkv;
     s.own = s.ranges > 0 ? (s.ranges + s.items) * (Hq / Hkv) : 0;
     s.chunk = prefix_chunk(N, Hq / Hkv, Hkv, n_prefix, sms);
@@ -861,7 +861,7 @@ extern "C" int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int nu
         const int rc = q4::sm_count(&sm_count);
         if (rc != LF_OK) return rc;
     }
-    *bytes = q4::sizes(num_seqs, num_q_heads, num_kv_heads, num_prefix_pages, max_pages, sm_count).bytes(head_dim);
+    *bytes = q4::sizes(num_seqs, num_q_heads, num_kv_heads, head_dim, num_prefix_pages, max_pages, sm_count).bytes(head_dim);
     clear_error();
     return LF_OK;
 }
@@ -890,7 +890,7 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
         const int rc = q4::sm_count(&sm_count);
         if (rc != LF_OK) return rc;
     }
-    const q4::Sizes z = q4::sizes(num_seqs, num_q_heads, num_kv_heads, num_prefix_pages, max_pages, sm_count);
+    const q4::Sizes z = q4::sizes(num_seqs, num_q_heads, num_kv_heads, head_dim, num_prefix_pages, max_pages, sm_count);
     LF_CHECK_ARG(workspace_bytes >= z.bytes(head_dim), "q4 decode: workspace too small (%zu < %zu bytes)",
                  workspace_bytes, z.bytes(head_dim));
     q4::DecodeArgs a{};

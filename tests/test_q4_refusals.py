@@ -113,7 +113,9 @@ def test_fork_and_pool_arguments():
 
 
 def test_workspace():
-    """(148 x 12 ranges + N Hkv items) x G partials, prefix chunks x N Hq partials, a span per item."""
+    """(148 x 12 ranges (16 of 64 dims) + N Hkv items) x G partials, prefix chunks x N Hq partials, a
+    span per item."""
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 64, 10, 0, 148) == (2368 + 6) * 2 * (256 + 8) + 6 * 8
     assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 0, 148) == (1776 + 6) * 2 * (512 + 8) + 6 * 8
     # a prefix of 16 pages or less is one chunk; no own pages, no ranges
     assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 10, 148) == 3 * 4 * (512 + 8) + 6 * 8
