@@ -20,8 +20,9 @@ def sm_count(index: int) -> int:
 
 
 def launch(name: str, device: torch.device, *args) -> None:
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
         return
     with torch.cuda.device(device):
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))

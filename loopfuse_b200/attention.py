@@ -327,11 +327,14 @@ def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
     if block_table.dim() != 2 or block_table.shape[0] != N or seq_lens.shape != (N,):
         raise LoopfuseError(_lib.LF_EINVAL, "block_table must be [N,max_pages], seq_lens [N]")
     dev = _one_device("paged_decode_q4", q, pages, block_table, seq_lens, out, workspace)
-    o = out if out is not None else torch.empty_like(q)
-    _require(o, "out")
-    if o.shape != q.shape:
-        raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: out must have q's shape")
-    lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    if out is None:
+        o = torch.empty_like(q)
+    else:
+        o = out
+        _require(o, "out")
+        if o.shape != q.shape:
+            raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: out must have q's shape")
+    lse = torch.empty((N, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if N == 0:
         return (o, lse) if return_lse else o
     max_pages, npre = block_table.shape[1], int(num_prefix_pages)

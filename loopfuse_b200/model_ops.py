@@ -129,30 +129,26 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     means none was given: its logprob is 0.  A token >= V gives NaN and is reported by
     ``lf_device_status``.  -inf logits have no probability; a row of nothing else has logprob -inf and
     entropy 0; a row with a NaN or +inf has NaN probabilities and entropy."""
-    if logits.device.type != "cuda" or tokens.device != logits.device:
+    dev, k = logits.device, int(top_k)
+    code = _LOGIT_TYPES.get(logits.dtype)
+    if not logits.is_cuda or tokens.device != dev:
         raise LoopfuseError(_lib.LF_EINVAL, "token_logprobs: logits and tokens must be on one CUDA device")
-    if logits.dtype not in _LOGIT_TYPES or logits.dim() != 2 or \
-            (logits.shape[1] > 1 and logits.stride(1) != 1):
+    if code is None or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise LoopfuseError(_lib.LF_EINVAL, "token_logprobs: logits must be bf16, fp16 or fp32 [T, V] "
                                             "with contiguous rows")
     T, V = logits.shape
-    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != (T,) or not tokens.is_contiguous():
+    wide = tokens.dtype is torch.int64
+    if not (wide or tokens.dtype is torch.int32) or tokens.shape != (T,) or not tokens.is_contiguous():
         raise LoopfuseError(_lib.LF_EINVAL, f"token_logprobs: tokens must be contiguous int64 or int32 [{T}]")
-    k = int(top_k)
     if not 0 <= k <= min(MAX_TOP_LOGPROBS, V):
         raise LoopfuseError(_lib.LF_EINVAL, f"token_logprobs: top_k = {k} outside 0..{min(MAX_TOP_LOGPROBS, V)}")
-    dev = logits.device
-    out = TokenLogprobs(torch.empty(T, dtype=torch.float32, device=dev),
-                        torch.empty(T, dtype=torch.float32, device=dev),
-                        torch.empty((T, k), dtype=torch.int64, device=dev),
-                        torch.empty((T, k), dtype=torch.float32, device=dev))
-    if T == 0:
-        return out
-    launch("lf_token_logprobs", dev, logits.data_ptr(), _LOGIT_TYPES[logits.dtype], logits.stride(0),
-           tokens.data_ptr(), int(tokens.dtype == torch.int64), T, V, k, out.logprob.data_ptr(),
-           out.entropy.data_ptr(), out.top_ids.data_ptr() if k else None,
-           out.top_logprobs.data_ptr() if k else None)
-    return out
+    logprob, entropy = torch.empty((2, T), dtype=torch.float32, device=dev).unbind(0)
+    top_ids = torch.empty((T, k), dtype=torch.int64, device=dev)
+    top = torch.empty((T, k), dtype=torch.float32, device=dev)
+    if T:
+        launch("lf_token_logprobs", dev, logits.data_ptr(), code, logits.stride(0), tokens.data_ptr(), wide,
+               T, V, k, logprob.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), top.data_ptr())
+    return TokenLogprobs(logprob, entropy, top_ids, top)
 
 
 # -- low-rank adapters ----------------------------------------------------------------------------
@@ -176,13 +172,15 @@ def lora_plan(adapter_ids: torch.Tensor, cu_tokens: torch.Tensor, total_tokens: 
     [N + 1]``: session ``i`` owns rows ``cu_tokens[i] .. cu_tokens[i + 1]``, ``total_tokens`` in
     all.  Ids outside ``[-1, num_adapters)`` count as none; they, and offsets that are not rising
     from 0 to ``total_tokens`` (nothing is written then), are reported by ``lf_device_status``."""
-    for t, n in ((adapter_ids, "adapter_ids"), (cu_tokens, "cu_tokens")):
-        if t.device.type != "cuda" or t.dtype != torch.int32 or not t.is_contiguous():
-            raise LoopfuseError(_lib.LF_EINVAL, f"lora_plan: {n} must be a contiguous CUDA int32 tensor")
-    n = adapter_ids.shape[0] if adapter_ids.dim() == 1 else -1
-    if cu_tokens.shape != (n + 1,) or cu_tokens.device != adapter_ids.device:
-        raise LoopfuseError(_lib.LF_EINVAL, "lora_plan: adapter_ids [N] and cu_tokens [N + 1] on one device")
-    total, adapters, dev = int(total_tokens), int(num_adapters), adapter_ids.device
+    i32, dev = torch.int32, adapter_ids.device
+    if not (adapter_ids.is_cuda and adapter_ids.dtype is i32 and cu_tokens.dtype is i32 and
+            cu_tokens.device == dev and adapter_ids.is_contiguous() and cu_tokens.is_contiguous()):
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_plan: adapter_ids and cu_tokens must be contiguous int32 "
+                                            "tensors on one CUDA device")
+    n = adapter_ids.numel()
+    if adapter_ids.shape != (n,) or cu_tokens.shape != (n + 1,):
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_plan: adapter_ids must be [N], cu_tokens [N + 1]")
+    total, adapters = int(total_tokens), int(num_adapters)
     size = _plan_bytes(n, total, adapters)
     buf = torch.empty(size, dtype=torch.uint8, device=dev)
     launch("lf_lora_plan", dev, adapter_ids.data_ptr(), cu_tokens.data_ptr(), n, total, adapters,
@@ -213,36 +211,37 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     32, 64 or 128 (pad with zeros), K and N multiples of 8.  In place on ``y`` unless ``out`` is
     given; rows without an adapter keep (or, with ``out``, are) ``y``'s."""
     res = y if out is None else out
-    for t, n, dim in ((y, "y", 2), (x, "x", 2), (res, "out", 2), (a, "a", 3), (b, "b", 3)):
-        if t.device.type != "cuda" or t.dtype != torch.bfloat16 or t.dim() != dim or \
-                t.device != plan.buffer.device:
-            raise LoopfuseError(_lib.LF_EINVAL, f"lora_add: {n} must be a {dim}-d bf16 tensor on the plan's device")
+    dev, bf16 = plan.buffer.device, torch.bfloat16
+    if not (y.is_cuda and y.dtype is bf16 and x.dtype is bf16 and res.dtype is bf16 and a.dtype is bf16 and
+            b.dtype is bf16 and y.device == dev and x.device == dev and res.device == dev and a.device == dev and
+            b.device == dev and y.dim() == 2 and x.dim() == 2 and a.dim() == 3 and b.dim() == 3):
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_add: y, x, out [T, .], a and b [adapters, ., .] must be bf16 "
+                                            "tensors on the plan's CUDA device")
     T, K = x.shape
-    N, R = y.shape[1], a.shape[2]
-    if T != plan.total_tokens or y.shape[0] != T or res.shape != y.shape or \
-            tuple(a.shape) != (plan.num_adapters, K, R) or tuple(b.shape) != (plan.num_adapters, R, N):
+    N, R, adapters = y.shape[1], a.shape[2], plan.num_adapters
+    if T != plan.total_tokens or y.shape[0] != T or res.shape != y.shape or a.shape != (adapters, K, R) or \
+            b.shape != (adapters, R, N):
         raise LoopfuseError(_lib.LF_EINVAL, f"lora_add: y {tuple(y.shape)}, x {tuple(x.shape)}, "
                                             f"a {tuple(a.shape)}, b {tuple(b.shape)} and a plan of "
-                                            f"{plan.total_tokens} tokens, {plan.num_adapters} adapters do not match")
+                                            f"{plan.total_tokens} tokens, {adapters} adapters do not match")
     if not (a.is_contiguous() and b.is_contiguous()):
         raise LoopfuseError(_lib.LF_EINVAL, "lora_add: a and b must be contiguous")
-    for t in (y, x, res):
-        if t.stride(1) != 1 or (T > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
-            raise LoopfuseError(_lib.LF_EINVAL, "lora_add: rows must be contiguous, their stride a multiple of 8")
+    sy, sx, so = y.stride(0), x.stride(0), res.stride(0)
+    if T <= 1:
+        sy, sx, so = N, K, N
+    if y.stride(1) != 1 or x.stride(1) != 1 or res.stride(1) != 1 or (sy | sx | so) % 8 or sy < N or sx < K or so < N:
+        raise LoopfuseError(_lib.LF_EINVAL, "lora_add: rows must be contiguous, their stride a multiple of 8")
     if R not in LORA_RANKS:
         raise LoopfuseError(_lib.LF_EINVAL, f"lora_add: rank {R} is not one of {LORA_RANKS} (pad with zeros)")
-    if scale is not None and (scale.device != y.device or scale.dtype != torch.float32 or
-                              tuple(scale.shape) != (plan.num_adapters,) or not scale.is_contiguous()):
+    if scale is not None and (scale.device != dev or scale.dtype is not torch.float32 or
+                              scale.shape != (adapters,) or not scale.is_contiguous()):
         raise LoopfuseError(_lib.LF_EINVAL, "lora_add: scale must be fp32 [adapters] on y's device")
     if T == 0:
         return res
-    dev = y.device
     sms = sm_count(dev.index)
-    need = _lora_workspace_bytes(plan.sessions, T, plan.num_adapters, K, R, sms)
+    need = _lora_workspace_bytes(plan.sessions, T, adapters, K, R, sms)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    launch("lf_lora_add", dev, y.data_ptr(), y.stride(0) if T > 1 else N, x.data_ptr(),
-           x.stride(0) if T > 1 else K, a.data_ptr(), b.data_ptr(),
+    launch("lf_lora_add", dev, y.data_ptr(), sy, x.data_ptr(), sx, a.data_ptr(), b.data_ptr(),
            scale.data_ptr() if scale is not None else None, plan.buffer.data_ptr(), plan.sessions, T,
-           plan.num_adapters, K, N, R, res.data_ptr(), res.stride(0) if T > 1 else N, ws.data_ptr(), need,
-           sms)
+           adapters, K, N, R, res.data_ptr(), so, ws.data_ptr(), need, sms)
     return res
