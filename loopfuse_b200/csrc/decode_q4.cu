@@ -44,6 +44,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace lf {
 namespace q4 {
 
@@ -447,18 +449,12 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
         for (int i = 0; i < kStages; ++i) sm100::mbar_init(bar + 8 * i, 1);
         sm100::fence_barrier_init();
     }
-    long mine = 0;
-    for (int n = threadIdx.x; n < a.N; n += kThreads) mine += own_units(a, n);
-    const long total = cta_sum(mine, buf) * a.Hkv;
-    const long share = max((total + a.ranges - 1) / a.ranges, (long)kMinUnits);
-    const int range = blockIdx.x * kWarps + warp;
-    const long begin = range * share, cta_begin = (long)blockIdx.x * kWarps * share;
-    // Sessions where the CTA's ranges start, a CTA's width of sessions at a time.
-    const long cta_last = min(cta_begin + (kWarps - 1) * share, total - 1);
-    long before = 0;
-    for (int n0 = 0; n0 < a.N && cta_begin < total && before * a.Hkv <= cta_last; n0 += kThreads) {
-        const int n = n0 + threadIdx.x;
-        const int u = n < a.N ? own_units(a, n) : 0;
+    // Units of a CTA's width of sessions, summed up to each: the first such chunk serves the total and,
+    // in most batches, the search.
+    long excl = 0, chunk = 0;                                    // units before this thread's session; of the chunk
+    int u = 0;
+    auto scan = [&](int n0) {
+        u = n0 + threadIdx.x < a.N ? own_units(a, n0 + threadIdx.x) : 0;
         long incl = u;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -467,15 +463,42 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
         }
         if (lane == 31) buf[warp] = incl;
         __syncthreads();
-        long excl = before + incl - u;
-        for (int w = 0; w < warp; ++w) excl += buf[w];
-        for (int w = 0; w < kWarps; ++w) before += buf[w];
+        excl = incl - u;
+        chunk = 0;
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const long at = cta_begin + w * share;
-            if (at >= excl * a.Hkv && at < (excl + u) * a.Hkv) {
-                s_before[w] = excl;
-                s_n[w] = n;
+            if (w < warp) excl += buf[w];
+            chunk += buf[w];
+        }
+        __syncthreads();
+    };
+    scan(0);
+    long total = chunk;
+    if (a.N > kThreads) {
+        long mine = 0;
+        for (int n = kThreads + threadIdx.x; n < a.N; n += kThreads) mine += own_units(a, n);
+        total += cta_sum(mine, buf);
+    }
+    total *= a.Hkv;
+    const long share = max((total + a.ranges - 1) / a.ranges, (long)kMinUnits);
+    const int range = blockIdx.x * kWarps + warp;
+    const long begin = range * share, cta_begin = (long)blockIdx.x * kWarps * share;
+    const long cta_last = min(cta_begin + (kWarps - 1) * share, total - 1);
+    if (cta_begin < total) {                                     // the sessions where the CTA's ranges start
+        long before = 0;
+        for (int n0 = 0;;) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const long at = cta_begin + w * share, from = before + excl;
+                if (at >= from * a.Hkv && at < (from + u) * a.Hkv) {
+                    s_before[w] = from;
+                    s_n[w] = n0 + threadIdx.x;
+                }
             }
+            before += chunk;
+            n0 += kThreads;
+            if (n0 >= a.N || before * a.Hkv > cta_last) break;
+            scan(n0);
         }
         __syncthreads();
     }
@@ -723,12 +746,15 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
         return (j < chunks ? a.pre_o + (pre0 + j) * D : a.own_o + (own0 + (long)(j - chunks) * a.G) * D) + V * lane;
     };
     typedef typename Vec<V>::T VT;
-    // the first slots' vectors are on their way while the weights are formed
-    constexpr int kEarly = 4;
-    VT early[kEarly];
+    // Vectors come in batches of kBatch at once, the first while the weights are formed.
+    constexpr int kBatch = 8;
+    VT x[kBatch];
+    auto fetch = [&](int t0) {
 #pragma unroll
-    for (int t = 0; t < kEarly; ++t)
-        if (t < total) early[t] = *reinterpret_cast<const VT*>(vec(t));
+        for (int t = 0; t < kBatch; ++t)
+            if (t0 + t < total) x[t] = *reinterpret_cast<const VT*>(vec(t0 + t));
+    };
+    fetch(0);
     float2 e = make_float2(-INFINITY, 0.f);
     if (lane < total) e = ml(lane);
     float M = e.x;
@@ -739,26 +765,22 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     const float ref = M == -INFINITY ? 0.f : M;
-    auto add = [&](float wt, const VT& x) {
-        const float* f = reinterpret_cast<const float*>(&x);
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(wt, f[i], acc[i]);
-    };
-    for (int j0 = 0; j0 < total; j0 += 32) {
-        if (j0 > 0) e = j0 + lane < total ? ml(j0 + lane) : make_float2(-INFINITY, 0.f);
-        const float w = e.x == -INFINITY ? 0.f : fast_exp2((e.x - ref) * a.qscale);
-        l = fmaf(w, e.y, l);
-        const int end = min(32, total - j0);
-        if (j0 == 0) {
-#pragma unroll
-            for (int t = 0; t < kEarly; ++t) {
-                const float wt = __shfl_sync(0xffffffffu, w, t);
-                if (t < total) add(wt, early[t]);
-            }
+    float w = 0.f;
+    for (int j0 = 0; j0 < total; j0 += kBatch) {
+        if (j0 % 32 == 0) {                                // weights of 32 slots, one a lane
+            if (j0 > 0) e = j0 + lane < total ? ml(j0 + lane) : make_float2(-INFINITY, 0.f);
+            w = e.x == -INFINITY ? 0.f : fast_exp2((e.x - ref) * a.qscale);
+            l = fmaf(w, e.y, l);
         }
-#pragma unroll 4
-        for (int t = j0 == 0 ? kEarly : 0; t < end; ++t)
-            add(__shfl_sync(0xffffffffu, w, t), *reinterpret_cast<const VT*>(vec(j0 + t)));
+        if (j0 > 0) fetch(j0);
+#pragma unroll
+        for (int t = 0; t < kBatch; ++t) {
+            const float wt = __shfl_sync(0xffffffffu, w, (j0 + t) % 32);
+            const float* f = reinterpret_cast<const float*>(&x[t]);
+            if (j0 + t < total)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] = fmaf(wt, f[i], acc[i]);
+        }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
@@ -772,13 +794,12 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
 // -- sizes ------------------------------------------------------------------------------------------
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-// Pages of a prefix chunk: halved from the whole prefix, down to 16, while the items are fewer than
-// two per SM.
+// Pages of a prefix chunk: as many chunks as keep every item resident at once (four CTAs an SM), of 8
+// pages at least.
 inline int prefix_chunk(int N, int G, int Hkv, int n_prefix, int sms) {
     const long groups = ceil_div((long)N * G, 8 * kWarps * kBlocks);
-    int c = n_prefix;
-    while (c > 16 && groups * Hkv * ceil_div(n_prefix, c) < 2L * sms) c = (c + 1) / 2;
-    return c > 0 ? c : 1;
+    const long chunks = std::max(1L, std::min(4L * sms / (groups * Hkv), n_prefix / 8L));
+    return n_prefix > 0 ? ceil_div(n_prefix, chunks) : 1;
 }
 
 // Sizes of the workspace's parts, in their order.
