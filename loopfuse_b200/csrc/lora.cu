@@ -388,6 +388,20 @@ expand_kernel(const Args g) {
             }
         }
     }
+    // h of the tile in registers for all blocks, where it fits (64 of a thread's at rank 64)
+    constexpr bool kHeld = R <= 64;
+    constexpr int MB = kTile / 16, KB = R / 16;
+    uint32_t ha[kHeld ? MB : 1][KB][4];
+    auto load_h = [&](int m, uint32_t (&a)[KB][4]) {
+#pragma unroll
+        for (int kk = 0; kk < KB; ++kk) ldsm4(sh + at<HC>(16 * m + (lane & 15), 2 * kk + (lane >> 4)), a[kk]);
+    };
+    if (kHeld && !copy_only) {
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < (kHeld ? MB : 1); ++m)
+            if (m < blocks) load_h(m, ha[m]);
+    }
     for (int blk = 0; blk < n_blocks; ++blk) {
         load(blk + 1);
         cp_wait<1>();
@@ -397,24 +411,21 @@ expand_kernel(const Args g) {
         if (!copy_only) {
             const int gq = lane >> 2, cq = lane & 3;
             constexpr int CJ = kCols / kExpandWarps / 16;   // 16-column pieces of a warp
-            uint32_t b[R / 16][CJ][4];                 // B of this warp's columns, for every row block
+            uint32_t b[KB][CJ][4];                     // B of this warp's columns, for every row block
 #pragma unroll
-            for (int kk = 0; kk < R / 16; ++kk)
+            for (int kk = 0; kk < KB; ++kk)
 #pragma unroll
                 for (int j = 0; j < CJ; ++j)
                     ldsm4_t(sb + at<YC>(16 * kk + (lane & 15), 2 * (CJ * warp + j) + (lane >> 4)), b[kk][j]);
-            for (int m = 0; m < blocks; ++m) {
+            auto rows16 = [&](int m, const uint32_t (&a)[KB][4]) {
                 float acc[2 * CJ][4] = {};
 #pragma unroll
-                for (int kk = 0; kk < R / 16; ++kk) {
-                    uint32_t a[4];
-                    ldsm4(sh + at<HC>(16 * m + (lane & 15), 2 * kk + (lane >> 4)), a);
+                for (int kk = 0; kk < KB; ++kk)
 #pragma unroll
                     for (int j = 0; j < CJ; ++j) {
-                        mma(acc[2 * j], a, b[kk][j][0], b[kk][j][1]);
-                        mma(acc[2 * j + 1], a, b[kk][j][2], b[kk][j][3]);
+                        mma(acc[2 * j], a[kk], b[kk][j][0], b[kk][j][1]);
+                        mma(acc[2 * j + 1], a[kk], b[kk][j][2], b[kk][j][3]);
                     }
-                }
 #pragma unroll
                 for (int j = 0; j < 2 * CJ; ++j)
 #pragma unroll
@@ -424,6 +435,17 @@ expand_kernel(const Args g) {
                         const uint32_t w = *p;
                         *p = pack_bf16x2(bf16lo_to_f32(w) + acc[j][2 * half], bf16hi_to_f32(w) + acc[j][2 * half + 1]);
                     }
+            };
+            if constexpr (kHeld) {
+#pragma unroll
+                for (int m = 0; m < MB; ++m)
+                    if (m < blocks) rows16(m, ha[m]);
+            } else {
+                for (int m = 0; m < blocks; ++m) {
+                    uint32_t a[KB][4];
+                    load_h(m, a);
+                    rows16(m, a);
+                }
             }
             __syncthreads();
         }
