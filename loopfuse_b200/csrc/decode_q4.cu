@@ -439,7 +439,10 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
     __shared__ long buf[kWarps];
     __shared__ long s_before[kWarps];          // units of one head before session s_n[w]
     __shared__ int s_n[kWarps];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // combine may be brought in
+    // Inputs are there after grid_wait(), or, behind the prefix kernel, from the start (it waited before
+    // it let this one begin); combine may read the lengths as soon as it is released.
+    if (a.n_chunks == 0) grid_wait();
+    grid_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     uint8_t* mem = smem + warp * OwnSmem<D>::kWarp;
     const uint8_t* qbuf = mem + kStages * UB;
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
             }
         } while (seg.next(a));
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");           // the prefix kernel's partials are there too
+    if (a.n_chunks > 0) grid_wait();                             // the prefix kernel's partials are there too
 }
 
 // -- shared prefix --------------------------------------------------------------------------------------
@@ -625,7 +628,8 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
     __shared__ __align__(8) uint64_t bars[kRing];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the own pages need nothing from here
+    grid_wait();
+    grid_release();                                              // the own pages need nothing from here
     const int chunk = blockIdx.x % a.n_chunks, h = blockIdx.x / a.n_chunks % a.Hkv;
     const int group = blockIdx.x / a.n_chunks / a.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -734,7 +738,7 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     const int n = (int)(row / a.Hq), hq = (int)(row % a.Hq), item = n * a.Hkv + hq / a.G;
     const int npages = (held(a, n) + kPage - 1) / kPage;
     const int chunks = a.n_prefix > 0 ? (min(npages, a.n_prefix) + a.chunk - 1) / a.chunk : 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");        // the partials are written
+    grid_wait();                                              // the partials are written
     int2 span = npages > a.n_prefix ? a.span[item] : make_int2(0, -1);
     span.x = max(0, min(span.x, a.ranges - 1));               // (a range that gave up leaves any bits there)
     span.y = max(span.x - 1, min(span.y, a.ranges - 1));
@@ -826,24 +830,6 @@ static int sm_count(int* out) {
     return LF_OK;
 }
 
-// `after`: may start while the stream's last kernel still runs (and waits for it itself).
-template <class... P, class... A>
-static int start(const char* what, bool after, void (*kernel)(P...), long blocks, size_t smem, cudaStream_t st, A... args) {
-    LF_CHECK_ARG(blocks <= 2147483647L, "%s: grid limits exceeded", what);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = after ? 1 : 0;
-    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-    return launch_status(what);
-}
-
 template <int D>
 static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st) {
     static PerContextOnce once;
@@ -855,16 +841,19 @@ static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st)
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
-    const long shared = (long)a.n_chunks * a.Hkv * a.groups;
+    const long shared = (long)a.n_chunks * a.Hkv * a.groups, rows = (long)a.N * a.Hq;
+    LF_CHECK_ARG(shared <= 2147483647L, "q4 decode: grid limits exceeded");
     if (shared > 0) {
-        rc = start("q4 decode prefix", false, prefix_kernel<D>, shared, PrefixSmem<D>::kBytes, st, a);
+        rc = launch_early("q4 decode prefix", prefix_kernel<D>, dim3((unsigned)shared), dim3(kThreads),
+                          PrefixSmem<D>::kBytes, st, a);
         if (rc != LF_OK) return rc;
     }
     if (a.ranges > 0) {
-        rc = start("q4 decode", shared > 0, own_kernel<D>, a.ranges / kWarps, OwnSmem<D>::kBytes, st, a);
+        rc = launch_early("q4 decode", own_kernel<D>, dim3(a.ranges / kWarps), dim3(kThreads), OwnSmem<D>::kBytes, st, a);
         if (rc != LF_OK) return rc;
     }
-    return start("q4 decode combine", true, combine_kernel<D>, ceil_div((long)a.N * a.Hq, kWarps), 0, st, a, o, lse);
+    return launch_early("q4 decode combine", combine_kernel<D>, dim3((unsigned)ceil_div(rows, kWarps)), dim3(kThreads),
+                        0, st, a, o, lse);
 }
 
 }  // namespace q4

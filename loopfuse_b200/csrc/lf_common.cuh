@@ -70,6 +70,30 @@ inline int launch_status(const char* what) {
     return LF_OK;
 }
 
+// A launch that may begin while the stream's last kernel still runs (programmatic dependent launch).
+// The kernel calls grid_wait() before it touches anything that kernel reads or writes, in every CTA
+// and on every path: a grid that ended without waiting would let its successor start too soon.
+template <class... P, class... A>
+int launch_early(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                 A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+    return launch_status(what);
+}
+// Returns once the kernels before this one in the stream are complete and their writes visible.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// From when every CTA has called this (or ended), the stream's next kernel may begin if launched early.
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // bf16 bit patterns -> fp32: a bf16 is the high half of the fp32 with the same value.

@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     };
 
     __shared__ float s_tok;
+    grid_wait();
     if (part == 0 && threadIdx.x == kThreads - 1) {    // the token's own logit, on its way meanwhile
         const int64_t tok = token(a, row);
         float f[2] = {0.f, 0.f};
@@ -477,12 +478,14 @@ static int launch(const Args& a, int rows, cudaStream_t st) {
     cfg.gridDim = dim3((unsigned)((long)rows * a.parts));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see launch_early
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)a.parts;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (a.k > 0) LF_CHECK_CUDA((cudaLaunchKernelEx(&cfg, logprobs_kernel<DT, true>, a)));
     else LF_CHECK_CUDA((cudaLaunchKernelEx(&cfg, logprobs_kernel<DT, false>, a)));
     return launch_status("token logprobs");

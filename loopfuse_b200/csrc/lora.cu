@@ -53,6 +53,7 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int
     int* off = sm + adapters + 1;                      // first sorted row
     int* til = off + adapters + 1;                     // first tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_wait();
     auto bucket = [&](int i) {
         const int a = ids[i];
         return a >= 0 && a < adapters ? a : adapters;
@@ -206,8 +207,8 @@ shrink_kernel(const Args g) {
     extern __shared__ __align__(128) uint8_t smem[];
     // x, y and the plan are there, and this memory's last readers are done; from here on the expansion
     // may be brought in and fetch y and B
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    grid_wait();
+    grid_release();
     const int tile = blockIdx.y, slice = blockIdx.x;
     if (tile >= g.head[0]) return;
     const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
@@ -327,7 +328,7 @@ expand_kernel(const Args g) {
     const int rows = t.z, first = t.y;
     const bool copy_only = t.x < 0;
     if (none || (copy_only && g.y == g.out)) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");      // no CTA ends before the kernel it follows
+        grid_wait();
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -359,7 +360,7 @@ expand_kernel(const Args g) {
         cp_commit();
     };
     load(0);
-    asm volatile("griddepcontrol.wait;" ::: "memory");          // h is there
+    grid_wait();                                                // h is there
     if (!copy_only) {
         if (g.slices == 1) {
             const uint16_t* h = reinterpret_cast<const uint16_t*>(g.part) + (long)first * R;
@@ -487,23 +488,11 @@ static int launch(const Args& g, int tiles, cudaStream_t st) {
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
-    // Both may start while the kernel before them still runs; they wait for it themselves.
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute pdl[1];
-    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    pdl[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = pdl;
-    cfg.numAttrs = 1;
-    cfg.stream = st;
-    cfg.gridDim = dim3(g.slices, tiles);
-    cfg.blockDim = dim3(32 * kShrinkWarps);
-    cfg.dynamicSmemBytes = ShrinkSmem<R>::kBytes;
-    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, shrink_kernel<R>, g));
-    cfg.gridDim = dim3(((g.N + kCols - 1) / kCols + g.cols - 1) / g.cols, tiles);
-    cfg.blockDim = dim3(32 * kExpandWarps);
-    cfg.dynamicSmemBytes = ExpandSmem<R>::kBytes;
-    LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, expand_kernel<R>, g));
-    return launch_status("lora expand");
+    const int e = launch_early("lora shrink", shrink_kernel<R>, dim3(g.slices, tiles), dim3(32 * kShrinkWarps),
+                               ShrinkSmem<R>::kBytes, st, g);
+    if (e != LF_OK) return e;
+    return launch_early("lora expand", expand_kernel<R>, dim3(((g.N + kCols - 1) / kCols + g.cols - 1) / g.cols, tiles),
+                        dim3(32 * kExpandWarps), ExpandSmem<R>::kBytes, st, g);
 }
 
 static int sm_count(int* out) {
@@ -550,9 +539,8 @@ extern "C" int lf_lora_plan(const int32_t* adapter_ids, const int32_t* cu_tokens
     });
     if (rc != LF_OK) return rc;
     const lora::Plan p = lora::views(static_cast<int32_t*>(plan), total_tokens, n, num_adapters);
-    lora::plan_kernel<<<1, pool::kMetaThreads, 3 * (num_adapters + 1) * 4, (cudaStream_t)stream>>>(
-        adapter_ids, cu_tokens, n, total_tokens, num_adapters, p);
-    return launch_status("lora plan");
+    return launch_early("lora plan", lora::plan_kernel, dim3(1), dim3(pool::kMetaThreads), 3 * (num_adapters + 1) * 4,
+                        (cudaStream_t)stream, adapter_ids, cu_tokens, n, total_tokens, num_adapters, p);
 }
 
 extern "C" int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int rank,

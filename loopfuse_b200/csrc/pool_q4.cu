@@ -49,6 +49,7 @@ template <int D>
 __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
     using F = Fmt<D>;
     constexpr int LPR = D / 8, RPW = 32 / LPR;          // lanes a row, rows a warp
+    grid_wait();
     if (a.status != nullptr && *reinterpret_cast<volatile int32_t*>(a.status) != LF_OK) return;
     const int H = a.Hq + 2 * a.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -220,6 +221,7 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
               int32_t* __restrict__ out_table, int N, int Hkv, int num_pages, int max_pages,
               int n_prefix, int out_pages) {
     using F = Fmt<D>;
+    grid_wait();
     const int chunks = (max_pages + kExpPages - 1) / kExpPages;
     const int n = blockIdx.x / chunks, j0 = (blockIdx.x % chunks) * kExpPages;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -372,7 +374,7 @@ extern "C" int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v
     if (n == 0 || total_tokens == 0) { clear_error(); return LF_OK; }
     LF_CHECK_ARG(k && v && block_table && start_pos && cu_tokens && pages, "q4 append: null pointer argument");
     LF_CHECK_ARG(head_dim == 64 || head_dim == 128, "q4 append: head_dim must be 64 or 128 (got %d)", head_dim);
-    LF_CHECK_ARG(num_q_heads >= 0 && num_kv_heads > 0 && num_pages > 0 && max_pages > 0 && table_rows > 0 &&
+    LF_CHECK_ARG(num_q_heads >= 0 && num_kv_heads > 0 && num_pages > 0 && max_pages > 0 && max_pages <= (1 << 26) && table_rows > 0 &&
                      num_layers > 0 && num_layers <= 65535,
                  "q4 append: bad shape");
     LF_CHECK_ARG(num_q_heads == 0 || (q && q_out && num_layers == 1), "q4 append: q needs q_out and one layer");
@@ -395,11 +397,8 @@ extern "C" int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v
     const int threads = 32 * (warps < most ? warps : most);
     const int blocks = total_tokens < 148 * 32 ? total_tokens : 148 * 32;
     const dim3 grid(blocks, num_layers);
-    if (head_dim == 128)
-        q4::append_kernel<128><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
-    else
-        q4::append_kernel<64><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
-    return launch_status("q4 append");
+    return launch_early("q4 append", head_dim == 128 ? q4::append_kernel<128> : q4::append_kernel<64>, grid,
+                        dim3(threads), 0, (cudaStream_t)stream, a);
 }
 
 extern "C" int lf_q4_expand(const void* pages, const int32_t* block_table, const int32_t* seq_lens,
@@ -412,20 +411,17 @@ extern "C" int lf_q4_expand(const void* pages, const int32_t* block_table, const
                      (out_pages == 0 || (k_out && v_out)),
                  "q4 expand: null pointer argument");
     LF_CHECK_ARG(head_dim == 64 || head_dim == 128, "q4 expand: head_dim must be 64 or 128 (got %d)", head_dim);
-    LF_CHECK_ARG(num_kv_heads > 0 && num_pages > 0 && max_pages > 0 && num_prefix_pages >= 0 &&
-                     num_prefix_pages <= max_pages,
+    LF_CHECK_ARG(num_kv_heads > 0 && num_pages > 0 && max_pages > 0 && max_pages <= (1 << 26) &&
+                     num_prefix_pages >= 0 && num_prefix_pages <= max_pages,
                  "q4 expand: bad shape");
     LF_CHECK_ARG(aligned16(pages) && (reinterpret_cast<uintptr_t>(k_out) & 31u) == 0 && aligned16(v_out),
                  "q4 expand: pages and v_out must be 16-byte aligned, k_out 32-byte aligned");
     const long blocks = (long)num_seqs * ((max_pages + q4::kExpPages - 1) / q4::kExpPages);
     LF_CHECK_ARG(blocks <= 2147483647L, "q4 expand: grid limits exceeded");
-    auto launch = [&](auto kernel) {
-        kernel<<<(unsigned)blocks, 32 * q4::kExpWarps, 0, (cudaStream_t)stream>>>(
-            static_cast<const uint8_t*>(pages), block_table, seq_lens, k_out, v_out, out_table, num_seqs,
-            num_kv_heads, num_pages, max_pages, num_prefix_pages, out_pages);
-    };
-    if (head_dim == 128) launch(q4::expand_kernel<128>); else launch(q4::expand_kernel<64>);
-    return launch_status("q4 expand");
+    return launch_early("q4 expand", head_dim == 128 ? q4::expand_kernel<128> : q4::expand_kernel<64>,
+                        dim3((unsigned)blocks), dim3(32 * q4::kExpWarps), 0, (cudaStream_t)stream,
+                        static_cast<const uint8_t*>(pages), block_table, seq_lens, k_out, v_out, out_table, num_seqs,
+                        num_kv_heads, num_pages, max_pages, num_prefix_pages, out_pages);
 }
 
 extern "C" int lf_q4_fork(const lf_pool_meta* m, int src_seq, const int32_t* dst_seqs, int n,
