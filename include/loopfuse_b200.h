@@ -395,7 +395,7 @@ int lf_pool_unregister_all(const lf_pool_meta* m, const lf_prefix_registry* r, v
  * rotated as in lf_pool_write_qkv first.  pages is [num_layers][num_pages][Hkv][18 * D].  A row
  * without a page, or past the rotation table, is not stored: *status (nullable, a pool's sticky
  * status; nothing is done when it is already set) becomes LF_EINVAL, or, without a status, the
- * device error word 222.  Strides multiples of 8, buffers 16-byte aligned. */
+ * device error word 252.  Strides multiples of 8, buffers 16-byte aligned. */
 int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v, int64_t q_stride_token,
                  int64_t stride_layer, int64_t stride_token, int64_t stride_head,
                  const int32_t* block_table, int table_rows, int max_pages, const int32_t* seq_ids,
@@ -409,8 +409,8 @@ int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v, int64_t q
  * each session's own pages in session order; out_table [num_seqs][max_pages] holds their ids (-1
  * past a session's pages).  Rows at or past a session's length are zeros; output pages past the
  * last session's are not written.  A session whose pages do not fit in out_pages is cut off there,
- * with -1 in out_table and the device error word 223; a page id outside [0, num_pages) reads page 0
- * (word 224).  k_out 32-byte aligned. */
+ * with -1 in out_table and the device error word 253; a page id outside [0, num_pages) reads page 0
+ * (word 254).  k_out 32-byte aligned. */
 int lf_q4_expand(const void* pages, const int32_t* block_table, const int32_t* seq_lens,
                  int num_prefix_pages, lf_bf16* k_out, lf_bf16* v_out, int32_t* out_table,
                  int num_seqs, int num_kv_heads, int head_dim, int num_pages, int max_pages,

@@ -27,16 +27,16 @@
 //           the chip alike and a warp starts up once.  A warp works alone, with a ring of kStages
 //           units whose copies run on across heads and sessions (the queries of a head come with
 //           its first unit).  The columns are the GQA group's heads.
-//   prefix  (chunk, KV head, group of 4 * 8/G sessions): the pages of a shared prefix; the 8 columns of
-//           a warp are G heads of 8/G sessions, and the four warps use the same staged pages, so
-//           that a prefix page is read once per 32 columns.  A kernel of its own, next to which the
-//           own one starts.  (Two blocks of 8 columns a warp, unpacking a page once for both: 227
-//           registers and half the warps, 65.6 against 57.6 us with 64 sessions on 4096 tokens.)
+//   prefix  the pages of a shared prefix, a kernel of its own, next to which the own one starts.  Long
+//           prefixes of many rows go to tiles of 128 rows on tcgen05 (decode_q4_prefix.cuh); here:
+//           (chunk, KV head, group of 4 * 8/G sessions): the 8 columns of a warp are G heads of 8/G
+//           sessions, and the four warps use the same staged pages, so that a prefix page is read once
+//           per 32 columns.
 // Every piece writes unnormalised fp32 partials (o, max, sum); a range's piece of item (session, KV
 // head) is partial number range + item, which no two pieces share as both grow along the ranges.
 // combine merges a row's partials, in order.
 //
-// Every barrier wait is bounded (site 221 in the device error word); a warp that gives up stops
+// Every barrier wait is bounded (site 251 in the device error word); a warp that gives up stops
 // computing and lets the copies in flight land, bounded again, before it leaves.
 #include "decode_common.cuh"
 #include "q4_common.cuh"
@@ -45,6 +45,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace lf {
 namespace q4 {
@@ -57,7 +58,6 @@ constexpr int kUnit = 2;                       // own: pages of a barrier, a sof
 constexpr int kStages = 2;                     // own: units in flight per warp
 constexpr int per_sm(int D) { return D == 64 ? 4 : 3; }   // own: resident CTAs of an SM (registers)
 constexpr int kMinUnits = 2;                   // own: units of a range
-constexpr int kBlocks = 1;                     // prefix: blocks of 8 columns of a warp
 constexpr int kRing = 16;                      // prefix: pages staged in a CTA, in two halves
 constexpr uint64_t kWaitNs = 2000000000ull;
 
@@ -144,21 +144,20 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     return r;
 }
 
-// A warp's attention state: B blocks of 8 columns (query rows), of which this lane holds 2c and
-// 2c + 1.  Scores and maxima are kept as q . k 2^-69 (q's sign carries the scale's).
-template <int D, int B, int U>
+// A warp's attention state: 8 columns (query rows), of which this lane holds 2c and 2c + 1.  Scores and maxima are kept as q . k 2^-69 (q's sign carries the scale's).
+template <int D, int U>
 struct State {
     static constexpr int NG = Fmt<D>::NG;
-    uint32_t qb[B][NG][4][2];                  // Q^T operand, column g: q 2^64, q 2^60
-    float qsum[B][NG][2];                      // sums of columns 2c, 2c + 1 over each group, 2^-69
-    float o[B][NG][4][4];                      // O^T: m-tile (16 dims) x 4; 2^-69, 2^-65 in rows g + 8
-    float corr[B][NG][4];                      // -8 sum(bf16(p s)): the same in every m-tile
-    float bias[B][NG][2];                      // this lane's share of sum p (b + 8 s)
-    float m[B][2], l[B][2];
+    uint32_t qb[NG][4][2];                     // Q^T operand, column g: q 2^64, q 2^60
+    float qsum[NG][2];                         // sums of columns 2c, 2c + 1 over each group, 2^-69
+    float o[NG][4][4];                         // O^T: m-tile (16 dims) x 4; 2^-69, 2^-65 in rows g + 8
+    float corr[NG][4];                         // -8 sum(bf16(p s)): the same in every m-tile
+    float bias[NG][2];                         // this lane's share of sum p (b + 8 s)
+    float m[2], l[2];
 
     // `row` is column g's query row (null: the column is unused); `flip` is 0x80008000 for a
     // negative scale.
-    __device__ __forceinline__ void init(int b, const uint16_t* row, uint32_t flip, int c) {
+    __device__ __forceinline__ void init(const uint16_t* row, uint32_t flip, int c) {
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
             uint4 x = make_uint4(0, 0, 0, 0), y = x;
@@ -170,33 +169,33 @@ struct State {
             float part = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                qb[b][gr][k / 2][k % 2] = mul_bf16x2(w[k] ^ flip, k % 2 == 0 ? 0x5F805F80u : 0x5D805D80u);
+                qb[gr][k / 2][k % 2] = mul_bf16x2(w[k] ^ flip, k % 2 == 0 ? 0x5F805F80u : 0x5D805D80u);
                 part += bf16lo_to_f32(w[k] ^ flip) + bf16hi_to_f32(w[k] ^ flip);
             }
             part += __shfl_xor_sync(0xffffffffu, part, 1);
             part += __shfl_xor_sync(0xffffffffu, part, 2);
             part *= 1.f / kDown;
-            qsum[b][gr][0] = __shfl_sync(0xffffffffu, part, 8 * c);
-            qsum[b][gr][1] = __shfl_sync(0xffffffffu, part, 8 * c + 4);
-            bias[b][gr][0] = bias[b][gr][1] = 0.f;
+            qsum[gr][0] = __shfl_sync(0xffffffffu, part, 8 * c);
+            qsum[gr][1] = __shfl_sync(0xffffffffu, part, 8 * c + 4);
+            bias[gr][0] = bias[gr][1] = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                corr[b][gr][k] = 0.f;
+                corr[gr][k] = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[b][gr][k][j] = 0.f;
+                for (int j = 0; j < 4; ++j) o[gr][k][j] = 0.f;
             }
         }
-        m[b][0] = m[b][1] = -INFINITY;
-        l[b][0] = l[b][1] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
     }
 
-    // Applies U staged pages, tokens tok0 .. tok0 + 16 U - 1; len[b] are the lengths of the
-    // lane's columns.  kMasked: some token may be at or past a column's length.  Such tokens take no
-    // part, whatever their codes and scales hold.
+    // Applies U staged pages, tokens tok0 .. tok0 + 16 U - 1; len: the lengths of the lane's columns.
+    // kMasked: some token may be at or past a column's length.  Such tokens take no part, whatever
+    // their codes and scales hold.
     template <bool kMasked>
-    __device__ __forceinline__ void unit(uint32_t base, int tok0, const int (&len)[B][2], float qscale, int lane) {
+    __device__ __forceinline__ void unit(uint32_t base, int tok0, const int (&len)[2], float qscale, int lane) {
         const int g = lane >> 2, c = lane & 3;
-        float s[B][U][4];                  // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
+        float s[U][4];                     // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
         uint32_t vp[U][2][NG];             // V params of tokens g, g + 8
 #pragma unroll
         for (int pg = 0; pg < U; ++pg) {
@@ -210,109 +209,98 @@ struct State {
             for (int gr = 0; gr < NG; ++gr) {
                 vp[pg][0][gr] = pa[NG + gr];
                 vp[pg][1][gr] = pb[NG + gr];
-                float acc[B][4];
+                float acc[4];
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const uint32_t a0 = codes(ka[2 * gr + w], 2 * k), a1 = codes(kb[2 * gr + w], 2 * k);
                         const uint32_t a2 = codes(ka[2 * gr + w], 2 * k + 1), a3 = codes(kb[2 * gr + w], 2 * k + 1);
-#pragma unroll
-                        for (int b = 0; b < B; ++b) {
-                            if (w == 0 && k == 0) {
-                                const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma(acc[b], a0, a1, a2, a3, qb[b][gr][0][0], qb[b][gr][0][1], zero);
-                            } else {
-                                mma(acc[b], a0, a1, a2, a3, qb[b][gr][2 * w + k][0], qb[b][gr][2 * w + k][1], acc[b]);
-                            }
+                        if (w == 0 && k == 0) {
+                            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma(acc, a0, a1, a2, a3, qb[gr][0][0], qb[gr][0][1], zero);
+                        } else {
+                            mma(acc, a0, a1, a2, a3, qb[gr][2 * w + k][0], qb[gr][2 * w + k][1], acc);
                         }
                     }
                 const float sa = bf16lo_to_f32(pa[gr]), sb = bf16lo_to_f32(pb[gr]);
                 const float ba = bf16hi_to_f32(pa[gr]), bb = bf16hi_to_f32(pb[gr]);
-#pragma unroll
-                for (int b = 0; b < B; ++b) {
-                    float(&t)[4] = s[b][pg];
-                    if (gr == 0) {
-                        t[0] = ba * qsum[b][gr][0];
-                        t[1] = ba * qsum[b][gr][1];
-                        t[2] = bb * qsum[b][gr][0];
-                        t[3] = bb * qsum[b][gr][1];
-                    } else {
-                        t[0] = fmaf(ba, qsum[b][gr][0], t[0]);
-                        t[1] = fmaf(ba, qsum[b][gr][1], t[1]);
-                        t[2] = fmaf(bb, qsum[b][gr][0], t[2]);
-                        t[3] = fmaf(bb, qsum[b][gr][1], t[3]);
-                    }
-                    t[0] = fmaf(sa, acc[b][0], t[0]);
-                    t[1] = fmaf(sa, acc[b][1], t[1]);
-                    t[2] = fmaf(sb, acc[b][2], t[2]);
-                    t[3] = fmaf(sb, acc[b][3], t[3]);
+                float(&t)[4] = s[pg];
+                if (gr == 0) {
+                    t[0] = ba * qsum[gr][0];
+                    t[1] = ba * qsum[gr][1];
+                    t[2] = bb * qsum[gr][0];
+                    t[3] = bb * qsum[gr][1];
+                } else {
+                    t[0] = fmaf(ba, qsum[gr][0], t[0]);
+                    t[1] = fmaf(ba, qsum[gr][1], t[1]);
+                    t[2] = fmaf(bb, qsum[gr][0], t[2]);
+                    t[3] = fmaf(bb, qsum[gr][1], t[3]);
                 }
+                t[0] = fmaf(sa, acc[0], t[0]);
+                t[1] = fmaf(sa, acc[1], t[1]);
+                t[2] = fmaf(sb, acc[2], t[2]);
+                t[3] = fmaf(sb, acc[3], t[3]);
             }
         }
-        bool keep[B][U][4];
+        bool keep[U][4];
         if (kMasked) {
-#pragma unroll
-            for (int b = 0; b < B; ++b)
 #pragma unroll
                 for (int pg = 0; pg < U; ++pg)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        keep[b][pg][j] = tok0 + kPage * pg + g + 8 * (j / 2) < len[b][j % 2];
-                        s[b][pg][j] = keep[b][pg][j] ? s[b][pg][j] : -INFINITY;
+                        keep[pg][j] = tok0 + kPage * pg + g + 8 * (j / 2) < len[j % 2];
+                        s[pg][j] = keep[pg][j] ? s[pg][j] : -INFINITY;
                     }
         }
+        float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]);
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            float x0 = fmaxf(s[b][0][0], s[b][0][2]), x1 = fmaxf(s[b][0][1], s[b][0][3]);
+        for (int pg = 1; pg < U; ++pg) {
+            x0 = fmaxf(x0, fmaxf(s[pg][0], s[pg][2]));
+            x1 = fmaxf(x1, fmaxf(s[pg][1], s[pg][3]));
+        }
+        // Only lanes of the column need agree, and only when the maximum grows.
+        if (__any_sync(0xffffffffu, x0 > m[0] || x1 > m[1])) {
 #pragma unroll
-            for (int pg = 1; pg < U; ++pg) {
-                x0 = fmaxf(x0, fmaxf(s[b][pg][0], s[b][pg][2]));
-                x1 = fmaxf(x1, fmaxf(s[b][pg][1], s[b][pg][3]));
+            for (int off = 4; off < 32; off <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
             }
-            // Only lanes of the column need agree, and only when the maximum grows.
-            if (__any_sync(0xffffffffu, x0 > m[b][0] || x1 > m[b][1])) {
+            const float n0 = fmaxf(m[0], x0), n1 = fmaxf(m[1], x1);
+            const float a0 = m[0] == n0 ? 1.f : fast_exp2((m[0] - n0) * qscale);
+            const float a1 = m[1] == n1 ? 1.f : fast_exp2((m[1] - n1) * qscale);
+            // (a column that had met no token has sums of zero: any finite factor will do)
+            const float f0 = m[0] == -INFINITY ? 0.f : a0, f1 = m[1] == -INFINITY ? 0.f : a1;
+            m[0] = n0;
+            m[1] = n1;
+            l[0] *= f0;
+            l[1] *= f1;
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
-                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
-                }
-                const float n0 = fmaxf(m[b][0], x0), n1 = fmaxf(m[b][1], x1);
-                const float a0 = m[b][0] == n0 ? 1.f : fast_exp2((m[b][0] - n0) * qscale);
-                const float a1 = m[b][1] == n1 ? 1.f : fast_exp2((m[b][1] - n1) * qscale);
-                // (a column that had met no token has sums of zero: any finite factor will do)
-                const float f0 = m[b][0] == -INFINITY ? 0.f : a0, f1 = m[b][1] == -INFINITY ? 0.f : a1;
-                m[b][0] = n0;
-                m[b][1] = n1;
-                l[b][0] *= f0;
-                l[b][1] *= f1;
+            for (int gr = 0; gr < NG; ++gr) {
+                bias[gr][0] *= f0;
+                bias[gr][1] *= f1;
 #pragma unroll
-                for (int gr = 0; gr < NG; ++gr) {
-                    bias[b][gr][0] *= f0;
-                    bias[b][gr][1] *= f1;
+                for (int j = 0; j < 4; ++j) corr[gr][j] *= (j & 1) ? f1 : f0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) corr[b][gr][j] *= (j & 1) ? f1 : f0;
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) o[b][gr][k][j] *= (j & 1) ? f1 : f0;
-                }
+                    for (int j = 0; j < 4; ++j) o[gr][k][j] *= (j & 1) ? f1 : f0;
             }
-            // a column that has met no token yet keeps a maximum of -inf; its scores are all -inf
-            const float r0 = (kMasked && m[b][0] == -INFINITY) ? 0.f : m[b][0] * -qscale;
-            const float r1 = (kMasked && m[b][1] == -INFINITY) ? 0.f : m[b][1] * -qscale;
+        }
+        // a column that has met no token yet keeps a maximum of -inf; its scores are all -inf
+        const float r0 = (kMasked && m[0] == -INFINITY) ? 0.f : m[0] * -qscale;
+        const float r1 = (kMasked && m[1] == -INFINITY) ? 0.f : m[1] * -qscale;
 #pragma unroll
-            for (int pg = 0; pg < U; ++pg)
+        for (int pg = 0; pg < U; ++pg)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float e = fast_exp2(fmaf(s[b][pg][j], qscale, (j & 1) ? r1 : r0));
-                    s[b][pg][j] = !kMasked || keep[b][pg][j] ? e : 0.f;
-                }
-#pragma unroll
-            for (int pg = 0; pg < U; ++pg) {
-                l[b][0] += s[b][pg][0] + s[b][pg][2];
-                l[b][1] += s[b][pg][1] + s[b][pg][3];
+            for (int j = 0; j < 4; ++j) {
+                const float e = fast_exp2(fmaf(s[pg][j], qscale, (j & 1) ? r1 : r0));
+                s[pg][j] = !kMasked || keep[pg][j] ? e : 0.f;
             }
+#pragma unroll
+        for (int pg = 0; pg < U; ++pg) {
+            l[0] += s[pg][0] + s[pg][2];
+            l[1] += s[pg][1] + s[pg][3];
         }
 #pragma unroll
         for (int pg = 0; pg < U; ++pg) {
@@ -326,34 +314,29 @@ struct State {
                 const float ba = fmaf(8.f, sa, bf16hi_to_f32(vp[pg][0][gr]));
                 const float bb = fmaf(8.f, sb, bf16hi_to_f32(vp[pg][1][gr]));
                 const float ua = sa * kUp, ub = sb * kUp;
-                uint32_t b0[B], b1[B];
+                uint32_t b0, b1;
+                const float(&e)[4] = s[pg];
+                float p[4] = {e[0] * ua, e[1] * ua, e[2] * ub, e[3] * ub};
+                if (kMasked) {
 #pragma unroll
-                for (int b = 0; b < B; ++b) {
-                    const float(&e)[4] = s[b][pg];
-                    float p[4] = {e[0] * ua, e[1] * ua, e[2] * ub, e[3] * ub};
-                    if (kMasked) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) p[j] = keep[b][pg][j] ? p[j] : 0.f;
-                        bias[b][gr][0] += (keep[b][pg][0] ? e[0] * ba : 0.f) + (keep[b][pg][2] ? e[2] * bb : 0.f);
-                        bias[b][gr][1] += (keep[b][pg][1] ? e[1] * ba : 0.f) + (keep[b][pg][3] ? e[3] * bb : 0.f);
-                    } else {
-                        bias[b][gr][0] = fmaf(e[0], ba, fmaf(e[2], bb, bias[b][gr][0]));
-                        bias[b][gr][1] = fmaf(e[1], ba, fmaf(e[3], bb, bias[b][gr][1]));
-                    }
-                    b0[b] = movm_t(pack_bf16x2(p[0], p[1]));
-                    b1[b] = movm_t(pack_bf16x2(p[2], p[3]));
-                    // -8 2^-133 in rows g, -128 2^-133 in rows g + 8
-                    mma(corr[b][gr], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0[b], b1[b], corr[b][gr]);
+                    for (int j = 0; j < 4; ++j) p[j] = keep[pg][j] ? p[j] : 0.f;
+                    bias[gr][0] += (keep[pg][0] ? e[0] * ba : 0.f) + (keep[pg][2] ? e[2] * bb : 0.f);
+                    bias[gr][1] += (keep[pg][1] ? e[1] * ba : 0.f) + (keep[pg][3] ? e[3] * bb : 0.f);
+                } else {
+                    bias[gr][0] = fmaf(e[0], ba, fmaf(e[2], bb, bias[gr][0]));
+                    bias[gr][1] = fmaf(e[1], ba, fmaf(e[3], bb, bias[gr][1]));
                 }
+                b0 = movm_t(pack_bf16x2(p[0], p[1]));
+                b1 = movm_t(pack_bf16x2(p[2], p[3]));
+                // -8 2^-133 in rows g, -128 2^-133 in rows g + 8
+                mma(corr[gr], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1, corr[gr]);
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const uint32_t a0 = codes(va[2 * gr + w], 2 * k), a1 = codes(va[2 * gr + w], 2 * k + 1);
                         const uint32_t a2 = codes(vb[2 * gr + w], 2 * k), a3 = codes(vb[2 * gr + w], 2 * k + 1);
-#pragma unroll
-                        for (int b = 0; b < B; ++b)
-                            mma(o[b][gr][2 * w + k], a0, a1, a2, a3, b0[b], b1[b], o[b][gr][2 * w + k]);
+                            mma(o[gr][2 * w + k], a0, a1, a2, a3, b0, b1, o[gr][2 * w + k]);
                     }
             }
         }
@@ -362,25 +345,22 @@ struct State {
     // Sums over the lanes that share a column; o then holds the whole unnormalised rows.
     __device__ __forceinline__ void finish() {
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
+        for (int off = 4; off < 32; off <<= 1) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], off);
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-                l[b][0] += __shfl_xor_sync(0xffffffffu, l[b][0], off);
-                l[b][1] += __shfl_xor_sync(0xffffffffu, l[b][1], off);
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr) {
-                    bias[b][gr][0] += __shfl_xor_sync(0xffffffffu, bias[b][gr][0], off);
-                    bias[b][gr][1] += __shfl_xor_sync(0xffffffffu, bias[b][gr][1], off);
-                }
+            for (int gr = 0; gr < NG; ++gr) {
+                bias[gr][0] += __shfl_xor_sync(0xffffffffu, bias[gr][0], off);
+                bias[gr][1] += __shfl_xor_sync(0xffffffffu, bias[gr][1], off);
             }
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        o[b][gr][k][j] = fmaf(o[b][gr][k][j] + corr[b][gr][j], j < 2 ? kDown : kDown / 16.f, bias[b][gr][j & 1]);
         }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[gr][k][j] = fmaf(o[gr][k][j] + corr[gr][j], j < 2 ? kDown : kDown / 16.f, bias[gr][j & 1]);
     }
 };
 
@@ -562,13 +542,13 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
         bool failed = false;
         do {
             const int item = seg.n * a.Hkv + seg.h, L = seg.L;
-            const int len[1][2] = {{L, L}};
-            State<D, 1, kUnit> st;
+            const int len[2] = {L, L};
+            State<D, kUnit> st;
             for (int j = seg.j; j < seg.j1; ++j) {
                 const int sl = used % kStages;
                 if (!warp_wait(bar + 8 * sl, (used / kStages) & 1)) {
                     if (lane == 0) {
-                        atomicCAS(&g_device_error, 0, 221);      // let the copies in flight land
+                        atomicCAS(&g_device_error, 0, 251);      // let the copies in flight land
                         for (uint32_t k = used; k < issued; ++k) wait_full(bar + 8 * (k % kStages), (k / kStages) & 1);
                     }
                     failed = true;
@@ -576,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
                 }
                 if (j == seg.j) {
                     const uint16_t* rows = reinterpret_cast<const uint16_t*>(qbuf + (q_out & 1) * OwnSmem<D>::kQ);
-                    st.init(0, g < a.G ? rows + g * D : nullptr, a.flip, c);
+                    st.init(g < a.G ? rows + g * D : nullptr, a.flip, c);
                     ++q_out;
                 }
                 const uint32_t blk = ring + (uint32_t)(sl * UB);
@@ -600,9 +580,9 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
 #pragma unroll
                     for (int k = 0; k < 4; k += 2)
                         *reinterpret_cast<float4*>(dst + out_dim(gr, k, g)) =
-                            make_float4(st.o[0][gr][k][col], st.o[0][gr][k][2 + col],
-                                        st.o[0][gr][k + 1][col], st.o[0][gr][k + 1][2 + col]);
-                if (g == 0) a.own_ml[slot + 2 * c + col] = make_float2(st.m[0][col], st.l[0][col]);
+                            make_float4(st.o[gr][k][col], st.o[gr][k][2 + col],
+                                        st.o[gr][k + 1][col], st.o[gr][k + 1][2 + col]);
+                if (g == 0) a.own_ml[slot + 2 * c + col] = make_float2(st.m[col], st.l[col]);
             }
             if (lane == 0) {
                 if (seg.j == 0) a.span[item].x = range;
@@ -619,8 +599,7 @@ struct PrefixSmem {
     static constexpr int kBytes = kRing * Fmt<D>::kBlockBytes + 128;
 };
 
-// One chunk of the prefix for the sessions of four warps (kBlocks blocks of 8 columns each) of one KV
-// head.  The staged pages are a ring of two halves, refilled half by half after a CTA barrier.
+// One chunk of the prefix for the sessions of four warps (8 columns each) of one KV head.  The staged pages are a ring of two halves, refilled half by half after a CTA barrier.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a) {
     using F = Fmt<D>;
@@ -634,12 +613,12 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
     const int group = blockIdx.x / a.n_chunks / a.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int spb = 8 / a.G;                                     // sessions of a block
-    const int first = group * kWarps * kBlocks * spb;
+    const int first = group * kWarps * spb;
     const int p_begin = chunk * a.chunk, p_end = min(p_begin + a.chunk, a.n_prefix);
     // The page ids come from the group's longest session, whose row holds every page that any
     // session here needs; pages past its length are not read.
     int best = -1, lead = first;
-    for (int i = lane; i < kWarps * kBlocks * spb; i += 32) {
+    for (int i = lane; i < kWarps * spb; i += 32) {
         const int L = held(a, first + i);
         if (L > best) { best = L; lead = first + i; }
     }
@@ -670,16 +649,11 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
     };
     issue_half(0);
     issue_half(kHalf);
-    State<D, kBlocks, 1> st;
-    int len[kBlocks][2], lmin = 0x7FFFFFFF;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-        const int base = first + (warp * kBlocks + b) * spb, n_g = base + g / a.G;
-        len[b][0] = held(a, base + (2 * c) / a.G);
-        len[b][1] = held(a, base + (2 * c + 1) / a.G);
-        lmin = min(lmin, min(len[b][0], len[b][1]));
-        st.init(b, n_g < a.N ? a.q + ((size_t)n_g * a.Hq + h * a.G + g % a.G) * D : nullptr, a.flip, c);
-    }
+    State<D, 1> st;
+    const int base = first + warp * spb, n_g = base + g / a.G;
+    const int len[2] = {held(a, base + (2 * c) / a.G), held(a, base + (2 * c + 1) / a.G)};
+    int lmin = min(len[0], len[1]);
+    st.init(n_g < a.N ? a.q + ((size_t)n_g * a.Hq + h * a.G + g % a.G) * D : nullptr, a.flip, c);
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) lmin = min(lmin, __shfl_xor_sync(0xffffffffu, lmin, off));
     bool failed = false;
@@ -687,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
         for (int k = k0; k < min(k0 + kHalf, pages); ++k) {
             const int sl = k % kRing;
             if (!failed && !warp_wait(bar + 8 * sl, (uint32_t)((k / kRing) & 1))) {
-                if (lane == 0) atomicCAS(&g_device_error, 0, 221);
+                if (lane == 0) atomicCAS(&g_device_error, 0, 251);
                 failed = true;
             }
             if (failed) continue;
@@ -706,22 +680,27 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
     st.finish();
     // rows of columns 2c and 2c + 1 go straight to their slots
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
+    for (int col = 0; col < 2; ++col) {
+        const int j = 2 * c + col, n = base + j / a.G;
+        if (n >= a.N) continue;
+        const size_t slot = ((size_t)n * a.Hq + h * a.G + j % a.G) * a.n_chunks + chunk;
 #pragma unroll
-        for (int col = 0; col < 2; ++col) {
-            const int j = 2 * c + col, n = first + (warp * kBlocks + b) * spb + j / a.G;
-            if (n >= a.N) continue;
-            const size_t slot = ((size_t)n * a.Hq + h * a.G + j % a.G) * a.n_chunks + chunk;
+        for (int gr = 0; gr < F::NG; ++gr)
 #pragma unroll
-            for (int gr = 0; gr < F::NG; ++gr)
-#pragma unroll
-                for (int k = 0; k < 4; k += 2)
-                    *reinterpret_cast<float4*>(a.pre_o + slot * D + out_dim(gr, k, g)) =
-                        make_float4(st.o[b][gr][k][col], st.o[b][gr][k][2 + col],
-                                    st.o[b][gr][k + 1][col], st.o[b][gr][k + 1][2 + col]);
-            if (g == 0) a.pre_ml[slot] = make_float2(st.m[b][col], st.l[b][col]);
-        }
+            for (int k = 0; k < 4; k += 2)
+                *reinterpret_cast<float4*>(a.pre_o + slot * D + out_dim(gr, k, g)) =
+                    make_float4(st.o[gr][k][col], st.o[gr][k][2 + col], st.o[gr][k + 1][col], st.o[gr][k + 1][2 + col]);
+        if (g == 0) a.pre_ml[slot] = make_float2(st.m[col], st.l[col]);
+    }
 }
+
+}  // namespace q4
+}  // namespace lf
+
+#include "decode_q4_prefix.cuh"
+
+namespace lf {
+namespace q4 {
 
 template <int V> struct Vec;
 template <> struct Vec<2> { typedef float2 T; };
@@ -798,12 +777,29 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
 // -- sizes ------------------------------------------------------------------------------------------
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-// Pages of a prefix chunk: as many chunks as keep every item resident at once (four CTAs an SM), of 8
-// pages at least.
-inline int prefix_chunk(int N, int G, int Hkv, int n_prefix, int sms) {
-    const long groups = ceil_div((long)N * G, 8 * kWarps * kBlocks);
+// Whether the prefix goes to tiles of 128 rows on tcgen05.  Both forms' times grow with rows x pages x
+// heads, the tiles' at less than half the rate but from 4 us more (barriers, tensor memory, more code to
+// fetch); they meet at about 2^25 row-pages x KV heads x dims.  Rows 64 x heads 8 of 128: 1024 pages 45
+// against 47 us, 512 pages 36 : 33; 128 rows: 512 pages 39 : 45, 256 pages 33 : 31; 256 rows: 512 pages
+// 47 : 74, 256 pages 37 : 45, 128 pages 31 : 31, 64 pages 29 : 25; 400 rows: 128 pages 36 : 41, 64 pages
+// 31 : 29.  64 dims: 512 rows x 4 heads: 512 pages 37 : 51, 256 pages 29 : 33, 128 pages 25 : 25.
+// (Decode times, a few own pages included.)  Up to 64 rows a tile is too empty.
+inline bool prefix_on_tc(int N, int G, int Hkv, int D, int n_prefix) {
+    return (long)N * G > 64 && (long)N * G * n_prefix * Hkv * D >= (1L << 25);
+}
+
+// Pages of a prefix chunk: as many chunks as keep every CTA resident at once (kTcPerSm an SM, of whole
+// steps; or four an SM, of 8 pages at least).
+inline int prefix_chunk(int N, int G, int Hkv, int D, int n_prefix, int sms) {
+    if (n_prefix <= 0) return 1;
+    if (prefix_on_tc(N, G, Hkv, D, n_prefix)) {
+        const long tiles = ceil_div((long)N * G, kTcRows), steps = ceil_div(n_prefix, kTcPages);
+        const long chunks = std::max(1L, std::min((long)kTcPerSm * sms / (tiles * Hkv), steps));
+        return ceil_div(steps, chunks) * kTcPages;
+    }
+    const long groups = ceil_div((long)N * G, 8 * kWarps);
     const long chunks = std::max(1L, std::min(4L * sms / (groups * Hkv), n_prefix / 8L));
-    return n_prefix > 0 ? ceil_div(n_prefix, chunks) : 1;
+    return ceil_div(n_prefix, chunks);
 }
 
 // Sizes of the workspace's parts, in their order.
@@ -817,7 +813,7 @@ inline Sizes sizes(int N, int Hq, int Hkv, int D, int n_prefix, int max_pages, i
     s.ranges = n_prefix < max_pages ? per_sm(D) * sms * kWarps : 0;
     s.items = (size_t)N * Hkv;
     s.own = s.ranges > 0 ? (s.ranges + s.items) * (Hq / Hkv) : 0;
-    s.chunk = prefix_chunk(N, Hq / Hkv, Hkv, n_prefix, sms);
+    s.chunk = prefix_chunk(N, Hq / Hkv, Hkv, D, n_prefix, sms);
     s.n_chunks = ceil_div(n_prefix, s.chunk);
     s.pre = (size_t)N * Hq * s.n_chunks;
     return s;
@@ -838,14 +834,19 @@ static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st)
                                            OwnSmem<D>::kBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            PrefixSmem<D>::kBytes));
+        LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           TcSmem<D>::kBytes));
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
     const long shared = (long)a.n_chunks * a.Hkv * a.groups, rows = (long)a.N * a.Hq;
     LF_CHECK_ARG(shared <= 2147483647L, "q4 decode: grid limits exceeded");
     if (shared > 0) {
-        rc = launch_early("q4 decode prefix", prefix_kernel<D>, dim3((unsigned)shared), dim3(kThreads),
-                          PrefixSmem<D>::kBytes, st, a);
+        rc = prefix_on_tc(a.N, a.G, a.Hkv, D, a.n_prefix)
+                 ? launch_early("q4 decode prefix", prefix_tc_kernel<D>, dim3((unsigned)shared), dim3(kTcThreads),
+                                TcSmem<D>::kBytes, st, a)
+                 : launch_early("q4 decode prefix", prefix_kernel<D>, dim3((unsigned)shared), dim3(kThreads),
+                                PrefixSmem<D>::kBytes, st, a);
         if (rc != LF_OK) return rc;
     }
     if (a.ranges > 0) {
@@ -922,7 +923,9 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
     a.n_prefix = num_prefix_pages;
     a.chunk = z.chunk;
     a.n_chunks = z.n_chunks;
-    a.groups = q4::ceil_div(num_seqs, q4::kWarps * q4::kBlocks * (8 / G));
+    a.groups = q4::prefix_on_tc(num_seqs, G, num_kv_heads, head_dim, num_prefix_pages)
+                   ? q4::ceil_div((long)num_seqs * G, q4::kTcRows)
+                   : q4::ceil_div(num_seqs, q4::kWarps * (8 / G));
     a.ranges = z.ranges;
     a.qscale = fabsf(scale) * kLog2e * q4::kDown;
     a.flip = scale < 0.f ? 0x80008000u : 0u;

@@ -37,7 +37,7 @@ struct AppendArgs {
 
 __device__ __forceinline__ void report(const AppendArgs& a) {
     if (a.status != nullptr) atomicCAS(a.status, LF_OK, LF_EINVAL);
-    else atomicCAS(&g_device_error, 0, 222);
+    else atomicCAS(&g_device_error, 0, 252);
 }
 
 // One CTA walks tokens (grid-stride, blockIdx.y the layer); a row of D dims of one head is D / 8
@@ -257,7 +257,7 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
         const int o = out_page(j);
         const bool fits = o < out_pages;
         out_table[(long)n * max_pages + j] = (j < np || j < n_prefix) && fits ? o : -1;
-        if (j < np && !fits) atomicCAS(&g_device_error, 0, 223);
+        if (j < np && !fits) atomicCAS(&g_device_error, 0, 253);
     }
     // shared pages are written once, from the longest session's row
     const int lead = best_n;
@@ -274,7 +274,7 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
         const int rows = min(kPage, L - j * kPage);     // <= 0: a prefix page past every session
         int page = rows > 0 ? bt[(long)n * max_pages + j] : 0;
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(num_pages)) {
-            if (lane == 0) atomicCAS(&g_device_error, 0, 224);
+            if (lane == 0) atomicCAS(&g_device_error, 0, 254);
             page = 0;
         }
         const uint8_t* blk = pages + ((long)page * Hkv + h) * F::kBlockBytes;

@@ -102,6 +102,52 @@ def test_decode_shared_prefix(Hq, Hkv, D, npre):
     check_decode(lens, Hq, Hkv, D, npre=npre, spoil=True)
 
 
+# rows x pages x KV heads x head_dim past 2^25: the prefix goes to tiles of 128 rows
+TILED = [(40, 32, 4, 128, 205), (130, 4, 4, 128, 505), (101, 8, 4, 64, 650), (33, 16, 2, 64, 993)]
+
+
+@pytest.mark.parametrize("N,Hq,Hkv,D,npre", TILED)
+def test_decode_long_shared_prefix_of_many_rows(N, Hq, Hkv, D, npre):
+    ends = [npre * 16 + x for x in (0, 1, 16, 130, 33, 7)] + [npre * 16 - 3, 1, 0, 8 * npre + 5, 500, 16 * npre - 16]
+    lens = [ends[(i * 7) % len(ends)] for i in range(N)]
+    check_decode(lens, Hq, Hkv, D, npre=npre, spoil=True)
+    check_decode([min(x, npre * 16) for x in lens], Hq, Hkv, D, npre=npre, scale=-0.4)   # peaked, negative
+
+
+@pytest.mark.parametrize("N,Hq,Hkv,D,npre", [(6, 8, 2, 128, 5), (5, 2, 2, 64, 40), TILED[0], TILED[3]])
+def test_nan_in_a_shared_prefix_reaches_the_rows_that_hold_it(N, Hq, Hkv, D, npre):
+    gen = torch.Generator().manual_seed(3)
+    at = npre * 8 + 3                                      # the token with NaN
+    lens = [npre * 16 + 20 if i % 2 else at - i % 3 for i in range(N)]
+    table, P = table_for(lens, npre, gen)
+    lead = next(i for i in range(N) if i % 2)
+    pages = random_pages(gen, P, Hkv, D)
+    q = torch.randn(N, Hq, D, generator=gen).bfloat16()
+    q[lead, 1] = math.nan
+
+    def run(kv):
+        x = pages.clone()
+        if kv is not None:
+            par = x[..., 16 * D:].contiguous().view(torch.bfloat16).view(P, Hkv, 16, 2, D // 64, 2)
+            par[int(table[lead, at // 16]), 0, at % 16, kv, 0] = math.nan
+            x[..., 16 * D:] = par.contiguous().view(torch.uint8).flatten(2)
+        return att.paged_decode_q4(q.cuda(), x.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                                   num_prefix_pages=npre).cpu()
+    clean, k_nan, v_nan = run(None), run(0), run(1)
+    assert torch.equal(clean.isnan().nonzero(), torch.cartesian_prod(
+        torch.tensor([lead]), torch.tensor([1]), torch.arange(D)))
+    G = Hq // Hkv
+    for i in range(N):
+        want = clean[i].clone()
+        if i % 2:
+            want[:G] = math.nan
+        assert torch.allclose(k_nan[i], want, rtol=0, atol=0, equal_nan=True)
+        want = clean[i].clone()
+        if i % 2:
+            want[:G, :64] = math.nan
+        assert torch.allclose(v_nan[i], want, rtol=0, atol=0, equal_nan=True)
+
+
 def test_decode_prefix_only_and_equal_to_unshared():
     lens = [96, 96, 96]
     check_decode(lens, 8, 2, 128, npre=6)
@@ -218,12 +264,12 @@ def test_append_without_a_page_stores_nothing_and_is_reported():
     for start in ([16, 16], [32, 1 << 20], [-1, -16]):       # no page, bad id, past the table, negative
         att.append_qkv_q4(qkv, dev, table, torch.tensor(start, dtype=torch.int32).cuda(),
                           torch.tensor([0, 1, 1], dtype=torch.int32).cuda(), 1)
-        assert drain_status() == [222]
+        assert drain_status() == [252]
     assert torch.equal(dev.cpu(), pages)
     cos, sin = (t.cuda() for t in rope_tables(4, 64))
     att.append_qkv_q4(qkv[:1], dev, table[:1], torch.tensor([4], dtype=torch.int32).cuda(),
                       torch.tensor([0, 1], dtype=torch.int32).cuda(), 1, rope=(cos, sin))
-    assert drain_status() == [222] and torch.equal(dev.cpu(), pages)
+    assert drain_status() == [252] and torch.equal(dev.cpu(), pages)
 
 
 # -- expansion --------------------------------------------------------------------------------------
@@ -262,12 +308,12 @@ def test_expansion_reports_too_few_output_pages_and_bad_ids():
     table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32).cuda()
     lens = torch.tensor([32, 20], dtype=torch.int32).cuda()
     k, v, out = att.expand_pages_q4(pages, table, lens, 3)
-    assert out.tolist() == [[0, 1], [2, -1]] and drain_status() == [223]
+    assert out.tolist() == [[0, 1], [2, -1]] and drain_status() == [253]
     full, _, _ = att.expand_pages_q4(pages, table, lens, 4)
     assert torch.equal(k, full[:3]) and drain_status() == []
     table[1, 1] = 9
     att.expand_pages_q4(pages, table, lens, 4)
-    assert drain_status() == [224]
+    assert drain_status() == [254]
 
 
 # -- streams, graphs, workspaces ---------------------------------------------------------------------
