@@ -423,7 +423,7 @@ int lf_q4_fork(const lf_pool_meta* m, int src_seq, const int32_t* dst_seqs, int 
 /* Paged split-KV decode over 4-bit pages: lf_decode_fwd's arguments and results (a session of
  * length 0 gives zeros and an lse of -inf), with one array of pages [P][Hkv][18 * D].  Hq / Hkv is 1, 2, 4 or 8.
  * The workspace comes from lf_q4_decode_workspace_size (sm_count <= 0, in both: the current
- * device's).  The sessions' own pages are cut into equal ranges, a few per SM; there is no split
+ * device's); where that is 0 bytes (few sessions, no prefix) it may be NULL.  The sessions' own pages are cut into equal ranges, a few per SM; there is no split
  * size to choose. */
 int lf_q4_decode_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                                 int max_pages, int num_prefix_pages, int sm_count, size_t* bytes);

@@ -269,7 +269,7 @@ def append_qkv_q4(qkv: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
         raise LoopfuseError(_lib.LF_EINVAL, "append_qkv_q4 expects bf16 rows qkv [T, (Hq + 2 Hkv) * D]")
     T = qkv.shape[0]
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=qkv.dtype, device=qkv.device)
+        q_out = torch.empty(T, Hq, D, dtype=qkv.dtype, device=qkv.device)
     _require(q_out, "q_out")
     if tuple(q_out.shape) != (T, Hq, D):
         raise LoopfuseError(_lib.LF_EINVAL, f"q_out must be [T, Hq, D] = {(T, Hq, D)}")
@@ -334,19 +334,18 @@ def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
         _require(o, "out")
         if o.shape != q.shape:
             raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: out must have q's shape")
-    lse = torch.empty((N, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty(N, Hq, dtype=torch.float32, device=dev) if return_lse else None
     if N == 0:
         return (o, lse) if return_lse else o
     max_pages, npre = block_table.shape[1], int(num_prefix_pages)
     scale = D ** -0.5 if scale is None else float(scale)
     sms = sm_count(dev.index)
     need = decode_q4_workspace_bytes(N, Hq, Hkv, D, max_pages, npre, sms)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     launch("lf_q4_decode_fwd", dev, q.data_ptr(), pages.data_ptr(), block_table.data_ptr(),
            seq_lens.data_ptr(), npre, o.data_ptr(), lse.data_ptr() if lse is not None else None,
-           workspace.data_ptr(), workspace.numel() * workspace.element_size(), N, Hq, Hkv, D, P,
-           max_pages, scale, sms)
+           workspace.data_ptr() if need else None, need, N, Hq, Hkv, D, P, max_pages, scale, sms)
     return (o, lse) if return_lse else o
 
 

@@ -32,7 +32,9 @@
 //           (chunk, KV head, group of 4 * 8/G sessions): the 8 columns of a warp are G heads of 8/G
 //           sessions, and the four warps use the same staged pages, so that a prefix page is read once
 //           per 32 columns.
-// Every piece writes unnormalised fp32 partials (o, max, sum); a range's piece of item (session, KV
+//   few     few sessions without a prefix, e.g. one: an item (session, KV head) is a cluster of up to 8
+//           CTAs, which merges its warps' partials on the chip; one launch and no workspace.
+// Every other piece writes unnormalised fp32 partials (o, max, sum); a range's piece of item (session, KV
 // head) is partial number range + item, which no two pieces share as both grow along the ranges.
 // combine merges a row's partials, in order.
 //
@@ -42,6 +44,7 @@
 #include "q4_common.cuh"
 #include "sm100_primitives.cuh"
 
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
@@ -49,6 +52,8 @@
 
 namespace lf {
 namespace q4 {
+
+namespace cg = cooperative_groups;
 
 using decode::checked_page;
 using decode::kThreads;
@@ -59,6 +64,7 @@ constexpr int kStages = 2;                     // own: units in flight per warp
 constexpr int per_sm(int D) { return D == 64 ? 4 : 3; }   // own: resident CTAs of an SM (registers)
 constexpr int kMinUnits = 2;                   // own: units of a range
 constexpr int kRing = 16;                      // prefix: pages staged in a CTA, in two halves
+constexpr int kMaxParts = 8;                   // few items: CTAs of an item, a cluster (portable size)
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct DecodeArgs {
@@ -71,6 +77,9 @@ struct DecodeArgs {
     int N, Hq, Hkv, G, num_pages, max_pages;
     int n_prefix, chunk, n_chunks, groups;     // shared prefix: pages, pages a chunk, chunks, session groups
     int ranges;                                // of the own pages: one per warp
+    int parts;                                 // few items: CTAs of an item (0: not few)
+    uint16_t* o;
+    float* lse;                                // nullable
     float qscale;                              // |scale| * log2(e) * 2^69
     uint32_t flip;                             // sign bits of a negative scale
 };
@@ -374,6 +383,9 @@ struct OwnSmem {
     static constexpr int kQ = 8 * D * 2;                   // queries of a KV head, at most 8 rows
     static constexpr int kWarp = kStages * kUnitBytes + 2 * kQ;
     static constexpr int kBytes = kWarps * kWarp + 128;
+    // few items: the warps' partials, [warp][row][D] fp32 and [warp][row] (max, sum)
+    static constexpr int kPart = kWarps * kWarp, kPartMl = kPart + kWarps * 8 * D * 4;
+    static constexpr int kFewBytes = kPartMl + kWarps * 8 * 8 + 128;
 };
 
 // Sum over the CTA's threads (every thread gets it).
@@ -409,12 +421,195 @@ struct Segment {
     }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeArgs a) {
+__device__ __forceinline__ uint8_t* align128(uint8_t* p) {
+    return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 127) & ~uintptr_t(127));
+}
+// A warp's barriers, one a unit in flight.
+__device__ __forceinline__ uint32_t init_ring(uint64_t* bars, int lane) {
+    const uint32_t bar = sm100::smem_addr(bars);
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) sm100::mbar_init(bar + 8 * i, 1);
+        sm100::fence_barrier_init();
+    }
+    return bar;
+}
+
+// A warp's segments, from `seg` on: copies, products, partials.  kFew: to the CTA's shared memory (part_o
+// [warp][8 rows][D]), else to the range's slots.  (`a` by value: by reference the ragged case takes 42.1
+// us, not 41.2.)
+template <int D, bool kFew>
+__device__ __forceinline__ void run_segments(const DecodeArgs a, Segment seg, int range, uint8_t* mem, uint32_t bar,
+                                             float* part_o, float2* part_ml) {
     using F = Fmt<D>;
     constexpr int UB = OwnSmem<D>::kUnitBytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const uint8_t* qbuf = mem + kStages * UB;
+    const uint32_t ring = sm100::smem_addr(mem), qring = ring + kStages * UB;
+    // What it copies: a segment that runs ahead.  Page ids of 16 units at a time, one page per
+    // lane (lane 2 i + p: page p of the i-th).
+    Segment pre = seg;
+    bool more = true, fresh = true;                          // fresh: the segment's first unit
+    int ids = 0, ids_at = 16;
+    uint32_t issued = 0, used = 0, q_in = 0;
+    const uint64_t policy = sm100::l2_evict_first_policy();  // read once
+    auto issue = [&]() {                                     // warp-uniform: one unit, if any is left
+        if (more && pre.j >= pre.j1) {
+            more = pre.next(a);
+            fresh = true;
+            ids_at = 16;
+        }
+        if (!more) return;
+        if (ids_at == 16) {
+            ids_at = 0;
+            const int p = a.n_prefix + (pre.j + lane / kUnit) * kUnit + lane % kUnit;
+            ids = p < (pre.L + kPage - 1) / kPage ? checked_page(a.bt[(size_t)pre.n * a.max_pages + p], a.num_pages) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, ids_at * kUnit + lane % kUnit);
+        const int last = __shfl_sync(0xffffffffu, page, kUnit - 1);
+        const int st = issued % kStages;
+        const uint32_t q_bytes = a.G * D * 2;
+        if (lane == 0)
+            sm100::mbar_arrive_expect_tx(bar + 8 * st, (last >= 0 ? UB : F::kBlockBytes) + (fresh ? q_bytes : 0));
+        __syncwarp();
+        if (lane < kUnit && page >= 0)
+            bulk_load(ring + (uint32_t)(st * UB + lane * F::kBlockBytes),
+                      a.pages + ((size_t)page * a.Hkv + pre.h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
+        if (fresh && lane == kUnit)
+            bulk_load(qring + (q_in & 1) * OwnSmem<D>::kQ, a.q + ((size_t)pre.n * a.Hq + pre.h * a.G) * D, q_bytes,
+                      bar + 8 * st, policy);
+        q_in += fresh;
+        fresh = false;
+        ++issued;
+        ++ids_at;
+        ++pre.j;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kStages; ++k) issue();
+    uint32_t q_out = 0;
+    bool failed = false;
+    do {
+        const int item = seg.n * a.Hkv + seg.h, L = seg.L;
+        const int len[2] = {L, L};
+        State<D, kUnit> st;
+        for (int j = seg.j; j < seg.j1; ++j) {
+            const int sl = used % kStages;
+            if (!warp_wait(bar + 8 * sl, (used / kStages) & 1)) {
+                if (lane == 0) {
+                    atomicCAS(&g_device_error, 0, 251);      // let the copies in flight land
+                    for (uint32_t k = used; k < issued; ++k) wait_full(bar + 8 * (k % kStages), (k / kStages) & 1);
+                }
+                failed = true;
+                break;
+            }
+            if (j == seg.j) {
+                const uint16_t* rows = reinterpret_cast<const uint16_t*>(qbuf + (q_out & 1) * OwnSmem<D>::kQ);
+                st.init(g < a.G ? rows + g * D : nullptr, a.flip, c);
+                ++q_out;
+            }
+            const uint32_t blk = ring + (uint32_t)(sl * UB);
+            const int tok0 = (a.n_prefix + j * kUnit) * kPage;
+            if (tok0 + kUnit * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
+            else st.template unit<true>(blk, tok0, len, a.qscale, lane);
+            __syncwarp();                                    // every lane has read the buffer
+            ++used;
+            issue();
+        }
+        if (failed) break;
+        st.finish();
+        // Columns 2c and 2c + 1 are heads of the group; lane g holds 2 dims of each m-tile.
+        const size_t slot = kFew ? (size_t)warp * 8 : (size_t)(range + item) * a.G;
+        float* out_o = kFew ? part_o : a.own_o;
+        float2* out_ml = kFew ? part_ml : a.own_ml;
+#pragma unroll
+        for (int col = 0; col < 2; ++col) {
+            if (2 * c + col >= a.G) continue;
+            float* dst = out_o + (slot + 2 * c + col) * D;
+#pragma unroll
+            for (int gr = 0; gr < F::NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 4; k += 2)
+                    *reinterpret_cast<float4*>(dst + out_dim(gr, k, g)) =
+                        make_float4(st.o[gr][k][col], st.o[gr][k][2 + col],
+                                    st.o[gr][k + 1][col], st.o[gr][k + 1][2 + col]);
+            if (g == 0) out_ml[slot + 2 * c + col] = make_float2(st.m[col], st.l[col]);
+        }
+        if (!kFew && lane == 0) {
+            if (seg.j == 0) a.span[item].x = range;
+            if (seg.j1 == seg.u) a.span[item].y = range;
+        }
+    } while (seg.next(a));
+}
+
+template <int V> struct Vec;
+template <> struct Vec<2> { typedef float2 T; };
+template <> struct Vec<4> { typedef float4 T; };
+
+// Weighted sum of `count` partials of a row, this lane's V dims: x(t) and ml(t) are loaded all at once.
+template <int V, int kMax, class X, class ML>
+__device__ __forceinline__ float2 merge_row(int count, float qscale, X x, ML ml, float (&acc)[V]) {
+    typedef typename Vec<V>::T VT;
+    VT v[kMax];
+    float2 e[kMax];
+#pragma unroll
+    for (int t = 0; t < kMax; ++t) {
+        e[t] = t < count ? *ml(t) : make_float2(-INFINITY, 0.f);
+        if (t < count) v[t] = *reinterpret_cast<const VT*>(x(t));
+    }
+    float M = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int t = 0; t < kMax; ++t) M = fmaxf(M, e[t].x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int t = 0; t < kMax; ++t)
+        if (e[t].y != 0.f) {                                     // (0: no token, and nothing was written)
+            const float w = e[t].x == M ? 1.f : fast_exp2((e[t].x - M) * qscale);
+            const float* f = reinterpret_cast<const float*>(&v[t]);
+            l = fmaf(w, e[t].y, l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+        }
+    return make_float2(M, l);
+}
+
+// The final rows of a cluster's item: over a CTA's warps, then over the CTAs through distributed shared
+// memory, a row each.
+template <int D>
+__device__ void merge_few(const DecodeArgs& a, float* part_o, float2* part_ml) {
+    constexpr int V = D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    cg::cluster_group cluster = cg::this_cluster();
+    float acc[V];
+    __syncthreads();
+    for (int r = warp; r < a.G; r += kWarps) {
+        const float2 e = merge_row<V, kWarps>(kWarps, a.qscale, [&](int w) { return part_o + (w * 8 + r) * D + V * lane; },
+                                              [&](int w) { return part_ml + w * 8 + r; }, acc);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < V; ++i) part_o[r * D + V * lane + i] = acc[i];
+        if (lane == 0) part_ml[r] = e;
+    }
+    cluster.sync();
+    const int item = blockIdx.x / a.parts, n = item / a.Hkv;
+    for (int r = (int)cluster.block_rank() + warp * a.parts; r < a.G; r += kWarps * a.parts) {
+        const float2 e = merge_row<V, kMaxParts>(
+            a.parts, a.qscale, [&](int t) { return cluster.map_shared_rank(part_o + r * D + V * lane, t); },
+            [&](int t) { return cluster.map_shared_rank(part_ml + r, t); }, acc);
+        const size_t row = (size_t)n * a.Hq + item % a.Hkv * a.G + r;
+        const float inv = e.y != 0.f ? 1.f / e.y : 0.f;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(a.o + row * D) + (V / 2) * lane;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) dst[i] = pack_bf16x2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+        if (a.lse != nullptr && lane == 0)
+            a.lse[row] = e.y != 0.f ? (e.x * a.qscale + log2f(e.y)) * kLn2 : -INFINITY;
+    }
+    cluster.sync();                                              // others may still read this CTA's shared memory
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeArgs a) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
     __shared__ long buf[kWarps];
     __shared__ long s_before[kWarps];          // units of one head before session s_n[w]
@@ -423,15 +618,9 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
     // it let this one begin); combine may read the lengths as soon as it is released.
     if (a.n_chunks == 0) grid_wait();
     grid_release();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    uint8_t* mem = smem + warp * OwnSmem<D>::kWarp;
-    const uint8_t* qbuf = mem + kStages * UB;
-    const uint32_t ring = sm100::smem_addr(mem), qring = ring + kStages * UB;
-    const uint32_t bar = sm100::smem_addr(bars + warp * kStages);
-    if (lane == 0) {
-        for (int i = 0; i < kStages; ++i) sm100::mbar_init(bar + 8 * i, 1);
-        sm100::fence_barrier_init();
-    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* mem = align128(smem_raw) + warp * OwnSmem<D>::kWarp;
+    const uint32_t bar = init_ring(bars + warp * kStages, lane);
     // Units of a CTA's width of sessions, summed up to each: the first such chunk serves the total and,
     // in most batches, the search.
     long excl = 0, chunk = 0;                                    // units before this thread's session; of the chunk
@@ -486,111 +675,46 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
         __syncthreads();
     }
     if (begin < total) {
-        Segment seg;                                             // what the warp computes on
+        Segment seg;
         seg.n = s_n[warp];
         seg.u = own_units(a, seg.n);
         seg.L = held(a, seg.n);
-        {
-            const long in = begin - s_before[warp] * a.Hkv, len = min(share, total - begin);
-            seg.h = (int)(in / seg.u);
-            seg.j = (int)(in % seg.u);
-            seg.j1 = (int)min((long)seg.u, seg.j + len);
-            seg.left = len - (seg.j1 - seg.j);
-        }
-        // What it copies: a segment that runs ahead.  Page ids of 16 units at a time, one page per
-        // lane (lane 2 i + p: page p of the i-th).
-        Segment pre = seg;
-        bool more = true, fresh = true;                          // fresh: the segment's first unit
-        int ids = 0, ids_at = 16;
-        uint32_t issued = 0, used = 0, q_in = 0;
-        const uint64_t policy = sm100::l2_evict_first_policy();  // read once
-        auto issue = [&]() {                                     // warp-uniform: one unit, if any is left
-            if (more && pre.j >= pre.j1) {
-                more = pre.next(a);
-                fresh = true;
-                ids_at = 16;
-            }
-            if (!more) return;
-            if (ids_at == 16) {
-                ids_at = 0;
-                const int p = a.n_prefix + (pre.j + lane / kUnit) * kUnit + lane % kUnit;
-                ids = p < (pre.L + kPage - 1) / kPage ? checked_page(a.bt[(size_t)pre.n * a.max_pages + p], a.num_pages) : -1;
-            }
-            const int page = __shfl_sync(0xffffffffu, ids, ids_at * kUnit + lane % kUnit);
-            const int last = __shfl_sync(0xffffffffu, page, kUnit - 1);
-            const int st = issued % kStages;
-            const uint32_t q_bytes = a.G * D * 2;
-            if (lane == 0)
-                sm100::mbar_arrive_expect_tx(bar + 8 * st, (last >= 0 ? UB : F::kBlockBytes) + (fresh ? q_bytes : 0));
-            __syncwarp();
-            if (lane < kUnit && page >= 0)
-                bulk_load(ring + (uint32_t)(st * UB + lane * F::kBlockBytes),
-                          a.pages + ((size_t)page * a.Hkv + pre.h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
-            if (fresh && lane == kUnit)
-                bulk_load(qring + (q_in & 1) * OwnSmem<D>::kQ, a.q + ((size_t)pre.n * a.Hq + pre.h * a.G) * D, q_bytes,
-                          bar + 8 * st, policy);
-            q_in += fresh;
-            fresh = false;
-            ++issued;
-            ++ids_at;
-            ++pre.j;
-        };
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < kStages; ++k) issue();
-        uint32_t q_out = 0;
-        bool failed = false;
-        do {
-            const int item = seg.n * a.Hkv + seg.h, L = seg.L;
-            const int len[2] = {L, L};
-            State<D, kUnit> st;
-            for (int j = seg.j; j < seg.j1; ++j) {
-                const int sl = used % kStages;
-                if (!warp_wait(bar + 8 * sl, (used / kStages) & 1)) {
-                    if (lane == 0) {
-                        atomicCAS(&g_device_error, 0, 251);      // let the copies in flight land
-                        for (uint32_t k = used; k < issued; ++k) wait_full(bar + 8 * (k % kStages), (k / kStages) & 1);
-                    }
-                    failed = true;
-                    break;
-                }
-                if (j == seg.j) {
-                    const uint16_t* rows = reinterpret_cast<const uint16_t*>(qbuf + (q_out & 1) * OwnSmem<D>::kQ);
-                    st.init(g < a.G ? rows + g * D : nullptr, a.flip, c);
-                    ++q_out;
-                }
-                const uint32_t blk = ring + (uint32_t)(sl * UB);
-                const int tok0 = (a.n_prefix + j * kUnit) * kPage;
-                if (tok0 + kUnit * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
-                else st.template unit<true>(blk, tok0, len, a.qscale, lane);
-                __syncwarp();                                    // every lane has read the buffer
-                ++used;
-                issue();
-            }
-            if (failed) break;
-            st.finish();
-            // Columns 2c and 2c + 1 are heads of the group; lane g holds 2 dims of each m-tile.
-            const size_t slot = (size_t)(range + item) * a.G;
-#pragma unroll
-            for (int col = 0; col < 2; ++col) {
-                if (2 * c + col >= a.G) continue;
-                float* dst = a.own_o + (slot + 2 * c + col) * D;
-#pragma unroll
-                for (int gr = 0; gr < F::NG; ++gr)
-#pragma unroll
-                    for (int k = 0; k < 4; k += 2)
-                        *reinterpret_cast<float4*>(dst + out_dim(gr, k, g)) =
-                            make_float4(st.o[gr][k][col], st.o[gr][k][2 + col],
-                                        st.o[gr][k + 1][col], st.o[gr][k + 1][2 + col]);
-                if (g == 0) a.own_ml[slot + 2 * c + col] = make_float2(st.m[col], st.l[col]);
-            }
-            if (lane == 0) {
-                if (seg.j == 0) a.span[item].x = range;
-                if (seg.j1 == seg.u) a.span[item].y = range;
-            }
-        } while (seg.next(a));
+        const long in = begin - s_before[warp] * a.Hkv, len = min(share, total - begin);
+        seg.h = (int)(in / seg.u);
+        seg.j = (int)(in % seg.u);
+        seg.j1 = (int)min((long)seg.u, seg.j + len);
+        seg.left = len - (seg.j1 - seg.j);
+        run_segments<D, false>(a, seg, range, mem, bar, nullptr, nullptr);
     }
     if (a.n_chunks > 0) grid_wait();                             // the prefix kernel's partials are there too
+}
+
+// Few items without a prefix.  An item is a cluster's: its units are cut over the cluster's warps, whose
+// partials are merged on the chip, so that the call is one launch.
+template <int D>
+__global__ void __launch_bounds__(kThreads, per_sm(D)) few_kernel(const DecodeArgs a) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+    grid_wait();
+    grid_release();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* smem = align128(smem_raw);
+    float* part_o = reinterpret_cast<float*>(smem + OwnSmem<D>::kPart);
+    float2* part_ml = reinterpret_cast<float2*>(smem + OwnSmem<D>::kPartMl);
+    if (lane < 8) part_ml[warp * 8 + lane] = make_float2(-INFINITY, 0.f);
+    const uint32_t bar = init_ring(bars + warp * kStages, lane);
+    const int item = blockIdx.x / a.parts, w = blockIdx.x % a.parts * kWarps + warp;
+    Segment seg;
+    seg.n = item / a.Hkv;
+    seg.h = item % a.Hkv;
+    seg.u = own_units(a, seg.n);
+    seg.L = held(a, seg.n);
+    const int share = (seg.u + a.parts * kWarps - 1) / (a.parts * kWarps);
+    seg.j = w * share;
+    seg.j1 = min(seg.u, seg.j + share);
+    seg.left = 0;
+    if (seg.j < seg.j1) run_segments<D, true>(a, seg, 0, smem + warp * OwnSmem<D>::kWarp, bar, part_o, part_ml);
+    merge_few<D>(a, part_o, part_ml);
 }
 
 // -- shared prefix --------------------------------------------------------------------------------------
@@ -702,17 +826,16 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
 namespace lf {
 namespace q4 {
 
-template <int V> struct Vec;
-template <> struct Vec<2> { typedef float2 T; };
-template <> struct Vec<4> { typedef float4 T; };
-
-// One warp per (session, query head): merges the row's partials, the prefix chunks first, by their
-// maxima.  A row without tokens gives zeros and an lse of -inf.
-template <int D>
-__global__ void __launch_bounds__(kThreads)
-combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__ lse) {
-    const int lane = threadIdx.x & 31;
-    const long row = (long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+// Merges the partials of a row (session, query head), the prefix chunks first, by their maxima.  A row
+// without tokens gives zeros and an lse of -inf.  R warps a row: 1, or kRowWarps where a row has many
+// partials (they take 32 of them in turn).
+constexpr int kRowWarps = 8, kManyPartials = 32;
+template <int D, int R>
+__global__ void __launch_bounds__(R == 1 ? kThreads : 32 * R)
+combine_kernel(const DecodeArgs a) {
+    constexpr int kRows = R == 1 ? kWarps : 1;             // rows of a CTA
+    const int lane = threadIdx.x & 31, part = R == 1 ? 0 : threadIdx.x >> 5;
+    const long row = (long)blockIdx.x * kRows + (R == 1 ? threadIdx.x >> 5 : 0);
     if (row >= (long)a.N * a.Hq) return;
     const int n = (int)(row / a.Hq), hq = (int)(row % a.Hq), item = n * a.Hkv + hq / a.G;
     const int npages = (held(a, n) + kPage - 1) / kPage;
@@ -737,7 +860,7 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
         for (int t = 0; t < kBatch; ++t)
             if (t0 + t < total) x[t] = *reinterpret_cast<const VT*>(vec(t0 + t));
     };
-    fetch(0);
+    fetch(32 * part);
     float2 e = make_float2(-INFINITY, 0.f);
     if (lane < total) e = ml(lane);
     float M = e.x;
@@ -749,13 +872,13 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     const float ref = M == -INFINITY ? 0.f : M;
     float w = 0.f;
-    for (int j0 = 0; j0 < total; j0 += kBatch) {
+    for (int j0 = R == 1 ? 0 : 32 * part; j0 < total; j0 += kBatch) {
         if (j0 % 32 == 0) {                                // weights of 32 slots, one a lane
             if (j0 > 0) e = j0 + lane < total ? ml(j0 + lane) : make_float2(-INFINITY, 0.f);
             w = e.x == -INFINITY ? 0.f : fast_exp2((e.x - ref) * a.qscale);
             l = fmaf(w, e.y, l);
         }
-        if (j0 > 0) fetch(j0);
+        if (j0 > (R == 1 ? 0 : 32 * part)) fetch(j0);
 #pragma unroll
         for (int t = 0; t < kBatch; ++t) {
             const float wt = __shfl_sync(0xffffffffu, w, (j0 + t) % 32);
@@ -764,14 +887,29 @@ combine_kernel(const DecodeArgs a, uint16_t* __restrict__ o, float* __restrict__
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[i] = fmaf(wt, f[i], acc[i]);
         }
+        if constexpr (R > 1) j0 += j0 % 32 == 32 - kBatch ? 32 * (R - 1) : 0;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if constexpr (R > 1) {                                 // the warps' sums, in order
+        __shared__ float s_acc[R][D], s_l[R];
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_acc[part][V * lane + i] = acc[i];
+        if (lane == 0) s_l[part] = l;
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int p = 1; p < R; ++p) {
+            l += s_l[p];
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += s_acc[p][V * lane + i];
+        }
+    }
     const float inv = total > 0 && l != 0.f ? 1.f / l : 0.f;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(o + row * D) + (V / 2) * lane;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.o + row * D) + (V / 2) * lane;
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) dst[i] = pack_bf16x2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    if (lse != nullptr && lane == 0) lse[row] = l != 0.f ? (ref * a.qscale + log2f(l)) * kLn2 : -INFINITY;
+    if (a.lse != nullptr && lane == 0) a.lse[row] = l != 0.f ? (ref * a.qscale + log2f(l)) * kLn2 : -INFINITY;
 }
 
 // -- sizes ------------------------------------------------------------------------------------------
@@ -802,16 +940,29 @@ inline int prefix_chunk(int N, int G, int Hkv, int D, int n_prefix, int sms) {
     return ceil_div(n_prefix, chunks);
 }
 
+// CTAs of an item when there are few items without a prefix (0: not few): 8, 4 or 2 that are all resident
+// at once.  A cluster is alone with its item's length, so the table may allow 8 units a warp at most.
+// Of equal lengths, 8 heads of 128: 1 session of 777 tokens 6.5 against 10.2 us (two launches, partials
+// through memory), 8000: 13.0 : 14.3, 16000: 20.1 : 17.1; 12 sessions of 777: 9.9 : 13.0, 4000: 19.8 :
+// 24.6; 24 of 777: 13.3 : 16.4.
+inline int few_parts(int N, int Hkv, int D, int n_prefix, int max_pages, int sms) {
+    if (n_prefix > 0) return 0;
+    int parts = kMaxParts;
+    while (parts > 1 && (long)N * Hkv * parts > (long)per_sm(D) * sms) parts /= 2;
+    return parts > 1 && max_pages <= 8 * kUnit * kWarps * parts ? parts : 0;
+}
+
 // Sizes of the workspace's parts, in their order.
 struct Sizes {
     size_t own, pre, items;                    // partials of the ranges, of the prefix; spans
-    int chunk, n_chunks, ranges;
+    int chunk, n_chunks, ranges, parts;
     size_t bytes(int D) const { return (own + pre) * (D * sizeof(float) + sizeof(float2)) + items * sizeof(int2); }
 };
 inline Sizes sizes(int N, int Hq, int Hkv, int D, int n_prefix, int max_pages, int sms) {
     Sizes s;
-    s.ranges = n_prefix < max_pages ? per_sm(D) * sms * kWarps : 0;
-    s.items = (size_t)N * Hkv;
+    s.parts = few_parts(N, Hkv, D, n_prefix, max_pages, sms);
+    s.ranges = n_prefix < max_pages && s.parts == 0 ? per_sm(D) * sms * kWarps : 0;
+    s.items = s.parts == 0 ? (size_t)N * Hkv : 0;
     s.own = s.ranges > 0 ? (s.ranges + s.items) * (Hq / Hkv) : 0;
     s.chunk = prefix_chunk(N, Hq / Hkv, Hkv, D, n_prefix, sms);
     s.n_chunks = ceil_div(n_prefix, s.chunk);
@@ -827,11 +978,13 @@ static int sm_count(int* out) {
 }
 
 template <int D>
-static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st) {
+static int launch(const DecodeArgs& a, cudaStream_t st) {
     static PerContextOnce once;
     int rc = once.run([] {
         LF_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            OwnSmem<D>::kBytes));
+        LF_CHECK_CUDA(cudaFuncSetAttribute(few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           OwnSmem<D>::kFewBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            PrefixSmem<D>::kBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -839,6 +992,9 @@ static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st)
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
+    if (a.parts > 0)
+        return launch_early_clusters("q4 decode", few_kernel<D>, a.parts, dim3((unsigned)(a.N * a.Hkv * a.parts)),
+                                     dim3(kThreads), OwnSmem<D>::kFewBytes, st, a);
     const long shared = (long)a.n_chunks * a.Hkv * a.groups, rows = (long)a.N * a.Hq;
     LF_CHECK_ARG(shared <= 2147483647L, "q4 decode: grid limits exceeded");
     if (shared > 0) {
@@ -853,8 +1009,13 @@ static int launch(const DecodeArgs& a, uint16_t* o, float* lse, cudaStream_t st)
         rc = launch_early("q4 decode", own_kernel<D>, dim3(a.ranges / kWarps), dim3(kThreads), OwnSmem<D>::kBytes, st, a);
         if (rc != LF_OK) return rc;
     }
-    return launch_early("q4 decode combine", combine_kernel<D>, dim3((unsigned)ceil_div(rows, kWarps)), dim3(kThreads),
-                        0, st, a, o, lse);
+    // A row's partials, at most: the prefix chunks and an equal share of the ranges.
+    const long most = a.n_chunks + std::min((long)a.ranges / (a.N * a.Hkv), (long)a.max_pages / (kUnit * kMinUnits)) + 1;
+    return most > kManyPartials
+               ? launch_early("q4 decode combine", combine_kernel<D, kRowWarps>, dim3((unsigned)rows), dim3(32 * kRowWarps),
+                              0, st, a)
+               : launch_early("q4 decode combine", combine_kernel<D, 1>, dim3((unsigned)ceil_div(rows, kWarps)),
+                              dim3(kThreads), 0, st, a);
 }
 
 }  // namespace q4
@@ -884,7 +1045,7 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
                                 int sm_count, void* stream) {
     LF_CHECK_ARG(num_seqs >= 0, "q4 decode: negative sizes");
     if (num_seqs == 0) { clear_error(); return LF_OK; }
-    LF_CHECK_ARG(q && pages && block_table && seq_lens && o && workspace, "q4 decode: null pointer argument");
+    LF_CHECK_ARG(q && pages && block_table && seq_lens && o, "q4 decode: null pointer argument");
     LF_CHECK_ARG(aligned16(q) && aligned16(pages) && aligned16(o) && aligned16(workspace),
                  "q4 decode: q, pages, o and workspace must be 16-byte aligned");
     LF_CHECK_ARG(head_dim == 128 || head_dim == 64, "q4 decode: head_dim must be 64 or 128 (got %d)", head_dim);
@@ -902,6 +1063,7 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
         if (rc != LF_OK) return rc;
     }
     const q4::Sizes z = q4::sizes(num_seqs, num_q_heads, num_kv_heads, head_dim, num_prefix_pages, max_pages, sm_count);
+    LF_CHECK_ARG(workspace != nullptr || z.bytes(head_dim) == 0, "q4 decode: null pointer argument");
     LF_CHECK_ARG(workspace_bytes >= z.bytes(head_dim), "q4 decode: workspace too small (%zu < %zu bytes)",
                  workspace_bytes, z.bytes(head_dim));
     q4::DecodeArgs a{};
@@ -927,8 +1089,11 @@ extern "C" int lf_q4_decode_fwd(const lf_bf16* q, const void* pages, const int32
                    ? q4::ceil_div((long)num_seqs * G, q4::kTcRows)
                    : q4::ceil_div(num_seqs, q4::kWarps * (8 / G));
     a.ranges = z.ranges;
+    a.parts = z.parts;
+    a.o = o;
+    a.lse = lse;
     a.qscale = fabsf(scale) * kLog2e * q4::kDown;
     a.flip = scale < 0.f ? 0x80008000u : 0u;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return head_dim == 128 ? q4::launch<128>(a, o, lse, st) : q4::launch<64>(a, o, lse, st);
+    return head_dim == 128 ? q4::launch<128>(a, st) : q4::launch<64>(a, st);
 }

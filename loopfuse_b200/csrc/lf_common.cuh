@@ -74,20 +74,28 @@ inline int launch_status(const char* what) {
 // The kernel calls grid_wait() before it touches anything that kernel reads or writes, in every CTA
 // and on every path: a grid that ended without waiting would let its successor start too soon.
 template <class... P, class... A>
-int launch_early(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                 A&&... args) {
+int launch_early_clusters(const char* what, void (*kernel)(P...), int cluster, dim3 grid, dim3 block, size_t smem,
+                          cudaStream_t st, A&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     LF_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
     return launch_status(what);
+}
+template <class... P, class... A>
+int launch_early(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                 A&&... args) {
+    return launch_early_clusters(what, kernel, 1, grid, block, smem, st, static_cast<A&&>(args)...);
 }
 // Returns once the kernels before this one in the stream are complete and their writes visible.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -474,21 +474,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
 
 template <int DT>
 static int launch(const Args& a, int rows, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long)rows * a.parts));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see launch_early
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)a.parts;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    if (a.k > 0) LF_CHECK_CUDA((cudaLaunchKernelEx(&cfg, logprobs_kernel<DT, true>, a)));
-    else LF_CHECK_CUDA((cudaLaunchKernelEx(&cfg, logprobs_kernel<DT, false>, a)));
-    return launch_status("token logprobs");
+    return launch_early_clusters("token logprobs", a.k > 0 ? logprobs_kernel<DT, true> : logprobs_kernel<DT, false>, a.parts,
+                                 dim3((unsigned)((long)rows * a.parts)), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace logprobs

@@ -142,9 +142,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
         raise LoopfuseError(_lib.LF_EINVAL, f"token_logprobs: tokens must be contiguous int64 or int32 [{T}]")
     if not 0 <= k <= min(MAX_TOP_LOGPROBS, V):
         raise LoopfuseError(_lib.LF_EINVAL, f"token_logprobs: top_k = {k} outside 0..{min(MAX_TOP_LOGPROBS, V)}")
-    logprob, entropy = torch.empty((2, T), dtype=torch.float32, device=dev).unbind(0)
-    top_ids = torch.empty((T, k), dtype=torch.int64, device=dev)
-    top = torch.empty((T, k), dtype=torch.float32, device=dev)
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    top_ids = torch.empty(T, k, dtype=torch.int64, device=dev)
+    top = torch.empty(T, k, dtype=torch.float32, device=dev)
     if T:
         launch("lf_token_logprobs", dev, logits.data_ptr(), code, logits.stride(0), tokens.data_ptr(), wide,
                T, V, k, logprob.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), top.data_ptr())

@@ -59,7 +59,7 @@ def check_decode(lens, Hq, Hkv, D, npre=0, scale=None, width=None, seed=0, spoil
     table, P = table_for(lens, npre, gen, width)
     pages = random_pages(gen, P, Hkv, D)
     if spoil:                             # NaN scales in every row that no session holds
-        par = pages[..., 16 * D:].contiguous().view(torch.bfloat16).view(P, Hkv, 16, -1)
+        par = pages[..., 16 * D:].clone().contiguous().view(torch.bfloat16).view(P, Hkv, 16, -1)
         for i, L in enumerate(lens):
             if L % 16 and L // 16 >= npre:
                 par[int(table[i, L // 16]), :, L % 16:] = math.nan
@@ -102,6 +102,32 @@ def test_decode_shared_prefix(Hq, Hkv, D, npre):
     check_decode(lens, Hq, Hkv, D, npre=npre, spoil=True)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (8, 8, 128), (12, 12, 64), (8, 1, 64)])
+@pytest.mark.parametrize("lens", [[1], [0], [16], [31], [777], [8192], [0, 4000, 1], [5, 0, 1023, 2048, 64, 1, 700]])
+def test_decode_of_few_sessions(Hq, Hkv, D, lens):
+    check_decode(lens, Hq, Hkv, D, spoil=True)
+    check_decode(lens, Hq, Hkv, D, scale=-0.7)
+
+
+def test_decode_of_few_sessions_equals_that_of_a_wide_table():
+    gen = torch.Generator().manual_seed(2)
+    lens = torch.tensor([777, 40], dtype=torch.int32).cuda()
+    table, P = table_for([777, 40], 0, gen)
+    pages = random_pages(gen, P, 2, 128).cuda()
+    q = torch.randn(2, 8, 128, generator=gen).bfloat16().cuda()
+    few = att.paged_decode_q4(q, pages, table.cuda(), lens)
+    wide = torch.full((2, 2000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    flat = att.paged_decode_q4(q, pages, wide.cuda(), lens)
+    assert ((few - flat).float().abs() <= 2 ** -6 * flat.float().abs().clamp_min(0.25)).all()   # two bf16 steps
+    assert torch.equal(few, att.paged_decode_q4(q, pages, table.cuda(), lens))
+
+
+def test_decode_of_few_long_sessions():
+    check_decode([40000, 20001], 8, 2, 128)                # many partials a row
+    check_decode([30000], 4, 4, 64, npre=3)
+
+
 # rows x pages x KV heads x head_dim past 2^25: the prefix goes to tiles of 128 rows
 TILED = [(40, 32, 4, 128, 205), (130, 4, 4, 128, 505), (101, 8, 4, 64, 650), (33, 16, 2, 64, 993)]
 
@@ -128,7 +154,7 @@ def test_nan_in_a_shared_prefix_reaches_the_rows_that_hold_it(N, Hq, Hkv, D, npr
     def run(kv):
         x = pages.clone()
         if kv is not None:
-            par = x[..., 16 * D:].contiguous().view(torch.bfloat16).view(P, Hkv, 16, 2, D // 64, 2)
+            par = x[..., 16 * D:].clone().contiguous().view(torch.bfloat16).view(P, Hkv, 16, 2, D // 64, 2)
             par[int(table[lead, at // 16]), 0, at % 16, kv, 0] = math.nan
             x[..., 16 * D:] = par.contiguous().view(torch.uint8).flatten(2)
         return att.paged_decode_q4(q.cuda(), x.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
