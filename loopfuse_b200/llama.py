@@ -281,6 +281,8 @@ class LlamaShaped:
         successor is not given), the entropy and the ``top_k`` alternatives there.  The LM head runs
         ``rows`` positions at a time, so no logits of the whole batch are held."""
         counts = [int(n) for n in counts]
+        if not sum(counts):
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, "score: the batch has no tokens")
         tokens = tokens.to(self.device).long()
         x = self._trunk(tokens, pool, states, counts, n_prefix_pages, None, adapters, adapter_ids)
         nxt = torch.full_like(tokens, -1)

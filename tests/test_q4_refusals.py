@@ -48,7 +48,7 @@ def test_tensors_off_the_gpu_and_of_other_types_are_refused():
     (dict(head_dim=96), b"head_dim"), (dict(num_q_heads=6), b"1, 2, 4 or 8"), (dict(num_q_heads=5), b"multiple"),
     (dict(q=P + 2), b"aligned"), (dict(pages=P + 8), b"aligned"), (dict(q=None), b"null"),
     (dict(num_prefix_pages=5), b"num_prefix_pages"), (dict(num_prefix_pages=-1), b"num_prefix_pages"),
-    (dict(workspace_bytes=16), b"workspace"), (dict(max_pages=1 << 27), b"max_pages"),
+    (dict(workspace_bytes=16, max_pages=600), b"workspace"), (dict(workspace=None, max_pages=600), b"null"), (dict(max_pages=1 << 27), b"max_pages"),
     (dict(num_seqs=1 << 29), b"too many"),
     (dict(num_seqs=-1), b"negative"), (dict(max_pages=0), b"max_pages"),
 ])
@@ -115,7 +115,11 @@ def test_fork_and_pool_arguments():
 def test_workspace():
     """(148 x 12 ranges (16 of 64 dims) + N Hkv items) x G partials, prefix chunks x N Hq partials, a
     span per item."""
-    assert att.decode_q4_workspace_bytes(3, 4, 2, 64, 10, 0, 148) == (2368 + 6) * 2 * (256 + 8) + 6 * 8
-    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 0, 148) == (1776 + 6) * 2 * (512 + 8) + 6 * 8
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 64, 513, 0, 148) == (2368 + 6) * 2 * (256 + 8) + 6 * 8
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 513, 0, 148) == (1776 + 6) * 2 * (512 + 8) + 6 * 8
+    # few items whose table allows 64 pages a CTA of their cluster (8, 4 or 2 of the 444 resident): none
+    assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 512, 0, 148) == 0
+    assert att.decode_q4_workspace_bytes(50, 4, 2, 128, 256, 0, 148) == 0 != att.decode_q4_workspace_bytes(50, 4, 2, 128, 257, 0, 148)
+    assert att.decode_q4_workspace_bytes(111, 4, 2, 128, 128, 0, 148) == 0 != att.decode_q4_workspace_bytes(112, 4, 2, 128, 128, 0, 148)
     # a prefix of 16 pages or less is one chunk; no own pages, no ranges
     assert att.decode_q4_workspace_bytes(3, 4, 2, 128, 10, 10, 148) == 3 * 4 * (512 + 8) + 6 * 8
