@@ -467,7 +467,8 @@ int lf_token_logprobs(const void* logits, int dtype, int64_t row_stride, const v
  * scale [num_adapters] (nullable: 1), all bf16 but the fp32 scale; inputs and outputs multiples of
  * 8; rank 16, 32, 64 or 128 (zero columns of A and rows of B pad a smaller one).  x . A is summed
  * in fp32 and scale * (x . A) is rounded once to bf16; y is added in fp32 and the sum rounded once.
- * n, total_tokens and num_adapters are the plan's.  num_adapters <= 4096. */
+ * n, total_tokens and num_adapters are the plan's.  num_adapters <= 4096.  Where
+ * lf_lora_workspace_size gives 0 bytes the workspace may be NULL. */
 int lf_lora_plan_size(int n, int total_tokens, int num_adapters, size_t* bytes);
 int lf_lora_plan(const int32_t* adapter_ids, const int32_t* cu_tokens, int n, int total_tokens,
                  int num_adapters, void* plan, size_t plan_bytes, void* stream);

@@ -6,7 +6,8 @@
 // share an adapter's weights between its sessions.  `shrink` computes h = x A per (tile, slice of the
 // inputs) into fp32 partials; `expand` sums a tile's partials in slice order, rounds scale * h once to
 // bf16 (the operand type; an error of at most 2^-8 of the adapter's own contribution) and adds h B
-// to y in fp32, rounded once.  No atomics: the same bits in every run.
+// to y in fp32, rounded once.  No atomics: the same bits in every run.  In a decode batch of adapters
+// enough to fill the chip, `few` does the work of both in one launch.
 //
 // Both products have a rank of 16 to 128 on one side, so the work is bound by moving x, y, A and B:
 // tiles come in by cp.async several stages ahead (rows of x and y are gathered, 16 bytes a copy),
@@ -15,10 +16,14 @@
 #include "pool_common.cuh"
 #include "sm100_primitives.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace lf {
 namespace lora {
+
+namespace cg = cooperative_groups;
 
 constexpr int kTile = 64;                              // rows of a tile
 constexpr int kMaxAdapters = 4096;
@@ -172,7 +177,7 @@ struct Args {
     const uint16_t *x, *y, *a, *b;
     uint16_t* out;
     const float* scale;
-    float* part;                                       // [slices][total][R]; with one slice, h [total][R] bf16
+    float* part;                                       // [slices][total][R]; with one slice, h [total][R] bf16; few_kernel: slices 0, none
     const int32_t *head, *tiles, *order;
     int64_t x_stride, y_stride, out_stride;            // elements between rows
     int total, K, N, slices, k_per;                    // k_per: inputs of a slice, a multiple of kStep
@@ -199,24 +204,14 @@ struct ShrinkSmem {
     static constexpr int kBytes = kRing > kRed ? kRing : kRed;
 };
 
-// CTA (slice of the inputs, tile).  Warps split the tile's 16-row blocks, and, where the tile has
-// fewer than eight, the 16-input steps of a stage; those partial sums are added in warp order.
-template <int R>
-__global__ void __launch_bounds__(32 * kShrinkWarps)
-shrink_kernel(const Args g) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    // x, y and the plan are there, and this memory's last readers are done; from here on the expansion
-    // may be brought in and fetch y and B
-    grid_wait();
-    grid_release();
-    const int tile = blockIdx.y, slice = blockIdx.x;
-    if (tile >= g.head[0]) return;
-    const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
-    if (t.x < 0) return;
+// Inputs k0 .. k1 - 1 of tile t's x A, 4 sums at a time to store(index in [rows][R], sums).  Warps split
+// the tile's 16-row blocks, and, where the tile has fewer than eight, the 16-input steps of a stage;
+// those partial sums are added in warp order.
+template <int R, class Store>
+__device__ __forceinline__ void shrink_tile(const Args g, const int4 t, int k0, int k1, uint8_t* smem, Store store) {
     const int rows = t.z, first = t.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int k0 = slice * g.k_per, k1 = min(g.K, k0 + g.k_per);
-    const int steps = (k1 - k0 + kStep - 1) / kStep;
+    const int steps = k1 > k0 ? (k1 - k0 + kStep - 1) / kStep : 0;
     const uint32_t base = sm100::smem_addr(smem);
     constexpr int XC = kStep / 8, AC = R / 8;          // chunks of a row
     constexpr int SZ = ShrinkSmem<R>::kX + ShrinkSmem<R>::kA;
@@ -288,52 +283,74 @@ shrink_kernel(const Args g) {
     }
     __syncthreads();
     const int used = kw < kStep / 16 ? kw : kStep / 16;  // warps past a stage's steps hold zeros
-    float* dst = g.part + ((long)slice * g.total + first) * R;
     for (int i = threadIdx.x * 4; i < rows * R; i += 32 * kShrinkWarps * 4) {
         float4 v = *reinterpret_cast<const float4*>(red + i);
         for (int w = 1; w < used; ++w) {
             const float4 o = *reinterpret_cast<const float4*>(red + (long)w * 16 * mb * R + i);
             v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
         }
-        if (g.slices > 1) {
-            *reinterpret_cast<float4*>(dst + i) = v;
-        } else {
-            const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.part) + (long)first * R + i) =
-                make_uint2(pack_bf16x2(v.x * sc, v.y * sc), pack_bf16x2(v.z * sc, v.w * sc));
-        }
+        store(i, v);
     }
 }
 
-constexpr int kCols = 128;                             // columns of an expand block
-constexpr int kExpandWarps = 4;                        // 32 columns each
-
+// CTA (slice of the inputs, tile).
 template <int R>
+__global__ void __launch_bounds__(32 * kShrinkWarps)
+shrink_kernel(const Args g) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    // x, y and the plan are there, and this memory's last readers are done; from here on the expansion
+    // may be brought in and fetch y and B
+    grid_wait();
+    grid_release();
+    const int tile = blockIdx.y, slice = blockIdx.x;
+    if (tile >= g.head[0]) return;
+    const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
+    if (t.x < 0) return;
+    const int k0 = slice * g.k_per, k1 = min(g.K, k0 + g.k_per);
+    if (g.slices > 1) {
+        float* dst = g.part + ((long)slice * g.total + t.y) * R;
+        shrink_tile<R>(g, t, k0, k1, smem, [&](int i, const float4& v) { *reinterpret_cast<float4*>(dst + i) = v; });
+    } else {
+        uint16_t* h = reinterpret_cast<uint16_t*>(g.part) + (long)t.y * R;
+        const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+        shrink_tile<R>(g, t, k0, k1, smem, [&](int i, const float4& v) {
+            *reinterpret_cast<uint2*>(h + i) = make_uint2(pack_bf16x2(v.x * sc, v.y * sc), pack_bf16x2(v.z * sc, v.w * sc));
+        });
+    }
+}
+
+constexpr int kExpandWarps = 4;                        // 32 columns each
+constexpr int kBlockCols = 32 * kExpandWarps;          // columns of a block of the expansion
+
+template <int R, int W>
 struct ExpandSmem {
+    static constexpr int kCols = 32 * W;               // columns of a block
     static constexpr int kH = kTile * R * 2, kB = R * kCols * 2, kY = kTile * kCols * 2;
     static constexpr int kBuf = kB + kY;
     static constexpr int kBytes = kH + 2 * kBuf;
 };
 
-// CTA (group of column blocks, tile): h of the tile once, then per block of 128 columns y + h B,
-// staged in shared memory, the next block's y and B on their way meanwhile.
+// 8 values of h, scaled and rounded, to a tile's h in shared memory.
 template <int R>
-__global__ void __launch_bounds__(32 * kExpandWarps)
-expand_kernel(const Args g) {
-    using S = ExpandSmem<R>;
-    extern __shared__ __align__(128) uint8_t smem[];
-    const int tile = blockIdx.y;
-    const bool none = tile >= g.head[0];
-    const int4 t = none ? make_int4(-1, 0, 0, 0) : reinterpret_cast<const int4*>(g.tiles)[tile];
+__device__ __forceinline__ void put_h(uint8_t* smem, int row, int chunk, const float (&v)[8], float sc) {
+    *reinterpret_cast<uint4*>(smem + at<R / 8>(row, chunk)) =
+        make_uint4(pack_bf16x2(v[0] * sc, v[1] * sc), pack_bf16x2(v[2] * sc, v[3] * sc),
+                   pack_bf16x2(v[4] * sc, v[5] * sc), pack_bf16x2(v[6] * sc, v[7] * sc));
+}
+
+// y + h B of tile t in column blocks block0, block0 + skip, ... (n_blocks), staged in shared memory, the
+// next block's y and B on their way meanwhile.  W warps; form() puts h (rows to the next multiple of 16,
+// zeros past the tile's) at the start of `smem` once the first block is on its way.
+template <int R, int W, class Form>
+__device__ __forceinline__ void expand_tile(const Args g, const int4 t, uint8_t* smem, int block0, int skip, int n_blocks,
+                                            Form form) {
+    using S = ExpandSmem<R, W>;
+    constexpr int kCols = S::kCols;
     const int rows = t.z, first = t.y;
     const bool copy_only = t.x < 0;
-    if (none || (copy_only && g.y == g.out)) {
-        grid_wait();
-        return;
-    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int YC = kCols / 8, HC = R / 8;
-    constexpr int T = 32 * kExpandWarps, RS = T / YC, NR = kTile / RS;   // rows of a pass, passes
+    constexpr int T = 32 * W, RS = T / YC, NR = kTile / RS;   // rows of a pass, passes
     const uint32_t sh = sm100::smem_addr(smem);
     const uint16_t* B = g.b + (long)(copy_only ? 0 : t.x) * R * g.N;
     const int c = threadIdx.x % YC, r0 = threadIdx.x / YC;      // this thread's chunk column, first row
@@ -341,12 +358,10 @@ expand_kernel(const Args g) {
     int tok[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) tok[i] = r0 + i * RS < rows ? g.order[first + r0 + i * RS] : -1;
-    const int n_first = blockIdx.x * g.cols * kCols;
-    const int n_blocks = min(g.cols, (g.N - n_first + kCols - 1) / kCols);
     // A thread copies in and writes out the same pieces of y, so a buffer's y needs no barrier between.
     auto load = [&](int blk) {
         if (blk < n_blocks) {
-            const int col = n_first + blk * kCols + 8 * c;
+            const int col = (block0 + blk * skip) * kCols + 8 * c;
             const uint32_t sb = sh + S::kH + (blk & 1) * S::kBuf, sy = sb + S::kB;
             const bool on = col < g.N;
 #pragma unroll
@@ -360,35 +375,7 @@ expand_kernel(const Args g) {
         cp_commit();
     };
     load(0);
-    grid_wait();                                                // h is there
-    if (!copy_only) {
-        if (g.slices == 1) {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(g.part) + (long)first * R;
-            for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
-                const int r = i / HC, ch = i % HC;
-                *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
-                    r < rows ? *reinterpret_cast<const uint4*>(h + (long)r * R + 8 * ch) : make_uint4(0, 0, 0, 0);
-            }
-        } else {                                       // partials summed in slice order, scaled, rounded
-            const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
-            for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
-                const int r = i / HC, ch = i % HC;
-                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (r < rows) {
-#pragma unroll 4
-                    for (int s = 0; s < g.slices; ++s) {
-                        const float4* p = reinterpret_cast<const float4*>(g.part + ((long)s * g.total + first + r) * R + 8 * ch);
-                        const float4 a = p[0], b = p[1];
-                        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-                        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-                    }
-                }
-                *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
-                    make_uint4(pack_bf16x2(v[0] * sc, v[1] * sc), pack_bf16x2(v[2] * sc, v[3] * sc),
-                               pack_bf16x2(v[4] * sc, v[5] * sc), pack_bf16x2(v[6] * sc, v[7] * sc));
-            }
-        }
-    }
+    form(sh, blocks);
     // h of the tile in registers for all blocks, where it fits (64 of a thread's at rank 64)
     constexpr bool kHeld = R <= 64;
     constexpr int MB = kTile / 16, KB = R / 16;
@@ -411,7 +398,7 @@ expand_kernel(const Args g) {
         uint8_t* yb = smem + S::kH + (blk & 1) * S::kBuf + S::kB;
         if (!copy_only) {
             const int gq = lane >> 2, cq = lane & 3;
-            constexpr int CJ = kCols / kExpandWarps / 16;   // 16-column pieces of a warp
+            constexpr int CJ = kCols / W / 16;   // 16-column pieces of a warp
             uint32_t b[KB][CJ][4];                     // B of this warp's columns, for every row block
 #pragma unroll
             for (int kk = 0; kk < KB; ++kk)
@@ -450,7 +437,7 @@ expand_kernel(const Args g) {
             }
             __syncthreads();
         }
-        const int col = n_first + blk * kCols + 8 * c;
+        const int col = (block0 + blk * skip) * kCols + 8 * c;
         if (col < g.N) {
 #pragma unroll
             for (int i = 0; i < NR; ++i)
@@ -459,6 +446,122 @@ expand_kernel(const Args g) {
                         *reinterpret_cast<const uint4*>(yb + at<YC>(r0 + i * RS, c));
         }
     }
+}
+
+// CTA (group of column blocks, tile).
+template <int R>
+__global__ void __launch_bounds__(32 * kExpandWarps)
+expand_kernel(const Args g) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int kCols = ExpandSmem<R, kExpandWarps>::kCols, HC = R / 8, T = 32 * kExpandWarps;
+    const int tile = blockIdx.y;
+    const bool none = tile >= g.head[0];
+    const int4 t = none ? make_int4(-1, 0, 0, 0) : reinterpret_cast<const int4*>(g.tiles)[tile];
+    if (none || (t.x < 0 && g.y == g.out)) {
+        grid_wait();
+        return;
+    }
+    const int block0 = blockIdx.x * g.cols;
+    const int n_blocks = min(g.cols, (g.N + kCols - 1) / kCols - block0);
+    expand_tile<R, kExpandWarps>(g, t, smem, block0, 1, n_blocks, [&](uint32_t, int blocks) {
+        const int rows = t.z, first = t.y;
+        const bool copy_only = t.x < 0;
+        grid_wait();                                                // h is there
+        if (!copy_only) {
+            if (g.slices == 1) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(g.part) + (long)first * R;
+                for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
+                    const int r = i / HC, ch = i % HC;
+                    *reinterpret_cast<uint4*>(smem + at<HC>(r, ch)) =
+                        r < rows ? *reinterpret_cast<const uint4*>(h + (long)r * R + 8 * ch) : make_uint4(0, 0, 0, 0);
+                }
+            } else {                                       // partials summed in slice order, scaled, rounded
+                const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+                for (int i = threadIdx.x; i < 16 * blocks * HC; i += T) {
+                    const int r = i / HC, ch = i % HC;
+                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (r < rows) {
+#pragma unroll 4
+                        for (int s = 0; s < g.slices; ++s) {
+                            const float4* p = reinterpret_cast<const float4*>(g.part + ((long)s * g.total + first + r) * R + 8 * ch);
+                            const float4 a = p[0], b = p[1];
+                            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                            v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+                        }
+                    }
+                    put_h<R>(smem, r, ch, v, sc);
+                }
+            }
+        }
+    });
+}
+
+// A decode batch's tiles (a few rows each): a cluster of kParts CTAs a tile, in one launch and without a
+// workspace (96 rows of 16 adapters, 4096 -> 6144, rank 16: 20.8 us a call, plan included, 24.8 in two).  Each CTA sums a
+// slice of the inputs; the sums are exchanged through distributed shared memory, added in slice order by
+// every CTA, and the column blocks shared out.
+constexpr int kParts = 8;                              // portable cluster size
+template <int R>
+struct FewSmem {
+    static constexpr int kPart = kTile * R * 4;        // this CTA's sums [row][R]
+    static constexpr int kRest = ShrinkSmem<R>::kBytes > ExpandSmem<R, kShrinkWarps>::kBytes
+                                     ? ShrinkSmem<R>::kBytes : ExpandSmem<R, kShrinkWarps>::kBytes;
+    static constexpr int kBytes = kPart + kRest;
+};
+template <int R>
+__global__ void __launch_bounds__(32 * kShrinkWarps)
+few_kernel(const Args g) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    grid_wait();
+    grid_release();
+    const int tile = blockIdx.x / kParts, slice = blockIdx.x % kParts;
+    if (tile >= g.head[0]) return;                     // (the whole cluster, here and below)
+    const int4 t = reinterpret_cast<const int4*>(g.tiles)[tile];
+    if (t.x < 0 && g.y == g.out) return;
+    cg::cluster_group cluster = cg::this_cluster();
+    float* part = reinterpret_cast<float*>(smem);
+    uint8_t* rest = smem + FewSmem<R>::kPart;
+    if (t.x >= 0) {
+        const int k0 = slice * g.k_per, k1 = min(g.K, k0 + g.k_per);
+        shrink_tile<R>(g, t, k0, k1, rest, [&](int i, const float4& v) { *reinterpret_cast<float4*>(part + i) = v; });
+        __syncthreads();                               // `rest` is free
+    }
+    constexpr int kCols = ExpandSmem<R, kShrinkWarps>::kCols, HC = R / 8;
+    const int all = (g.N + kCols - 1) / kCols, n_blocks = all > slice ? (all - slice + kParts - 1) / kParts : 0;
+    expand_tile<R, kShrinkWarps>(g, t, rest, slice, kParts, n_blocks, [&](uint32_t, int blocks) {
+        if (t.x < 0) return;
+        const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+        cluster.sync();
+        for (int i = threadIdx.x; i < 16 * blocks * HC; i += 32 * kShrinkWarps) {
+            const int r = i / HC, ch = i % HC;
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (r < t.z) {
+                float4 x[kParts][2];
+#pragma unroll
+                for (int s = 0; s < kParts; ++s) {
+                    const float4* p = reinterpret_cast<const float4*>(cluster.map_shared_rank(part + r * R + 8 * ch, s));
+                    x[s][0] = p[0];
+                    x[s][1] = p[1];
+                }
+#pragma unroll
+                for (int s = 0; s < kParts; ++s) {
+                    v[0] += x[s][0].x; v[1] += x[s][0].y; v[2] += x[s][0].z; v[3] += x[s][0].w;
+                    v[4] += x[s][1].x; v[5] += x[s][1].y; v[6] += x[s][1].z; v[7] += x[s][1].w;
+                }
+            }
+            put_h<R>(rest, r, ch, v, sc);
+        }
+        cluster.sync();                                // others may still read this CTA's sums
+    });
+}
+
+// Whether the tiles' clusters are one launch's work: three quarters of the SMs at least, two CTAs of one
+// at most.  Fewer leave SMs empty (10 tiles, 4096 -> 28672, rank 16: 22.5 us against 20.5 in two launches; 14
+// tiles 22.5 : 26.6), more, and ranks above 32, wait too long for one another in a CTA (19 tiles, 4096 -> 6144:
+// rank 16 14.3 : 16.4, 32 16.4 : 18.4, 64 26.7 : 20.5; 66 tiles of rank 64 125 : 76).
+inline bool is_few(int total, int n, int adapters, int rank, int sms) {
+    const long ctas = max_tiles(total, n, adapters) * kParts;
+    return rank <= 32 && 4 * ctas >= 3L * sms && ctas <= 2L * sms;
 }
 
 inline int slices_for(int total, int n, int adapters, int K, int sms) {
@@ -484,15 +587,23 @@ static int launch(const Args& g, int tiles, cudaStream_t st) {
         LF_CHECK_CUDA(cudaFuncSetAttribute(shrink_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            ShrinkSmem<R>::kBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(expand_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           ExpandSmem<R>::kBytes));
+                                           ExpandSmem<R, kExpandWarps>::kBytes));
+        if constexpr (R <= 32)
+            LF_CHECK_CUDA(cudaFuncSetAttribute(few_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               FewSmem<R>::kBytes));
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
+    if constexpr (R <= 32) {
+        if (g.slices == 0)
+            return launch_early_clusters("lora", few_kernel<R>, kParts, dim3((unsigned)(tiles * kParts)),
+                                         dim3(32 * kShrinkWarps), FewSmem<R>::kBytes, st, g);
+    }
     const int e = launch_early("lora shrink", shrink_kernel<R>, dim3(g.slices, tiles), dim3(32 * kShrinkWarps),
                                ShrinkSmem<R>::kBytes, st, g);
     if (e != LF_OK) return e;
-    return launch_early("lora expand", expand_kernel<R>, dim3(((g.N + kCols - 1) / kCols + g.cols - 1) / g.cols, tiles),
-                        dim3(32 * kExpandWarps), ExpandSmem<R>::kBytes, st, g);
+    return launch_early("lora expand", expand_kernel<R>, dim3(((g.N + kBlockCols - 1) / kBlockCols + g.cols - 1) / g.cols, tiles),
+                        dim3(32 * kExpandWarps), ExpandSmem<R, kExpandWarps>::kBytes, st, g);
 }
 
 static int sm_count(int* out) {
@@ -553,7 +664,8 @@ extern "C" int lf_lora_workspace_size(int n, int total_tokens, int num_adapters,
         rc = lora::sm_count(&sm_count);
         if (rc != LF_OK) return rc;
     }
-    *bytes = (size_t)lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count) * total_tokens * rank * 4;
+    *bytes = lora::is_few(total_tokens, n, num_adapters, rank, sm_count)
+                 ? 0 : (size_t)lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count) * total_tokens * rank * 4;
     clear_error();
     return LF_OK;
 }
@@ -570,7 +682,7 @@ extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x,
     LF_CHECK_ARG(inputs > 0 && inputs % 8 == 0 && outputs > 0 && outputs % 8 == 0,
                  "lora: inputs and outputs must be positive multiples of 8");
     if (total_tokens == 0) { clear_error(); return LF_OK; }
-    LF_CHECK_ARG(y && x && a && b && plan && out && workspace, "lora: null pointer argument");
+    LF_CHECK_ARG(y && x && a && b && plan && out, "lora: null pointer argument");
     LF_CHECK_ARG(aligned16(y) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(out) &&
                      aligned16(plan) && aligned16(workspace) && y_stride % 8 == 0 && x_stride % 8 == 0 &&
                      out_stride % 8 == 0,
@@ -583,8 +695,10 @@ extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x,
         if (rc != LF_OK) return rc;
     }
     lora::Args g{};
-    g.slices = lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count);
+    const bool few = lora::is_few(total_tokens, n, num_adapters, rank, sm_count);
+    g.slices = few ? 0 : lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count);
     const size_t need = (size_t)g.slices * total_tokens * rank * 4;
+    LF_CHECK_ARG(workspace != nullptr || need == 0, "lora: null pointer argument");
     LF_CHECK_ARG(workspace_bytes >= need, "lora: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
     const lora::Plan p = lora::views(const_cast<int32_t*>(static_cast<const int32_t*>(plan)), total_tokens, n, num_adapters);
     g.x = x;
@@ -604,9 +718,10 @@ extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x,
     g.K = inputs;
     g.N = outputs;
     const int steps = (inputs + lora::kStep - 1) / lora::kStep;
-    g.k_per = (steps + g.slices - 1) / g.slices * lora::kStep;
+    const int cuts = few ? lora::kParts : g.slices;
+    g.k_per = (steps + cuts - 1) / cuts * lora::kStep;
     const int tiles = (int)lora::max_tiles(total_tokens, n, num_adapters);
-    g.cols = lora::column_blocks((outputs + lora::kCols - 1) / lora::kCols, tiles, rank, sm_count);
+    g.cols = lora::column_blocks((outputs + lora::kBlockCols - 1) / lora::kBlockCols, tiles, rank, sm_count);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (rank) {
         case 16: return lora::launch<16>(g, tiles, st);

@@ -241,8 +241,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         return res
     sms = sm_count(dev.index)
     need = _lora_workspace_bytes(plan.sessions, T, adapters, K, R, sms)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     launch("lf_lora_add", dev, y.data_ptr(), sy, x.data_ptr(), sx, a.data_ptr(), b.data_ptr(),
            scale.data_ptr() if scale is not None else None, plan.buffer.data_ptr(), plan.sessions, T,
-           adapters, K, N, R, res.data_ptr(), so, ws.data_ptr(), need, sms)
+           adapters, K, N, R, res.data_ptr(), so, ws.data_ptr() if need else None, need, sms)
     return res
