@@ -59,7 +59,9 @@ using decode::checked_page;
 using decode::kThreads;
 using decode::kWarps;
 
-constexpr int kUnit = 2;                       // own: pages of a barrier, a softmax step, a buffer
+// own: pages of a unit (a barrier, a softmax step, a buffer).  GP: heads of a group whose units are packed
+// (1 or 2, of 64 dims), or 0.
+constexpr int unit_pages(int GP) { return GP > 0 ? 4 : 2; }
 constexpr int kStages = 2;                     // own: units in flight per warp
 constexpr int per_sm(int D) { return D == 64 ? 4 : 3; }   // own: resident CTAs of an SM (registers)
 constexpr int kMinUnits = 2;                   // own: units of a range
@@ -88,9 +90,10 @@ __device__ __forceinline__ int held(const DecodeArgs& a, int n) {
     return n < a.N ? min(max(a.lens[n], 0), a.max_pages * kPage) : 0;
 }
 // Units of a session's own pages.
+template <int U>
 __device__ __forceinline__ int own_units(const DecodeArgs& a, int n) {
     const int own = (held(a, n) + kPage - 1) / kPage - a.n_prefix;
-    return own > 0 ? (own + kUnit - 1) / kUnit : 0;
+    return own > 0 ? (own + U - 1) / U : 0;
 }
 
 // Waits for a phase; false after kWaitNs.
@@ -351,8 +354,11 @@ struct State {
         }
     }
 
+    // The head that column g stands for, or -1.
+    static __device__ __forceinline__ int head_of(int g, int G) { return g < G ? g : -1; }
+
     // Sums over the lanes that share a column; o then holds the whole unnormalised rows.
-    __device__ __forceinline__ void finish() {
+    __device__ __forceinline__ void finish(float) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
@@ -373,13 +379,209 @@ struct State {
     }
 };
 
+// The same for groups of G = 1 or 2 heads of 64 dims, 4 pages at once: column n stands for head n % G over
+// page n / G, so that the softmax's arithmetic, the same for 8 columns as for one, serves 4 pages.  A page's
+// MMAs get the operand with the other pages' columns zero, and all add to the same accumulators.  Columns
+// keep their own maximum and sums; those of a head are joined at the end.
+// 96 sessions x 12 heads of 64 x 4000 tokens: 73 us, 85 with two pages a unit in columns of their own;
+// 1 to 1280 tokens: 21.5 and 23.8; 64 sessions x 8 heads of 2 x 6000: 53 and 61; 300 tokens: 15.4 and 14.7.
+// (A chain of MMAs for each page: 74.4.)
+template <int G>
+struct Packed {
+    static constexpr int U = 4, NG = 1;
+    uint32_t qb[4][2];                         // Q^T operand, column g: q 2^64, q 2^60
+    float qsum[2];
+    float o[1][4][4];
+    float corr[4];
+    float bias[2];
+    float m[2], l[2];
+
+    static __device__ __forceinline__ int head_of(int g, int) { return g < U * G ? g % G : -1; }
+
+    __device__ __forceinline__ void init(const uint16_t* row, uint32_t flip, int c) {
+        State<64, 1> one;
+        one.init(row, flip, c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            qb[k][0] = one.qb[0][k][0];
+            qb[k][1] = one.qb[0][k][1];
+            corr[k] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[0][k][j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            qsum[j] = one.qsum[0][j];
+            bias[j] = l[j] = 0.f;
+            m[j] = -INFINITY;
+        }
+    }
+
+    template <bool kMasked>
+    __device__ __forceinline__ void unit(uint32_t base, int tok0, const int (&len)[2], float qscale, int lane) {
+        using F = Fmt<64>;
+        const int g = lane >> 2, c = lane & 3;
+        float acc[2][4];                       // pages 0 and 1, 2 and 3
+#pragma unroll
+        for (int p = 0; p < U; ++p) {
+            const uint32_t blk = base + (uint32_t)(p * F::kBlockBytes);
+            const uint32_t sel = g / G == p ? 0xFFFFFFFFu : 0u;
+            uint32_t ka[2], kb[2];
+            lds<2>(blk + g * 32 + c * 8, ka);
+            lds<2>(blk + (g + 8) * 32 + c * 8, kb);
+            float(&d)[4] = acc[p / 2];
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t a0 = codes(ka[w], 2 * k), a1 = codes(kb[w], 2 * k);
+                    const uint32_t a2 = codes(ka[w], 2 * k + 1), a3 = codes(kb[w], 2 * k + 1);
+                    const uint32_t b0 = qb[2 * w + k][0] & sel, b1 = qb[2 * w + k][1] & sel;
+                    if (p % 2 == 0 && w == 0 && k == 0) {
+                        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma(d, a0, a1, a2, a3, b0, b1, zero);
+                    } else {
+                        mma(d, a0, a1, a2, a3, b0, b1, d);
+                    }
+                }
+        }
+        // This lane's columns 2c, 2c + 1 and the pages they stand for (past the last one: any page, masked).
+        const int p0 = (2 * c / G) % U, p1 = ((2 * c + 1) / G) % U;
+        const bool live = 2 * c < U * G;
+        float s[4], vs[4], vb[4];              // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
+        bool keep[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (G == 2 && j % 2 == 1) continue;          // the same page: below
+            const int page = j % 2 == 0 ? p0 : p1, tok = g + 8 * (j / 2);
+            uint32_t par[2];
+            lds<2>(base + (uint32_t)(page * F::kBlockBytes + F::kParOff + tok * 8), par);
+            const float ks = bf16lo_to_f32(par[0]), kl = bf16hi_to_f32(par[0]);
+            vs[j] = bf16lo_to_f32(par[1]);
+            vb[j] = fmaf(8.f, vs[j], bf16hi_to_f32(par[1]));
+            s[j] = fmaf(ks, acc[0][j] + acc[1][j], kl * qsum[j % 2]);
+            if (G == 2) {
+                vs[j + 1] = vs[j];
+                vb[j + 1] = vb[j];
+                s[j + 1] = fmaf(ks, acc[0][j + 1] + acc[1][j + 1], kl * qsum[1]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int page = j % 2 == 0 ? p0 : p1;
+            keep[j] = live && (!kMasked || tok0 + kPage * page + g + 8 * (j / 2) < len[0]);
+            if (kMasked || G == 1) s[j] = keep[j] ? s[j] : -INFINITY;
+        }
+        float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+        if (__any_sync(0xffffffffu, x0 > m[0] || x1 > m[1])) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+            }
+            const float n0 = fmaxf(m[0], x0), n1 = fmaxf(m[1], x1);
+            const float f0 = m[0] == -INFINITY ? 0.f : (m[0] == n0 ? 1.f : fast_exp2((m[0] - n0) * qscale));
+            const float f1 = m[1] == -INFINITY ? 0.f : (m[1] == n1 ? 1.f : fast_exp2((m[1] - n1) * qscale));
+            m[0] = n0;
+            m[1] = n1;
+            l[0] *= f0;
+            l[1] *= f1;
+            bias[0] *= f0;
+            bias[1] *= f1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) corr[j] *= (j & 1) ? f1 : f0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[0][k][j] *= (j & 1) ? f1 : f0;
+        }
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0] * -qscale, r1 = m[1] == -INFINITY ? 0.f : m[1] * -qscale;
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float e = fast_exp2(fmaf(s[j], qscale, (j & 1) ? r1 : r0));
+            if (kMasked || G == 1) e = keep[j] ? e : 0.f;
+            l[j & 1] += e;
+            // what a masked token's scales hold does not count
+            bias[j & 1] = kMasked || G == 1 ? bias[j & 1] + (keep[j] ? e * vb[j] : 0.f) : fmaf(e, vb[j], bias[j & 1]);
+            p[j] = e * (vs[j] * kUp);
+            if (kMasked || G == 1) p[j] = keep[j] ? p[j] : 0.f;
+        }
+        const uint32_t b0 = movm_t(pack_bf16x2(p[0], p[1])), b1 = movm_t(pack_bf16x2(p[2], p[3]));
+        mma(corr, 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1, corr);
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            const uint32_t blk = base + (uint32_t)(q * F::kBlockBytes) + F::kVOff;
+            const uint32_t sel = g / G == q ? 0xFFFFFFFFu : 0u;
+            uint32_t va[2], vb2[2];            // tokens 2c, 2c + 1 and 2c + 8, 2c + 9
+            lds<2>(blk + lane * 8, va);
+            lds<2>(blk + 256 + lane * 8, vb2);
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    mma(o[0][2 * w + k], codes(va[w], 2 * k), codes(va[w], 2 * k + 1), codes(vb2[w], 2 * k),
+                        codes(vb2[w], 2 * k + 1), b0 & sel, b1 & sel, o[0][2 * w + k]);
+        }
+    }
+
+    // Sums over lanes and over the columns of a head; columns 0 .. G - 1 then hold the rows.
+    __device__ __forceinline__ void finish(float qscale) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
+                bias[j] += __shfl_xor_sync(0xffffffffu, bias[j], off);
+            }
+        }
+        float M[2] = {m[0], m[1]};
+        if (G == 1) M[0] = M[1] = fmaxf(M[0], M[1]);
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) M[j] = fmaxf(M[j], __shfl_xor_sync(0xffffffffu, M[j], off));
+        float w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            // (a column that has met no token has sums of zero, or of NaN: any finite weight will do)
+            w[j] = m[j] == M[j] ? 1.f : (m[j] == -INFINITY ? 0.f : fast_exp2((m[j] - M[j]) * qscale));
+            m[j] = M[j];
+        }
+        auto join = [&](float x0, float x1, float& y0, float& y1) {
+            x0 *= w[0];
+            x1 *= w[1];
+            if (G == 1) x0 += x1;
+#pragma unroll
+            for (int off = 1; off < 4; off <<= 1) {
+                x0 += __shfl_xor_sync(0xffffffffu, x0, off);
+                if (G == 2) x1 += __shfl_xor_sync(0xffffffffu, x1, off);
+            }
+            y0 = x0;
+            y1 = x1;
+        };
+        join(l[0], l[1], l[0], l[1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                o[0][k][j] = fmaf(o[0][k][j] + corr[j], j < 2 ? kDown : kDown / 16.f, bias[j & 1]);
+            join(o[0][k][0], o[0][k][1], o[0][k][0], o[0][k][1]);
+            join(o[0][k][2], o[0][k][3], o[0][k][2], o[0][k][3]);
+        }
+    }
+};
+template <int D, int GP> struct StateOf { typedef State<D, 2> T; };
+template <> struct StateOf<64, 1> { typedef Packed<1> T; };
+template <> struct StateOf<64, 2> { typedef Packed<2> T; };
+
 // Dim of accumulator row g of m-tile k of group gr (row g + 8 is the next dim).
 __device__ __forceinline__ int out_dim(int gr, int k, int g) { return gr * kGroup + 8 * g + 2 * k; }
 
 // -- own pages ----------------------------------------------------------------------------------------
-template <int D>
+template <int D, int GP>
 struct OwnSmem {
-    static constexpr int kUnitBytes = kUnit * Fmt<D>::kBlockBytes;
+    static constexpr int kUnitBytes = unit_pages(GP) * Fmt<D>::kBlockBytes;
     static constexpr int kQ = 8 * D * 2;                   // queries of a KV head, at most 8 rows
     static constexpr int kWarp = kStages * kUnitBytes + 2 * kQ;
     static constexpr int kBytes = kWarps * kWarp + 128;
@@ -406,11 +608,12 @@ struct Segment {
     int n, h, j, j1, u, L;
     long left;
     // Moves on to the next segment; false at the range's end.
+    template <int U>
     __device__ __forceinline__ bool next(const DecodeArgs& a) {
         if (left <= 0) return false;
         if (++h == a.Hkv) {
             h = 0;
-            do { u = own_units(a, ++n); } while (u == 0 && n < a.N);
+            do { u = own_units<U>(a, ++n); } while (u == 0 && n < a.N);
             if (u == 0) return false;                            // (not met: units are left)
             L = held(a, n);
         }
@@ -437,45 +640,46 @@ __device__ __forceinline__ uint32_t init_ring(uint64_t* bars, int lane) {
 // A warp's segments, from `seg` on: copies, products, partials.  kFew: to the CTA's shared memory (part_o
 // [warp][8 rows][D]), else to the range's slots.  (`a` by value: by reference the ragged case takes 42.1
 // us, not 41.2.)
-template <int D, bool kFew>
+template <int D, int GP, bool kFew>
 __device__ __forceinline__ void run_segments(const DecodeArgs a, Segment seg, int range, uint8_t* mem, uint32_t bar,
                                              float* part_o, float2* part_ml) {
     using F = Fmt<D>;
-    constexpr int UB = OwnSmem<D>::kUnitBytes;
+    constexpr int U = unit_pages(GP), UB = OwnSmem<D, GP>::kUnitBytes;
+    typedef typename StateOf<D, GP>::T St;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint8_t* qbuf = mem + kStages * UB;
     const uint32_t ring = sm100::smem_addr(mem), qring = ring + kStages * UB;
-    // What it copies: a segment that runs ahead.  Page ids of 16 units at a time, one page per
-    // lane (lane 2 i + p: page p of the i-th).
+    // What it copies: a segment that runs ahead.  Page ids of 32 / U units at a time, one page per
+    // lane (lane U i + p: page p of the i-th).
     Segment pre = seg;
     bool more = true, fresh = true;                          // fresh: the segment's first unit
-    int ids = 0, ids_at = 16;
+    int ids = 0, ids_at = 32 / U;
     uint32_t issued = 0, used = 0, q_in = 0;
     const uint64_t policy = sm100::l2_evict_first_policy();  // read once
     auto issue = [&]() {                                     // warp-uniform: one unit, if any is left
         if (more && pre.j >= pre.j1) {
-            more = pre.next(a);
+            more = pre.template next<U>(a);
             fresh = true;
-            ids_at = 16;
+            ids_at = 32 / U;
         }
         if (!more) return;
-        if (ids_at == 16) {
+        if (ids_at == 32 / U) {
             ids_at = 0;
-            const int p = a.n_prefix + (pre.j + lane / kUnit) * kUnit + lane % kUnit;
+            const int p = a.n_prefix + (pre.j + lane / U) * U + lane % U;
             ids = p < (pre.L + kPage - 1) / kPage ? checked_page(a.bt[(size_t)pre.n * a.max_pages + p], a.num_pages) : -1;
         }
-        const int page = __shfl_sync(0xffffffffu, ids, ids_at * kUnit + lane % kUnit);
-        const int last = __shfl_sync(0xffffffffu, page, kUnit - 1);
+        const int page = __shfl_sync(0xffffffffu, ids, ids_at * U + lane % U);
+        const int n_pages = __popc(__ballot_sync(0xffffffffu, lane < U && page >= 0));
         const int st = issued % kStages;
         const uint32_t q_bytes = a.G * D * 2;
         if (lane == 0)
-            sm100::mbar_arrive_expect_tx(bar + 8 * st, (last >= 0 ? UB : F::kBlockBytes) + (fresh ? q_bytes : 0));
+            sm100::mbar_arrive_expect_tx(bar + 8 * st, n_pages * F::kBlockBytes + (fresh ? q_bytes : 0));
         __syncwarp();
-        if (lane < kUnit && page >= 0)
+        if (lane < U && page >= 0)
             bulk_load(ring + (uint32_t)(st * UB + lane * F::kBlockBytes),
                       a.pages + ((size_t)page * a.Hkv + pre.h) * F::kBlockBytes, F::kBlockBytes, bar + 8 * st, policy);
-        if (fresh && lane == kUnit)
-            bulk_load(qring + (q_in & 1) * OwnSmem<D>::kQ, a.q + ((size_t)pre.n * a.Hq + pre.h * a.G) * D, q_bytes,
+        if (fresh && lane == U)
+            bulk_load(qring + (q_in & 1) * OwnSmem<D, GP>::kQ, a.q + ((size_t)pre.n * a.Hq + pre.h * a.G) * D, q_bytes,
                       bar + 8 * st, policy);
         q_in += fresh;
         fresh = false;
@@ -491,7 +695,7 @@ __device__ __forceinline__ void run_segments(const DecodeArgs a, Segment seg, in
     do {
         const int item = seg.n * a.Hkv + seg.h, L = seg.L;
         const int len[2] = {L, L};
-        State<D, kUnit> st;
+        St st;
         for (int j = seg.j; j < seg.j1; ++j) {
             const int sl = used % kStages;
             if (!warp_wait(bar + 8 * sl, (used / kStages) & 1)) {
@@ -503,20 +707,21 @@ __device__ __forceinline__ void run_segments(const DecodeArgs a, Segment seg, in
                 break;
             }
             if (j == seg.j) {
-                const uint16_t* rows = reinterpret_cast<const uint16_t*>(qbuf + (q_out & 1) * OwnSmem<D>::kQ);
-                st.init(g < a.G ? rows + g * D : nullptr, a.flip, c);
+                const uint16_t* rows = reinterpret_cast<const uint16_t*>(qbuf + (q_out & 1) * OwnSmem<D, GP>::kQ);
+                const int head = St::head_of(g, a.G);
+                st.init(head >= 0 ? rows + head * D : nullptr, a.flip, c);
                 ++q_out;
             }
             const uint32_t blk = ring + (uint32_t)(sl * UB);
-            const int tok0 = (a.n_prefix + j * kUnit) * kPage;
-            if (tok0 + kUnit * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
+            const int tok0 = (a.n_prefix + j * U) * kPage;
+            if (tok0 + U * kPage <= L) st.template unit<false>(blk, tok0, len, a.qscale, lane);
             else st.template unit<true>(blk, tok0, len, a.qscale, lane);
             __syncwarp();                                    // every lane has read the buffer
             ++used;
             issue();
         }
         if (failed) break;
-        st.finish();
+        st.finish(a.qscale);
         // Columns 2c and 2c + 1 are heads of the group; lane g holds 2 dims of each m-tile.
         const size_t slot = kFew ? (size_t)warp * 8 : (size_t)(range + item) * a.G;
         float* out_o = kFew ? part_o : a.own_o;
@@ -538,7 +743,7 @@ __device__ __forceinline__ void run_segments(const DecodeArgs a, Segment seg, in
             if (seg.j == 0) a.span[item].x = range;
             if (seg.j1 == seg.u) a.span[item].y = range;
         }
-    } while (seg.next(a));
+    } while (seg.template next<U>(a));
 }
 
 template <int V> struct Vec;
@@ -607,7 +812,7 @@ __device__ void merge_few(const DecodeArgs& a, float* part_o, float2* part_ml) {
     cluster.sync();                                              // others may still read this CTA's shared memory
 }
 
-template <int D>
+template <int D, int GP>
 __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeArgs a) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
@@ -619,14 +824,14 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
     if (a.n_chunks == 0) grid_wait();
     grid_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint8_t* mem = align128(smem_raw) + warp * OwnSmem<D>::kWarp;
+    uint8_t* mem = align128(smem_raw) + warp * OwnSmem<D, GP>::kWarp;
     const uint32_t bar = init_ring(bars + warp * kStages, lane);
     // Units of a CTA's width of sessions, summed up to each: the first such chunk serves the total and,
     // in most batches, the search.
     long excl = 0, chunk = 0;                                    // units before this thread's session; of the chunk
     int u = 0;
     auto scan = [&](int n0) {
-        u = n0 + threadIdx.x < a.N ? own_units(a, n0 + threadIdx.x) : 0;
+        u = n0 + threadIdx.x < a.N ? own_units<unit_pages(GP)>(a, n0 + threadIdx.x) : 0;
         long incl = u;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -648,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
     long total = chunk;
     if (a.N > kThreads) {
         long mine = 0;
-        for (int n = kThreads + threadIdx.x; n < a.N; n += kThreads) mine += own_units(a, n);
+        for (int n = kThreads + threadIdx.x; n < a.N; n += kThreads) mine += own_units<unit_pages(GP)>(a, n);
         total += cta_sum(mine, buf);
     }
     total *= a.Hkv;
@@ -677,21 +882,21 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) own_kernel(const DecodeAr
     if (begin < total) {
         Segment seg;
         seg.n = s_n[warp];
-        seg.u = own_units(a, seg.n);
+        seg.u = own_units<unit_pages(GP)>(a, seg.n);
         seg.L = held(a, seg.n);
         const long in = begin - s_before[warp] * a.Hkv, len = min(share, total - begin);
         seg.h = (int)(in / seg.u);
         seg.j = (int)(in % seg.u);
         seg.j1 = (int)min((long)seg.u, seg.j + len);
         seg.left = len - (seg.j1 - seg.j);
-        run_segments<D, false>(a, seg, range, mem, bar, nullptr, nullptr);
+        run_segments<D, GP, false>(a, seg, range, mem, bar, nullptr, nullptr);
     }
     if (a.n_chunks > 0) grid_wait();                             // the prefix kernel's partials are there too
 }
 
 // Few items without a prefix.  An item is a cluster's: its units are cut over the cluster's warps, whose
 // partials are merged on the chip, so that the call is one launch.
-template <int D>
+template <int D, int GP>
 __global__ void __launch_bounds__(kThreads, per_sm(D)) few_kernel(const DecodeArgs a) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kWarps * kStages];
@@ -699,21 +904,21 @@ __global__ void __launch_bounds__(kThreads, per_sm(D)) few_kernel(const DecodeAr
     grid_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* smem = align128(smem_raw);
-    float* part_o = reinterpret_cast<float*>(smem + OwnSmem<D>::kPart);
-    float2* part_ml = reinterpret_cast<float2*>(smem + OwnSmem<D>::kPartMl);
+    float* part_o = reinterpret_cast<float*>(smem + OwnSmem<D, GP>::kPart);
+    float2* part_ml = reinterpret_cast<float2*>(smem + OwnSmem<D, GP>::kPartMl);
     if (lane < 8) part_ml[warp * 8 + lane] = make_float2(-INFINITY, 0.f);
     const uint32_t bar = init_ring(bars + warp * kStages, lane);
     const int item = blockIdx.x / a.parts, w = blockIdx.x % a.parts * kWarps + warp;
     Segment seg;
     seg.n = item / a.Hkv;
     seg.h = item % a.Hkv;
-    seg.u = own_units(a, seg.n);
+    seg.u = own_units<unit_pages(GP)>(a, seg.n);
     seg.L = held(a, seg.n);
     const int share = (seg.u + a.parts * kWarps - 1) / (a.parts * kWarps);
     seg.j = w * share;
     seg.j1 = min(seg.u, seg.j + share);
     seg.left = 0;
-    if (seg.j < seg.j1) run_segments<D, true>(a, seg, 0, smem + warp * OwnSmem<D>::kWarp, bar, part_o, part_ml);
+    if (seg.j < seg.j1) run_segments<D, GP, true>(a, seg, 0, smem + warp * OwnSmem<D, GP>::kWarp, bar, part_o, part_ml);
     merge_few<D>(a, part_o, part_ml);
 }
 
@@ -801,7 +1006,7 @@ __global__ void __launch_bounds__(kThreads, 4) prefix_kernel(const DecodeArgs a)
         }
         issue_half(k0 + kRing);
     }
-    st.finish();
+    st.finish(a.qscale);
     // rows of columns 2c and 2c + 1 go straight to their slots
 #pragma unroll
     for (int col = 0; col < 2; ++col) {
@@ -941,7 +1146,7 @@ inline int prefix_chunk(int N, int G, int Hkv, int D, int n_prefix, int sms) {
 }
 
 // CTAs of an item when there are few items without a prefix (0: not few): 8, 4 or 2 that are all resident
-// at once.  A cluster is alone with its item's length, so the table may allow 8 units a warp at most.
+// at once.  A cluster is alone with its item's length, so the table may allow 16 pages a warp at most.
 // Of equal lengths, 8 heads of 128: 1 session of 777 tokens 6.5 against 10.2 us (two launches, partials
 // through memory), 8000: 13.0 : 14.3, 16000: 20.1 : 17.1; 12 sessions of 777: 9.9 : 13.0, 4000: 19.8 :
 // 24.6; 24 of 777: 13.3 : 16.4.
@@ -949,7 +1154,7 @@ inline int few_parts(int N, int Hkv, int D, int n_prefix, int max_pages, int sms
     if (n_prefix > 0) return 0;
     int parts = kMaxParts;
     while (parts > 1 && (long)N * Hkv * parts > (long)per_sm(D) * sms) parts /= 2;
-    return parts > 1 && max_pages <= 8 * kUnit * kWarps * parts ? parts : 0;
+    return parts > 1 && max_pages <= 64 * parts ? parts : 0;
 }
 
 // Sizes of the workspace's parts, in their order.
@@ -977,14 +1182,37 @@ static int sm_count(int* out) {
     return LF_OK;
 }
 
+template <int D, int GP>
+static int launch_own(const DecodeArgs& a, cudaStream_t st) {
+    static PerContextOnce once;
+    const int rc = once.run([] {
+        LF_CHECK_CUDA(cudaFuncSetAttribute((own_kernel<D, GP>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           OwnSmem<D, GP>::kBytes));
+        LF_CHECK_CUDA(cudaFuncSetAttribute((few_kernel<D, GP>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           OwnSmem<D, GP>::kFewBytes));
+        return LF_OK;
+    });
+    if (rc != LF_OK) return rc;
+    return a.parts > 0
+               ? launch_early_clusters("q4 decode", few_kernel<D, GP>, a.parts, dim3((unsigned)(a.N * a.Hkv * a.parts)),
+                                       dim3(kThreads), OwnSmem<D, GP>::kFewBytes, st, a)
+               : launch_early("q4 decode", own_kernel<D, GP>, dim3(a.ranges / kWarps), dim3(kThreads),
+                              OwnSmem<D, GP>::kBytes, st, a);
+}
+template <int D>
+static int launch_own_of(const DecodeArgs& a, cudaStream_t st) {
+    if constexpr (D == 64) {
+        if (a.G == 1) return launch_own<64, 1>(a, st);
+        if (a.G == 2) return launch_own<64, 2>(a, st);
+    }
+    return launch_own<D, 0>(a, st);
+}
+
 template <int D>
 static int launch(const DecodeArgs& a, cudaStream_t st) {
+    if (a.parts > 0) return launch_own_of<D>(a, st);
     static PerContextOnce once;
     int rc = once.run([] {
-        LF_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           OwnSmem<D>::kBytes));
-        LF_CHECK_CUDA(cudaFuncSetAttribute(few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           OwnSmem<D>::kFewBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            PrefixSmem<D>::kBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -992,9 +1220,6 @@ static int launch(const DecodeArgs& a, cudaStream_t st) {
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
-    if (a.parts > 0)
-        return launch_early_clusters("q4 decode", few_kernel<D>, a.parts, dim3((unsigned)(a.N * a.Hkv * a.parts)),
-                                     dim3(kThreads), OwnSmem<D>::kFewBytes, st, a);
     const long shared = (long)a.n_chunks * a.Hkv * a.groups, rows = (long)a.N * a.Hq;
     LF_CHECK_ARG(shared <= 2147483647L, "q4 decode: grid limits exceeded");
     if (shared > 0) {
@@ -1006,11 +1231,11 @@ static int launch(const DecodeArgs& a, cudaStream_t st) {
         if (rc != LF_OK) return rc;
     }
     if (a.ranges > 0) {
-        rc = launch_early("q4 decode", own_kernel<D>, dim3(a.ranges / kWarps), dim3(kThreads), OwnSmem<D>::kBytes, st, a);
+        rc = launch_own_of<D>(a, st);
         if (rc != LF_OK) return rc;
     }
     // A row's partials, at most: the prefix chunks and an equal share of the ranges.
-    const long most = a.n_chunks + std::min((long)a.ranges / (a.N * a.Hkv), (long)a.max_pages / (kUnit * kMinUnits)) + 1;
+    const long most = a.n_chunks + std::min((long)a.ranges / (a.N * a.Hkv), (long)a.max_pages / (2 * kMinUnits)) + 1;
     return most > kManyPartials
                ? launch_early("q4 decode combine", combine_kernel<D, kRowWarps>, dim3((unsigned)rows), dim3(32 * kRowWarps),
                               0, st, a)
