@@ -60,8 +60,8 @@ using decode::kThreads;
 using decode::kWarps;
 
 // own: pages of a unit (a barrier, a softmax step, a buffer).  GP: heads of a group whose units are packed
-// (1 or 2, of 64 dims), or 0.
-constexpr int unit_pages(int GP) { return GP > 0 ? 4 : 2; }
+// (4, or 1 or 2 of 64 dims), or 0.
+constexpr int unit_pages(int GP) { return GP == 1 || GP == 2 ? 4 : 2; }
 constexpr int kStages = 2;                     // own: units in flight per warp
 constexpr int per_sm(int D) { return D == 64 ? 4 : 3; }   // own: resident CTAs of an SM (registers)
 constexpr int kMinUnits = 2;                   // own: units of a range
@@ -379,98 +379,121 @@ struct State {
     }
 };
 
-// The same for groups of G = 1 or 2 heads of 64 dims, 4 pages at once: column n stands for head n % G over
-// page n / G, so that the softmax's arithmetic, the same for 8 columns as for one, serves 4 pages.  A page's
-// MMAs get the operand with the other pages' columns zero, and all add to the same accumulators.  Columns
-// keep their own maximum and sums; those of a head are joined at the end.
-// 96 sessions x 12 heads of 64 x 4000 tokens: 73 us, 85 with two pages a unit in columns of their own;
-// 1 to 1280 tokens: 21.5 and 23.8; 64 sessions x 8 heads of 2 x 6000: 53 and 61; 300 tokens: 15.4 and 14.7.
-// (A chain of MMAs for each page: 74.4.)
-template <int G>
+// The same for groups of fewer than 8 heads, a unit's pages at once: column n stands for head n % G over
+// page n / G, so that the softmax's arithmetic, the same for 8 columns as for one, serves all of them.  A
+// page's MMAs get the operand with the other pages' columns zero, and all add to the same accumulators.
+// Columns keep their own maximum and sums; those of a head are joined at the end.
+// 4 heads, 2 pages: 480 instructions a unit of 128 dims, 522 with pages in columns of their own; 64 sessions of
+// 4096 .. 16384 tokens 149.5 us, 154.0.  1 or 2 heads of 64 dims, 4 pages: 96 sessions x 12 heads x 4000 tokens
+// 73 us, 85; 1 to 1280 tokens 21.5 and 23.8; 64 sessions x 8 heads of 2 x 6000 53 and 61; 300 tokens 15.4
+// and 14.7.  (One or two heads of 128 dims would need 4 pages of twice the size in flight: State.)
+template <int D, int G>
 struct Packed {
-    static constexpr int U = 4, NG = 1;
-    uint32_t qb[4][2];                         // Q^T operand, column g: q 2^64, q 2^60
-    float qsum[2];
-    float o[1][4][4];
-    float corr[4];
-    float bias[2];
+    static constexpr int U = unit_pages(G), NG = Fmt<D>::NG;
+    // copies of q: one a page with the other pages' columns zero, where they fit (masked at use with 4 heads:
+    // ragged 42.8 us, not 41.6)
+    static constexpr int QM = U == 2 ? U : 1;
+    uint32_t qb[QM][NG][4][2];                 // Q^T operand, column g: q 2^64, q 2^60
+    float qsum[NG][2];
+    float o[NG][4][4];
+    float corr[NG][4];
+    float bias[NG][2];
     float m[2], l[2];
 
     static __device__ __forceinline__ int head_of(int g, int) { return g < U * G ? g % G : -1; }
 
     __device__ __forceinline__ void init(const uint16_t* row, uint32_t flip, int c) {
-        State<64, 1> one;
+        State<D, 1> one;
         one.init(row, flip, c);
+        const int page = (threadIdx.x & 31) / 4 / G;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            qb[k][0] = one.qb[0][k][0];
-            qb[k][1] = one.qb[0][k][1];
-            corr[k] = 0.f;
+        for (int gr = 0; gr < NG; ++gr) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[0][k][j] = 0.f;
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int q = 0; q < QM; ++q)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) qb[q][gr][k][j] = QM == 1 || page == q ? one.qb[gr][k][j] : 0u;
+                corr[gr][k] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[gr][k][j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                qsum[gr][j] = one.qsum[gr][j];
+                bias[gr][j] = 0.f;
+            }
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            qsum[j] = one.qsum[0][j];
-            bias[j] = l[j] = 0.f;
-            m[j] = -INFINITY;
-        }
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
     }
 
     template <bool kMasked>
     __device__ __forceinline__ void unit(uint32_t base, int tok0, const int (&len)[2], float qscale, int lane) {
-        using F = Fmt<64>;
+        using F = Fmt<D>;
         const int g = lane >> 2, c = lane & 3;
-        float acc[2][4];                       // pages 0 and 1, 2 and 3
+        constexpr int kAcc = 2;                // chains of MMAs a group (one: ragged 41.6 us, two 41.2)
+        float acc[kAcc][NG][4];
 #pragma unroll
         for (int p = 0; p < U; ++p) {
             const uint32_t blk = base + (uint32_t)(p * F::kBlockBytes);
-            const uint32_t sel = g / G == p ? 0xFFFFFFFFu : 0u;
-            uint32_t ka[2], kb[2];
-            lds<2>(blk + g * 32 + c * 8, ka);
-            lds<2>(blk + (g + 8) * 32 + c * 8, kb);
-            float(&d)[4] = acc[p / 2];
+            const uint32_t sel = QM > 1 || g / G == p ? 0xFFFFFFFFu : 0u;
+            uint32_t ka[2 * NG], kb[2 * NG];
+            lds<2 * NG>(blk + g * (32 * NG) + c * (8 * NG), ka);
+            lds<2 * NG>(blk + (g + 8) * (32 * NG) + c * (8 * NG), kb);
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+            for (int gr = 0; gr < NG; ++gr) {
+                float(&d)[4] = acc[p * kAcc / U][gr];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t a0 = codes(ka[w], 2 * k), a1 = codes(kb[w], 2 * k);
-                    const uint32_t a2 = codes(ka[w], 2 * k + 1), a3 = codes(kb[w], 2 * k + 1);
-                    const uint32_t b0 = qb[2 * w + k][0] & sel, b1 = qb[2 * w + k][1] & sel;
-                    if (p % 2 == 0 && w == 0 && k == 0) {
-                        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma(d, a0, a1, a2, a3, b0, b1, zero);
-                    } else {
-                        mma(d, a0, a1, a2, a3, b0, b1, d);
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t a0 = codes(ka[2 * gr + w], 2 * k), a1 = codes(kb[2 * gr + w], 2 * k);
+                        const uint32_t a2 = codes(ka[2 * gr + w], 2 * k + 1), a3 = codes(kb[2 * gr + w], 2 * k + 1);
+                        const uint32_t(&q)[2] = qb[QM > 1 ? p : 0][gr][2 * w + k];
+                        if (p % (U / kAcc) == 0 && w == 0 && k == 0) {
+                            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma(d, a0, a1, a2, a3, q[0] & sel, q[1] & sel, zero);
+                        } else {
+                            mma(d, a0, a1, a2, a3, q[0] & sel, q[1] & sel, d);
+                        }
                     }
-                }
+            }
         }
         // This lane's columns 2c, 2c + 1 and the pages they stand for (past the last one: any page, masked).
-        const int p0 = (2 * c / G) % U, p1 = ((2 * c + 1) / G) % U;
+        const int page[2] = {(2 * c / G) % U, ((2 * c + 1) / G) % U};
         const bool live = 2 * c < U * G;
-        float s[4], vs[4], vb[4];              // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
+        float s[4];                            // (token g, col 2c), (g, 2c+1), (g+8, 2c), (g+8, 2c+1)
+        float vs[4][NG], vb[4][NG];
         bool keep[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (G == 2 && j % 2 == 1) continue;          // the same page: below
-            const int page = j % 2 == 0 ? p0 : p1, tok = g + 8 * (j / 2);
-            uint32_t par[2];
-            lds<2>(base + (uint32_t)(page * F::kBlockBytes + F::kParOff + tok * 8), par);
-            const float ks = bf16lo_to_f32(par[0]), kl = bf16hi_to_f32(par[0]);
-            vs[j] = bf16lo_to_f32(par[1]);
-            vb[j] = fmaf(8.f, vs[j], bf16hi_to_f32(par[1]));
-            s[j] = fmaf(ks, acc[0][j] + acc[1][j], kl * qsum[j % 2]);
-            if (G == 2) {
-                vs[j + 1] = vs[j];
-                vb[j + 1] = vb[j];
-                s[j + 1] = fmaf(ks, acc[0][j + 1] + acc[1][j + 1], kl * qsum[1]);
+            if (G > 1 && j % 2 == 1) continue;           // the same page: below
+            uint32_t par[2 * NG];
+            lds<2 * NG>(base + (uint32_t)(page[j % 2] * F::kBlockBytes + F::kParOff + (g + 8 * (j / 2)) * (8 * NG)), par);
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                const float ks = bf16lo_to_f32(par[gr]), kl = bf16hi_to_f32(par[gr]);
+                vs[j][gr] = bf16lo_to_f32(par[NG + gr]);
+                vb[j][gr] = fmaf(8.f, vs[j][gr], bf16hi_to_f32(par[NG + gr]));
+#pragma unroll
+                for (int i = 0; i < (G > 1 ? 2 : 1); ++i) {
+                    float x = acc[0][gr][j + i];
+                    if (kAcc > 1) x += acc[kAcc - 1][gr][j + i];
+                    const float y = kl * qsum[gr][(j + i) % 2];
+                    s[j + i] = gr == 0 ? fmaf(ks, x, y) : fmaf(ks, x, fmaf(kl, qsum[gr][(j + i) % 2], s[j + i]));
+                }
+                if (G > 1) {
+                    vs[j + 1][gr] = vs[j][gr];
+                    vb[j + 1][gr] = vb[j][gr];
+                }
             }
         }
+        constexpr bool kSome = kMasked || U * G < 8;     // some columns or tokens do not count
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int page = j % 2 == 0 ? p0 : p1;
-            keep[j] = live && (!kMasked || tok0 + kPage * page + g + 8 * (j / 2) < len[0]);
-            if (kMasked || G == 1) s[j] = keep[j] ? s[j] : -INFINITY;
+            keep[j] = live && (!kMasked || tok0 + kPage * page[j % 2] + g + 8 * (j / 2) < len[0]);
+            if (kSome) s[j] = keep[j] ? s[j] : -INFINITY;
         }
         float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
         if (__any_sync(0xffffffffu, x0 > m[0] || x1 > m[1])) {
@@ -486,42 +509,57 @@ struct Packed {
             m[1] = n1;
             l[0] *= f0;
             l[1] *= f1;
-            bias[0] *= f0;
-            bias[1] *= f1;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) corr[j] *= (j & 1) ? f1 : f0;
+            for (int gr = 0; gr < NG; ++gr) {
+                bias[gr][0] *= f0;
+                bias[gr][1] *= f1;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+                for (int j = 0; j < 4; ++j) corr[gr][j] *= (j & 1) ? f1 : f0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[0][k][j] *= (j & 1) ? f1 : f0;
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[gr][k][j] *= (j & 1) ? f1 : f0;
+            }
         }
         const float r0 = m[0] == -INFINITY ? 0.f : m[0] * -qscale, r1 = m[1] == -INFINITY ? 0.f : m[1] * -qscale;
-        float p[4];
+        float e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float e = fast_exp2(fmaf(s[j], qscale, (j & 1) ? r1 : r0));
-            if (kMasked || G == 1) e = keep[j] ? e : 0.f;
-            l[j & 1] += e;
-            // what a masked token's scales hold does not count
-            bias[j & 1] = kMasked || G == 1 ? bias[j & 1] + (keep[j] ? e * vb[j] : 0.f) : fmaf(e, vb[j], bias[j & 1]);
-            p[j] = e * (vs[j] * kUp);
-            if (kMasked || G == 1) p[j] = keep[j] ? p[j] : 0.f;
+            e[j] = fast_exp2(fmaf(s[j], qscale, (j & 1) ? r1 : r0));
+            if (kSome) e[j] = keep[j] ? e[j] : 0.f;
+            l[j & 1] += e[j];
         }
-        const uint32_t b0 = movm_t(pack_bf16x2(p[0], p[1])), b1 = movm_t(pack_bf16x2(p[2], p[3]));
-        mma(corr, 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1, corr);
+        uint32_t b0[NG], b1[NG];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {      // what a masked token's scales hold does not count
+                float& bs = bias[gr][j & 1];
+                bs = kSome ? bs + (keep[j] ? e[j] * vb[j][gr] : 0.f) : fmaf(e[j], vb[j][gr], bs);
+                p[j] = e[j] * (vs[j][gr] * kUp);
+                if (kSome) p[j] = keep[j] ? p[j] : 0.f;
+            }
+            b0[gr] = movm_t(pack_bf16x2(p[0], p[1]));
+            b1[gr] = movm_t(pack_bf16x2(p[2], p[3]));
+            mma(corr[gr], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0[gr], b1[gr], corr[gr]);
+        }
 #pragma unroll
         for (int q = 0; q < U; ++q) {
-            const uint32_t blk = base + (uint32_t)(q * F::kBlockBytes) + F::kVOff;
+            const uint32_t blk = base + (uint32_t)(q * F::kBlockBytes) + F::kVOff + lane * (8 * NG);
             const uint32_t sel = g / G == q ? 0xFFFFFFFFu : 0u;
-            uint32_t va[2], vb2[2];            // tokens 2c, 2c + 1 and 2c + 8, 2c + 9
-            lds<2>(blk + lane * 8, va);
-            lds<2>(blk + 256 + lane * 8, vb2);
+            uint32_t va[2 * NG], vc[2 * NG];   // tokens 2c, 2c + 1 and 2c + 8, 2c + 9
+            lds<2 * NG>(blk, va);
+            lds<2 * NG>(blk + 256 * NG, vc);
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+            for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    mma(o[0][2 * w + k], codes(va[w], 2 * k), codes(va[w], 2 * k + 1), codes(vb2[w], 2 * k),
-                        codes(vb2[w], 2 * k + 1), b0 & sel, b1 & sel, o[0][2 * w + k]);
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        mma(o[gr][2 * w + k], codes(va[2 * gr + w], 2 * k), codes(va[2 * gr + w], 2 * k + 1),
+                            codes(vc[2 * gr + w], 2 * k), codes(vc[2 * gr + w], 2 * k + 1), b0[gr] & sel, b1[gr] & sel,
+                            o[gr][2 * w + k]);
         }
     }
 
@@ -532,13 +570,15 @@ struct Packed {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
-                bias[j] += __shfl_xor_sync(0xffffffffu, bias[j], off);
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) bias[gr][j] += __shfl_xor_sync(0xffffffffu, bias[gr][j], off);
             }
         }
+        constexpr int kFirst = G == 4 ? 2 : 1; // lanes of a head's columns: c and those kFirst, 2 kFirst, ... away
         float M[2] = {m[0], m[1]};
         if (G == 1) M[0] = M[1] = fmaxf(M[0], M[1]);
 #pragma unroll
-        for (int off = 1; off < 4; off <<= 1)
+        for (int off = kFirst; off < 4; off <<= 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j) M[j] = fmaxf(M[j], __shfl_xor_sync(0xffffffffu, M[j], off));
         float w[2];
@@ -553,27 +593,28 @@ struct Packed {
             x1 *= w[1];
             if (G == 1) x0 += x1;
 #pragma unroll
-            for (int off = 1; off < 4; off <<= 1) {
+            for (int off = kFirst; off < 4; off <<= 1) {
                 x0 += __shfl_xor_sync(0xffffffffu, x0, off);
-                if (G == 2) x1 += __shfl_xor_sync(0xffffffffu, x1, off);
+                if (G > 1) x1 += __shfl_xor_sync(0xffffffffu, x1, off);
             }
             y0 = x0;
             y1 = x1;
         };
         join(l[0], l[1], l[0], l[1]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                o[0][k][j] = fmaf(o[0][k][j] + corr[j], j < 2 ? kDown : kDown / 16.f, bias[j & 1]);
-            join(o[0][k][0], o[0][k][1], o[0][k][0], o[0][k][1]);
-            join(o[0][k][2], o[0][k][3], o[0][k][2], o[0][k][3]);
-        }
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[gr][k][j] = fmaf(o[gr][k][j] + corr[gr][j], j < 2 ? kDown : kDown / 16.f, bias[gr][j & 1]);
+                join(o[gr][k][0], o[gr][k][1], o[gr][k][0], o[gr][k][1]);
+                join(o[gr][k][2], o[gr][k][3], o[gr][k][2], o[gr][k][3]);
+            }
     }
 };
-template <int D, int GP> struct StateOf { typedef State<D, 2> T; };
-template <> struct StateOf<64, 1> { typedef Packed<1> T; };
-template <> struct StateOf<64, 2> { typedef Packed<2> T; };
+template <int D, int GP> struct StateOf { typedef Packed<D, GP> T; };
+template <int D> struct StateOf<D, 0> { typedef State<D, 2> T; };
 
 // Dim of accumulator row g of m-tile k of group gr (row g + 8 is the next dim).
 __device__ __forceinline__ int out_dim(int gr, int k, int g) { return gr * kGroup + 8 * g + 2 * k; }
@@ -1205,6 +1246,7 @@ static int launch_own_of(const DecodeArgs& a, cudaStream_t st) {
         if (a.G == 1) return launch_own<64, 1>(a, st);
         if (a.G == 2) return launch_own<64, 2>(a, st);
     }
+    if (a.G == 4) return launch_own<D, 4>(a, st);
     return launch_own<D, 0>(a, st);
 }
 
