@@ -472,7 +472,7 @@ int lf_token_logprobs(const void* logits, int dtype, int64_t row_stride, const v
 int lf_lora_plan_size(int n, int total_tokens, int num_adapters, size_t* bytes);
 int lf_lora_plan(const int32_t* adapter_ids, const int32_t* cu_tokens, int n, int total_tokens,
                  int num_adapters, void* plan, size_t plan_bytes, void* stream);
-int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int rank,
+int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int outputs, int rank,
                            int sm_count, size_t* bytes);
 int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x, int64_t x_stride,
                 const lf_bf16* a, const lf_bf16* b, const float* scale, const void* plan, int n,

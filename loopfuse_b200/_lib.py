@@ -98,7 +98,7 @@ _SIGS.update({
     "lf_token_logprobs": [_P, _I, c_int64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "lf_lora_plan_size": [_I, _I, _I, POINTER(c_size_t)],
     "lf_lora_plan": [_P, _P, _I, _I, _I, _P, c_size_t, _P],
-    "lf_lora_workspace_size": [_I, _I, _I, _I, _I, _I, POINTER(c_size_t)],
+    "lf_lora_workspace_size": [_I, _I, _I, _I, _I, _I, _I, POINTER(c_size_t)],
     "lf_lora_add": [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, c_int64, _P,
                     c_size_t, _I, _P],
 })

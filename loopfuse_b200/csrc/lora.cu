@@ -6,8 +6,8 @@
 // share an adapter's weights between its sessions.  `shrink` computes h = x A per (tile, slice of the
 // inputs) into fp32 partials; `expand` sums a tile's partials in slice order, rounds scale * h once to
 // bf16 (the operand type; an error of at most 2^-8 of the adapter's own contribution) and adds h B
-// to y in fp32, rounded once.  No atomics: the same bits in every run.  In a decode batch of adapters
-// enough to fill the chip, `few` does the work of both in one launch.
+// to y in fp32, rounded once.  No atomics: the same bits in every run.  In most decode
+// batches `few` does the work of both in one launch.
 //
 // Both products have a rank of 16 to 128 on one side, so the work is bound by moving x, y, A and B:
 // tiles come in by cp.async several stages ahead (rows of x and y are gathered, 16 bytes a copy),
@@ -497,20 +497,24 @@ expand_kernel(const Args g) {
 }
 
 // A decode batch's tiles (a few rows each): a cluster of kParts CTAs a tile, in one launch and without a
-// workspace (96 rows of 16 adapters, 4096 -> 6144, rank 16: 20.8 us a call, plan included, 24.8 in two).  Each CTA sums a
+// workspace (96 rows of 16 adapters, 4096 -> 6144, rank 16: 19.7 us a call, plan included, 24.1 in two).  Each CTA sums a
 // slice of the inputs; the sums are exchanged through distributed shared memory, added in slice order by
 // every CTA, and the column blocks shared out.
 constexpr int kParts = 8;                              // portable cluster size
-template <int R>
+// kAhead: with an SM to itself a CTA has memory of its own for the column blocks, and the first is on its way
+// during the sums (5 tiles, 4096 -> 6144, rank 16: 12.3 us, 14.3 without).  For up to half of the SMs: clusters
+// of 8 such CTAs do not cover them all (18 tiles, 4096 -> 28672: 36.9 us, 24.6 without).
+template <int R, bool kAhead>
 struct FewSmem {
-    static constexpr int kPart = kTile * R * 4;        // this CTA's sums [row][R]
-    static constexpr int kRest = ShrinkSmem<R>::kBytes > ExpandSmem<R, kShrinkWarps>::kBytes
-                                     ? ShrinkSmem<R>::kBytes : ExpandSmem<R, kShrinkWarps>::kBytes;
-    static constexpr int kBytes = kPart + kRest;
+    static constexpr int kRing = kTile * R * 4;        // before it this CTA's sums [row][R]
+    static constexpr int kShrink = ShrinkSmem<R>::kBytes, kExpand = ExpandSmem<R, kShrinkWarps>::kBytes;
+    static constexpr int kBlocks = kRing + (kAhead ? kShrink : 0);
+    static constexpr int kBytes = kAhead || kExpand > kShrink ? kBlocks + kExpand : kRing + kShrink;
 };
-template <int R>
+template <int R, bool kAhead>
 __global__ void __launch_bounds__(32 * kShrinkWarps)
 few_kernel(const Args g) {
+    using S = FewSmem<R, kAhead>;
     extern __shared__ __align__(128) uint8_t smem[];
     grid_wait();
     grid_release();
@@ -520,10 +524,13 @@ few_kernel(const Args g) {
     if (t.x < 0 && g.y == g.out) return;
     cg::cluster_group cluster = cg::this_cluster();
     float* part = reinterpret_cast<float*>(smem);
-    uint8_t* rest = smem + FewSmem<R>::kPart;
-    if (t.x >= 0) {
+    uint8_t* rest = smem + S::kBlocks;
+    auto sums = [&]() {
         const int k0 = slice * g.k_per, k1 = min(g.K, k0 + g.k_per);
-        shrink_tile<R>(g, t, k0, k1, rest, [&](int i, const float4& v) { *reinterpret_cast<float4*>(part + i) = v; });
+        shrink_tile<R>(g, t, k0, k1, smem + S::kRing, [&](int i, const float4& v) { *reinterpret_cast<float4*>(part + i) = v; });
+    };
+    if (!kAhead && t.x >= 0) {
+        sums();
         __syncthreads();                               // `rest` is free
     }
     constexpr int kCols = ExpandSmem<R, kShrinkWarps>::kCols, HC = R / 8;
@@ -531,6 +538,7 @@ few_kernel(const Args g) {
     expand_tile<R, kShrinkWarps>(g, t, rest, slice, kParts, n_blocks, [&](uint32_t, int blocks) {
         if (t.x < 0) return;
         const float sc = g.scale != nullptr ? g.scale[t.x] : 1.f;
+        if (kAhead) sums();
         cluster.sync();
         for (int i = threadIdx.x; i < 16 * blocks * HC; i += 32 * kShrinkWarps) {
             const int r = i / HC, ch = i % HC;
@@ -555,13 +563,15 @@ few_kernel(const Args g) {
     });
 }
 
-// Whether the tiles' clusters are one launch's work: three quarters of the SMs at least, two CTAs of one
-// at most.  Fewer leave SMs empty (10 tiles, 4096 -> 28672, rank 16: 22.5 us against 20.5 in two launches; 14
-// tiles 22.5 : 26.6), more, and ranks above 32, wait too long for one another in a CTA (19 tiles, 4096 -> 6144:
-// rank 16 14.3 : 16.4, 32 16.4 : 18.4, 64 26.7 : 20.5; 66 tiles of rank 64 125 : 76).
-inline bool is_few(int total, int n, int adapters, int rank, int sms) {
-    const long ctas = max_tiles(total, n, adapters) * kParts;
-    return rank <= 32 && 4 * ctas >= 3L * sms && ctas <= 2L * sms;
+// Whether one launch of clusters does it (few_kernel).  Its CTAs fill three quarters of the SMs at least,
+// and two fit each (14 tiles, 4096 -> 28672, rank 16: 22.5 us against 26.6 in two launches; 10 tiles 22.5 :
+// 20.5; 19 tiles, 4096 -> 6144, rank 16 14.3 : 16.4, 32 16.4 : 18.4, 64 26.7 : 20.5); or the work is
+// small enough for fewer (1 to 10 tiles of rank 16, up to 8192 wide, a few rows each: 10 to 12 us both, and a
+// launch and a workspace less for the host: 4 us).
+inline bool is_few(int total, int n, int adapters, int inputs, int outputs, int rank, int sms) {
+    const long tiles = max_tiles(total, n, adapters), ctas = tiles * kParts;
+    if (rank > 32 || ctas > 2L * sms) return false;
+    return 4 * ctas >= 3L * sms || (rank == 16 && inputs <= 8192 && outputs <= 8192 && total <= 16 * tiles);
 }
 
 inline int slices_for(int total, int n, int adapters, int K, int sms) {
@@ -581,23 +591,28 @@ inline int column_blocks(int blocks, int tiles, int rank, int sms) {
 }
 
 template <int R>
-static int launch(const Args& g, int tiles, cudaStream_t st) {
+static int launch(const Args& g, int tiles, int sms, cudaStream_t st) {
     static PerContextOnce once;
     const int rc = once.run([] {
         LF_CHECK_CUDA(cudaFuncSetAttribute(shrink_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            ShrinkSmem<R>::kBytes));
         LF_CHECK_CUDA(cudaFuncSetAttribute(expand_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            ExpandSmem<R, kExpandWarps>::kBytes));
-        if constexpr (R <= 32)
-            LF_CHECK_CUDA(cudaFuncSetAttribute(few_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               FewSmem<R>::kBytes));
+        if constexpr (R <= 32) {
+            LF_CHECK_CUDA(cudaFuncSetAttribute((few_kernel<R, true>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               FewSmem<R, true>::kBytes));
+            LF_CHECK_CUDA(cudaFuncSetAttribute((few_kernel<R, false>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               FewSmem<R, false>::kBytes));
+        }
         return LF_OK;
     });
     if (rc != LF_OK) return rc;
     if constexpr (R <= 32) {
+        const dim3 grid((unsigned)(tiles * kParts)), block(32 * kShrinkWarps);
         if (g.slices == 0)
-            return launch_early_clusters("lora", few_kernel<R>, kParts, dim3((unsigned)(tiles * kParts)),
-                                         dim3(32 * kShrinkWarps), FewSmem<R>::kBytes, st, g);
+            return 2 * tiles * kParts <= sms
+                       ? launch_early_clusters("lora", few_kernel<R, true>, kParts, grid, block, FewSmem<R, true>::kBytes, st, g)
+                       : launch_early_clusters("lora", few_kernel<R, false>, kParts, grid, block, FewSmem<R, false>::kBytes, st, g);
     }
     const int e = launch_early("lora shrink", shrink_kernel<R>, dim3(g.slices, tiles), dim3(32 * kShrinkWarps),
                                ShrinkSmem<R>::kBytes, st, g);
@@ -654,17 +669,17 @@ extern "C" int lf_lora_plan(const int32_t* adapter_ids, const int32_t* cu_tokens
                         (cudaStream_t)stream, adapter_ids, cu_tokens, n, total_tokens, num_adapters, p);
 }
 
-extern "C" int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int rank,
-                                      int sm_count, size_t* bytes) {
+extern "C" int lf_lora_workspace_size(int n, int total_tokens, int num_adapters, int inputs, int outputs,
+                                      int rank, int sm_count, size_t* bytes) {
     LF_CHECK_ARG(bytes != nullptr, "lora: bytes is null");
     int rc = lora::check_sizes(n, total_tokens, num_adapters);
     if (rc != LF_OK) return rc;
-    LF_CHECK_ARG(inputs > 0 && rank > 0, "lora: bad workspace arguments");
+    LF_CHECK_ARG(inputs > 0 && outputs > 0 && rank > 0, "lora: bad workspace arguments");
     if (sm_count <= 0) {
         rc = lora::sm_count(&sm_count);
         if (rc != LF_OK) return rc;
     }
-    *bytes = lora::is_few(total_tokens, n, num_adapters, rank, sm_count)
+    *bytes = lora::is_few(total_tokens, n, num_adapters, inputs, outputs, rank, sm_count)
                  ? 0 : (size_t)lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count) * total_tokens * rank * 4;
     clear_error();
     return LF_OK;
@@ -695,7 +710,7 @@ extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x,
         if (rc != LF_OK) return rc;
     }
     lora::Args g{};
-    const bool few = lora::is_few(total_tokens, n, num_adapters, rank, sm_count);
+    const bool few = lora::is_few(total_tokens, n, num_adapters, inputs, outputs, rank, sm_count);
     g.slices = few ? 0 : lora::slices_for(total_tokens, n, num_adapters, inputs, sm_count);
     const size_t need = (size_t)g.slices * total_tokens * rank * 4;
     LF_CHECK_ARG(workspace != nullptr || need == 0, "lora: null pointer argument");
@@ -724,9 +739,9 @@ extern "C" int lf_lora_add(const lf_bf16* y, int64_t y_stride, const lf_bf16* x,
     g.cols = lora::column_blocks((outputs + lora::kBlockCols - 1) / lora::kBlockCols, tiles, rank, sm_count);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (rank) {
-        case 16: return lora::launch<16>(g, tiles, st);
-        case 32: return lora::launch<32>(g, tiles, st);
-        case 64: return lora::launch<64>(g, tiles, st);
-        default: return lora::launch<128>(g, tiles, st);
+        case 16: return lora::launch<16>(g, tiles, sm_count, st);
+        case 32: return lora::launch<32>(g, tiles, sm_count, st);
+        case 64: return lora::launch<64>(g, tiles, sm_count, st);
+        default: return lora::launch<128>(g, tiles, sm_count, st);
     }
 }

@@ -197,9 +197,9 @@ def _plan_bytes(n: int, total: int, adapters: int) -> int:
 
 
 @lru_cache(maxsize=4096)
-def _lora_workspace_bytes(n: int, total: int, adapters: int, inputs: int, rank: int, sms: int) -> int:
+def _lora_workspace_bytes(n: int, total: int, adapters: int, inputs: int, outputs: int, rank: int, sms: int) -> int:
     need = _lib.c_size_t(0)
-    _lib.call("lf_lora_workspace_size", n, total, adapters, inputs, rank, sms, _lib.ctypes.byref(need))
+    _lib.call("lf_lora_workspace_size", n, total, adapters, inputs, outputs, rank, sms, _lib.ctypes.byref(need))
     return int(need.value)
 
 
@@ -240,7 +240,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     if T == 0:
         return res
     sms = sm_count(dev.index)
-    need = _lora_workspace_bytes(plan.sessions, T, adapters, K, R, sms)
+    need = _lora_workspace_bytes(plan.sessions, T, adapters, K, N, R, sms)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     launch("lf_lora_add", dev, y.data_ptr(), sy, x.data_ptr(), sx, a.data_ptr(), b.data_ptr(),
            scale.data_ptr() if scale is not None else None, plan.buffer.data_ptr(), plan.sessions, T,

@@ -101,10 +101,11 @@ def test_many_sessions_and_long_ones():
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("K,N", [(8, 8), (72, 264), (136, 2056), (1032, 512), (4096, 6144)])
 def test_decode_batches_of_many_adapters(R, in_place, K, N):
-    """14 to 37 tiles: a cluster a tile."""
+    """14 to 37 tiles, and fewer of a few rows each: a cluster a tile."""
     check([(5 * i) % 17 - 1 for i in range(40)], [(1, 1, 2, 0, 1, 40, 1, 17)[i % 8] for i in range(40)], K, N, R, 16,
           in_place=in_place)
     check([i % 14 for i in range(30)], [1] * 30, K, N, R, 14, scale=False, in_place=in_place)
+    check([2, -1, 0, 2, 1], [1, 3, 1, 0, 20], K, N, R, 3, in_place=in_place)
 
 
 @pytest.mark.parametrize("in_place", [False, True])

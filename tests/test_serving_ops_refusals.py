@@ -28,7 +28,7 @@ def test_logprobs_arguments(change, words):
 @pytest.mark.parametrize("change,words", [
     (dict(rank=8), b"rank"), (dict(rank=48), b"rank"), (dict(inputs=60), b"multiples of 8"), (dict(outputs=0), b"multiples of 8"),
     (dict(y=P + 2), b"aligned"), (dict(x_stride=65), b"aligned"), (dict(y_stride=64), b"overlap"), (dict(plan=None), b"null"),
-    (dict(workspace_bytes=8), b"workspace"), (dict(num_adapters=0), b"adapters"), (dict(num_adapters=4097), b"adapters"),
+    (dict(workspace_bytes=8, rank=64), b"workspace"), (dict(workspace=None, rank=64), b"null"), (dict(num_adapters=0), b"adapters"), (dict(num_adapters=4097), b"adapters"),
     (dict(total_tokens=-1), b"negative"), (dict(out=P, out_stride=136), b"in place"), (dict(total_tokens=1 << 30), b"too many"),
 ])
 def test_lora_arguments(change, words):
@@ -50,7 +50,9 @@ def test_plan_arguments_and_sizes():
     assert lib.lf_lora_plan(P, P, 3, 130, 5, P, 16, None) == _lib.LF_EINVAL
     assert lib.lf_lora_plan(P, P, 3, 130, 5, P + 4, 1 << 20, None) == _lib.LF_EINVAL
     assert lib.lf_lora_plan(None, P, 3, 130, 5, P, 1 << 20, None) == _lib.LF_EINVAL
-    _lib.call("lf_lora_workspace_size", 1, 1, 1, 4096, 16, 148, ctypes.byref(n))
+    _lib.call("lf_lora_workspace_size", 1, 1, 1, 4096, 6144, 16, 148, ctypes.byref(n))
+    assert n.value == 0                                             # one launch of clusters
+    _lib.call("lf_lora_workspace_size", 1, 1, 1, 4096, 28672, 16, 148, ctypes.byref(n))
     assert n.value % (16 * 4) == 0 and n.value >= 16 * 4
 
 
