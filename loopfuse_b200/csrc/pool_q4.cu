@@ -22,6 +22,14 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Both halves of a bf16 pair as fp32.
+__device__ __forceinline__ uint64_t pair_of(uint32_t w) { return sm100::f2_pack(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
+
 struct AppendArgs {
     const uint16_t *q, *k, *v;
     int64_t q_token, kv_layer, kv_token, kv_head;      // strides in elements
@@ -41,29 +49,31 @@ __device__ __forceinline__ void report(const AppendArgs& a) {
 }
 
 // One CTA walks tokens (grid-stride, blockIdx.y the layer); a row of D dims of one head is D / 8
-// lanes of 8 dims, heads ordered q (Hq), k (Hkv), v (Hkv).  Rotation uses the partner lane's 8 dims
-// and rounds every product and sum separately, then to bf16, as an eager fp32 evaluation does; the
-// codes are those of the rounded values.  A row that has no page, or no rotation table row, is not
-// stored and is reported.
+// lanes of 8 dims: the queries' rows, then k's and v's, from the last warp on.  Rotation uses the partner
+// lane's 8 dims and rounds every product and sum separately, then to bf16, as an eager fp32
+// evaluation does; the codes are those of the rounded values.  A row that has no page, or no rotation
+// table row, is not stored and is reported.
 template <int D>
 __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
     using F = Fmt<D>;
     constexpr int LPR = D / 8, RPW = 32 / LPR;          // lanes a row, rows a warp
     grid_wait();
     if (a.status != nullptr && *reinterpret_cast<volatile int32_t*>(a.status) != LF_OK) return;
-    const int H = a.Hq + 2 * a.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const int l = lane % LPR;
+    const int l = lane % LPR, row0 = warp * RPW + lane / LPR;   // this lane's first query row
+    const int kv0 = (warps - 1 - warp) * RPW + lane / LPR;      // and k or v row: the last warps begin
+    const int H2 = 2 * a.Hkv, skip = warps * RPW;
     const long layer = blockIdx.y;
     for (int t = blockIdx.x; t < a.total; t += gridDim.x) {
-        // This warp's first row is on its way while the token is looked up.
-        auto source = [&](int h) -> const uint16_t* {
-            if (h < a.Hq) return a.q + t * a.q_token + (long)h * D + 8 * l;
-            const bool k = h < a.Hq + a.Hkv;
-            return (k ? a.k : a.v) + layer * a.kv_layer + t * a.kv_token + (h - a.Hq - (k ? 0 : a.Hkv)) * a.kv_head + 8 * l;
+        // This lane's first rows are on their way while the token is looked up.
+        const uint16_t* qs = a.q + t * a.q_token + (long)row0 * D + 8 * l;
+        auto source = [&](int h) -> const uint16_t* {           // k rows, then v rows
+            const bool v = h >= a.Hkv;
+            return (v ? a.v : a.k) + layer * a.kv_layer + t * a.kv_token + (h - (v ? a.Hkv : 0)) * a.kv_head + 8 * l;
         };
-        uint4 ahead = make_uint4(0, 0, 0, 0);
-        if (warp * RPW + lane / LPR < H) ahead = *reinterpret_cast<const uint4*>(source(warp * RPW + lane / LPR));
+        uint4 q_next = make_uint4(0, 0, 0, 0), kv_next = q_next;
+        if (row0 < a.Hq) q_next = *reinterpret_cast<const uint4*>(qs);
+        if (kv0 < H2) kv_next = *reinterpret_cast<const uint4*>(source(kv0));
         int lo = 0;                                    // the last session i with cu[i] <= t, 32 probes at a time
         for (int len = a.n; len > 1;) {
             const int step = (len + 31) / 32, i = lo + lane * step;
@@ -80,47 +90,46 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
             page = a.table[(long)row * a.table_stride + pos / kPage];
         const bool page_ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages);
         if (!(page_ok && pos_ok) && threadIdx.x == 0) report(a);
-        float cs[8], sn[8];                            // this lane's dims, the same in every row
+        float cs[8], sn[8];                            // this lane's dims, the same in every row: -s, s by half
         if (a.cos != nullptr) {
             const long off = (long)(pos_ok ? pos : 0) * (D / 2) + (8 * l) % (D / 2);
+            const float sign = l < LPR / 2 ? -1.f : 1.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos + off) + j);
                 const float4 n = __ldg(reinterpret_cast<const float4*>(a.sin + off) + j);
-                const float sign = l < LPR / 2 ? -1.f : 1.f;
                 cs[4 * j] = c.x; cs[4 * j + 1] = c.y; cs[4 * j + 2] = c.z; cs[4 * j + 3] = c.w;
                 sn[4 * j] = sign * n.x; sn[4 * j + 1] = sign * n.y;
                 sn[4 * j + 2] = sign * n.z; sn[4 * j + 3] = sign * n.w;
             }
         }
-        for (int r0 = warp * RPW; r0 < H; r0 += warps * RPW) {
-            const int h = r0 + lane / LPR;
-            const bool live = h < H;
-            const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
-            const int kh = h - a.Hq - (is_k ? 0 : a.Hkv);
-            const uint4 x = ahead;
-            ahead = make_uint4(0, 0, 0, 0);
-            if (h + warps * RPW < H) ahead = *reinterpret_cast<const uint4*>(source(h + warps * RPW));
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            const bool turn = live && (is_q || is_k);
-            if (a.cos != nullptr && __any_sync(0xffffffffu, turn)) {   // every lane takes the shuffles
+        // x1 c - x2 s in the first half of a row, x2 c + x1 s in the second; a warp's lanes together.
+        auto rotate = [&](uint32_t (&w)[4], bool turn) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], LPR / 2);
-                    // x1 c - x2 s in the first half of a row, x2 c + x1 s in the second (sn is -s, s)
-                    const float lo = __fadd_rn(__fmul_rn(bf16lo_to_f32(w[j]), cs[2 * j]),
-                                               __fmul_rn(bf16lo_to_f32(other), sn[2 * j]));
-                    const float hi = __fadd_rn(__fmul_rn(bf16hi_to_f32(w[j]), cs[2 * j + 1]),
-                                               __fmul_rn(bf16hi_to_f32(other), sn[2 * j + 1]));
-                    if (turn) w[j] = pack_bf16x2(lo, hi);
-                }
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t o = __shfl_xor_sync(0xffffffffu, w[j], LPR / 2);
+                // (scalar: a packed multiplication and addition may be fused)
+                const float lo = __fadd_rn(__fmul_rn(bf16lo_to_f32(w[j]), cs[2 * j]), __fmul_rn(bf16lo_to_f32(o), sn[2 * j]));
+                const float hi = __fadd_rn(__fmul_rn(bf16hi_to_f32(w[j]), cs[2 * j + 1]), __fmul_rn(bf16hi_to_f32(o), sn[2 * j + 1]));
+                if (turn) w[j] = pack_bf16x2(lo, hi);
             }
-            if (__all_sync(0xffffffffu, is_q || !live)) {   // query rows: no groups to form
-                if (live && pos_ok)
-                    *reinterpret_cast<uint4*>(a.q_out + ((long)t * a.Hq + h) * D + 8 * l) =
-                        make_uint4(w[0], w[1], w[2], w[3]);
-                continue;
-            }
+        };
+        uint16_t* qd = a.q_out + ((long)t * a.Hq + row0) * D + 8 * l;
+        for (int h = row0, r0 = warp * RPW; r0 < a.Hq; r0 += skip, h += skip) {
+            uint32_t w[4] = {q_next.x, q_next.y, q_next.z, q_next.w};
+            qs += skip * D;
+            if (h + skip < a.Hq) q_next = *reinterpret_cast<const uint4*>(qs);
+            if (a.cos != nullptr) rotate(w, true);
+            if (h < a.Hq && pos_ok) *reinterpret_cast<uint4*>(qd) = make_uint4(w[0], w[1], w[2], w[3]);
+            qd += skip * D;
+        }
+        for (int h = kv0, r0 = (warps - 1 - warp) * RPW; r0 < H2; r0 += skip, h += skip) {
+            const bool live = h < H2, is_k = h < a.Hkv;
+            const int kh = h - (is_k ? 0 : a.Hkv);
+            uint32_t w[4] = {kv_next.x, kv_next.y, kv_next.z, kv_next.w};
+            kv_next = make_uint4(0, 0, 0, 0);
+            if (h + skip < H2) kv_next = *reinterpret_cast<const uint4*>(source(h + skip));
+            if (a.cos != nullptr && __any_sync(0xffffffffu, is_k)) rotate(w, is_k);
             // {-min, max} of the group (8 lanes) as a bf16 pair, NaN if it holds one
             uint32_t ext;
             {
@@ -130,14 +139,7 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
 #pragma unroll
                 for (int off = 1; off < 8; off <<= 1) ext = max2(ext, __shfl_xor_sync(0xffffffffu, ext, off));
             }
-            if (!live) continue;
-            if (is_q) {
-                if (pos_ok)
-                    *reinterpret_cast<uint4*>(a.q_out + ((long)t * a.Hq + h) * D + 8 * l) =
-                        make_uint4(w[0], w[1], w[2], w[3]);
-                continue;
-            }
-            if (!page_ok || !pos_ok) continue;
+            if (!live || !page_ok || !pos_ok) continue;
             const float mn = -bf16lo_to_f32(ext), span = __fsub_rn(bf16hi_to_f32(ext), mn);
             uint32_t par = 0x7FC07FC0u;                // NaN, NaN
             uint32_t n[8];                             // the codes plus kMagicBits
@@ -146,27 +148,29 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
             if (span < kMaxSpan) {                     // (not NaN)
                 par = pack_bf16x2(__fdiv_rn(span, 15.f), mn);
                 const float s = bf16lo_to_f32(par);
-                float d[8];
+                uint64_t d[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    d[2 * j] = __fsub_rn(bf16lo_to_f32(w[j]), mn);
-                    d[2 * j + 1] = __fsub_rn(bf16hi_to_f32(w[j]), mn);
-                }
+                for (int j = 0; j < 4; ++j) d[j] = sm100::fadd2(pair_of(w[j]), sm100::f2_pack(-mn, -mn));
                 if (s >= kSmallest) {
                     // d / s rounded to nearest from the rounded reciprocal and the exact remainder of the
                     // first quotient (Markstein's theorem); at most 15.03, so that adding 1.5 * 2^23
                     // leaves rint(d / s), ties to even, in the low bits.
                     const float r = __frcp_rn(s);
+                    const uint64_t r2 = sm100::f2_pack(r, r), s2 = sm100::f2_pack(-s, -s), m2 = sm100::f2_pack(kMagic, kMagic);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float q0 = __fmul_rn(d[j], r);
-                        const float q1 = fmaf(fmaf(-q0, s, d[j]), r, q0);
-                        n[j] = __float_as_uint(__fadd_rn(q1, kMagic));
+                    for (int j = 0; j < 4; ++j) {
+                        const uint64_t q0 = fmul2(d[j], r2);
+                        const float2 q1 = sm100::f2_unpack(sm100::fadd2(sm100::ffma2(sm100::ffma2(q0, s2, d[j]), r2, q0), m2));
+                        n[2 * j] = __float_as_uint(q1.x);
+                        n[2 * j + 1] = __float_as_uint(q1.y);
                     }
                 } else if (s > 0.f) {                  // remainders would underflow
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        n[j] = __float_as_uint(__fadd_rn(fminf(rintf(__fdiv_rn(d[j], s)), 15.f), kMagic));
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 x = sm100::f2_unpack(d[j]);
+                        n[2 * j] = __float_as_uint(__fadd_rn(fminf(rintf(__fdiv_rn(x.x, s)), 15.f), kMagic));
+                        n[2 * j + 1] = __float_as_uint(__fadd_rn(fminf(rintf(__fdiv_rn(x.y, s)), 15.f), kMagic));
+                    }
                 }
             }
             const int tok = pos % kPage, grp = l / 8, in = l % 8;   // group, 8-dim piece of it
