@@ -140,6 +140,41 @@ def test_decode_long_shared_prefix_of_many_rows(N, Hq, Hkv, D, npre):
     check_decode([min(x, npre * 16) for x in lens], Hq, Hkv, D, npre=npre, scale=-0.4)   # peaked, negative
 
 
+def test_long_shared_prefix_beside_other_work_and_captured():
+    """Two decodes and a prefill attention, all with tensor memory, on three streams; then from a graph."""
+    N, Hq, Hkv, D, npre = 80, 32, 8, 128, 160
+    gen = torch.Generator().manual_seed(9)
+    lens = [npre * 16 + 5 + 3 * i for i in range(N)]
+    table, P = table_for(lens, npre, gen)
+    pages = [random_pages(gen, P, Hkv, D).cuda() for _ in range(2)]
+    q = torch.randn(N, Hq, D, generator=gen).bfloat16().cuda()
+    table, lens = table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    x = torch.randn(2, 8, 1500, 128, generator=gen).bfloat16().cuda()
+    k, v = x[:, :4].contiguous(), x[:, 4:].contiguous()
+
+    def decode(i):
+        return att.paged_decode_q4(q, pages[i], table, lens, num_prefix_pages=npre)
+    alone = [decode(0), decode(1), att.prefill_attention_fwd(x, k, v)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(15):
+        got = []
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(decode(i) if i < 2 else att.prefill_attention_fwd(x, k, v))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a, b = decode(0), decode(1)
+    for _ in range(3):
+        a.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, alone[0]) and torch.equal(b, alone[1])
+    assert drain_status() == []
+
+
 @pytest.mark.parametrize("N,Hq,Hkv,D,npre", [(6, 8, 2, 128, 5), (5, 2, 2, 64, 40), TILED[0], TILED[3]])
 def test_nan_in_a_shared_prefix_reaches_the_rows_that_hold_it(N, Hq, Hkv, D, npre):
     gen = torch.Generator().manual_seed(3)
