@@ -21,7 +21,7 @@ def sm_count(index: int) -> int:
 
 def launch(name: str, device: torch.device, *args) -> None:
     index = device.index
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:         # (a tensor is there: CUDA has been set up)
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
         return
     with torch.cuda.device(device):

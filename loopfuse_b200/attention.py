@@ -308,6 +308,22 @@ def decode_q4_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int
     return int(n.value)
 
 
+def _check_decode_q4(q, pages, block_table, seq_lens, out, workspace) -> None:
+    _require(q, "q")
+    D = q4_head_dim(pages)
+    _require(block_table, "block_table", torch.int32)
+    _require(seq_lens, "seq_lens", torch.int32)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise LoopfuseError(_lib.LF_EINVAL, f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
+    if block_table.dim() != 2 or block_table.shape[0] != q.shape[0] or seq_lens.shape != q.shape[:1]:
+        raise LoopfuseError(_lib.LF_EINVAL, "block_table must be [N,max_pages], seq_lens [N]")
+    _one_device("paged_decode_q4", q, pages, block_table, seq_lens, out, workspace)
+    if out is not None:
+        _require(out, "out")
+        if out.shape != q.shape:
+            raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: out must have q's shape")
+
+
 def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor,
                     seq_lens: torch.Tensor, num_prefix_pages: int = 0,
                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
@@ -316,24 +332,18 @@ def paged_decode_q4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
     (one layer), ``block_table [N, max_pages]`` and ``seq_lens [N]`` int32, Hq / Hkv 1, 2, 4 or 8.
     With ``num_prefix_pages > 0`` the first that many block-table entries must be the same pages
     for all sessions.  A session of length 0 gives zeros and an LSE of -inf."""
-    _require(q, "q")
-    D = q4_head_dim(pages)
-    _require(block_table, "block_table", torch.int32)
-    _require(seq_lens, "seq_lens", torch.int32)
-    if q.dim() != 3 or q.shape[2] != D:
-        raise LoopfuseError(_lib.LF_EINVAL, f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
-    N, Hq, _ = q.shape
-    P, Hkv, _ = pages.shape
-    if block_table.dim() != 2 or block_table.shape[0] != N or seq_lens.shape != (N,):
-        raise LoopfuseError(_lib.LF_EINVAL, "block_table must be [N,max_pages], seq_lens [N]")
-    dev = _one_device("paged_decode_q4", q, pages, block_table, seq_lens, out, workspace)
-    if out is None:
-        o = torch.empty_like(q)
-    else:
-        o = out
-        _require(o, "out")
-        if o.shape != q.shape:
-            raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: out must have q's shape")
+    dev, i32, ps, qs = q.device, torch.int32, pages.shape, q.shape
+    # In one go; what is wrong, if anything is, is named by the checks one by one.
+    if not (q.is_cuda and pages.device == dev and block_table.device == dev and seq_lens.device == dev and
+            q.dtype is torch.bfloat16 and pages.dtype is torch.uint8 and block_table.dtype is i32 and
+            seq_lens.dtype is i32 and q.is_contiguous() and pages.is_contiguous() and
+            block_table.is_contiguous() and seq_lens.is_contiguous() and len(qs) == 3 and len(ps) == 3 and
+            ps[2] == 18 * qs[2] and (qs[2] == 128 or qs[2] == 64) and block_table.dim() == 2 and
+            block_table.shape[0] == qs[0] and seq_lens.shape == qs[:1] and out is None and workspace is None):
+        _check_decode_q4(q, pages, block_table, seq_lens, out, workspace)
+    N, Hq, D = qs
+    P, Hkv, _ = ps
+    o = torch.empty_like(q) if out is None else out
     lse = torch.empty(N, Hq, dtype=torch.float32, device=dev) if return_lse else None
     if N == 0:
         return (o, lse) if return_lse else o

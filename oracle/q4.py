@@ -81,7 +81,8 @@ def decode(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: List
     The bound counts: o's rounding to bf16 (half a step, 2^-8); the rounding of ``p s`` to bf16,
     which multiplies ``n - 8`` (2^-8 of ``sum p s |n - 8|``); the scores' fp32 sums of products
     ``q n s`` and of ``b sum(q)``, seven additions of magnitude at most ``(15 s + |b|) sum |q|`` with
-    2^-22 each (truncating accumulators); fp32 exponentials and sums (2^-20 of ``sum p |v|``)."""
+    2^-22 each (truncating accumulators; where a long prefix is taken in tiles, 17 additions of 2^-23, half
+    of them while the sum is still growing: 13.5 of 2^-23); fp32 exponentials and sums (2^-20 of ``sum p |v|``)."""
     N, Hq, D = q.shape
     Hkv = pages.shape[1]
     G, ng = Hq // Hkv, D // GROUP
