@@ -18,11 +18,11 @@
 // CTAs fit an SM.  A NaN among a token's scales must not reach rows that do not hold the token: its tile
 // of V is then zero and B brings the NaN, behind the row's mask.
 //
-// 64 sessions x 4 heads a KV head on 4096 tokens: the whole decode takes 43.4 us, 51.6 with the warp-MMA
-// form; 256 sessions: 80 and 145.  What bounds it: a step's chain unpack - S - softmax - P . V, 2400
+// 64 sessions x 4 heads a KV head on 4096 tokens: the whole decode takes 45.3 us, 52.7 with the warp-MMA
+// form; 256 sessions: 81 and 146.  What bounds it: a step's chain unpack - S - softmax - P . V, 2400
 // cycles for the two CTAs of an SM together, half of that the softmax's and unpacking's instructions, and
 // about 10 us around the 8 steps of a CTA (first pages and code from HBM, partials written).  Measured
-// and not kept, same case: scales applied by the softmax threads (S of each group apart: two 16-byte
+// and not kept, same case when it took 43.4: scales applied by the softmax threads (S of each group apart: two 16-byte
 // shared loads a token and row) 51.1; pages through a ring of bulk copies 45.8; one CTA an SM with twice
 // the steps 47.3; chunks merged over clusters of 8 CTAs 46.0; one softmax body, masked always, 46.2.
 // Waits are bounded (sites 255..259 in the device error word); after one gives up every role leaves.
