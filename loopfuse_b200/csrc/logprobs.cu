@@ -24,8 +24,9 @@
 // (maximum, then lowest index); it starts from the lanes' best vectors of the first slice, and a
 // later slice is searched only when some lane's maximum reaches the list's k-th.  Lists are merged by
 // bitonic exchanges, in the CTA through shared memory and in the cluster through distributed shared
-// memory, and the values of the last k vectors are read again and sorted: one launch, no workspace,
-// no atomics, the same result in every run.
+// memory, and the values of the last k vectors are read again, each counting those above it: one launch,
+// no workspace, no atomics, the same result in every run.  64 rows of 128256 bf16 (16 MB, in L2): 12.6 us
+// with 20 alternatives, 6.5 without any; one row 7.9 and 3.5.
 #include "lf_common.cuh"
 
 #include <cooperative_groups.h>
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     typedef typename E::T T;
     constexpr int N = E::N;
     constexpr uint32_t kSlice = 32u * N * kVecs;       // values of a warp's slice
-    __shared__ u64 s_list[kWarps][32];
+    __shared__ __align__(16) u64 s_list[kWarps][32];
     __shared__ Stat s_stat[kWarps];
     __shared__ u64 c_list[kMaxParts][32];              // the cluster's, in its first CTA
     __shared__ Stat c_stat[kMaxParts];
@@ -421,46 +422,51 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     auto logp = [&](float v) { return bad ? NAN : (none ? -INFINITY : (v - st.m) - ln_s); };
     if (kTop) {
         // The values of the k best vectors that reach the k-th vector's maximum hold the k best values
-        // (at least k do); they are gathered, sorted 32 at a time and merged.
+        // (at least k do); they are packed, and each counts those above it.
         const u64 mine = lists[0][lane];
         const bool have = mine != 0 && lane < a.k;
         const uint32_t u = key_index(mine) * N;
         const u64 last = __shfl_sync(kAll, mine, a.k - 1);   // 0: fewer than k vectors
         const float bar = last == 0 ? -INFINITY : key_value(last);
-        u64 best = 0, key = 0;
-        int count = 0;                                 // candidates waiting in `key`, one a lane
         float val[N];
+        unsigned in = 0;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const uint32_t p = u + e;
             float f[2] = {-INFINITY, 0.f};
-            if (have && p >= lead && p < end) E::unpack((uint32_t)base[p], f);
+            const bool inside = have && p >= lead && p < end;
+            if (inside) E::unpack((uint32_t)base[p], f);
             val[e] = f[0];
+            in |= (inside && !(f[0] < bar) ? 1u : 0u) << e;
         }
+        int at = __popc(in);                           // where this lane's begin
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint32_t p = u + e;
-            const bool in = have && p >= lead && p < end && !(val[e] < bar);
-            const unsigned mask = __ballot_sync(kAll, in);
-            if (mask == 0) continue;
-            const u64 cand = in ? make_key(val[e], p - lead) : 0;
-            const int n = __popc(mask);
-            if (count + n > 32) {
-                best = merge_lists(best, sort_desc(key, lane), lane);
-                key = 0;
-                count = 0;
-            }
-            // the j-th candidate goes to lane count + j
-            const int j = lane - count;
-            const int src = j >= 0 && j < n ? (int)__fns(mask, 0, j + 1) : 0;
-            const u64 got = __shfl_sync(kAll, cand, src);
-            if (j >= 0 && j < n) key = got;
-            count += n;
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(kAll, at, off);
+            if (lane >= off) at += o;
         }
-        best = merge_lists(best, sort_desc(key, lane), lane);
-        if (lane < a.k) {
-            a.ids[row * a.k + lane] = (int64_t)key_index(best);
-            a.top[row * a.k + lane] = logp(key_value(best));
+        const int n = __shfl_sync(kAll, at, 31);       // at most 32 N
+        at -= __popc(in);
+        static_assert(kWarps * 32 >= 32 * N, "room for the candidates");
+        u64* cand = &s_list[0][0];                     // (the lists have been read)
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if ((in >> e) & 1u) cand[at++] = make_key(val[e], u + e - lead);
+        if (lane == 0 && (n & 1)) cand[n] = 0;
+        __syncwarp();
+        for (int c = lane; c < n; c += 32) {
+            const u64 key = cand[c];
+            int pos = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; j += 2) {
+                const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(cand + j);
+                pos += (o.x > key) + (o.y > key);
+            }
+            if (pos < a.k) {
+                a.ids[row * a.k + pos] = (int64_t)key_index(key);
+                a.top[row * a.k + pos] = logp(key_value(key));
+            }
         }
     }
     if (lane == 0) {
