@@ -102,6 +102,12 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 // From when every CTA has called this (or ended), the stream's next kernel may begin if launched early.
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// The two halves of a barrier of the cluster's threads.  A CTA may touch another one's shared memory only
+// once that one is known to run: every thread arrives at the start of the kernel and waits before the
+// first such access, with its work in between.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // bf16 bit patterns -> fp32: a bf16 is the high half of the fp32 with the same value.

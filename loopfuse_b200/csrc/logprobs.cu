@@ -25,8 +25,8 @@
 // later slice is searched only when some lane's maximum reaches the list's k-th.  Lists are merged by
 // bitonic exchanges, in the CTA through shared memory and in the cluster through distributed shared
 // memory, and the values of the last k vectors are read again, each counting those above it: one launch,
-// no workspace, no atomics, the same result in every run.  64 rows of 128256 bf16 (16 MB, in L2): 12.6 us
-// with 20 alternatives, 6.5 without any; one row 7.9 and 3.5.
+// no workspace, no atomics, the same result in every run.  64 rows of 128256 bf16 (16 MB, in L2): 12.9 us
+// with 20 alternatives, 6.5 without any; one row 7.9 and 3.6.
 #include "lf_common.cuh"
 
 #include <cooperative_groups.h>
@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     };
 
     __shared__ float s_tok;
+    if (a.parts > 1) cluster_arrive();                 // waited for before the first remote store
     grid_wait();
     if (part == 0 && threadIdx.x == kThreads - 1) {    // the token's own logit, on its way meanwhile
         const int64_t tok = token(a, row);
@@ -405,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     Stat* stats = s_stat;
     if (a.parts > 1) {
         cg::cluster_group cluster = cg::this_cluster();
+        cluster_wait();                                // the first CTA runs
         if (warp == 0) {
             if (kTop) *cluster.map_shared_rank(&c_list[part][lane], 0) = s_list[0][lane];
             if (lane == 0) *cluster.map_shared_rank(&c_stat[part], 0) = s_stat[0];

@@ -196,3 +196,20 @@ def test_captured_repeated_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     empty = mo.token_logprobs(x[:0], tok[:0], top_k=2)
     assert empty.logprob.shape == (0,) and empty.top_ids.shape == (0, 2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [16385, 32800, 65537, 70001])
+def test_parts_of_a_row_that_end_early(V, dtype):
+    """A row cut over 2, 4 or 8 CTAs whose last ones have little or nothing to read: they hand over their
+    lists while the first is still at work."""
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    for T in (1, 3, 70):
+        x = (3 * torch.randn(T, V, generator=gen, device="cuda")).to(dtype)
+        tok = torch.randint(0, V, (T,), generator=gen, device="cuda")
+        x[0, V - 1] = 30.0                                 # the best of a row in its last, short part
+        for k in (0, 1, 32):
+            first = check(x, tok, k)
+            for _ in range(5):
+                assert all(torch.equal(a, b) for a, b in zip(first, mo.token_logprobs(x, tok, top_k=k)))
+    assert drain_status() == []
