@@ -309,11 +309,11 @@ __global__ void __launch_bounds__(kTcThreads, kTcPerSm) prefix_tc_kernel(const D
             return k < pages ? checked_page(row[k], a.num_pages) : -1;
         };
         auto get4 = [](const uint8_t* p, uint32_t* d) {
-            const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+            const uint4 t = *reinterpret_cast<const uint4*>(p);
             d[0] = t.x; d[1] = t.y; d[2] = t.z; d[3] = t.w;
         };
         auto get2 = [](const uint8_t* p, uint32_t* d) {
-            const uint2 t = __ldg(reinterpret_cast<const uint2*>(p));
+            const uint2 t = *reinterpret_cast<const uint2*>(p);
             d[0] = t.x; d[1] = t.y;
         };
         auto load = [&](int page, Raw& x) {            // zeros for a page past the chunk
@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(kTcThreads, kTcPerSm) prefix_tc_kernel(const D
                 get2(blk + (half * 8 + g) * 32 + c * 8, x.k);
                 get2(blk + F::kVOff + half * 256 + lane * 8, x.v);
                 get2(par + g * 8, x.pk);
-                x.pv[0][0] = __ldg(reinterpret_cast<const uint32_t*>(par + 2 * c * 8 + 4));
-                x.pv[1][0] = __ldg(reinterpret_cast<const uint32_t*>(par + (2 * c + 1) * 8 + 4));
+                x.pv[0][0] = *reinterpret_cast<const uint32_t*>(par + 2 * c * 8 + 4);
+                x.pv[1][0] = *reinterpret_cast<const uint32_t*>(par + (2 * c + 1) * 8 + 4);
             }
         };
         const int tk = w * 8 + g, tv = w * 8 + 2 * c;

@@ -72,7 +72,8 @@ inline int launch_status(const char* what) {
 
 // A launch that may begin while the stream's last kernel still runs (programmatic dependent launch).
 // The kernel calls grid_wait() before it touches anything that kernel reads or writes, in every CTA
-// and on every path: a grid that ended without waiting would let its successor start too soon.
+// and on every path: a grid that ended without waiting would let its successor start too soon.  It reads
+// through coherent loads (ld_stream, no __ldg, no __restrict__).
 template <class... P, class... A>
 int launch_early_clusters(const char* what, void (*kernel)(P...), int cluster, dim3 grid, dim3 block, size_t smem,
                           cudaStream_t st, A&&... args) {
@@ -130,6 +131,16 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 __device__ __forceinline__ uint4 ldg_stream(const void* p) {
     uint4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+
+// The same through coherent loads, for kernels that begin early: what the stream's last kernel writes is
+// not read-only for as long as they run, which the read-only path and __restrict__ would promise.
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                  : "l"(p));
     return r;

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
         const uint32_t u0 = slice * kSlice + lane * N;
         if (slice * kSlice >= lead && (slice + 1) * kSlice <= end) {   // warp-uniform: whole slice
 #pragma unroll
-            for (int i = 0; i < kVecs; ++i) v[i] = ldg_stream(base + u0 + i * 32 * N);
+            for (int i = 0; i < kVecs; ++i) v[i] = ld_stream(base + u0 + i * 32 * N);
             return;
         }
 #pragma unroll
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
             const uint32_t u = u0 + i * 32 * N;
             uint32_t w[4] = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
             if (u >= lead && u + N <= end) {
-                v[i] = ldg_stream(base + u);
+                v[i] = ld_stream(base + u);
                 continue;
             }
 #pragma unroll

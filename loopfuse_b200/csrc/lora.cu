@@ -49,7 +49,7 @@ inline Plan views(int32_t* p, int total, int n, int adapters) {
 
 // One CTA.  Bucket b < adapters holds adapter b's sessions, bucket `adapters` those without one.
 __global__ void __launch_bounds__(pool::kMetaThreads)
-plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ cu, int n, int total, int adapters,
+plan_kernel(const int32_t* ids, const int32_t* cu, int n, int total, int adapters,
             Plan p) {
     extern __shared__ int sm[];
     __shared__ int2 buf[32];

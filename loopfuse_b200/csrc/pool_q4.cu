@@ -98,8 +98,8 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
             const float sign = l < LPR / 2 ? -1.f : 1.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos + off) + j);
-                const float4 n = __ldg(reinterpret_cast<const float4*>(a.sin + off) + j);
+                const float4 c = reinterpret_cast<const float4*>(a.cos + off)[j];
+                const float4 n = reinterpret_cast<const float4*>(a.sin + off)[j];
                 cs[4 * j] = c.x; cs[4 * j + 1] = c.y; cs[4 * j + 2] = c.z; cs[4 * j + 3] = c.w;
                 sn[4 * j] = sign * n.x; sn[4 * j + 1] = sign * n.y;
                 sn[4 * j + 2] = sign * n.z; sn[4 * j + 3] = sign * n.w;
@@ -222,9 +222,8 @@ __device__ __forceinline__ uint32_t values(uint32_t w, uint32_t s2, uint32_t b2)
 // become zeros, so that the prefill kernel's masked products see no stale bits.
 template <int D>
 __global__ void __launch_bounds__(32 * kExpWarps)
-expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
-              const int32_t* __restrict__ lens, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo,
-              int32_t* __restrict__ out_table, int N, int Hkv, int num_pages, int max_pages,
+expand_kernel(const uint8_t* pages, const int32_t* bt, const int32_t* lens, uint16_t* ko, uint16_t* vo,
+              int32_t* out_table, int N, int Hkv, int num_pages, int max_pages,
               int n_prefix, int out_pages) {
     using F = Fmt<D>;
     grid_wait();
@@ -292,20 +291,20 @@ expand_kernel(const uint8_t* __restrict__ pages, const int32_t* __restrict__ bt,
             const uint8_t* kp = blk + (half * 8 + g) * (32 * F::NG) + c * (8 * F::NG);
             const uint8_t* vp = blk + F::kVOff + half * (256 * F::NG) + lane * (8 * F::NG);
             if constexpr (F::NG == 2) {
-                const uint4 a = ldg_stream(kp), b = ldg_stream(vp);
+                const uint4 a = ld_stream(kp), b = ld_stream(vp);
                 kw[half][0] = a.x; kw[half][1] = a.y; kw[half][2] = a.z; kw[half][3] = a.w;
                 vw[half][0] = b.x; vw[half][1] = b.y; vw[half][2] = b.z; vw[half][3] = b.w;
             } else {
-                const uint2 a = __ldg(reinterpret_cast<const uint2*>(kp));
-                const uint2 b = __ldg(reinterpret_cast<const uint2*>(vp));
+                const uint2 a = *reinterpret_cast<const uint2*>(kp);
+                const uint2 b = *reinterpret_cast<const uint2*>(vp);
                 kw[half][0] = a.x; kw[half][1] = a.y;
                 vw[half][0] = b.x; vw[half][1] = b.y;
             }
 #pragma unroll
             for (int grp = 0; grp < F::NG; ++grp) {
-                pk[half][grp] = __ldg(par + (half * 8 + g) * 2 * F::NG + grp);
-                pv[half][0][grp] = __ldg(par + ((half * 8 + 2 * c) * 2 + 1) * F::NG + grp);
-                pv[half][1][grp] = __ldg(par + ((half * 8 + 2 * c) * 2 + 3) * F::NG + grp);
+                pk[half][grp] = par[(half * 8 + g) * 2 * F::NG + grp];
+                pv[half][0][grp] = par[((half * 8 + 2 * c) * 2 + 1) * F::NG + grp];
+                pv[half][1][grp] = par[((half * 8 + 2 * c) * 2 + 3) * F::NG + grp];
             }
         }
 #pragma unroll

@@ -38,3 +38,29 @@ def test_other_ctas_shared_memory_is_reached_behind_a_cluster_barrier(name, at):
     barrier = r"\bcluster\.sync\(\)|\bcluster_wait\(\)"
     assert re.search(barrier, text[function_start(text, at):at]), "no barrier before"
     assert re.search(barrier, text[at:].split("\n}\n")[0]), "no barrier after"
+
+
+EARLY = sorted({(name, k) for name, text in SOURCES.items()
+                for m in re.finditer(r"launch_early(?:_clusters)?\(\"([^;]*);", text)
+                for k in re.findall(r"\b(\w+_kernel)\b", m.group(1))})
+
+
+def test_kernels_that_begin_early_are_found():
+    assert len(EARLY) >= 10 and ("logprobs.cu", "logprobs_kernel") in EARLY and ("pool_q4.cu", "append_kernel") in EARLY
+
+
+@pytest.mark.parametrize("name,kernel", EARLY)
+def test_a_kernel_that_begins_early_reads_through_coherent_loads(name, kernel):
+    """What the stream's last kernel writes changes during the lifetime of a kernel that begins early.  So
+    neither non-coherent loads (their memory has to be read-only for as long as the kernel runs) nor
+    __restrict__ (it lets the compiler take such loads, or move a load up over the wait)."""
+    files = [name] + [f for f in SOURCES if f.endswith(".cuh") and f in SOURCES[name] and kernel in SOURCES[f]]
+    found = 0
+    for f in files:
+        text = SOURCES[f]
+        for m in re.finditer(r"\b%s\(([^;{}]*)\)\s*\{" % kernel, text):
+            found += 1
+            assert "__restrict__" not in m.group(1)
+            body = text[m.end():].split("\n}\n")[0]
+            assert not re.search(r"\b__ldg\(|\bldg_stream\(|\.nc\b", body)
+    assert found >= 1
