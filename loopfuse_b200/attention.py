@@ -309,6 +309,8 @@ def decode_q4_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int
 
 
 def _check_decode_q4(q, pages, block_table, seq_lens, out, workspace) -> None:
+    if workspace is not None and not workspace.is_contiguous():
+        raise LoopfuseError(_lib.LF_EINVAL, "paged_decode_q4: workspace must be contiguous")
     _require(q, "q")
     D = q4_head_dim(pages)
     _require(block_table, "block_table", torch.int32)

@@ -44,6 +44,14 @@ def test_tensors_off_the_gpu_and_of_other_types_are_refused():
         att.expand_pages_q4(pages, i32[None], i32, 1)
 
 
+def test_a_workspace_with_gaps_is_refused():
+    """Its bytes are counted as if they followed one another: the partials would go past its end."""
+    pages, i32 = torch.zeros(2, 1, 18 * 64, dtype=torch.uint8), torch.zeros(1, dtype=torch.int32)
+    for ws in (torch.zeros(1 << 16, dtype=torch.uint8)[::2], torch.zeros(64, 64)[:, :32]):
+        with pytest.raises(LoopfuseError, match="workspace"):
+            att.paged_decode_q4(torch.zeros(1, 1, 64).bfloat16(), pages, i32[None], i32, workspace=ws)
+
+
 @pytest.mark.parametrize("change,words", [
     (dict(head_dim=96), b"head_dim"), (dict(num_q_heads=6), b"1, 2, 4 or 8"), (dict(num_q_heads=5), b"multiple"),
     (dict(q=P + 2), b"aligned"), (dict(pages=P + 8), b"aligned"), (dict(q=None), b"null"),
