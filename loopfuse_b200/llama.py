@@ -95,11 +95,11 @@ class LoraAdapters:
                  seed: Optional[int] = None, std: float = 0.02):
         if rank not in mo.LORA_RANKS:
             raise _lib.LoopfuseError(_lib.LF_EINVAL, f"rank {rank} is not one of {mo.LORA_RANKS}")
+        if not 1 <= num_adapters <= mo.MAX_ADAPTERS:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"num_adapters must be 1..{mo.MAX_ADAPTERS}, got {num_adapters}")
         c = cfg
         self.num_adapters, self.rank, self.device = num_adapters, rank, torch.device(device)
-        nq = c.q_heads * c.head_dim
-        self.shapes = {"qkv": (c.d_model, nq + 2 * c.kv_heads * c.head_dim), "o": (nq, c.d_model),
-                       "gate_up": (c.d_model, 2 * c.ffn), "down": (c.ffn, c.d_model)}
+        self.shapes = self.shapes_of(c)
         g = None
         if seed is not None:
             g = torch.Generator(device=self.device).manual_seed(seed)
@@ -111,6 +111,23 @@ class LoraAdapters:
         self.weights = [{k: (w(num_adapters, i, rank), w(num_adapters, rank, o))
                          for k, (i, o) in self.shapes.items()} for _ in range(c.layers)]
         self.scale = torch.ones(num_adapters, dtype=torch.float32, device=self.device)
+
+    @staticmethod
+    def shapes_of(c: LlamaConfig) -> dict:
+        """(inputs, outputs) of each projection that takes an adapter."""
+        nq = c.q_heads * c.head_dim
+        return {"qkv": (c.d_model, nq + 2 * c.kv_heads * c.head_dim), "o": (nq, c.d_model),
+                "gate_up": (c.d_model, 2 * c.ffn), "down": (c.ffn, c.d_model)}
+
+    def check(self, cfg: LlamaConfig, device: torch.device, ids: Optional[Sequence[int]], n: int) -> None:
+        """Raises unless these are adapters of a model of ``cfg`` on ``device`` and ``ids`` (None: not
+        looked at) names one, or -1, for each of ``n`` sessions."""
+        if self.shapes != self.shapes_of(cfg) or len(self.weights) != cfg.layers or self.scale.device != device:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, "the adapters' layers, shapes or device are not the model's")
+        if ids is not None and (len(ids) != n or
+                                (n and not (-1 <= min(ids) and max(ids) < self.num_adapters))):
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"adapter_ids must name one adapter for each of {n} sessions, "
+                                                     f"-1 (none) or 0..{self.num_adapters - 1}")
 
     def set(self, index: int, layer: int, name: str, a: torch.Tensor, b: torch.Tensor,
             scale: float = 1.0) -> None:
@@ -257,6 +274,8 @@ class LlamaShaped:
         logits with ``return_logits``).  With ``top_logprobs`` (0 to 32 alternatives): ``(tokens,
         TokenLogprobs)`` of the tokens chosen.  ``adapter_ids`` names each session's adapter (-1:
         none).  ``n_prefix_pages``: leading pages that are the same for every session listed."""
+        if top_logprobs is not None:
+            self._check_top("top_logprobs", top_logprobs)
         x = self._trunk(tokens, pool, states, counts, n_prefix_pages, timer, adapters, adapter_ids)
         last = torch.tensor([int(n) for n in counts], device=self.device).cumsum(0) - 1
         h = self._norm_in(x[last].contiguous(), None, self.final_norm)
@@ -283,6 +302,9 @@ class LlamaShaped:
         counts = [int(n) for n in counts]
         if not sum(counts):
             raise _lib.LoopfuseError(_lib.LF_EINVAL, "score: the batch has no tokens")
+        self._check_top("top_k", top_k)
+        if rows < 1:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"score: rows must be at least 1, got {rows}")
         tokens = tokens.to(self.device).long()
         x = self._trunk(tokens, pool, states, counts, n_prefix_pages, None, adapters, adapter_ids)
         nxt = torch.full_like(tokens, -1)
@@ -293,11 +315,30 @@ class LlamaShaped:
                  for i in range(0, h.shape[0], rows)]
         return mo.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
 
+    # What a batch can be refused for is refused before the pool's sessions grow.
+    def _check_top(self, what: str, k: int) -> None:
+        most = min(mo.MAX_TOP_LOGPROBS, self.cfg.vocab)
+        if not 0 <= k <= most:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"{what} = {k} outside 0..{most}")
+
+    def _check_batch(self, tokens, pool, states, counts, n_prefix_pages, adapters, adapter_ids) -> None:
+        if len(counts) != len(states) or min(counts, default=0) < 0 or tokens.numel() != sum(counts):
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"{tokens.numel()} tokens and counts {counts} do not match "
+                                                     f"{len(states)} sessions")
+        if not 0 <= n_prefix_pages <= pool.max_pages_per_seq:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"n_prefix_pages = {n_prefix_pages} outside "
+                                                     f"0..{pool.max_pages_per_seq}")
+        if (adapters is None) != (adapter_ids is None):
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, "adapters need one adapter id per session")
+        if adapters is not None:
+            adapters.check(self.cfg, self.embed.device, adapter_ids, len(states))
+
     def _trunk(self, tokens, pool, states, counts, n_prefix_pages, timer, adapters, adapter_ids):
         """Every layer for the batch's new tokens; returns the residual stream ``[T, d_model]``."""
         c = self.cfg
         counts = [int(x) for x in counts]
         T = sum(counts)
+        self._check_batch(tokens, pool, states, counts, n_prefix_pages, adapters, adapter_ids)
         starts_host = [s.current_len for s in states]
         start = pool.reserve(states, counts)
         index = pool.batch_index(states, counts)
@@ -320,8 +361,6 @@ class LlamaShaped:
                 self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         adapted = None
         if adapters is not None:
-            if adapter_ids is None or len(adapter_ids) != len(states):
-                raise _lib.LoopfuseError(_lib.LF_EINVAL, "adapters need one adapter id per session")
             adapted = _Adapted(adapters, pool._ids(adapter_ids), index[1], T)
         if timer is not None:
             timer.lap("setup")
@@ -389,6 +428,8 @@ class GraphedDecode:
     def __init__(self, model: "LlamaShaped", pool: KVPool, pad: KVState, n_prefix_pages: int = 0,
                  adapters: Optional[LoraAdapters] = None):
         self.model, self.pool, self.pad, self.npp = model, pool, pad, n_prefix_pages
+        if adapters is not None:
+            adapters.check(model.cfg, model.embed.device, None, 0)
         self.adapters = adapters
         self.graphs = {}
         self.status_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
@@ -463,8 +504,12 @@ class GraphedDecode:
         (the first ``len(states)`` rows are valid).  ``adapter_ids``: each session's adapter (-1 or
         not given: none), when the graphs were built with ``adapters``."""
         n = len(states)
-        if adapter_ids is not None and (self.adapters is None or len(adapter_ids) != n):
-            raise _lib.LoopfuseError(_lib.LF_EINVAL, "adapter_ids need adapters and one id per session")
+        if len(tokens) != n:
+            raise _lib.LoopfuseError(_lib.LF_EINVAL, f"{len(tokens)} tokens do not match {n} sessions")
+        if adapter_ids is not None:
+            if self.adapters is None:
+                raise _lib.LoopfuseError(_lib.LF_EINVAL, "adapter_ids need a graph built with adapters")
+            self.adapters.check(self.model.cfg, self.model.embed.device, adapter_ids, n)
         nb = _bucket(n)
         s = self.graphs.get(nb)
         if s is None:

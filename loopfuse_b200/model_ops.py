@@ -154,6 +154,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
 
 # -- low-rank adapters ----------------------------------------------------------------------------
 LORA_RANKS = (16, 32, 64, 128)
+MAX_ADAPTERS = 4096
 
 
 @dataclass
