@@ -271,8 +271,8 @@ class LlamaShaped:
                 adapters: Optional[LoraAdapters] = None,
                 adapter_ids: Optional[Sequence[int]] = None, top_logprobs: Optional[int] = None):
         """Advance each session by ``counts[i]`` tokens; the greedy next token of each (their fp32
-        logits with ``return_logits``).  With ``top_logprobs`` (0 to 32 alternatives): ``(tokens,
-        TokenLogprobs)`` of the tokens chosen.  ``adapter_ids`` names each session's adapter (-1:
+        logits with ``return_logits``).  With ``top_logprobs`` (0 to 32 alternatives): the same and the
+        ``TokenLogprobs`` of the greedy tokens, a pair.  ``adapter_ids`` names each session's adapter (-1:
         none).  ``n_prefix_pages``: leading pages that are the same for every session listed."""
         if top_logprobs is not None:
             self._check_top("top_logprobs", top_logprobs)
@@ -281,12 +281,10 @@ class LlamaShaped:
         h = self._norm_in(x[last].contiguous(), None, self.final_norm)
         logits = h @ self.lm_head
         _lap(timer, "lm_head")
-        if return_logits:
-            out = logits.float()
-        else:
-            out = torch.argmax(logits, dim=-1)
-            if top_logprobs is not None:
-                out = out, mo.token_logprobs(logits, out, top_k=top_logprobs)
+        out = logits.float() if return_logits else torch.argmax(logits, dim=-1)
+        if top_logprobs is not None:
+            chosen = torch.argmax(logits, dim=-1) if return_logits else out
+            out = out, mo.token_logprobs(logits, chosen, top_k=top_logprobs)
         _lap(timer, "argmax")
         return out
 

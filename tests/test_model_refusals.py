@@ -108,3 +108,17 @@ def test_a_refused_batch_leaves_the_pool_as_it_was():
             m.forward(toks, pool, states, [2, 1], **kw)
     assert pool.snapshot() == before and torch.equal(pool.pages, pages)
     assert [s.current_len for s in states] == [2, 1] and first.shape == (2,)
+
+
+def test_logits_and_alternatives_can_be_asked_for_together(model, monkeypatch):
+    x = torch.randn(3, TINY.d_model, generator=torch.Generator().manual_seed(0)).bfloat16()
+    monkeypatch.setattr(model, "fused_ops", False)
+    monkeypatch.setattr(model, "_trunk", lambda *a: x.clone())
+    monkeypatch.setattr(mo, "token_logprobs", lambda logits, tokens, top_k: ("logprobs", tokens, top_k))
+    pool = Pool()
+    states, toks = batch(pool)
+    logits = model.forward(toks, pool, states, [2, 1], return_logits=True)
+    chosen, lp = model.forward(toks, pool, states, [2, 1], top_logprobs=4)
+    both = model.forward(toks, pool, states, [2, 1], return_logits=True, top_logprobs=4)
+    assert torch.equal(both[0], logits) and torch.equal(chosen, logits.argmax(-1))
+    assert both[1][0] == "logprobs" and torch.equal(both[1][1], chosen) and both[1][2] == 4
