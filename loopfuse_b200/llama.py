@@ -88,8 +88,10 @@ def _lap(timer: Optional[OpTimer], name: str) -> None:
 class LoraAdapters:
     """Low-rank adapters of the four projections of every layer, ``num_adapters`` of rank ``rank``:
     per layer and projection ``a [num_adapters, inputs, rank]``, ``b [num_adapters, rank, outputs]``
-    (bf16, in ``weights``), and one ``scale [num_adapters]`` (fp32).  Ranks are 16, 32, 64 or 128;
-    a smaller adapter is padded with zeros (``set``).  ``seed`` None leaves all of them zero."""
+    (bf16, in ``weights``) and a scale for each adapter (``scales [layers, projections, num_adapters]``,
+    fp32, in the order of ``shapes``), and besides one ``scale [num_adapters]`` of whole adapters, which
+    multiplies those.  Ranks are 16, 32, 64 or 128; a smaller adapter is padded with zeros (``set``).
+    ``seed`` None leaves all weights zero; scales begin as ones."""
 
     def __init__(self, cfg: LlamaConfig, num_adapters: int, rank: int, device="cuda",
                  seed: Optional[int] = None, std: float = 0.02):
@@ -111,6 +113,7 @@ class LoraAdapters:
         self.weights = [{k: (w(num_adapters, i, rank), w(num_adapters, rank, o))
                          for k, (i, o) in self.shapes.items()} for _ in range(c.layers)]
         self.scale = torch.ones(num_adapters, dtype=torch.float32, device=self.device)
+        self.scales = torch.ones((c.layers, len(self.shapes), num_adapters), dtype=torch.float32, device=self.device)
 
     @staticmethod
     def shapes_of(c: LlamaConfig) -> dict:
@@ -131,7 +134,8 @@ class LoraAdapters:
 
     def set(self, index: int, layer: int, name: str, a: torch.Tensor, b: torch.Tensor,
             scale: float = 1.0) -> None:
-        """Adapter ``index`` of one projection: ``a [inputs, r]``, ``b [r, outputs]``, r <= rank."""
+        """Adapter ``index`` of one projection: ``a [inputs, r]``, ``b [r, outputs]``, r <= rank, and its
+        scale there."""
         i, o = self.shapes[name]
         r = a.shape[1]
         if tuple(a.shape) != (i, r) or tuple(b.shape) != (r, o) or r > self.rank or \
@@ -143,7 +147,7 @@ class LoraAdapters:
         wb[index].zero_()
         wa[index, :, :r] = a
         wb[index, :r] = b
-        self.scale[index] = scale
+        self.scales[layer, list(self.shapes).index(name), index] = scale
 
 
 class _Adapted:
@@ -152,10 +156,12 @@ class _Adapted:
     def __init__(self, adapters: LoraAdapters, ids: torch.Tensor, cu: torch.Tensor, total: int):
         self.adapters = adapters
         self.plan = mo.lora_plan(ids, cu, total, adapters.num_adapters)
+        self.scales = adapters.scales * adapters.scale
+        self.place = {name: i for i, name in enumerate(adapters.shapes)}
 
     def add(self, y: torch.Tensor, x: torch.Tensor, layer: int, name: str) -> torch.Tensor:
         a, b = self.adapters.weights[layer][name]
-        return mo.lora_add(y, x, a, b, self.plan, self.adapters.scale)
+        return mo.lora_add(y, x, a, b, self.plan, self.scales[layer, self.place[name]])
 
 
 class LlamaShaped:
