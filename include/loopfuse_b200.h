@@ -393,9 +393,10 @@ int lf_pool_unregister_all(const lf_pool_meta* m, const lf_prefix_registry* r, v
  * h*stride_head + d.  num_q_heads > 0 (one layer): q rows of num_q_heads * D at t*q_stride_token
  * are copied to q_out [total_tokens, num_q_heads, D].  rope_cos / rope_sin (nullable): q and k are
  * rotated as in lf_pool_write_qkv first.  pages is [num_layers][num_pages][Hkv][18 * D].  A row
- * without a page, or past the rotation table, is not stored: *status (nullable, a pool's sticky
- * status; nothing is done when it is already set) becomes LF_EINVAL, or, without a status, the
- * device error word 252.  Strides multiples of 8, buffers 16-byte aligned. */
+ * without a page, past the rotation table or of no session (before cu_tokens[0], from cu_tokens[n]
+ * on) is not stored, nor is q of the last two kinds: *status (nullable, a pool's sticky status;
+ * nothing is done when it is already set) becomes LF_EINVAL, or, without a status, the device error
+ * word 252.  Strides multiples of 8, buffers 16-byte aligned. */
 int lf_q4_append(const lf_bf16* q, const lf_bf16* k, const lf_bf16* v, int64_t q_stride_token,
                  int64_t stride_layer, int64_t stride_token, int64_t stride_head,
                  const int32_t* block_table, int table_rows, int max_pages, const int32_t* seq_ids,

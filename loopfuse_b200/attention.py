@@ -251,7 +251,9 @@ def append_qkv_q4(qkv: torch.Tensor, pages: torch.Tensor, block_table: torch.Ten
     cu_tokens[i]`` of ``block_table [N, max_pages]``, into ``pages [P, Hkv, 18 * D]``; q and k are
     first rotated with ``rope = (cos, sin)`` (``[rows, D/2]`` fp32, "rotate half").  Returns the
     rotated q ``[T, Hq, D]`` (``q_out`` when given).  Block-table rows and pages are the caller's to
-    reserve; a token without a page is not stored and is reported by ``lf_device_status``.
+    reserve; a token without a page, or a row of no session (before ``cu_tokens[0]`` or from
+    ``cu_tokens[N]`` on: its q is not written either), is not stored and is reported by
+    ``lf_device_status``.
     """
     D = q4_head_dim(pages)
     P, Hkv, _ = pages.shape

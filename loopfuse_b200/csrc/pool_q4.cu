@@ -53,8 +53,8 @@ __device__ __forceinline__ void report(const AppendArgs& a) {
 // One CTA walks tokens (grid-stride, blockIdx.y the layer); a row of D dims of one head is D / 8
 // lanes of 8 dims: the queries' rows, then k's and v's, from the last warp on.  Rotation uses the partner
 // lane's 8 dims and rounds every product and sum separately, then to bf16, as an eager fp32
-// evaluation does; the codes are those of the rounded values.  A row that has no page, or no rotation
-// table row, is not stored and is reported.
+// evaluation does; the codes are those of the rounded values.  A row that has no session, no page, or no
+// rotation table row is not stored and is reported.
 template <int D>
 __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
     using F = Fmt<D>;
@@ -84,9 +84,11 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
             lo += k * step;
             len = min(step, len - k * step);
         }
-        const int pos = a.start[lo] + (t - a.cu[lo]);
+        const int begin = a.cu[lo];
+        const bool owned = t >= begin && t < a.cu[lo + 1];     // (no: before the first session or behind the last)
+        const int pos = owned ? a.start[lo] + (t - begin) : -1;
         const int row = a.seq_ids != nullptr ? a.seq_ids[lo] : lo;
-        const bool pos_ok = a.cos == nullptr || (pos >= 0 && pos < a.rope_rows);
+        const bool pos_ok = owned && (a.cos == nullptr || (pos >= 0 && pos < a.rope_rows));
         int page = -1;
         if (row >= 0 && row < a.table_rows && pos >= 0 && pos / kPage < a.table_stride)
             page = a.table[(long)row * a.table_stride + pos / kPage];

@@ -333,6 +333,41 @@ def test_append_without_a_page_stores_nothing_and_is_reported():
     assert drain_status() == [252] and torch.equal(dev.cpu(), pages)
 
 
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 4, 2), (64, 3, 3)])
+@pytest.mark.parametrize("turn", [False, True])
+@pytest.mark.parametrize("cu,T", [([2, 5], 5), ([0, 3], 7), ([3, 3, 4, 9], 11), ([0, 0], 2), ([6, 6, 6], 9)])
+def test_append_leaves_rows_of_no_session_alone(D, Hq, Hkv, turn, cu, T):
+    """Rows before cu[0] and from cu[n] on, as of a padded batch: no page, no q, one report."""
+    gen = torch.Generator().manual_seed(T + D)
+    N = len(cu) - 1
+    start = [20 + 3 * i for i in range(N)]
+    table, P = table_for([64] * N, gen=gen)
+    pages = random_pages(gen, P, Hkv, D)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=gen).bfloat16().cuda()
+    rope = tuple(t.cuda() for t in rope_tables(64, D)) if turn else None
+    i32 = dict(dtype=torch.int32, device="cuda")
+    runs = []
+    for rows, offsets in ((qkv, cu), (qkv[cu[0]:cu[-1]], [c - cu[0] for c in cu])):
+        dev, q = pages.cuda(), torch.full((rows.shape[0], Hq, D), 7.0, dtype=torch.bfloat16, device="cuda")
+        att.append_qkv_q4(rows, dev, table.cuda(), torch.tensor(start, **i32), torch.tensor(offsets, **i32), Hq,
+                          rope=rope, q_out=q)
+        runs.append((dev, q, drain_status()))
+    (dev, q, status), (dev2, q2, status2) = runs
+    assert torch.equal(dev, dev2) and torch.equal(q[cu[0]:cu[-1]], q2)
+    assert (q[:cu[0]] == 7).all() and (q[cu[-1]:] == 7).all()
+    assert status == [252] and status2 == []
+    # with a pool's status: that instead of the device's word
+    st = torch.zeros(1, **i32)
+    dev = pages.cuda()
+    base, row = qkv.data_ptr(), qkv.shape[1]
+    tb, sp, ct = table.cuda(), torch.tensor(start, **i32), torch.tensor(cu, **i32)
+    _lib.call("lf_q4_append", None, base + Hq * D * 2, base + (Hq + Hkv) * D * 2, 0, 0, row, D, tb.data_ptr(), N,
+              table.shape[1], None, sp.data_ptr(), ct.data_ptr(), N, T, None, None, 0, None, dev.data_ptr(), P, 1, 0,
+              Hkv, D, st.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert st.item() == _lib.LF_EINVAL and drain_status() == []
+
+
 # -- expansion --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("D,Hkv", [(128, 2), (64, 3)])
 @pytest.mark.parametrize("npre", [0, 2])
