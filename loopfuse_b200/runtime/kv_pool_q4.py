@@ -36,6 +36,9 @@ class QuantKVPool(KVPool):
     @classmethod
     def from_config(cls, kv_config: dict, device: str = "cuda", max_slots: int = 8,
                     num_pages: Optional[int] = None) -> "QuantKVPool":
+        dtype = kv_config.get("dtype", "bf16")
+        if dtype != "bf16":
+            raise LoopfuseError(_lib.LF_EINVAL, f"QuantKVPool takes bf16 K/V, got {dtype}")
         return cls(num_layers=kv_config["num_layers"], num_heads=kv_config["num_heads"],
                    head_dim=kv_config["head_dim"], max_seq_len=kv_config["max_seq_len"],
                    device=device, max_slots=max_slots, num_kv_heads=kv_config.get("num_kv_heads"),

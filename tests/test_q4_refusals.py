@@ -120,6 +120,18 @@ def test_fork_and_pool_arguments():
         QuantKVPool(1, 1, 64, 64, device="cpu")
 
 
+def test_a_config_of_another_type_is_refused_as_by_the_constructor(monkeypatch):
+    cfg = {"num_layers": 1, "num_heads": 2, "head_dim": 64, "max_seq_len": 64}
+    for dtype in ("fp16", "fp32", "int8"):
+        with pytest.raises(LoopfuseError, match="bf16"):
+            QuantKVPool.from_config(dict(cfg, dtype=dtype))
+    made = []
+    monkeypatch.setattr(QuantKVPool, "__init__", lambda self, *a, **kw: made.append(kw.get("dtype", torch.bfloat16)))
+    for more in ({}, {"dtype": "bf16"}):
+        QuantKVPool.from_config(dict(cfg, **more))
+    assert made == [torch.bfloat16] * 2
+
+
 def test_workspace():
     """(148 x 12 ranges (16 of 64 dims) + N Hkv items) x G partials, prefix chunks x N Hq partials, a
     span per item."""
