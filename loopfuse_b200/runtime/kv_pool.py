@@ -511,10 +511,11 @@ class KVPool:
             raise LoopfuseError(_lib.LF_EINVAL, "write_qkv: q_out must be contiguous [T, Hq, D]")
         if rope is not None:
             for t in rope:
-                if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
-                        t.shape[1] != D // 2 or t.device != self.device:
-                    raise LoopfuseError(_lib.LF_EINVAL, "write_qkv: rope tables must be "
-                                                        "contiguous fp32 [rows, D/2] on the pool device")
+                if len(rope) != 2 or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
+                        t.shape[1] != D // 2 or t.device != self.device or t.shape != rope[0].shape or \
+                        t.shape[0] == 0:
+                    raise LoopfuseError(_lib.LF_EINVAL, "write_qkv: rope must be two contiguous fp32 tables "
+                                                        "[rows, D/2] on the pool device")
         self._write_qkv(ids, start, cu_t, total, layer, qkv, q_out, rope, stream)
 
     # -- prefix-hash dedup (content-addressed KV fusion) ----------------------------------
