@@ -379,25 +379,31 @@ class KVPool:
             return
         tdim = 1 if layout == "lthd" else 2
         counts = [int(k.shape[tdim]) for k in keys]
-        start = self._reserve(states, counts, stream)
         total = sum(counts)
         if total == 0:
+            self._reserve(states, counts, stream)
             return
         if len(keys) == 1:
             k_all, v_all = keys[0], values[0]
         else:
             k_all = torch.cat(list(keys), dim=tdim)
             v_all = torch.cat(list(values), dim=tdim)
+        shape = (self.num_layers, total, self.num_kv_heads, self.head_dim) if layout == "lthd" else \
+            (self.num_layers, self.num_kv_heads, total, self.head_dim)
         for t in (k_all, v_all):
-            if t.device != self.device or t.dtype != self.dtype or t.stride(-1) != 1:
-                raise LoopfuseError(_lib.LF_EINVAL, "new K/V must be on the pool's device, in the "
-                                                    "pool dtype, with contiguous head_dim")
+            if t.device != self.device or t.dtype != self.dtype or t.stride(-1) != 1 or tuple(t.shape) != shape:
+                raise LoopfuseError(_lib.LF_EINVAL, f"new K/V must be {list(shape)} on the pool's device, in "
+                                                    "the pool dtype, with contiguous head_dim")
         if v_all.stride() != k_all.stride():
             v_all = v_all.contiguous()
             k_all = k_all.contiguous()
         sl = k_all.stride(0)
         st_tok = k_all.stride(1) if layout == "lthd" else k_all.stride(2)
         st_head = k_all.stride(2) if layout == "lthd" else k_all.stride(1)
+        for x in (k_all.data_ptr() // 2, v_all.data_ptr() // 2, sl, st_tok, st_head):
+            if x % 8:
+                raise LoopfuseError(_lib.LF_EINVAL, "new K/V rows must be 16-byte aligned")
+        start = self._reserve(states, counts, stream)
         cu = [0]
         for c in counts:
             cu.append(cu[-1] + c)

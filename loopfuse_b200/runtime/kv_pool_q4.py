@@ -79,9 +79,6 @@ class QuantKVPool(KVPool):
 
     def _write_kv(self, ids, start, cu, n, total, keys, values, s_layer, s_token, s_head, layer,
                   layers, stream) -> None:
-        for s in (s_layer, s_token, s_head):
-            if s % 8:
-                raise LoopfuseError(_lib.LF_EINVAL, "new K/V rows must be 16-byte aligned")
         self._quantise(None, keys.data_ptr(), values.data_ptr(), 0, s_layer, s_token, s_head, ids,
                        start, cu, n, total, layer, layers, None, None, stream)
 

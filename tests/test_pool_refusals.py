@@ -29,3 +29,32 @@ def test_write_qkv_takes_rotation_tables_of_one_shape_only(kind):
     assert p.stored == []
     p.write_qkv(None, None, 0, qkv, q, None, rope=(cos, cos.clone()), index=index)
     assert len(p.stored) == 1
+
+
+def state():
+    from loopfuse_b200.runtime.kv_pool import KVState
+    return KVState(0, None)
+
+
+@pytest.mark.parametrize("kind", [KVPool, QuantKVPool])
+def test_append_refuses_rows_before_the_session_grows(kind):
+    p = bare(kind)
+    p._reserve = lambda *a: pytest.fail("reserved")
+    good = torch.zeros(1, 3, 1, 64).bfloat16()
+    odd = torch.zeros(1, 3, 1, 128).bfloat16()[..., ::2]
+    wide = torch.zeros(1, 3, 2, 64).bfloat16()
+    for k, v in ((good.float(), good), (good, good.float()), (odd, odd), (wide, wide), (good, good[:, :2]),
+                 (good.expand(2, 3, 1, 64), good.expand(2, 3, 1, 64))):
+        with pytest.raises(LoopfuseError):
+            p.append([state()], [k], [v])
+
+
+def test_a_4bit_append_refuses_unaligned_rows_before_the_session_grows():
+    p = bare(QuantKVPool)
+    p._reserve = lambda *a: pytest.fail("reserved")
+    k = torch.zeros(1, 3, 1, 68).bfloat16()[..., :64]           # 136 bytes from row to row
+    with pytest.raises(LoopfuseError, match="aligned"):
+        p.append([state()], [k], [k])
+    k = torch.zeros(1, 3, 1, 72).bfloat16()[..., 4:68]          # begins 8 bytes off
+    with pytest.raises(LoopfuseError, match="aligned"):
+        p.append([state()], [k], [k])
