@@ -179,6 +179,13 @@ class AgentLoop:
         return out
 
     # -- per-kernel attribution ------------------------------------------------------------------
+    def _kv_bytes(self, phase: str) -> float:
+        """Bytes that attention moves for a token of the cache, over the layers.  A 4-bit cache (9/16 of a
+        byte a value) is expanded before a prefill attends to it: bf16 pages written and read."""
+        c = self.model.cfg
+        per_value = 2.0 if self.cfg.kv_bits == 16 else 9 / 16 + (4.0 if phase == "prefill" else 0.0)
+        return 2 * c.kv_heads * c.head_dim * c.layers * per_value
+
     def _op_work(self, T: int, n_out: int, attn_flops: float, attn_bytes: float) -> dict:
         """Algorithmic (FLOPs, HBM bytes) per op class of one forward of ``T`` new tokens
         (``n_out`` sessions' last positions go through the LM head), summed over the layers."""
@@ -192,7 +199,8 @@ class AgentLoop:
         w = {"qkv_gemm": gemm(T, d, qkv), "o_gemm": gemm(T, nq, d),
              "gate_up_gemm": gemm(T, d, 2 * f), "down_gemm": gemm(T, f, d)}
         out = {k: (L * v[0], L * v[1]) for k, v in w.items()}
-        out["qkv_rope_append"] = (0.0, L * 2.0 * T * (qkv + nq + 2 * nkv))
+        stored = 2 * nkv * (2.0 if self.cfg.kv_bits == 16 else 9 / 16)
+        out["qkv_rope_append"] = (0.0, L * T * (2.0 * (qkv + nq) + stored))
         out["attention"] = (attn_flops, attn_bytes)
         out["add_rmsnorm"] = (0.0, L * 2 * 4.0 * T * d * 2)
         out["swiglu"] = (0.0, L * 2.0 * T * 3 * f)
@@ -208,10 +216,9 @@ class AgentLoop:
         from .analysis import kernel_roofline
         from .llama import OpTimer
         c, pool = self.model.cfg, self.pool
-        # K+V bytes per token of the cache; a 4-bit cache is prefilled from its bf16 expansion
-        kv_tok = c.kv_heads * c.head_dim * c.layers * (4 if self.cfg.kv_bits == 16 else 9 / 8)
         res = {}
         for phase in ("decode", "prefill"):
+            kv_tok = self._kv_bytes(phase)
             chosen = sessions if phase == "decode" else sessions[:self.PROFILE_SESSIONS]
             states = [s.state for s in chosen]
             n = len(states)
