@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
                 for (int j = 0; j < 4; ++j) d[j] = sm100::fadd2(pair_of(w[j]), sm100::f2_pack(-mn, -mn));
                 if (s >= kSmallest) {
                     // d / s rounded to nearest from the rounded reciprocal and the exact remainder of the
-                    // first quotient (Markstein's theorem); at most 15.03, so that adding 1.5 * 2^23
+                    // first quotient (Markstein's theorem).  s is off by 2^-8 of itself at most, so d / s
+                    // is at most 15 (1 + 2^-8) < 15.06 and rounds to 15 without a limit: adding 1.5 * 2^23
                     // leaves rint(d / s), ties to even, in the low bits.
                     const float r = __frcp_rn(s);
                     const uint64_t r2 = sm100::f2_pack(r, r), s2 = sm100::f2_pack(-s, -s), m2 = sm100::f2_pack(kMagic, kMagic);

@@ -333,6 +333,29 @@ def test_append_without_a_page_stores_nothing_and_is_reported():
     assert drain_status() == [252] and torch.equal(dev.cpu(), pages)
 
 
+@pytest.mark.parametrize("power", [-100, -88, -20, 0, 40])
+def test_append_of_groups_whose_scale_is_rounded_down_most(power):
+    """Span / 15 halfway between two bf16 values: the largest code is that of 15 (1 + 2^-8) steps."""
+    gen = torch.Generator().manual_seed(1)
+    D, unit = 64, 2.0 ** power
+    rows = (torch.rand(4, 3, D, generator=gen) * 15).bfloat16().float()
+    rows[..., 0], rows[..., 1] = -15 / 256, 15.0
+    rows[1::2] = -rows[1::2]
+    rows = (rows * unit).bfloat16()
+    for x in rows[:, 1:].reshape(-1, D):                     # (the case is what it claims to be)
+        n, s, low = q4.quantise(x)
+        assert float(s) == unit and int(n.max()) == 15
+        assert float(((x.double() - low) / s).max()) == 15 + 15 / 256
+    pages = torch.zeros(1, 1, 18 * D, dtype=torch.uint8)
+    dev = pages.cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    att.append_qkv_q4(rows.reshape(4, -1).cuda(), dev, torch.zeros(1, 1, **i32), torch.zeros(1, **i32),
+                      torch.tensor([0, 4], **i32), 1)
+    for t in range(4):
+        q4.write_token(pages, 0, 0, t, rows[t, 1], rows[t, 2])
+    assert torch.equal(dev.cpu(), pages) and drain_status() == []
+
+
 @pytest.mark.parametrize("D,Hq,Hkv", [(128, 4, 2), (64, 3, 3)])
 @pytest.mark.parametrize("turn", [False, True])
 @pytest.mark.parametrize("cu,T", [([2, 5], 5), ([0, 3], 7), ([3, 3, 4, 9], 11), ([0, 0], 2), ([6, 6, 6], 9)])
