@@ -1,9 +1,9 @@
 // Appending K/V to 4-bit pages, and expanding 4-bit pages to bf16 pages for the prefill kernel.
 //
 // Both are passes over memory: the append reads each new K/V value once and writes 4.5 bits of it, the
-// expansion reads 4.5 bits and writes 16.  3796 tokens of 32 q and 8 k/v heads of 128: the append takes 26 us
+// expansion reads 4.5 bits and writes 16.  3796 tokens of 32 q and 8 k/v heads of 128: the append takes 28 us
 // (82 MB; issue slots and latencies, 150 instructions a row pair), the expansion of their 32 sessions'
-// contexts 57 us (283 MB, 4.9 TB/s).  The format is described in q4_common.cuh.
+// contexts 58 us (280 MB, 4.8 TB/s).  The format is described in q4_common.cuh.
 #include "pool_common.cuh"
 #include "q4_common.cuh"
 #include "sm100_primitives.cuh"
